@@ -1,0 +1,524 @@
+// zq_attn_q4.hip -- attention over the 4-bit KV cache of include/zq_kv.h.
+//
+// Rows are (query token, head of the kv head) pairs, r = t * G + g, of one
+// (sequence, kv head): the G heads that share keys are rows of one matrix
+// product, so a held row is read and decoded once for all of them.
+//
+//   s[r][p] = scale * q_r . k_p        p < visible(r)
+//   out[r]  = sum_p exp(s - lse) v_p,  lse = log sum_p exp(s)
+//   weight[p] (+)= sum_r exp(s - lse)
+//
+// The held values are exact in fp16 (11 significant bits), so they are single
+// operands of the f16 MFMA; queries and softmax weights are fp32 and go in as two
+// fp16 parts h + l (22 bits), accumulated in fp32.
+#include "../../include/zq_hip.h"
+#include "zq_internal.hpp"
+#include "zq_kv.hpp"
+
+#include <math.h>
+
+namespace zq {
+namespace {
+
+typedef float v4f_t __attribute__((ext_vector_type(4)));
+
+struct AttnQ4 {
+    zq_kv_q4 c;
+    const float* q;
+    float* out;
+    const int32_t* lens;
+    const int32_t* counts;
+    size_t stride;      // floats between the query tokens
+    float* part;        // partial outputs [head][row][split][D], where splits > 1
+    float* part_ml;     // their (max, sum) pairs [head][row][split][2]
+    float* lse;         // [head][row], log2 units, where weights are wanted
+    float scale2;       // scale * log2(e): scores are in log2 units
+    uint32_t tokens, G, KH, heads_kv;  // heads_kv = seqs * KH
+    uint32_t rows;      // tokens * G
+    uint32_t splits;
+    int full, add;
+};
+
+// What a sequence's rows see.
+struct Seq {
+    uint32_t s, kh, head, live, len;
+};
+__device__ __forceinline__ Seq seq_of(const AttnQ4& a, uint32_t head) {
+    Seq x;
+    x.head = head;
+    x.s = head / a.KH;
+    x.kh = head % a.KH;
+    const int32_t n = a.counts ? a.counts[x.s] : int32_t(a.tokens);
+    x.live = uint32_t(min(max(n, 0), int32_t(a.tokens)));  // live query tokens
+    x.len = uint32_t(clamp_len(a.lens[x.s], a.c.capacity));
+    return x;
+}
+// slots that query token t sees
+__device__ __forceinline__ uint32_t visible(const AttnQ4& a, const Seq& x, uint32_t t) {
+    return a.full ? x.len : uint32_t(min(uint64_t(x.len) + t + 1, uint64_t(a.c.capacity)));
+}
+
+__device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
+__device__ __forceinline__ float max_groups(float v) {  // over the four lanes that share lane & 15
+    v = fmaxf(v, __shfl_xor(v, 16));
+    return fmaxf(v, __shfl_xor(v, 32));
+}
+__device__ __forceinline__ float sum_groups(float v) {
+    v += __shfl_xor(v, 16);
+    return v + __shfl_xor(v, 32);
+}
+
+// ---- few rows: 16 rows a workgroup, keys split over waves and workgroups ----------
+// v_mfma_f32_16x16x32_f16 throughout, computed transposed (S^T = K Q^T, O^T = V^T
+// P^T) so that nothing crosses lanes between the two products:
+//  * lane (i = lane & 15, g = lane >> 4) loads codes of key 8 (i >> 2) + 4 t + (i & 3)
+//    of a 32-key tile for the two 16-key products t = 0, 1, the g-th quarter of its
+//    row; the dimension that a k slot stands for is the same for K and Q and need not
+//    be in order.  Lane (i, g) then holds the scores of row i and keys 8 g ... 8 g + 7;
+//  * which is what the second product's B operand wants of it.  Its A operand is V^T:
+//    lane (i, g) loads the i-th 1/16 of the rows of keys 8 g ... 8 g + 7 and picks
+//    one nibble position of two rows with one v_perm.
+// K and V so go from HBM into the operands without LDS, a wave takes whole tiles on
+// its own, and the running maximum is only moved (and the sums rescaled) when a score
+// passes it by 2^8: weights stay below 2^14, within fp16.
+constexpr int kWaves = 4;
+constexpr float kShift = 6.0f;  // weights are 2^(s - max + kShift)
+constexpr float kSlack = 8.0f;  // how far a score may pass the running maximum
+
+// The k-slot order of a dword's 8 nibbles (nibbles2 of w, w >> 4, w >> 8, w >> 12):
+// elements 0, 2, 16, 18, 1, 3, 17, 19 of the block from the dword's first byte on.
+__device__ __forceinline__ h8_t dequant8(uint32_t w, h2_t d) {
+    const h2_t a = nibbles2(w) * d, b = nibbles2(w >> 4) * d, c = nibbles2(w >> 8) * d, e = nibbles2(w >> 12) * d;
+    return h8_t{a.x, a.y, b.x, b.y, c.x, c.y, e.x, e.y};
+}
+
+template <int D>
+struct KTile {  // a wave's part of 32 keys
+    static constexpr int KB = D / 8;   // bytes of a row that a lane takes (2 steps a dword... one a dword)
+    static constexpr int KW = KB / 4;  // dwords, = MFMA steps
+    static constexpr int NS = KB > 16 ? KB / 16 : 1;  // scales of a lane's part
+    uint32_t w[2][KW];
+    uint16_t sc[2][NS];
+};
+template <int D>
+struct VTile {
+    static constexpr int VB = D / 32;  // bytes of a row that a lane takes
+    static constexpr int VW = VB > 4 ? VB / 4 : 1;
+    uint32_t w[8][VW];
+    h8_t sc;  // of the 8 keys
+};
+
+template <int D>
+__device__ __forceinline__ void load_k(KTile<D>& t, const AttnQ4& a, uint32_t head, uint32_t key0, int i, int g) {
+    using K = KTile<D>;
+    const size_t cap = a.c.capacity;
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+        const uint32_t key = key0 + 8 * (i >> 2) + 4 * u + (i & 3);
+        const uint8_t* p = a.c.k + (size_t(head) * cap + key) * (D / 2) + g * K::KB;
+        if constexpr (K::KB == 8) {
+            const uint2 x = *reinterpret_cast<const uint2*>(p);
+            t.w[u][0] = x.x;
+            t.w[u][1] = x.y;
+        } else {
+#pragma unroll
+            for (int j = 0; j < K::KW / 4; ++j) {
+                const uint4 x = reinterpret_cast<const uint4*>(p)[j];
+                t.w[u][4 * j] = x.x;
+                t.w[u][4 * j + 1] = x.y;
+                t.w[u][4 * j + 2] = x.z;
+                t.w[u][4 * j + 3] = x.w;
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < K::NS; ++j)
+            t.sc[u][j] = a.c.k_scale[(size_t(head) * (D / 32) + (g * K::KB) / 16 + j) * cap + key];
+    }
+}
+template <int D>
+__device__ __forceinline__ void load_v(VTile<D>& t, const AttnQ4& a, uint32_t head, uint32_t key0, int i, int g) {
+    using V = VTile<D>;
+    const size_t cap = a.c.capacity;
+    const uint8_t* p = a.c.v + (size_t(head) * cap + key0 + 8 * g) * (D / 2) + i * V::VB;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+        if constexpr (V::VB == 2) t.w[k][0] = *reinterpret_cast<const uint16_t*>(p + k * (D / 2));
+        else if constexpr (V::VB == 4) t.w[k][0] = *reinterpret_cast<const uint32_t*>(p + k * (D / 2));
+        else {
+            const uint2 x = *reinterpret_cast<const uint2*>(p + k * (D / 2));
+            t.w[k][0] = x.x;
+            t.w[k][1] = x.y;
+        }
+    }
+    t.sc = *reinterpret_cast<const h8_t*>(a.c.v_scale + (size_t(head) * (D / 32) + (i * V::VB) / 16) * cap + key0 + 8 * g);
+}
+// scores of 32 keys and 16 rows: s[4 u + r] = row i, key 8 g + 4 u + r
+template <int D>
+__device__ __forceinline__ void scores(const KTile<D>& t, const h8_t (&qh)[D / 32], const h8_t (&ql)[D / 32], float (&s)[8]) {
+    using K = KTile<D>;
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+        v4f_t acc = {0, 0, 0, 0};
+#pragma unroll
+        for (int j = 0; j < K::KW; ++j) {
+            const _Float16 d = __builtin_bit_cast(_Float16, t.sc[u][K::NS > 1 ? j / 4 : 0]);
+            const h8_t k = dequant8(t.w[u][j], h2_t{d, d});
+            acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, qh[j], acc, 0, 0, 0);
+            acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, ql[j], acc, 0, 0, 0);
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) s[4 * u + r] = acc[r];
+    }
+}
+
+// Query row r of a (sequence, kv head), as operands: scaled to its own power of two
+// (the returned 2^-e takes it off the scores again), split into two fp16 parts.
+// Rows past the live ones are zero.
+template <int D>
+__device__ __forceinline__ float load_q(const AttnQ4& a, const Seq& x, uint32_t r, bool ok, int g, h8_t (&qh)[D / 32],
+                                        h8_t (&ql)[D / 32]) {
+    constexpr int KB = D / 8;
+    const uint32_t t = ok ? r / a.G : 0, hg = ok ? r % a.G : 0;
+    const float* q = a.q + (size_t(x.s) * a.tokens + t) * a.stride + size_t(x.kh * a.G + hg) * D;
+    float4 v[D / 32][2];
+    float m = 0.0f;
+#pragma unroll
+    for (int j = 0; j < D / 32; ++j) {
+        const int byte = g * KB + 4 * j, dim = byte / 16 * 32 + byte % 16;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            v[j][h] = ok ? *reinterpret_cast<const float4*>(q + dim + 16 * h) : make_float4(0, 0, 0, 0);
+            v[j][h].x *= a.scale2;
+            v[j][h].y *= a.scale2;
+            v[j][h].z *= a.scale2;
+            v[j][h].w *= a.scale2;
+            m = fmaxf(m, fmaxf(fmaxf(fabsf(v[j][h].x), fabsf(v[j][h].y)), fmaxf(fabsf(v[j][h].z), fabsf(v[j][h].w))));
+        }
+    }
+    m = max_groups(m);
+    const int e = m > 0.0f ? min(max(15 - __builtin_amdgcn_frexp_expf(m), -120), 120) : 0;
+    const float f = pow2f(e);
+#pragma unroll
+    for (int j = 0; j < D / 32; ++j) {
+        const float o[8] = {v[j][0].x, v[j][0].z, v[j][1].x, v[j][1].z, v[j][0].y, v[j][0].w, v[j][1].y, v[j][1].w};
+#pragma unroll
+        for (int k = 0; k < 8; ++k) split_h(o[k] * f, qh[j], ql[j], k);
+    }
+    return pow2f(-e);
+}
+
+// Tiles of 32 keys that a row tile's rows see, and how many a split takes.
+struct Cut {
+    uint32_t keys, tiles, per, used;
+};
+__device__ __forceinline__ Cut cut_of(const AttnQ4& a, const Seq& x, uint32_t r0) {
+    Cut c;
+    const uint32_t last = min(r0 + 15, x.live * a.G - 1) / a.G;
+    c.keys = visible(a, x, last);
+    c.tiles = (c.keys + 31) / 32;
+    c.per = max((c.tiles + a.splits - 1) / a.splits, uint32_t(kWaves));
+    c.used = max((c.tiles + c.per - 1) / c.per, 1u);
+    return c;
+}
+
+template <int D>
+__global__ __launch_bounds__(kWaves * 64) void attn_q4_few_kernel(AttnQ4 a) {
+    constexpr int NT = D / 16;  // 16-row O^T tiles
+    using V = VTile<D>;
+    __shared__ float so[kWaves][NT * 4][64];
+    __shared__ float sm[kWaves][16], sl[kWaves][16];
+    // the (sequence, kv head) runs fastest: with 8 of them, all row tiles and splits
+    // of one lie on one XCD and share its L2
+    const uint32_t head = blockIdx.x % a.heads_kv, rest = blockIdx.x / a.heads_kv;
+    const uint32_t sp = rest % a.splits, r0 = rest / a.splits * 16;
+    const Seq x = seq_of(a, head);
+    if (r0 >= x.live * a.G) return;
+    const Cut cut = cut_of(a, x, r0);
+    if (sp >= cut.used) return;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, g = lane >> 4;
+    const uint32_t r = r0 + i;
+    const bool ok = r < x.live * a.G;
+    const uint32_t lim = ok ? visible(a, x, r / a.G) : 0;
+    // tiles below it need no mask: every live row sees them
+    const uint32_t whole = visible(a, x, r0 / a.G) / 32;
+
+    h8_t qh[D / 32], ql[D / 32];
+    const float c = load_q<D>(a, x, r, ok, g, qh, ql);
+    v4f_t o[NT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) o[n] = v4f_t{0, 0, 0, 0};
+    float m = -INFINITY, l = 0.0f;
+
+    const uint32_t t1 = min((sp + 1) * cut.per, cut.tiles);
+    uint32_t t = sp * cut.per + wave;
+    KTile<D> kt;
+    VTile<D> vt;
+    if (t < t1) {
+        load_k<D>(kt, a, head, t * 32, i, g);
+        load_v<D>(vt, a, head, t * 32, i, g);
+    }
+    for (; t < t1; t += kWaves) {
+        float s[8];
+        scores<D>(kt, qh, ql, s);
+        const VTile<D> vn = vt;
+        if (t + kWaves < t1) {
+            load_k<D>(kt, a, head, (t + kWaves) * 32, i, g);
+            load_v<D>(vt, a, head, (t + kWaves) * 32, i, g);
+        }
+        h8_t vsc = vn.sc;
+        if (t >= whole) {
+            const uint32_t key = t * 32 + 8 * g;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                s[k] = key + k < lim ? s[k] : -INFINITY;
+                vsc[k] = key + k < cut.keys ? vsc[k] : _Float16(0);  // rows that hold nothing: their scale may be any bits
+            }
+        }
+        float mx = fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])), fmaxf(fmaxf(s[4], s[5]), fmaxf(s[6], s[7]))) * c;
+        if (__any(mx > m + kSlack)) {
+            const float mn = fmaxf(m, max_groups(mx));
+            const float f = exp2_(m - (mn == -INFINITY ? 0.0f : mn));  // 0 where nothing was summed yet
+            m = mn;
+            l *= f;
+#pragma unroll
+            for (int n = 0; n < NT; ++n) o[n] *= f;
+        }
+        const float ms = (m == -INFINITY ? 0.0f : m) - kShift;
+        h8_t ph, pl;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const float p = exp2_(fmaf(s[k], c, -ms));
+            l += p;
+            split_h(p, ph, pl, k);
+        }
+        h2_t d[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) d[k] = h2_t{vsc[2 * k], vsc[2 * k + 1]};
+#pragma unroll
+        for (int y = 0; y < V::VB; ++y) {  // byte y of a lane's part: two nibbles, two O^T tiles
+            h8_t lo, hi;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const uint32_t sel = 0x0c000c00u | uint32_t((4 + (y & 3)) << 16) | uint32_t(y & 3);
+                const uint32_t u = __builtin_amdgcn_perm(vn.w[2 * k + 1][y / 4], vn.w[2 * k][y / 4], sel);
+                const h2_t a0 = nibbles2(u) * d[k], a1 = nibbles2(u >> 4) * d[k];
+                lo[2 * k] = a0.x;
+                lo[2 * k + 1] = a0.y;
+                hi[2 * k] = a1.x;
+                hi[2 * k + 1] = a1.y;
+            }
+            o[2 * y] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo, ph, o[2 * y], 0, 0, 0);
+            o[2 * y] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo, pl, o[2 * y], 0, 0, 0);
+            o[2 * y + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi, ph, o[2 * y + 1], 0, 0, 0);
+            o[2 * y + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi, pl, o[2 * y + 1], 0, 0, 0);
+        }
+    }
+    // ---- the four waves' sums as one ----
+    l = sum_groups(l);
+    if (g == 0) {
+        sm[wave][i] = m;
+        sl[wave][i] = l;
+    }
+    __syncthreads();
+    float M = sm[0][i], L = 0.0f;
+#pragma unroll
+    for (int w = 1; w < kWaves; ++w) M = fmaxf(M, sm[w][i]);
+    const float Ms = M == -INFINITY ? 0.0f : M;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) L += sl[w][i] * exp2_(sm[w][i] - Ms);
+    const float f = exp2_(m - Ms);
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) so[wave][n * 4 + k][lane] = o[n][k] * f;
+    __syncthreads();
+    if (!ok) return;
+    const bool direct = cut.used == 1;
+    const size_t row = size_t(head) * a.rows + r;
+    if (wave == 0 && g == 0) {
+        if (!direct) {
+            float* ml = a.part_ml + (row * a.splits + sp) * 2;
+            ml[0] = M;
+            ml[1] = L;
+        } else if (a.lse) {
+            a.lse[row] = M - kShift + log2f(L);
+        }
+    }
+    float* dst = direct ? a.out + ((size_t(x.s) * a.tokens + r / a.G) * a.KH * a.G + x.kh * a.G + r % a.G) * D
+                        : a.part + (row * a.splits + sp) * D;
+    const float inv = direct ? (L > 0.0f ? 1.0f / L : (L == 0.0f ? 0.0f : L)) : 1.0f;  // no key: 0; NaN stays
+    // lane (i, g), register k of tile n = 2 y + h: row i, byte (4 g + k) VB + y of the
+    // codes, its low or high nibble.  Wave w takes k = w.
+    {
+        const int k = wave;
+        const int byte = (4 * g + k) * V::VB, dim = byte / 16 * 32 + byte % 16;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            float v[V::VB];
+#pragma unroll
+            for (int y = 0; y < V::VB; ++y) {
+                float t = 0.0f;
+#pragma unroll
+                for (int w = 0; w < kWaves; ++w) t += so[w][(2 * y + h) * 4 + k][lane];
+                v[y] = t * inv;
+            }
+            float* p = dst + dim + 16 * h;
+            if constexpr (V::VB == 2) {
+                *reinterpret_cast<float2*>(p) = make_float2(v[0], v[1]);
+            } else {
+#pragma unroll
+                for (int y = 0; y < V::VB; y += 4)
+                    *reinterpret_cast<float4*>(p + y) = make_float4(v[y], v[y + 1], v[y + 2], v[y + 3]);
+            }
+        }
+    }
+}
+
+// One wave a row: the splits' partial outputs as one.  Splits are few (at most
+// 128), their maxima and sums are held by the lanes.
+template <int D>
+__global__ __launch_bounds__(256) void attn_q4_combine_kernel(AttnQ4 a) {
+    const uint32_t id = blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63;
+    const uint32_t head = id / a.rows, r = id % a.rows;
+    if (head >= a.heads_kv) return;
+    const Seq x = seq_of(a, head);
+    if (r >= x.live * a.G) return;
+    const Cut cut = cut_of(a, x, r / 16 * 16);
+    if (cut.used == 1) return;  // written by the split itself
+    const size_t row = size_t(head) * a.rows + r;
+    const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + row * a.splits;
+    const float2 none = make_float2(-INFINITY, 0.0f);
+    const float2 p0 = uint32_t(lane) < cut.used ? ml[lane] : none;
+    const float2 p1 = uint32_t(lane) + 64 < cut.used ? ml[lane + 64] : none;
+    const float M = wave_max(fmaxf(p0.x, p1.x)), Ms = M == -INFINITY ? 0.0f : M;
+    const float w0 = exp2_(p0.x - Ms), w1 = exp2_(p1.x - Ms);
+    const float L = wave_sum(p0.y * w0 + p1.y * w1);
+    constexpr int E = D / 64;
+    const float* part = a.part + row * a.splits * D + lane * E;
+    float acc[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc[e] = 0.0f;
+    for (uint32_t j = 0; j < cut.used; ++j) {
+        const float w = j < 64 ? __shfl(w0, int(j)) : __shfl(w1, int(j - 64));
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[e] = fmaf(part[size_t(j) * D + e], w, acc[e]);
+    }
+    const float inv = L > 0.0f ? 1.0f / L : (L == 0.0f ? 0.0f : L);
+    float* dst = a.out + ((size_t(x.s) * a.tokens + r / a.G) * a.KH * a.G + x.kh * a.G + r % a.G) * D + lane * E;
+#pragma unroll
+    for (int e = 0; e < E; ++e) dst[e] = acc[e] * inv;
+    if (a.lse && lane == 0) a.lse[row] = M - kShift + log2f(L);
+}
+
+// ---- the rows' weights ----------------------------------------------------------
+// A wave holds 32 keys and goes over all query rows that see any of them, so every
+// key's sum has one owner and one order.
+template <int D>
+__global__ __launch_bounds__(kWaves * 64) void attn_q4_weights_kernel(AttnQ4 a) {
+    const uint32_t head = blockIdx.x % a.heads_kv, kb = blockIdx.x / a.heads_kv;
+    const Seq x = seq_of(a, head);
+    if (!x.live) return;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, g = lane >> 4;
+    const uint32_t rows = x.live * a.G, keys = visible(a, x, x.live - 1);
+    const uint32_t key0 = (kb * kWaves + wave) * 32;
+    if (key0 >= keys) return;
+    KTile<D> kt;
+    load_k<D>(kt, a, head, key0, i, g);
+    float w[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) w[k] = 0.0f;
+    // first token that sees key0
+    const uint32_t ta = a.full || key0 < x.len ? 0 : key0 - x.len;
+    for (uint32_t r0 = ta * a.G / 16 * 16; r0 < rows; r0 += 16) {
+        const uint32_t r = r0 + i;
+        const bool ok = r < rows;
+        h8_t qh[D / 32], ql[D / 32];
+        const float c = load_q<D>(a, x, r, ok, g, qh, ql);
+        const float lse = ok ? a.lse[size_t(head) * a.rows + r] : 0.0f;
+        const uint32_t lim = ok ? visible(a, x, r / a.G) : 0;
+        float s[8];
+        scores<D>(kt, qh, ql, s);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) w[k] += key0 + 8 * g + k < lim ? exp2_(fmaf(s[k], c, -lse)) : 0.0f;
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) w[k] = group_sum<16>(w[k]);
+    float* dst = a.c.weight + size_t(head) * a.c.capacity + key0 + 8 * g;
+    if (i < 8 && key0 + 8 * g + i < keys) {
+        float v = w[0];
+#pragma unroll
+        for (int k = 1; k < 8; ++k) v = i == k ? w[k] : v;
+        dst[i] = a.add ? dst[i] + v : v;
+    }
+}
+
+// How many workgroups share a row tile's keys: enough for three workgroups a CU
+// (12 of the 16-row kernel's waves), at least one tile a wave.
+uint32_t splits_of(const zq_kv_q4& c, size_t rows) {
+    const size_t base = c.seqs * c.kv_heads * ((rows + 15) / 16);
+    const size_t want = (size_t(device_cu_count()) * 3 + base - 1) / base;
+    const size_t most = (c.capacity / 32 + kWaves - 1) / kWaves;
+    return uint32_t(want < most ? (want < 128 ? want : 128) : (most < 128 ? most : 128));
+}
+
+size_t up256(size_t n) { return (n + 255) / 256 * 256; }
+
+}  // namespace
+
+size_t attention_q4_bytes(const zq_kv_q4& c, size_t tokens, size_t heads, int flags) {
+    const size_t rows = tokens * (heads / c.kv_heads), all = c.seqs * c.kv_heads * rows;
+    const size_t splits = splits_of(c, rows);
+    size_t n = 0;
+    if (splits > 1) n += up256(all * splits * c.head_dim * 4) + up256(all * splits * 8);
+    if (flags & ZQ_ATTN_Q4_WEIGHTS) n += up256(all * 4);
+    return n;
+}
+
+hipError_t launch_attention_q4(const zq_kv_q4& c, const float* q, float* out, size_t tokens, size_t heads, size_t stride,
+                               const int32_t* lens, const int32_t* counts, float scale, int flags, void* ws,
+                               hipStream_t stream) {
+    AttnQ4 a{};
+    a.c = c;
+    a.q = q;
+    a.out = out;
+    a.lens = lens;
+    a.counts = counts;
+    a.stride = stride;
+    a.scale2 = float(double(scale) * 1.4426950408889634);
+    a.tokens = uint32_t(tokens);
+    a.KH = uint32_t(c.kv_heads);
+    a.G = uint32_t(heads / c.kv_heads);
+    a.heads_kv = uint32_t(c.seqs * c.kv_heads);
+    a.rows = uint32_t(tokens) * a.G;
+    a.splits = splits_of(c, a.rows);
+    a.full = (flags & ZQ_ATTN_Q4_FULL) != 0;
+    a.add = (flags & ZQ_ATTN_Q4_ADD) != 0;
+    const size_t all = size_t(a.heads_kv) * a.rows;
+    uint8_t* p = static_cast<uint8_t*>(ws);
+    if (a.splits > 1) {
+        a.part = reinterpret_cast<float*>(p);
+        p += up256(all * a.splits * c.head_dim * 4);
+        a.part_ml = reinterpret_cast<float*>(p);
+        p += up256(all * a.splits * 8);
+    }
+    if (flags & ZQ_ATTN_Q4_WEIGHTS) a.lse = reinterpret_cast<float*>(p);
+    const size_t blocks = size_t(a.heads_kv) * a.splits * ((a.rows + 15) / 16);
+    const size_t key_blocks = size_t(a.heads_kv) * ((c.capacity / 32 + kWaves - 1) / kWaves);
+    if (blocks > 0x7fffffffu || key_blocks > 0x7fffffffu) return hipErrorInvalidValue;
+#define ZQ_ATTN_D(KERNEL, GRID, THREADS)                                                                \
+    do {                                                                                                \
+        if (c.head_dim == 64) hipLaunchKernelGGL(KERNEL<64>, dim3(uint32_t(GRID)), dim3(THREADS), 0, stream, a);        \
+        else if (c.head_dim == 128) hipLaunchKernelGGL(KERNEL<128>, dim3(uint32_t(GRID)), dim3(THREADS), 0, stream, a); \
+        else hipLaunchKernelGGL(KERNEL<256>, dim3(uint32_t(GRID)), dim3(THREADS), 0, stream, a);                        \
+        const hipError_t e = hipGetLastError();                                                         \
+        if (e != hipSuccess) return e;                                                                  \
+    } while (0)
+    ZQ_ATTN_D(attn_q4_few_kernel, blocks, kWaves * 64);
+    if (a.splits > 1) ZQ_ATTN_D(attn_q4_combine_kernel, (all + 3) / 4, 256);
+    if (a.lse) ZQ_ATTN_D(attn_q4_weights_kernel, key_blocks, kWaves * 64);
+#undef ZQ_ATTN_D
+    return hipSuccess;
+}
+
+}  // namespace zq

@@ -1,0 +1,527 @@
+// zq_kv.hip -- the 4-bit KV cache of include/zq_kv.h: append, read-back,
+// eviction, and the C entry points (the attention's kernels are in
+// zq_attn_q4.hip).
+#include "../../include/zq_hip.h"
+#include "zq_internal.hpp"
+#include "zq_kv.hpp"
+
+#include <math.h>
+
+namespace zq {
+namespace {
+
+constexpr int kT = 256;
+
+// ---- append ------------------------------------------------------------------
+// One lane takes four consecutive elements of a row's key and of its value, so 8
+// lanes hold a block and D / 4 lanes a row; a wave takes 256 / D rows (one row =
+// one token of one kv head).  Bound by the fp32 rows it reads: 8 D bytes a row
+// against D + D / 8 written.
+// The block's scale is an eighth of its element of largest magnitude, negated,
+// so that this element gets code 0 and all 16 codes are in use.  m / -8 is exact;
+// rounding it to bf16 leaves (code - 8) * d with at most 11 significant bits,
+// which fp16 holds exactly: the attention's matrix operands need no second part.
+// The quotient x / d of the correctly rounded division lies on a half only if the
+// exact one does (x is on d's grid near such a quotient, and the next x on either
+// side is a relative 2^-24 away, at least half a spacing of the quotient), so
+// rintf gives the nearest code of the exact quotient.
+struct Q4Block {
+    uint32_t codes;  // lanes 0..3 of the block's 8: bytes 4 l .. 4 l + 3
+    uint16_t scale;
+};
+__device__ __forceinline__ uint32_t group8_max(uint32_t v) {
+    v = max(v, uint32_t(__builtin_amdgcn_update_dpp(0, int(v), kDppXor1, 0xF, 0xF, false)));
+    v = max(v, uint32_t(__builtin_amdgcn_update_dpp(0, int(v), kDppXor2, 0xF, 0xF, false)));
+    return max(v, uint32_t(__builtin_amdgcn_update_dpp(0, int(v), kDppHalfMirror, 0xF, 0xF, false)));
+}
+__device__ __forceinline__ Q4Block quantize_block(float4 x, bool poison, bool is_key) {
+    const float e[4] = {x.x, x.y, x.z, x.w};
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) m = max(m, __float_as_uint(e[i]) & 0x7fffffffu);
+    m = group8_max(m);
+    // the first element that has the largest magnitude: as 2 * (32 - index) + sign, so the max is the first
+    const uint32_t l8 = threadIdx.x & 7u;
+    uint32_t at = 0;
+#pragma unroll
+    for (int i = 3; i >= 0; --i) {
+        const uint32_t u = __float_as_uint(e[i]);
+        if ((u & 0x7fffffffu) == m) at = 2u * (32u - (4u * l8 + uint32_t(i))) + (u >> 31);
+    }
+    at = group8_max(at);
+    const float top = __uint_as_float(m | ((at & 1u) << 31));
+    uint32_t u = __float_as_uint(top / -8.0f);
+    u = (u + 0x7fffu + ((u >> 16) & 1u)) & 0xffff0000u;  // bf16, to nearest even (m is finite here or unused)
+    const _Float16 h = _Float16(fminf(fmaxf(__uint_as_float(u), -4096.0f), 4096.0f));
+    const float d = float(h);
+    uint32_t c = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float r = d != 0.0f ? fminf(fmaxf(rintf(e[i] / d), -8.0f), 7.0f) : 0.0f;
+        c |= (poison ? 8u : uint32_t(int(r) + 8)) << (8 * i);
+    }
+    Q4Block b;
+    const uint32_t hi = uint32_t(__shfl(int(c), int(threadIdx.x & 63u) ^ 4));  // elements 16 on: the block's lanes 4..7
+    b.codes = c | (hi << 4);
+    b.scale = poison ? (is_key ? 0x7e00u : 0u) : (d != 0.0f ? __builtin_bit_cast(uint16_t, h) : uint16_t(0));
+    return b;
+}
+
+template <int D>
+__global__ __launch_bounds__(kT) void kv_q4_append_kernel(const float* __restrict__ k, const float* __restrict__ v,
+                                                          zq_kv_q4 c, uint32_t tokens, size_t stride,
+                                                          const int32_t* __restrict__ lens,
+                                                          const int32_t* __restrict__ counts,
+                                                          const int32_t* __restrict__ first_pos, uint32_t rows) {
+    constexpr uint32_t RL = D / 4;  // lanes of a row
+    const uint32_t KH = uint32_t(c.kv_heads);
+    const uint32_t id = blockIdx.x * (kT / RL) + threadIdx.x / RL, l = threadIdx.x % RL;
+    const uint32_t row = min(id, rows - 1);  // every lane of a wave takes part in the block's reductions
+    const uint32_t kh = row % KH, st = row / KH, t = st % tokens, s = st / tokens;
+    const int32_t len = lens[s];
+    const int32_t n = counts ? counts[s] : int32_t(tokens);
+    const bool live = id < rows && int32_t(t) < n && len >= 0 && size_t(len) + t < c.capacity;
+    const size_t slot = live ? size_t(len) + t : 0;
+    const size_t src = size_t(st) * stride + size_t(kh) * D + 4 * l;
+    const float4 z = make_float4(0, 0, 0, 0);
+    const float4 kx = live ? *reinterpret_cast<const float4*>(k + src) : z;
+    const float4 vx = live ? *reinterpret_cast<const float4*>(v + src) : z;
+    auto odd = [](float4 x) {  // any exponent of all ones: NaN or infinity
+        const uint32_t e = 0x7f800000u;
+        return (__float_as_uint(x.x) & e) == e || (__float_as_uint(x.y) & e) == e || (__float_as_uint(x.z) & e) == e ||
+               (__float_as_uint(x.w) & e) == e;
+    };
+    const uint64_t bad = __ballot(odd(kx) || odd(vx));
+    const uint32_t row0 = (threadIdx.x & 63u) / RL * RL;  // first lane of this row in the wave
+    const bool poison = ((bad >> row0) & (RL == 64 ? ~uint64_t(0) : (uint64_t(1) << (RL & 63u)) - 1)) != 0;
+    const Q4Block bk = quantize_block(kx, poison, true);
+    const Q4Block bv = quantize_block(vx, poison, false);
+    if (!live) return;
+    const size_t head = size_t(s) * KH + kh, at = head * c.capacity + slot;
+    const uint32_t b = l / 8, l8 = l % 8;
+    if (l8 < 4) {
+        *reinterpret_cast<uint32_t*>(c.k + at * (D / 2) + b * 16 + l8 * 4) = bk.codes;
+        *reinterpret_cast<uint32_t*>(c.v + at * (D / 2) + b * 16 + l8 * 4) = bv.codes;
+    } else if (l8 == 4) {
+        const size_t sc = (head * (D / 32) + b) * c.capacity + slot;
+        c.k_scale[sc] = bk.scale;
+        c.v_scale[sc] = bv.scale;
+    }
+    if (l == 0) {
+        if (c.weight) c.weight[at] = 0.0f;
+        if (c.pos) c.pos[at] = (first_pos ? first_pos[s] : len) + int32_t(t);
+    }
+}
+
+// ---- read ----------------------------------------------------------------------
+// A lane gives four elements (the low or the high nibbles of four bytes), so a
+// row's stores are as wide as its fp32 elements allow: bound by those.
+template <int D>
+__global__ __launch_bounds__(kT) void kv_q4_read_kernel(zq_kv_q4 c, float* __restrict__ k, float* __restrict__ v,
+                                                        uint32_t tokens, const int32_t* __restrict__ first,
+                                                        const int32_t* __restrict__ counts, uint32_t rows) {
+    constexpr uint32_t RL = D / 4;
+    const uint32_t KH = uint32_t(c.kv_heads);
+    const uint32_t row = blockIdx.x * (kT / RL) + threadIdx.x / RL, l = threadIdx.x % RL;
+    if (row >= rows) return;
+    const uint32_t kh = row % KH, st = row / KH, t = st % tokens, s = st / tokens;
+    const int32_t f = first[s];
+    if (int32_t(t) >= (counts ? counts[s] : int32_t(tokens)) || f < 0 || size_t(f) + t >= c.capacity) return;
+    const size_t slot = size_t(f) + t, head = size_t(s) * KH + kh, at = head * c.capacity + slot;
+    const uint32_t b = l / 8, l8 = l % 8;
+    const size_t code = at * (D / 2) + b * 16 + (l8 & 3u) * 4, sc = (head * (D / 32) + b) * c.capacity + slot;
+    const size_t dst = (size_t(st) * KH + kh) * D + 4 * l;
+    auto four = [&](const uint8_t* codes, const uint16_t* scales) {
+        const uint32_t w = *reinterpret_cast<const uint32_t*>(codes + code) >> (l8 & 4u);
+        const float d = half_bits_to_float(scales[sc]);
+        return make_float4(float(int(w & 15u) - 8) * d, float(int((w >> 8) & 15u) - 8) * d,
+                           float(int((w >> 16) & 15u) - 8) * d, float(int((w >> 24) & 15u) - 8) * d);
+    };
+    if (k) *reinterpret_cast<float4*>(k + dst) = four(c.k, c.k_scale);
+    if (v) *reinterpret_cast<float4*>(v + dst) = four(c.v, c.v_scale);
+}
+
+// ---- evict ---------------------------------------------------------------------
+// Two launches.  The first, one workgroup a (sequence, kv head), finds the rows
+// that stay and, for every slot below the new length, the slot its row comes from;
+// it also moves weight and pos, which it alone knows the old values of.  The second
+// copies the rows.  Free slots are filled from above the new length, so what is
+// written and what is read never meet, in place or not, and only evicted slots are
+// written in place.
+constexpr int kEvT = 1024;
+
+// Order of a row: protected ones, then by weight (-0 = +0), a NaN last.
+__device__ __forceinline__ uint32_t evict_key(float w, bool held) {
+    if (held) return 0xffffffffu;
+    if (w != w) return 0u;
+    const uint32_t u = __float_as_uint(w + 0.0f);
+    return (u >> 31) ? ~u : (u | 0x80000000u);
+}
+
+struct EvictLists {
+    int32_t* from;   // [keep] the slot that slot j's row comes from
+    int32_t* holes;  // [keep] free slots below the new length, ascending
+    int32_t* above;  // [keep] kept slots from the new length on, ascending
+};
+
+__global__ __launch_bounds__(kEvT) void kv_q4_evict_select_kernel(zq_kv_q4 c, zq_kv_q4 dst, int in_place,
+                                                                  const int32_t* __restrict__ lens, uint32_t keep,
+                                                                  uint32_t recent, uint32_t first,
+                                                                  const int32_t* __restrict__ next_pos,
+                                                                  int32_t* __restrict__ ws) {
+    __shared__ uint32_t hist[256];
+    __shared__ uint32_t pick[2];  // the byte found, and the rows wanted among those that have it
+    __shared__ uint32_t sums[3][kEvT / 64];
+    const uint32_t head = blockIdx.x, s = head / uint32_t(c.kv_heads);
+    const uint32_t n = uint32_t(clamp_len(lens[s], c.capacity)), kept = min(n, keep);
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const float* w = c.weight + size_t(head) * c.capacity;
+    const int32_t* pos = c.pos + size_t(head) * c.capacity;
+    float* dw = dst.weight + size_t(head) * dst.capacity;
+    int32_t* dp = dst.pos + size_t(head) * dst.capacity;
+    int32_t* from = ws + size_t(head) * 3 * keep;
+    int32_t* holes = from + keep;
+    int32_t* above = holes + keep;
+    if (n <= keep) {  // uniform: everything stays
+        for (uint32_t i = tid; i < n; i += kEvT) {
+            from[i] = int32_t(i);
+            if (!in_place) {
+                dw[i] = w[i];
+                dp[i] = pos[i];
+            }
+        }
+        return;
+    }
+    const int64_t newest = int64_t(next_pos ? next_pos[s] : int32_t(n)) - recent;
+    auto key = [&](uint32_t i) {
+        const int32_t p = pos[i];
+        return evict_key(w[i], p >= 0 && (int64_t(p) >= newest || p < int64_t(first)));
+    };
+    // the key of rank `kept`, byte by byte from the top: want = rows still to be found among those that share its bytes so far
+    uint32_t prefix = 0, want = kept;
+    for (int shift = 24; shift >= 0; shift -= 8) {
+        for (int i = tid; i < 256; i += kEvT) hist[i] = 0;
+        __syncthreads();
+        for (uint32_t i = tid; i < n; i += kEvT) {
+            const uint32_t x = key(i);
+            if (shift == 24 || (x >> (shift + 8)) == (prefix >> (shift + 8))) atomicAdd(&hist[(x >> shift) & 255u], 1u);
+        }
+        __syncthreads();
+        if (wave == 0) {  // lane l holds bins 255 - 4 l down to 252 - 4 l; rows in higher bins than its own by a scan
+            uint32_t h[4], t = 0;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) t += h[j] = hist[255 - 4 * lane - j];
+            uint32_t up = t;
+            for (int o = 1; o < 64; o <<= 1) {
+                const uint32_t x = uint32_t(__shfl_up(int(up), o));
+                if (lane >= o) up += x;
+            }
+            uint32_t before = up - t;  // rows of higher bins
+            if (before < want && want <= up) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    if (before < want && want <= before + h[j]) {
+                        pick[0] = uint32_t(255 - 4 * lane - j);
+                        pick[1] = want - before;
+                    }
+                    before += h[j];
+                }
+            }
+        }
+        __syncthreads();
+        prefix |= pick[0] << shift;
+        want = pick[1];
+        __syncthreads();
+    }
+    // in slot order: a row stays if its key is above the found one, or equal and among the first `want`
+    uint32_t equal = 0, free_n = 0, above_n = 0;  // counts of the chunks before this one
+    for (uint32_t i0 = 0; i0 < n; i0 += kEvT) {
+        const uint32_t i = i0 + tid;
+        const uint32_t x = i < n ? key(i) : 0u;
+        const bool eq = i < n && x == prefix;
+        const uint64_t beq = __ballot(eq), below = (uint64_t(1) << lane) - 1;
+        if (lane == 0) sums[0][wave] = uint32_t(__popcll(beq));
+        __syncthreads();
+        uint32_t r = equal + uint32_t(__popcll(beq & below)), all = 0;
+        for (int k = 0; k < kEvT / 64; ++k) {
+            const uint32_t t = sums[0][k];
+            r += k < wave ? t : 0u;
+            all += t;
+        }
+        equal += all;
+        const bool stay = i < n && (x > prefix || (eq && r < want));
+        const bool hole = i < kept && !stay, up = i >= kept && stay;
+        const uint64_t bh = __ballot(hole), bu = __ballot(up);
+        if (lane == 0) {
+            sums[1][wave] = uint32_t(__popcll(bh));
+            sums[2][wave] = uint32_t(__popcll(bu));
+        }
+        __syncthreads();
+        uint32_t rh = free_n + uint32_t(__popcll(bh & below)), ru = above_n + uint32_t(__popcll(bu & below));
+        for (int k = 0; k < kEvT / 64; ++k) {
+            const uint32_t a = sums[1][k], b = sums[2][k];
+            rh += k < wave ? a : 0u;
+            ru += k < wave ? b : 0u;
+            free_n += a;
+            above_n += b;
+        }
+        if (hole) holes[rh] = int32_t(i);
+        if (up) above[ru] = int32_t(i);
+        if (i < kept && stay) {
+            from[i] = int32_t(i);
+            if (!in_place) {
+                dw[i] = w[i];
+                dp[i] = pos[i];
+            }
+        }
+        // the next chunk writes sums[0] behind this chunk's second barrier, and sums[1], [2] behind its own first
+    }
+    __syncthreads();  // the lists, written by other waves of this workgroup
+    for (uint32_t x = tid; x < free_n; x += kEvT) {
+        const int32_t h = holes[x], a = above[x];
+        from[h] = a;
+        dw[h] = w[a];
+        dp[h] = pos[a];
+    }
+    if (!in_place) return;
+    __syncthreads();  // every moved weight and pos has been read
+    for (uint32_t i = kept + tid; i < n; i += kEvT) {
+        dw[i] = -INFINITY;
+        dp[i] = -1;
+    }
+}
+
+// A workgroup copies 64 rows of one (sequence, kv head): codes in 16-byte parts,
+// scales one by one from their planes.
+constexpr uint32_t kMoveRows = 64;
+__global__ __launch_bounds__(kT) void kv_q4_evict_move_kernel(zq_kv_q4 c, zq_kv_q4 dst, int in_place,
+                                                              const int32_t* __restrict__ lens, uint32_t keep,
+                                                              const int32_t* __restrict__ ws, uint32_t parts) {
+    const uint32_t head = blockIdx.x / parts, j0 = blockIdx.x % parts * kMoveRows;
+    const uint32_t s = head / uint32_t(c.kv_heads), D = uint32_t(c.head_dim);
+    const uint32_t kept = min(uint32_t(clamp_len(lens[s], c.capacity)), keep);
+    if (j0 >= kept) return;
+    const uint32_t rows = min(kept - j0, kMoveRows);
+    const int32_t* from = ws + size_t(head) * 3 * keep + j0;
+    const uint32_t P = D / 32;  // 16-byte parts of a row's codes, and its scales
+    const size_t src = size_t(head) * c.capacity, to = size_t(head) * dst.capacity + j0;
+    for (uint32_t e = threadIdx.x; e < rows * P; e += kT) {
+        const uint32_t j = e / P, p = e % P;
+        const uint32_t f = uint32_t(from[j]);
+        if (in_place && f == j0 + j) continue;
+        const size_t a = (src + f) * P + p, b = (to + j) * P + p;
+        reinterpret_cast<uint4*>(dst.k)[b] = reinterpret_cast<const uint4*>(c.k)[a];
+        reinterpret_cast<uint4*>(dst.v)[b] = reinterpret_cast<const uint4*>(c.v)[a];
+    }
+    for (uint32_t e = threadIdx.x; e < rows * P; e += kT) {
+        const uint32_t j = e % rows, p = e / rows;
+        const uint32_t f = uint32_t(from[j]);
+        if (in_place && f == j0 + j) continue;
+        const size_t a = (size_t(head) * P + p) * c.capacity + f, b = (size_t(head) * P + p) * dst.capacity + j0 + j;
+        dst.k_scale[b] = c.k_scale[a];
+        dst.v_scale[b] = c.v_scale[a];
+    }
+}
+
+}  // namespace
+
+bool kv_q4_ok(const zq_kv_q4* c) {
+    auto a16 = [](const void* p) { return p && (reinterpret_cast<uintptr_t>(p) & 15u) == 0; };
+    auto a4 = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0; };
+    return c && a16(c->k) && a16(c->v) && a16(c->k_scale) && a16(c->v_scale) && a4(c->weight) && a4(c->pos) &&
+           (c->head_dim == 64 || c->head_dim == 128 || c->head_dim == 256) && c->capacity && c->capacity % 32 == 0 &&
+           c->capacity <= kKvMaxCapacity && c->seqs && c->kv_heads && c->seqs <= kKvMaxHeads &&
+           c->kv_heads <= kKvMaxHeads && c->seqs * c->kv_heads <= kKvMaxHeads;
+}
+
+hipError_t launch_kv_q4_append(const zq_kv_q4& c, const float* k, const float* v, size_t tokens, size_t stride,
+                               const int32_t* lens, const int32_t* counts, const int32_t* first_pos,
+                               hipStream_t stream) {
+    const uint32_t rows = uint32_t(c.seqs * tokens * c.kv_heads);
+    const uint32_t per = uint32_t(kT / (c.head_dim / 4));
+    const dim3 grid((rows + per - 1) / per);
+#define ZQ_KV(DD)                                                                                                \
+    hipLaunchKernelGGL(kv_q4_append_kernel<DD>, grid, dim3(kT), 0, stream, k, v, c, uint32_t(tokens), stride, lens, \
+                       counts, first_pos, rows)
+    if (c.head_dim == 64) ZQ_KV(64);
+    else if (c.head_dim == 128) ZQ_KV(128);
+    else ZQ_KV(256);
+#undef ZQ_KV
+    return hipGetLastError();
+}
+
+hipError_t launch_kv_q4_read(const zq_kv_q4& c, float* k, float* v, size_t tokens, const int32_t* first,
+                             const int32_t* counts, hipStream_t stream) {
+    const uint32_t rows = uint32_t(c.seqs * tokens * c.kv_heads);
+    const uint32_t per = uint32_t(kT / (c.head_dim / 4));
+    const dim3 grid((rows + per - 1) / per);
+#define ZQ_KV(DD) \
+    hipLaunchKernelGGL(kv_q4_read_kernel<DD>, grid, dim3(kT), 0, stream, c, k, v, uint32_t(tokens), first, counts, rows)
+    if (c.head_dim == 64) ZQ_KV(64);
+    else if (c.head_dim == 128) ZQ_KV(128);
+    else ZQ_KV(256);
+#undef ZQ_KV
+    return hipGetLastError();
+}
+
+size_t kv_q4_evict_bytes(const zq_kv_q4& c, size_t keep) {
+    return c.seqs * c.kv_heads * 3 * (keep < c.capacity ? keep : c.capacity) * sizeof(int32_t);
+}
+
+hipError_t launch_kv_q4_evict(const zq_kv_q4& c, const zq_kv_q4& dst, bool in_place, const int32_t* lens, size_t keep,
+                              size_t recent, size_t first, const int32_t* next_pos, void* ws, hipStream_t stream) {
+    const uint32_t heads = uint32_t(c.seqs * c.kv_heads), kp = uint32_t(keep < c.capacity ? keep : c.capacity);
+    hipLaunchKernelGGL(kv_q4_evict_select_kernel, dim3(heads), dim3(kEvT), 0, stream, c, dst, in_place ? 1 : 0, lens, kp,
+                       uint32_t(recent), uint32_t(first), next_pos, static_cast<int32_t*>(ws));
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    const uint32_t parts = (kp + kMoveRows - 1) / kMoveRows;
+    hipLaunchKernelGGL(kv_q4_evict_move_kernel, dim3(heads * parts), dim3(kT), 0, stream, c, dst, in_place ? 1 : 0, lens,
+                       kp, static_cast<const int32_t*>(ws), parts);
+    return hipGetLastError();
+}
+
+}  // namespace zq
+
+// ---- C entry points --------------------------------------------------------------
+namespace {
+
+bool a16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+bool a4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0; }
+
+int status(hipError_t e) { return e == hipSuccess ? ZQ_OK : e == hipErrorInvalidValue ? ZQ_ERR_ARG : ZQ_ERR_HIP; }
+
+// The device that holds the cache made current for the call's launches, and the
+// caller's device again after it.
+class OnDeviceOf {
+public:
+    explicit OnDeviceOf(const void* p) {
+        hipPointerAttribute_t a;
+        if (hipPointerGetAttributes(&a, p) != hipSuccess) {
+            (void)hipGetLastError();
+            int n = 0;
+            st_ = hipGetDeviceCount(&n) == hipSuccess && n > 0 ? ZQ_ERR_ARG : ZQ_ERR_NO_DEVICE;
+            (void)hipGetLastError();
+            return;
+        }
+        if (a.type != hipMemoryTypeDevice && a.type != hipMemoryTypeManaged) {
+            st_ = ZQ_ERR_ARG;  // an address of the host: a kernel that used it would fault
+            return;
+        }
+        if (hipGetDevice(&was_) != hipSuccess) st_ = ZQ_ERR_HIP;
+        else if (a.device != was_) {
+            moved_ = hipSetDevice(a.device) == hipSuccess;
+            if (!moved_) st_ = ZQ_ERR_HIP;
+        }
+    }
+    ~OnDeviceOf() {
+        if (moved_) (void)hipSetDevice(was_);
+    }
+    int status() const { return st_; }
+
+private:
+    int was_ = 0, st_ = ZQ_OK;
+    bool moved_ = false;
+};
+
+bool tokens_ok(const zq_kv_q4& c, size_t tokens, size_t heads) {
+    return tokens && tokens <= zq::kKvMaxRows && heads <= zq::kKvMaxHeads && c.seqs * heads <= zq::kKvMaxRows / tokens;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t zq_kv_q4_bytes(size_t kv_heads, size_t head_dim, size_t capacity) {
+    if (!kv_heads || kv_heads > zq::kKvMaxHeads || (head_dim != 64 && head_dim != 128 && head_dim != 256) || !capacity ||
+        capacity % 32 || capacity > zq::kKvMaxCapacity)
+        return 0;
+    return 2 * kv_heads * capacity * (head_dim / 2 + head_dim / 16);
+}
+
+int zq_hip_kv_q4_append_dev(const zq_kv_q4* cache, const float* k, const float* v, size_t tokens, size_t stride,
+                            const int32_t* lens, const int32_t* counts, const int32_t* first_pos, void* stream) {
+    if (!zq::kv_q4_ok(cache) || !k || !v || !lens || !a16(k) || !a16(v) || !a4(lens) || !a4(counts) || !a4(first_pos) ||
+        !tokens_ok(*cache, tokens, cache->kv_heads))
+        return ZQ_ERR_ARG;
+    const size_t width = cache->kv_heads * cache->head_dim;
+    if (!stride) stride = width;
+    if (stride < width || stride % 4 || stride > (size_t(1) << 31)) return ZQ_ERR_ARG;
+    const OnDeviceOf dev(cache->k);
+    if (dev.status() != ZQ_OK) return dev.status();
+    return status(zq::launch_kv_q4_append(*cache, k, v, tokens, stride, lens, counts, first_pos,
+                                          static_cast<hipStream_t>(stream)));
+}
+
+int zq_hip_kv_q4_read_dev(const zq_kv_q4* cache, float* k, float* v, size_t tokens, const int32_t* first,
+                          const int32_t* counts, void* stream) {
+    if (!zq::kv_q4_ok(cache) || (!k && !v) || !first || !a16(k) || !a16(v) || !a4(first) || !a4(counts) ||
+        !tokens_ok(*cache, tokens, cache->kv_heads))
+        return ZQ_ERR_ARG;
+    const OnDeviceOf dev(cache->k);
+    if (dev.status() != ZQ_OK) return dev.status();
+    return status(zq::launch_kv_q4_read(*cache, k, v, tokens, first, counts, static_cast<hipStream_t>(stream)));
+}
+
+size_t zq_hip_attention_q4_workspace_bytes(const zq_kv_q4* cache, size_t tokens, size_t heads, int flags) {
+    if (!zq::kv_q4_ok(cache) || !heads || heads % cache->kv_heads || !tokens_ok(*cache, tokens, heads)) return 0;
+    return zq::attention_q4_bytes(*cache, tokens, heads, flags);
+}
+
+int zq_hip_attention_q4_dev(const zq_kv_q4* cache, const float* q, float* out, size_t tokens, size_t heads,
+                            size_t stride, const int32_t* lens, const int32_t* counts, float scale, int flags,
+                            void* workspace, size_t workspace_bytes, void* stream) {
+    if (!zq::kv_q4_ok(cache) || !q || !out || !lens || !a16(q) || !a16(out) || !a4(lens) || !a4(counts) || !heads ||
+        heads % cache->kv_heads || !tokens_ok(*cache, tokens, heads))
+        return ZQ_ERR_ARG;
+    const int known = ZQ_ATTN_Q4_FULL | ZQ_ATTN_Q4_WEIGHTS | ZQ_ATTN_Q4_ADD;
+    if ((flags & ~known) || ((flags & ZQ_ATTN_Q4_ADD) && !(flags & ZQ_ATTN_Q4_WEIGHTS)) ||
+        ((flags & ZQ_ATTN_Q4_WEIGHTS) && !cache->weight))
+        return ZQ_ERR_ARG;
+    const size_t width = heads * cache->head_dim;
+    if (!stride) stride = width;
+    if (stride < width || stride % 4 || stride > (size_t(1) << 31)) return ZQ_ERR_ARG;
+    const size_t need = zq::attention_q4_bytes(*cache, tokens, heads, flags);
+    if (need && (!workspace || workspace_bytes < need || !a16(workspace))) return ZQ_ERR_ARG;
+    const OnDeviceOf dev(cache->k);
+    if (dev.status() != ZQ_OK) return dev.status();
+    return status(zq::launch_attention_q4(*cache, q, out, tokens, heads, stride, lens, counts, scale, flags, workspace,
+                                          static_cast<hipStream_t>(stream)));
+}
+
+size_t zq_hip_kv_q4_evict_workspace_bytes(const zq_kv_q4* cache, size_t keep) {
+    if (!zq::kv_q4_ok(cache) || !keep) return 0;
+    return zq::kv_q4_evict_bytes(*cache, keep);
+}
+
+int zq_hip_kv_q4_evict_dev(const zq_kv_q4* cache, const zq_kv_q4* dst, const int32_t* lens, size_t keep, size_t recent,
+                           size_t first, const int32_t* next_pos, void* workspace, size_t workspace_bytes,
+                           void* stream) {
+    if (!zq::kv_q4_ok(cache) || !cache->weight || !cache->pos || !lens || !a4(lens) || !a4(next_pos) || !keep ||
+        recent > keep || first > keep - recent || !workspace || !a16(workspace))
+        return ZQ_ERR_ARG;
+    if (recent > 0x7fffffffu || first > 0x7fffffffu) return ZQ_ERR_ARG;
+    if (!dst) dst = cache;
+    const bool in_place = dst->k == cache->k;
+    if (in_place) {
+        if (dst->v != cache->v || dst->k_scale != cache->k_scale || dst->v_scale != cache->v_scale ||
+            dst->weight != cache->weight || dst->pos != cache->pos || dst->seqs != cache->seqs ||
+            dst->kv_heads != cache->kv_heads || dst->head_dim != cache->head_dim || dst->capacity != cache->capacity)
+            return ZQ_ERR_ARG;
+    } else if (!zq::kv_q4_ok(dst) || !dst->weight || !dst->pos || dst->seqs != cache->seqs ||
+               dst->kv_heads != cache->kv_heads || dst->head_dim != cache->head_dim ||
+               dst->capacity < (keep < cache->capacity ? keep : cache->capacity) || dst->v == cache->v ||
+               dst->k_scale == cache->k_scale || dst->v_scale == cache->v_scale || dst->weight == cache->weight ||
+               dst->pos == cache->pos) {
+        return ZQ_ERR_ARG;
+    }
+    if (workspace_bytes < zq::kv_q4_evict_bytes(*cache, keep)) return ZQ_ERR_ARG;
+    const size_t parts = ((keep < cache->capacity ? keep : cache->capacity) + 63) / 64;
+    if (parts * cache->seqs * cache->kv_heads > 0x7fffffffu) return ZQ_ERR_ARG;
+    const OnDeviceOf dev(cache->k);
+    if (dev.status() != ZQ_OK) return dev.status();
+    return status(zq::launch_kv_q4_evict(*cache, *dst, in_place, lens, keep, recent, first, next_pos, workspace,
+                                         static_cast<hipStream_t>(stream)));
+}
+
+}  // extern "C"

@@ -22,6 +22,7 @@ OK, DECLINED = 0, 1
 ERR_ARG, ERR_NO_DEVICE, ERR_OOM, ERR_HIP, ERR_TOO_LARGE = -1, -2, -3, -4, -5
 WEIGHT_TAIL_PAD = 64
 MAX_BATCH = 8
+ATTN_Q4_FULL, ATTN_Q4_WEIGHTS, ATTN_Q4_ADD = 1, 2, 4
 
 _P = ctypes.c_void_p
 _S = ctypes.c_size_t
@@ -129,6 +130,26 @@ GGUF_SIGNATURES = {
     "zq_gguf_meta_value": (ctypes.c_char_p, [_P, ctypes.c_char_p]),
 }
 
+class KVCacheQ4(ctypes.Structure):
+    """zq_kv_q4 (include/zq_kv.h)."""
+    _fields_ = [(n, _P) for n in ("k", "v", "k_scale", "v_scale", "weight", "pos")] + [
+        (n, _S) for n in ("seqs", "kv_heads", "head_dim", "capacity")]
+
+
+# Every symbol include/zq_kv.h declares.
+_KV = ctypes.POINTER(KVCacheQ4)
+KV_SIGNATURES = {
+    "zq_kv_q4_bytes": (_S, [_S, _S, _S]),
+    "zq_hip_kv_q4_append_dev": (ctypes.c_int, [_KV, _P, _P, _S, _S, _P, _P, _P, _P]),
+    "zq_hip_kv_q4_read_dev": (ctypes.c_int, [_KV, _P, _P, _S, _P, _P, _P]),
+    "zq_hip_attention_q4_workspace_bytes": (_S, [_KV, _S, _S, ctypes.c_int]),
+    "zq_hip_attention_q4_dev": (ctypes.c_int, [_KV, _P, _P, _S, _S, _S, _P, _P, ctypes.c_float, ctypes.c_int, _P, _S,
+                                               _P]),
+    "zq_hip_kv_q4_evict_workspace_bytes": (_S, [_KV, _S]),
+    "zq_hip_kv_q4_evict_dev": (ctypes.c_int, [_KV, _KV, _P, _S, _S, _S, _P, _P, _S, _P]),
+}
+
+
 class ModelConfig(ctypes.Structure):
     _fields_ = [(n, ctypes.c_uint32) for n in ("embedding", "layers", "heads", "kv_heads", "head_dim", "ffn", "vocab",
                                                "context", "max_positions", "rope_dim")] + [
@@ -176,7 +197,7 @@ def lib():
             raise RuntimeError(f"{path} is missing: build it with `python -m zeninfer_amd.build` "
                                "(there is no CPU fallback for this path)")
         L = ctypes.CDLL(path)
-        for name, (res, args) in {**SIGNATURES, **GGUF_SIGNATURES, **MODEL_SIGNATURES}.items():
+        for name, (res, args) in {**SIGNATURES, **GGUF_SIGNATURES, **KV_SIGNATURES, **MODEL_SIGNATURES}.items():
             fn = getattr(L, name)
             fn.restype = res
             fn.argtypes = args
@@ -571,3 +592,105 @@ def synth_weights_dev(fmt, seed, w, rows, cols, stream=None):
 def synth_normal_dev(seed, out, n, stream=None):
     _need(out, 4 * n, "synth_normal_dev out")
     return check(lib().zq_hip_synth_normal_dev(seed, _dptr(out), n, _stream(stream)), "zq_hip_synth_normal_dev")
+
+
+# ---- 4-bit KV cache (include/zq_kv.h) --------------------------------------
+def kv_q4_bytes(kv_heads, head_dim, capacity):
+    return lib().zq_kv_q4_bytes(kv_heads, head_dim, capacity)
+
+
+class KVQ4:
+    """A 4-bit KV cache over the caller's device arrays (zq_kv_q4): codes k and v
+    [seqs][kv_heads][capacity][head_dim / 2], scales [seqs][kv_heads][head_dim / 32]
+    [capacity], and optionally weight and pos [seqs][kv_heads][capacity].  The arrays
+    are checked once, here, and kept alive with the handle."""
+
+    def __init__(self, k, v, k_scale, v_scale, seqs, kv_heads, head_dim, capacity, weight=None, pos=None):
+        dev = _device_index()
+        rows = seqs * kv_heads * capacity
+        arrays = [(k, rows * (head_dim // 2), "k"), (v, rows * (head_dim // 2), "v"),
+                  (k_scale, rows * (head_dim // 32) * 2, "k_scale"), (v_scale, rows * (head_dim // 32) * 2, "v_scale"),
+                  (weight, rows * 4, "weight"), (pos, rows * 4, "pos")]
+        self.c = KVCacheQ4(*[_need(t, n, f"KVQ4 {name}", dev) for t, n, name in arrays], seqs, kv_heads, head_dim,
+                           capacity)
+        self.arrays = [t for t, _, _ in arrays]
+        self.seqs, self.kv_heads, self.head_dim, self.capacity = seqs, kv_heads, head_dim, capacity
+        self.ref = ctypes.byref(self.c)
+
+
+def _need_rows(t, seqs, tokens, stride, width, what, dev):
+    """Device address of [seqs][tokens][stride] fp32 rows of which width floats are used.  With a stride, a view of
+    the columns of a wider buffer will do (its storage must hold the last row)."""
+    n = 4 * ((seqs * tokens - 1) * (stride or width) + width)
+    if t is None or isinstance(t, int) or not stride or t.is_contiguous():
+        return _need(t, n, what, dev)
+    _check_device(t, what)
+    have = t.untyped_storage().nbytes() - t.storage_offset() * t.element_size()
+    if t.stride(-1) != 1 or t.stride(-2) != stride:
+        raise ValueError(f"{what}: rows must be {stride} floats apart and their elements adjacent")
+    if have < n:
+        raise ValueError(f"{what}: buffer holds {have} bytes, the call needs {n}")
+    return t.data_ptr()
+
+
+def kv_q4_append_dev(cache, k, v, tokens, lens, counts=None, first_pos=None, stride=0, stream=None):
+    """New tokens' keys and values [seqs][tokens][stride] into slots lens ... of every sequence."""
+    dev = _device_index()
+    width = cache.kv_heads * cache.head_dim
+    k = _need_rows(k, cache.seqs, tokens, stride, width, "kv_q4_append_dev k", dev)
+    v = _need_rows(v, cache.seqs, tokens, stride, width, "kv_q4_append_dev v", dev)
+    n = 4 * cache.seqs
+    lens = _need(lens, n, "kv_q4_append_dev lens", dev)
+    counts = _need(counts, n, "kv_q4_append_dev counts", dev)
+    first_pos = _need(first_pos, n, "kv_q4_append_dev first_pos", dev)
+    return check(lib().zq_hip_kv_q4_append_dev(cache.ref, k, v, tokens, stride, lens, counts, first_pos,
+                                               _stream(stream)), "zq_hip_kv_q4_append_dev")
+
+
+def kv_q4_read_dev(cache, k, v, tokens, first, counts=None, stream=None):
+    """Rows first ... of every sequence as fp32 [seqs][tokens][kv_heads * head_dim]; k or v may be None."""
+    dev = _device_index()
+    n = 4 * cache.seqs * tokens * cache.kv_heads * cache.head_dim
+    k = _need(k, n, "kv_q4_read_dev k", dev)
+    v = _need(v, n, "kv_q4_read_dev v", dev)
+    n = 4 * cache.seqs
+    first = _need(first, n, "kv_q4_read_dev first", dev)
+    counts = _need(counts, n, "kv_q4_read_dev counts", dev)
+    return check(lib().zq_hip_kv_q4_read_dev(cache.ref, k, v, tokens, first, counts, _stream(stream)),
+                 "zq_hip_kv_q4_read_dev")
+
+
+def attention_q4_workspace_bytes(cache, tokens, heads, flags=0):
+    return lib().zq_hip_attention_q4_workspace_bytes(cache.ref, tokens, heads, flags)
+
+
+def attention_q4_dev(cache, q, out, tokens, heads, lens, scale, counts=None, stride=0, flags=0, workspace=None,
+                     workspace_bytes=0, stream=None):
+    """Attention of q [seqs][tokens][stride] over the cache into out [seqs][tokens][heads * head_dim]."""
+    dev = _device_index()
+    width = heads * cache.head_dim
+    q = _need_rows(q, cache.seqs, tokens, stride, width, "attention_q4_dev q", dev)
+    out = _need(out, 4 * cache.seqs * tokens * width, "attention_q4_dev out", dev)
+    n = 4 * cache.seqs
+    lens = _need(lens, n, "attention_q4_dev lens", dev)
+    counts = _need(counts, n, "attention_q4_dev counts", dev)
+    workspace = _need(workspace, workspace_bytes, "attention_q4_dev workspace", dev)
+    return check(lib().zq_hip_attention_q4_dev(cache.ref, q, out, tokens, heads, stride, lens, counts, scale, flags,
+                                               workspace, workspace_bytes, _stream(stream)), "zq_hip_attention_q4_dev")
+
+
+def kv_q4_evict_workspace_bytes(cache, keep):
+    return lib().zq_hip_kv_q4_evict_workspace_bytes(cache.ref, keep)
+
+
+def kv_q4_evict_dev(cache, lens, keep, recent, first, next_pos=None, dst=None, workspace=None, workspace_bytes=0,
+                    stream=None):
+    """Keeps the `keep` rows of the most weight (the `recent` newest and `first` first ones always), in place or in dst."""
+    dev = _device_index()
+    n = 4 * cache.seqs
+    lens = _need(lens, n, "kv_q4_evict_dev lens", dev)
+    next_pos = _need(next_pos, n, "kv_q4_evict_dev next_pos", dev)
+    workspace = _need(workspace, workspace_bytes, "kv_q4_evict_dev workspace", dev)
+    return check(lib().zq_hip_kv_q4_evict_dev(cache.ref, dst.ref if dst is not None else None, lens, keep, recent, first,
+                                              next_pos, workspace, workspace_bytes, _stream(stream)),
+                 "zq_hip_kv_q4_evict_dev")

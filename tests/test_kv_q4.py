@@ -549,7 +549,7 @@ def test_attention_far_scores(zq, T):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("D,T,G", [(64, 1, 8), (128, 2, 4), (256, 1, 1)])
+@pytest.mark.parametrize("D,T,G", [(64, 1, 8), (128, 2, 4), (256, 1, 1), (64, 20, 8), (128, 40, 4), (256, 70, 1)])
 def test_attention_of_a_long_cache(zq, D, T, G):
     """Keys split over many workgroups, and the capacity far above the length."""
     r = np.random.default_rng(D)

@@ -17,6 +17,8 @@
 
 #include <math.h>
 
+#include <algorithm>
+
 namespace zq {
 namespace {
 
@@ -36,7 +38,7 @@ struct AttnQ4 {
     uint32_t tokens, G, KH, heads_kv;  // heads_kv = seqs * KH
     uint32_t rows;      // tokens * G
     uint32_t splits;
-    int full, add;
+    int full, add, many;
 };
 
 // What a sequence's rows see.
@@ -58,6 +60,11 @@ __device__ __forceinline__ uint32_t visible(const AttnQ4& a, const Seq& x, uint3
     return a.full ? x.len : uint32_t(min(uint64_t(x.len) + t + 1, uint64_t(a.c.capacity)));
 }
 
+// A weight as two fp16 parts; the second is rounded by the instruction that forms it.
+__device__ __forceinline__ void split_p(float p, h8_t& h, h8_t& l, int i) {
+    h[i] = _Float16(p);
+    l[i] = _Float16(fmaf(float(h[i]), -1.0f, p));
+}
 __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ __forceinline__ float max_groups(float v) {  // over the four lanes that share lane & 15
     v = fmaxf(v, __shfl_xor(v, 16));
@@ -87,8 +94,9 @@ constexpr float kSlack = 8.0f;  // how far a score may pass the running maximum
 
 // The k-slot order of a dword's 8 nibbles (nibbles2 of w, w >> 4, w >> 8, w >> 12):
 // elements 0, 2, 16, 18, 1, 3, 17, 19 of the block from the dword's first byte on.
-__device__ __forceinline__ h8_t dequant8(uint32_t w, h2_t d) {
-    const h2_t a = nibbles2(w) * d, b = nibbles2(w >> 4) * d, c = nibbles2(w >> 8) * d, e = nibbles2(w >> 12) * d;
+__device__ __forceinline__ h8_t dequant8(uint32_t w, h2_t d, uint32_t one) {
+    const h2_t a = nibbles2(w, one) * d, b = nibbles2(w >> 4, one) * d, c = nibbles2(w >> 8, one) * d,
+               e = nibbles2(w >> 12, one) * d;
     return h8_t{a.x, a.y, b.x, b.y, c.x, c.y, e.x, e.y};
 }
 
@@ -154,7 +162,8 @@ __device__ __forceinline__ void load_v(VTile<D>& t, const AttnQ4& a, uint32_t he
 }
 // scores of 32 keys and 16 rows: s[4 u + r] = row i, key 8 g + 4 u + r
 template <int D>
-__device__ __forceinline__ void scores(const KTile<D>& t, const h8_t (&qh)[D / 32], const h8_t (&ql)[D / 32], float (&s)[8]) {
+__device__ __forceinline__ void scores(const KTile<D>& t, const h8_t (&qh)[D / 32], const h8_t (&ql)[D / 32], uint32_t one,
+                                       float (&s)[8]) {
     using K = KTile<D>;
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
@@ -162,7 +171,7 @@ __device__ __forceinline__ void scores(const KTile<D>& t, const h8_t (&qh)[D / 3
 #pragma unroll
         for (int j = 0; j < K::KW; ++j) {
             const _Float16 d = __builtin_bit_cast(_Float16, t.sc[u][K::NS > 1 ? j / 4 : 0]);
-            const h8_t k = dequant8(t.w[u][j], h2_t{d, d});
+            const h8_t k = dequant8(t.w[u][j], h2_t{d, d}, one);
             acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, qh[j], acc, 0, 0, 0);
             acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, ql[j], acc, 0, 0, 0);
         }
@@ -242,6 +251,7 @@ __global__ __launch_bounds__(kWaves * 64) void attn_q4_few_kernel(AttnQ4 a) {
     // tiles below it need no mask: every live row sees them
     const uint32_t whole = visible(a, x, r0 / a.G) / 32;
 
+    const uint32_t one = code_bits();
     h8_t qh[D / 32], ql[D / 32];
     const float c = load_q<D>(a, x, r, ok, g, qh, ql);
     v4f_t o[NT];
@@ -259,7 +269,7 @@ __global__ __launch_bounds__(kWaves * 64) void attn_q4_few_kernel(AttnQ4 a) {
     }
     for (; t < t1; t += kWaves) {
         float s[8];
-        scores<D>(kt, qh, ql, s);
+        scores<D>(kt, qh, ql, one, s);
         const VTile<D> vn = vt;
         if (t + kWaves < t1) {
             load_k<D>(kt, a, head, (t + kWaves) * 32, i, g);
@@ -289,7 +299,7 @@ __global__ __launch_bounds__(kWaves * 64) void attn_q4_few_kernel(AttnQ4 a) {
         for (int k = 0; k < 8; ++k) {
             const float p = exp2_(fmaf(s[k], c, -ms));
             l += p;
-            split_h(p, ph, pl, k);
+            split_p(p, ph, pl, k);
         }
         h2_t d[4];
 #pragma unroll
@@ -301,7 +311,7 @@ __global__ __launch_bounds__(kWaves * 64) void attn_q4_few_kernel(AttnQ4 a) {
             for (int k = 0; k < 4; ++k) {
                 const uint32_t sel = 0x0c000c00u | uint32_t((4 + (y & 3)) << 16) | uint32_t(y & 3);
                 const uint32_t u = __builtin_amdgcn_perm(vn.w[2 * k + 1][y / 4], vn.w[2 * k][y / 4], sel);
-                const h2_t a0 = nibbles2(u) * d[k], a1 = nibbles2(u >> 4) * d[k];
+                const h2_t a0 = nibbles2(u, one) * d[k], a1 = nibbles2(u >> 4, one) * d[k];
                 lo[2 * k] = a0.x;
                 lo[2 * k + 1] = a0.y;
                 hi[2 * k] = a1.x;
@@ -374,6 +384,339 @@ __global__ __launch_bounds__(kWaves * 64) void attn_q4_few_kernel(AttnQ4 a) {
     }
 }
 
+// ---- many rows: tiles of 128 rows, keys decoded once a tile into LDS ----------------
+// v_mfma_f32_32x32x16_f16, transposed as above.  A workgroup takes 128 rows; its
+// waves stand in four groups of 32 rows, for D <= 128 twice, each half with its 32
+// keys of every staged 64 (their sums are merged at the end), so a SIMD holds two
+// waves whose matrix and vector work overlap.  For D = 256 a wave needs more than 256
+// registers, and four waves take both halves.
+//  * the keys of a step are decoded into LDS as fp16, K row-major with the dwords' own
+//    element order, V transposed, into two buffers each, one barrier a step: decoding
+//    a value takes two vector instructions, which 128 rows share;
+//  * row rho of the S^T product reads key rho with bits 2 and 3 exchanged, so that a
+//    lane's 16 scores are those of keys 8 h .. 8 h + 7 and 16 + 8 h .. (h = lane >> 5):
+//    the B operands of the second product as they are, and V^T is read in 16-byte runs.
+constexpr uint32_t kTileRows = 128;
+typedef float v16f_t __attribute__((ext_vector_type(16)));
+
+template <int D>
+struct Big {
+    static constexpr int KG = D <= 128 ? 2 : 1;  // 32-key parts of a step, each with waves of its own
+    static constexpr int T = 256 * KG;           // threads
+    static constexpr int TK = 32 * KG;           // keys of a step
+    static constexpr int HP = D + 8;             // halves of a K row in LDS: 16-byte reads of 32 rows, no conflict
+    static constexpr int KP = TK + 8;            // halves of a V^T row
+    static constexpr int NT = D / 32, KS = D / 16;
+    static constexpr int kTasks = TK * NT;       // blocks of K, and 8-key column groups of V, of a step: at most 256
+    static constexpr size_t kK = size_t(TK) * HP, kV = size_t(D) * KP;  // halves of one buffer of each
+    static constexpr size_t kMerge = KG == 2 ? size_t(4) * 64 * (NT * 16 + 2) * 4 : 0;
+    static constexpr size_t kQ = size_t(kTileRows) * HP;  // halves of one part of the queries
+    static constexpr size_t kLds = std::max({4 * (kK + kV), 4 * kQ, kMerge});
+    static_assert(kTasks <= 256 && kTasks % 64 == 0, "one task a thread, whole waves");
+};
+
+// Task e of K: key e / (D / 32), block e % (D / 32).  Task e of V: 8 keys, two bytes
+// of their rows (four dimensions); the key group's low bit runs fastest, so that the
+// 16-byte LDS writes of 16 lanes meet all banks.
+template <int D>
+struct KStage {
+    uint4 w;
+    _Float16 d;
+};
+template <int D>
+struct VStage {
+    uint16_t w[8];
+    h8_t d;
+};
+template <int D>
+__device__ __forceinline__ void load_kstage(KStage<D>& r, const AttnQ4& a, uint32_t head, uint32_t key0, int e) {
+    const size_t cap = a.c.capacity;
+    const int key = e / (D / 32), b = e % (D / 32);
+    r.w = *reinterpret_cast<const uint4*>(a.c.k + (size_t(head) * cap + key0 + key) * (D / 2) + b * 16);
+    r.d = __builtin_bit_cast(_Float16, a.c.k_scale[(size_t(head) * (D / 32) + b) * cap + key0 + key]);
+}
+template <int D>
+__device__ __forceinline__ void store_kstage(const KStage<D>& r, _Float16* kt, uint32_t one, int e) {
+    const int key = e / (D / 32), b = e % (D / 32);
+    const h2_t d = {r.d, r.d};
+    h8_t* p = reinterpret_cast<h8_t*>(kt + key * Big<D>::HP + b * 32);
+    p[0] = dequant8(r.w.x, d, one);
+    p[1] = dequant8(r.w.y, d, one);
+    p[2] = dequant8(r.w.z, d, one);
+    p[3] = dequant8(r.w.w, d, one);
+}
+template <int D>
+__device__ __forceinline__ void load_vstage(VStage<D>& r, const AttnQ4& a, uint32_t head, uint32_t key0, int e) {
+    const size_t cap = a.c.capacity;
+    const int ch = (e >> 1) % (D / 4), o = (e & 1) + 2 * (e / (D / 2));
+    const uint8_t* p = a.c.v + (size_t(head) * cap + key0 + 8 * o) * (D / 2) + 2 * ch;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) r.w[k] = *reinterpret_cast<const uint16_t*>(p + k * (D / 2));
+    r.d = *reinterpret_cast<const h8_t*>(a.c.v_scale + (size_t(head) * (D / 32) + ch / 8) * cap + key0 + 8 * o);
+}
+// keys: how many of the step hold rows that are seen (the others' scale may be any bits)
+template <int D>
+__device__ __forceinline__ void store_vstage(const VStage<D>& r, _Float16* vt, uint32_t keys, uint32_t one, int e) {
+    const int ch = (e >> 1) % (D / 4), o = (e & 1) + 2 * (e / (D / 2));
+    h8_t s = r.d;
+    if (keys < uint32_t(Big<D>::TK))
+#pragma unroll
+        for (int k = 0; k < 8; ++k) s[k] = uint32_t(8 * o + k) < keys ? s[k] : _Float16(0);
+    const int dim = ch / 8 * 32 + 2 * (ch % 8);
+#pragma unroll
+    for (int y = 0; y < 2; ++y) {
+        h8_t lo, hi;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const uint32_t u = __builtin_amdgcn_perm(uint32_t(r.w[2 * k + 1]), uint32_t(r.w[2 * k]),
+                                                     0x0c000c00u | uint32_t((4 + y) << 16) | uint32_t(y));
+            const h2_t d = {s[2 * k], s[2 * k + 1]};
+            const h2_t a0 = nibbles2(u, one) * d, a1 = nibbles2(u >> 4, one) * d;
+            lo[2 * k] = a0.x;
+            lo[2 * k + 1] = a0.y;
+            hi[2 * k] = a1.x;
+            hi[2 * k + 1] = a1.y;
+        }
+        *reinterpret_cast<h8_t*>(vt + (dim + y) * Big<D>::KP + 8 * o) = lo;
+        *reinterpret_cast<h8_t*>(vt + (dim + y + 16) * Big<D>::KP + 8 * o) = hi;
+    }
+}
+
+// Steps of `unit` keys that a tile's rows see, and how many a split takes.
+__device__ __forceinline__ Cut big_cut(const AttnQ4& a, const Seq& x, uint32_t r0, uint32_t unit) {
+    Cut c;
+    const uint32_t last = min(r0 + kTileRows - 1, x.live * a.G - 1) / a.G;
+    c.keys = visible(a, x, last);
+    c.tiles = (c.keys + unit - 1) / unit;
+    c.per = max((c.tiles + a.splits - 1) / a.splits, 1u);
+    c.used = max((c.tiles + c.per - 1) / c.per, 1u);
+    return c;
+}
+
+// The tile's query rows into LDS as operands (a row's own power of two taken off, two
+// fp16 parts, the dwords' element order): whole rows are read by neighbouring lanes,
+// where operand loads straight from memory would touch 64 lines each.
+template <int D>
+__device__ __forceinline__ void stage_q(const AttnQ4& a, const Seq& x, uint32_t r0, _Float16* hi, _Float16* lo,
+                                        float* inv, int tid) {
+    constexpr int RL = D / 4, RW = Big<D>::T / RL;  // lanes of a row, rows of a pass
+    const int l = tid % RL, dim = 4 * l;
+    const int pos = (dim / 32 * 4 + dim % 16 / 4) * 8 + (dim % 32 >= 16 ? 2 : 0);
+    const uint32_t rows = x.live * a.G;
+#pragma unroll 4
+    for (int j = 0; j < int(kTileRows); j += RW) {
+        const int row = j + tid / RL;
+        const uint32_t r = r0 + row;
+        const uint32_t t = r / a.G, hg = r % a.G;
+        float4 v = make_float4(0, 0, 0, 0);
+        if (r < rows) v = *reinterpret_cast<const float4*>(a.q + (size_t(x.s) * a.tokens + t) * a.stride +
+                                                           size_t(x.kh * a.G + hg) * D + dim);
+        v.x *= a.scale2;
+        v.y *= a.scale2;
+        v.z *= a.scale2;
+        v.w *= a.scale2;
+        float m = fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w)));
+#pragma unroll
+        for (int o = RL / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+        const int e = m > 0.0f ? min(max(15 - __builtin_amdgcn_frexp_expf(m), -120), 120) : 0;
+        const float f = pow2f(e);
+        if (l == 0) inv[row] = pow2f(-e);
+        h4_t h, w;
+        split_h(v.x * f, h, w, 0);
+        split_h(v.z * f, h, w, 1);
+        split_h(v.y * f, h, w, 2);
+        split_h(v.w * f, h, w, 3);
+        _Float16* ph = hi + row * Big<D>::HP + pos;
+        _Float16* pl = lo + row * Big<D>::HP + pos;
+        *reinterpret_cast<h2_t*>(ph) = h2_t{h.x, h.y};
+        *reinterpret_cast<h2_t*>(ph + 4) = h2_t{h.z, h.w};
+        *reinterpret_cast<h2_t*>(pl) = h2_t{w.x, w.y};
+        *reinterpret_cast<h2_t*>(pl + 4) = h2_t{w.z, w.w};
+    }
+}
+
+template <int D>
+__global__ __launch_bounds__(Big<D>::T) void attn_q4_many_kernel(AttnQ4 a) {
+    using B = Big<D>;
+    extern __shared__ __align__(16) uint8_t lds[];
+    __shared__ float inv_q[kTileRows];
+    const uint32_t head = blockIdx.x % a.heads_kv, rest = blockIdx.x / a.heads_kv;
+    const uint32_t sp = rest % a.splits, tiles = (a.rows + kTileRows - 1) / kTileRows;
+    const uint32_t r0 = (tiles - 1 - rest / a.splits) * kTileRows;  // the tiles that see most come first
+    const Seq x = seq_of(a, head);
+    const uint32_t rows = x.live * a.G;
+    if (r0 >= rows) return;
+    const Cut cut = big_cut(a, x, r0, B::TK);
+    if (sp >= cut.used) return;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l32 = lane & 31, lh = lane >> 5;
+    const int kg = B::KG == 2 ? wave >> 2 : 0;
+    const uint32_t rw = r0 + 32 * (wave & 3), r = rw + l32;
+    const bool ok = r < rows;
+    const uint32_t lim = ok ? visible(a, x, r / a.G) : 0;
+    // of the wave's rows: keys that some see, and that all (live ones) see
+    const uint32_t most = rw < rows ? visible(a, x, min(rw + 31, rows - 1) / a.G) : 0;
+    const uint32_t whole = rw < rows ? visible(a, x, rw / a.G) : 0;
+
+    const uint32_t t0 = sp * cut.per, t1 = min(t0 + cut.per, cut.tiles);
+    _Float16* kbuf = reinterpret_cast<_Float16*>(lds);
+    _Float16* vbuf = kbuf + 2 * B::kK;
+    // K by the first 256 threads, V by the others (by the same ones where there are no others)
+    const int e = tid & 255;
+    const bool kr = (B::KG == 1 || tid < 256) && e < B::kTasks, vr = (B::KG == 1 || tid >= 256) && e < B::kTasks;
+    const uint32_t one = code_bits();
+    auto put_v = [&](const VStage<D>& s, uint32_t t) {
+        store_vstage<D>(s, vbuf + (t & 1) * B::kV, min(cut.keys - t * B::TK, uint32_t(B::TK)), one, e);
+    };
+    KStage<D> ks;
+    VStage<D> vs;
+    if (t0 < t1) {
+        if (kr) load_kstage<D>(ks, a, head, t0 * B::TK, e);
+        if (vr) load_vstage<D>(vs, a, head, t0 * B::TK, e);
+    }
+    h8_t qh[B::KS], ql[B::KS];
+    stage_q<D>(a, x, r0, kbuf, kbuf + B::kQ, inv_q, tid);
+    __syncthreads();
+    const int qrow = 32 * (wave & 3) + l32;
+    const float c = inv_q[qrow];
+#pragma unroll
+    for (int j = 0; j < B::KS; ++j) {
+        qh[j] = *reinterpret_cast<const h8_t*>(kbuf + qrow * B::HP + j * 16 + 8 * lh);
+        ql[j] = *reinterpret_cast<const h8_t*>(kbuf + B::kQ + qrow * B::HP + j * 16 + 8 * lh);
+    }
+    __syncthreads();  // K and V take its place
+    v16f_t o[B::NT], s;
+#pragma unroll
+    for (int n = 0; n < B::NT; ++n)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) o[n][v] = 0.0f;
+    float m = -INFINITY, l = 0.0f;
+    if (t0 < t1) {
+        if (kr) {
+            store_kstage<D>(ks, kbuf + (t0 & 1) * B::kK, one, e);
+            if (t0 + 1 < t1) {
+                load_kstage<D>(ks, a, head, (t0 + 1) * B::TK, e);
+                store_kstage<D>(ks, kbuf + ((t0 + 1) & 1) * B::kK, one, e);
+            }
+        }
+        if (vr) put_v(vs, t0);
+    }
+    __syncthreads();
+    // this lane's part of a K row: bits 2 and 3 of the row exchanged
+    const int krow = 32 * kg + ((l32 & 0x13) | (l32 & 4) << 1 | (l32 & 8) >> 1), koff = krow * B::HP + 8 * lh;
+    const int voff = l32 * B::KP + 32 * kg + 8 * lh;
+    auto product = [&](uint32_t t) {
+        const _Float16* kt = kbuf + (t & 1) * B::kK + koff;
+        v16f_t y;
+#pragma unroll
+        for (int v = 0; v < 16; ++v) y[v] = 0.0f;
+#pragma unroll
+        for (int j = 0; j < B::KS; ++j) {
+            const h8_t k = *reinterpret_cast<const h8_t*>(kt + j * 16);
+            y = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, qh[j], y, 0, 0, 0);
+            y = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, ql[j], y, 0, 0, 0);
+        }
+        return y;
+    };
+    if (t0 < t1) s = product(t0);
+    // Step t: the weights of its scores and, between their instructions, the next
+    // step's scores; then the second product.  K is decoded two steps ahead and V one.
+    for (uint32_t t = t0; t < t1; ++t) {
+        __syncthreads();  // K of t + 1 and V of t are written, K of t and V of t - 1 are read no more
+        if (kr && t + 2 < t1) load_kstage<D>(ks, a, head, (t + 2) * B::TK, e);
+        if (vr && t + 1 < t1) load_vstage<D>(vs, a, head, (t + 1) * B::TK, e);
+        const uint32_t key0 = t * B::TK + 32 * kg;
+        if (key0 < most) {  // uniform in the wave, and for no later step where it is not
+            if (key0 + 32 > whole) {
+#pragma unroll
+                for (int v = 0; v < 16; ++v) s[v] = key0 + 16 * (v >> 3) + 8 * lh + (v & 7) < lim ? s[v] : -INFINITY;
+            }
+            float mx = s[0];
+#pragma unroll
+            for (int v = 1; v < 16; ++v) mx = fmaxf(mx, s[v]);
+            mx *= c;
+            if (__any(mx > m + kSlack)) {
+                const float mn = fmaxf(m, fmaxf(mx, __shfl_xor(mx, 32)));
+                const float f = exp2_(m - (mn == -INFINITY ? 0.0f : mn));
+                m = mn;
+                l *= f;
+#pragma unroll
+                for (int n = 0; n < B::NT; ++n)
+#pragma unroll
+                    for (int v = 0; v < 16; ++v) o[n][v] *= f;
+            }
+            const float ms = (m == -INFINITY ? 0.0f : m) - kShift;
+            // (of a step past the last one: what the buffer holds, not used)
+            const v16f_t next = product(t + 1);
+            h8_t ph[2], pl[2];
+#pragma unroll
+            for (int v = 0; v < 16; ++v) {
+                const float p = exp2_(fmaf(s[v], c, -ms));
+                l += p;
+                split_p(p, ph[v >> 3], pl[v >> 3], v & 7);
+            }
+            s = next;
+            const _Float16* vt = vbuf + (t & 1) * B::kV + voff;
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int n = 0; n < B::NT; ++n) {
+                    const h8_t v = *reinterpret_cast<const h8_t*>(vt + 32 * n * B::KP + 16 * u);
+                    o[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, ph[u], o[n], 0, 0, 0);
+                    o[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, pl[u], o[n], 0, 0, 0);
+                }
+        }
+        if (kr && t + 2 < t1) store_kstage<D>(ks, kbuf + (t & 1) * B::kK, one, e);
+        if (vr && t + 1 < t1) put_v(vs, t + 1);
+    }
+    // ---- the two key halves of a row as one ----
+    l += __shfl_xor(l, 32);
+    float M = m, L = l;
+    if constexpr (B::KG == 2) {
+        float* mrg = reinterpret_cast<float*>(lds) + size_t(wave & 3) * 64 * (B::NT * 16 + 2);
+        __syncthreads();  // the buffers are read no more
+        if (kg == 1) {
+#pragma unroll
+            for (int n = 0; n < B::NT; ++n)
+#pragma unroll
+                for (int v = 0; v < 16; ++v) mrg[(n * 16 + v) * 64 + lane] = o[n][v];
+            mrg[B::NT * 16 * 64 + lane] = m;
+            mrg[(B::NT * 16 + 1) * 64 + lane] = l;
+        }
+        __syncthreads();
+        if (kg == 1) return;
+        const float m1 = mrg[B::NT * 16 * 64 + lane], l1 = mrg[(B::NT * 16 + 1) * 64 + lane];
+        M = fmaxf(m, m1);
+        const float Ms = M == -INFINITY ? 0.0f : M;
+        const float f0 = exp2_(m - Ms), f1 = exp2_(m1 - Ms);
+        L = l * f0 + l1 * f1;
+#pragma unroll
+        for (int n = 0; n < B::NT; ++n)
+#pragma unroll
+            for (int v = 0; v < 16; ++v) o[n][v] = o[n][v] * f0 + mrg[(n * 16 + v) * 64 + lane] * f1;
+    }
+    if (!ok) return;
+    const bool direct = cut.used == 1;
+    const size_t row = size_t(head) * a.rows + r;
+    if (lh == 0) {
+        if (!direct) {
+            float* ml = a.part_ml + (row * a.splits + sp) * 2;
+            ml[0] = M;
+            ml[1] = L;
+        } else if (a.lse) {
+            a.lse[row] = M - kShift + log2f(L);
+        }
+    }
+    float* dst = direct ? a.out + ((size_t(x.s) * a.tokens + r / a.G) * a.KH * a.G + x.kh * a.G + r % a.G) * D
+                        : a.part + (row * a.splits + sp) * D;
+    const float inv = direct ? (L > 0.0f ? 1.0f / L : (L == 0.0f ? 0.0f : L)) : 1.0f;
+#pragma unroll
+    for (int n = 0; n < B::NT; ++n)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            *reinterpret_cast<float4*>(dst + 32 * n + 8 * j + 4 * lh) =
+                make_float4(o[n][4 * j] * inv, o[n][4 * j + 1] * inv, o[n][4 * j + 2] * inv, o[n][4 * j + 3] * inv);
+}
+
 // One wave a row: the splits' partial outputs as one.  Splits are few (at most
 // 128), their maxima and sums are held by the lanes.
 template <int D>
@@ -384,7 +727,7 @@ __global__ __launch_bounds__(256) void attn_q4_combine_kernel(AttnQ4 a) {
     if (head >= a.heads_kv) return;
     const Seq x = seq_of(a, head);
     if (r >= x.live * a.G) return;
-    const Cut cut = cut_of(a, x, r / 16 * 16);
+    const Cut cut = a.many ? big_cut(a, x, r / kTileRows * kTileRows, Big<D>::TK) : cut_of(a, x, r / 16 * 16);
     if (cut.used == 1) return;  // written by the split itself
     const size_t row = size_t(head) * a.rows + r;
     const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + row * a.splits;
@@ -423,6 +766,7 @@ __global__ __launch_bounds__(kWaves * 64) void attn_q4_weights_kernel(AttnQ4 a) 
     const uint32_t rows = x.live * a.G, keys = visible(a, x, x.live - 1);
     const uint32_t key0 = (kb * kWaves + wave) * 32;
     if (key0 >= keys) return;
+    const uint32_t one = code_bits();
     KTile<D> kt;
     load_k<D>(kt, a, head, key0, i, g);
     float w[8];
@@ -438,7 +782,7 @@ __global__ __launch_bounds__(kWaves * 64) void attn_q4_weights_kernel(AttnQ4 a) 
         const float lse = ok ? a.lse[size_t(head) * a.rows + r] : 0.0f;
         const uint32_t lim = ok ? visible(a, x, r / a.G) : 0;
         float s[8];
-        scores<D>(kt, qh, ql, s);
+        scores<D>(kt, qh, ql, one, s);
 #pragma unroll
         for (int k = 0; k < 8; ++k) w[k] += key0 + 8 * g + k < lim ? exp2_(fmaf(s[k], c, -lse)) : 0.0f;
     }
@@ -453,13 +797,20 @@ __global__ __launch_bounds__(kWaves * 64) void attn_q4_weights_kernel(AttnQ4 a) 
     }
 }
 
-// How many workgroups share a row tile's keys: enough for three workgroups a CU
-// (12 of the 16-row kernel's waves), at least one tile a wave.
-uint32_t splits_of(const zq_kv_q4& c, size_t rows) {
-    const size_t base = c.seqs * c.kv_heads * ((rows + 15) / 16);
-    const size_t want = (size_t(device_cu_count()) * 3 + base - 1) / base;
-    const size_t most = (c.capacity / 32 + kWaves - 1) / kWaves;
-    return uint32_t(want < most ? (want < 128 ? want : 128) : (most < 128 ? most : 128));
+// Which kernel takes a call, and how many workgroups share a row tile's keys.
+struct Plan {
+    bool many;
+    uint32_t splits;
+};
+Plan plan_of(const zq_kv_q4& c, size_t rows) {
+    Plan p;
+    p.many = rows > 64;
+    const size_t tile = p.many ? kTileRows : 16;
+    const size_t base = c.seqs * c.kv_heads * ((rows + tile - 1) / tile);
+    const size_t want = (size_t(device_cu_count()) * (p.many ? 1 : 3) + base - 1) / base;
+    const size_t most = p.many ? (c.capacity + 511) / 512 : (c.capacity / 32 + kWaves - 1) / kWaves;
+    p.splits = uint32_t(std::max<size_t>(1, std::min<size_t>({want, most, 128})));
+    return p;
 }
 
 size_t up256(size_t n) { return (n + 255) / 256 * 256; }
@@ -468,7 +819,7 @@ size_t up256(size_t n) { return (n + 255) / 256 * 256; }
 
 size_t attention_q4_bytes(const zq_kv_q4& c, size_t tokens, size_t heads, int flags) {
     const size_t rows = tokens * (heads / c.kv_heads), all = c.seqs * c.kv_heads * rows;
-    const size_t splits = splits_of(c, rows);
+    const size_t splits = plan_of(c, rows).splits;
     size_t n = 0;
     if (splits > 1) n += up256(all * splits * c.head_dim * 4) + up256(all * splits * 8);
     if (flags & ZQ_ATTN_Q4_WEIGHTS) n += up256(all * 4);
@@ -491,7 +842,9 @@ hipError_t launch_attention_q4(const zq_kv_q4& c, const float* q, float* out, si
     a.G = uint32_t(heads / c.kv_heads);
     a.heads_kv = uint32_t(c.seqs * c.kv_heads);
     a.rows = uint32_t(tokens) * a.G;
-    a.splits = splits_of(c, a.rows);
+    const Plan plan = plan_of(c, a.rows);
+    a.splits = plan.splits;
+    a.many = plan.many;
     a.full = (flags & ZQ_ATTN_Q4_FULL) != 0;
     a.add = (flags & ZQ_ATTN_Q4_ADD) != 0;
     const size_t all = size_t(a.heads_kv) * a.rows;
@@ -503,7 +856,8 @@ hipError_t launch_attention_q4(const zq_kv_q4& c, const float* q, float* out, si
         p += up256(all * a.splits * 8);
     }
     if (flags & ZQ_ATTN_Q4_WEIGHTS) a.lse = reinterpret_cast<float*>(p);
-    const size_t blocks = size_t(a.heads_kv) * a.splits * ((a.rows + 15) / 16);
+    const size_t tile = a.many ? kTileRows : 16;
+    const size_t blocks = size_t(a.heads_kv) * a.splits * ((a.rows + tile - 1) / tile);
     const size_t key_blocks = size_t(a.heads_kv) * ((c.capacity / 32 + kWaves - 1) / kWaves);
     if (blocks > 0x7fffffffu || key_blocks > 0x7fffffffu) return hipErrorInvalidValue;
 #define ZQ_ATTN_D(KERNEL, GRID, THREADS)                                                                \
@@ -514,7 +868,18 @@ hipError_t launch_attention_q4(const zq_kv_q4& c, const float* q, float* out, si
         const hipError_t e = hipGetLastError();                                                         \
         if (e != hipSuccess) return e;                                                                  \
     } while (0)
-    ZQ_ATTN_D(attn_q4_few_kernel, blocks, kWaves * 64);
+    if (a.many) {
+#define ZQ_ATTN_MANY(DD)                                                                                          \
+    hipLaunchKernelGGL(attn_q4_many_kernel<DD>, dim3(uint32_t(blocks)), dim3(Big<DD>::T), Big<DD>::kLds, stream, a)
+        if (c.head_dim == 64) ZQ_ATTN_MANY(64);
+        else if (c.head_dim == 128) ZQ_ATTN_MANY(128);
+        else ZQ_ATTN_MANY(256);
+#undef ZQ_ATTN_MANY
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    } else {
+        ZQ_ATTN_D(attn_q4_few_kernel, blocks, kWaves * 64);
+    }
     if (a.splits > 1) ZQ_ATTN_D(attn_q4_combine_kernel, (all + 3) / 4, 256);
     if (a.lse) ZQ_ATTN_D(attn_q4_weights_kernel, key_blocks, kWaves * 64);
 #undef ZQ_ATTN_D

@@ -32,9 +32,16 @@ hipError_t launch_attention_q4(const zq_kv_q4& c, const float* q, float* out, si
 typedef _Float16 h2_t __attribute__((ext_vector_type(2)));
 
 // Two nibbles at bits 0..3 and 16..19 of u as fp16 code - 8: 0x6400 | n is
-// 1024 + n, and the difference to 1032 is exact.
-__device__ __forceinline__ h2_t nibbles2(uint32_t u) {
-    const h2_t x = __builtin_bit_cast(h2_t, (u & 0x000f000fu) | 0x64006400u);
+// 1024 + n, and the difference to 1032 is exact.  `one` is 0x64006400 in a vector
+// register (code_bits()): with it the mask and the or are one instruction, which
+// takes no two literals.
+__device__ __forceinline__ uint32_t code_bits() {
+    uint32_t x = 0x64006400u;
+    asm("" : "+v"(x));  // no constant to the compiler
+    return x;
+}
+__device__ __forceinline__ h2_t nibbles2(uint32_t u, uint32_t one) {
+    const h2_t x = __builtin_bit_cast(h2_t, (u & 0x000f000fu) | one);
     return x - h2_t{_Float16(1032.0f), _Float16(1032.0f)};
 }
 __device__ __forceinline__ int32_t clamp_len(int32_t n, size_t most) {

@@ -496,28 +496,37 @@ __device__ __forceinline__ Cut big_cut(const AttnQ4& a, const Seq& x, uint32_t r
 // The tile's query rows into LDS as operands (a row's own power of two taken off, two
 // fp16 parts, the dwords' element order): whole rows are read by neighbouring lanes,
 // where operand loads straight from memory would touch 64 lines each.
-template <int D>
-__device__ __forceinline__ void stage_q(const AttnQ4& a, const Seq& x, uint32_t r0, _Float16* hi, _Float16* lo,
-                                        float* inv, int tid) {
-    constexpr int RL = D / 4, RW = Big<D>::T / RL;  // lanes of a row, rows of a pass
-    const int l = tid % RL, dim = 4 * l;
-    const int pos = (dim / 32 * 4 + dim % 16 / 4) * 8 + (dim % 32 >= 16 ? 2 : 0);
-    const uint32_t rows = x.live * a.G;
-#pragma unroll 4
-    for (int j = 0; j < int(kTileRows); j += RW) {
-        const int row = j + tid / RL;
-        const uint32_t r = r0 + row;
+template <int D, int T, int N>
+struct QStage {  // what a thread of T holds of N rows
+    static constexpr int RL = D / 4, J = N * RL / T;  // lanes of a row, passes
+    float4 v[J];
+};
+template <int D, int T, int N>
+__device__ __forceinline__ void load_qstage(QStage<D, T, N>& s, const AttnQ4& a, const Seq& x, uint32_t r0, int tid) {
+    using S = QStage<D, T, N>;
+#pragma unroll
+    for (int j = 0; j < S::J; ++j) {
+        const uint32_t r = r0 + uint32_t(j * (T / S::RL) + tid / S::RL);
         const uint32_t t = r / a.G, hg = r % a.G;
-        float4 v = make_float4(0, 0, 0, 0);
-        if (r < rows) v = *reinterpret_cast<const float4*>(a.q + (size_t(x.s) * a.tokens + t) * a.stride +
-                                                           size_t(x.kh * a.G + hg) * D + dim);
-        v.x *= a.scale2;
-        v.y *= a.scale2;
-        v.z *= a.scale2;
-        v.w *= a.scale2;
+        s.v[j] = r < x.live * a.G ? *reinterpret_cast<const float4*>(a.q + (size_t(x.s) * a.tokens + t) * a.stride +
+                                                                     size_t(x.kh * a.G + hg) * D + tid % S::RL * 4)
+                                  : make_float4(0, 0, 0, 0);
+    }
+}
+template <int D, int T, int N>
+__device__ __forceinline__ void store_qstage(const QStage<D, T, N>& s, float scale2, _Float16* hi, _Float16* lo,
+                                             float* inv, int tid) {
+    using S = QStage<D, T, N>;
+    constexpr int HP = D + 8;
+    const int l = tid % S::RL, dim = 4 * l;
+    const int pos = (dim / 32 * 4 + dim % 16 / 4) * 8 + (dim % 32 >= 16 ? 2 : 0);
+#pragma unroll
+    for (int j = 0; j < S::J; ++j) {
+        const int row = j * (T / S::RL) + tid / S::RL;
+        const float4 v = make_float4(s.v[j].x * scale2, s.v[j].y * scale2, s.v[j].z * scale2, s.v[j].w * scale2);
         float m = fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w)));
 #pragma unroll
-        for (int o = RL / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+        for (int o = S::RL / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
         const int e = m > 0.0f ? min(max(15 - __builtin_amdgcn_frexp_expf(m), -120), 120) : 0;
         const float f = pow2f(e);
         if (l == 0) inv[row] = pow2f(-e);
@@ -526,8 +535,8 @@ __device__ __forceinline__ void stage_q(const AttnQ4& a, const Seq& x, uint32_t 
         split_h(v.z * f, h, w, 1);
         split_h(v.y * f, h, w, 2);
         split_h(v.w * f, h, w, 3);
-        _Float16* ph = hi + row * Big<D>::HP + pos;
-        _Float16* pl = lo + row * Big<D>::HP + pos;
+        _Float16* ph = hi + row * HP + pos;
+        _Float16* pl = lo + row * HP + pos;
         *reinterpret_cast<h2_t*>(ph) = h2_t{h.x, h.y};
         *reinterpret_cast<h2_t*>(ph + 4) = h2_t{h.z, h.w};
         *reinterpret_cast<h2_t*>(pl) = h2_t{w.x, w.y};
@@ -574,7 +583,11 @@ __global__ __launch_bounds__(Big<D>::T) void attn_q4_many_kernel(AttnQ4 a) {
         if (vr) load_vstage<D>(vs, a, head, t0 * B::TK, e);
     }
     h8_t qh[B::KS], ql[B::KS];
-    stage_q<D>(a, x, r0, kbuf, kbuf + B::kQ, inv_q, tid);
+    {
+        QStage<D, B::T, int(kTileRows)> qs;
+        load_qstage(qs, a, x, r0, tid);
+        store_qstage(qs, a.scale2, kbuf, kbuf + B::kQ, inv_q, tid);
+    }
     __syncthreads();
     const int qrow = 32 * (wave & 3) + l32;
     const float c = inv_q[qrow];
@@ -755,45 +768,157 @@ __global__ __launch_bounds__(256) void attn_q4_combine_kernel(AttnQ4 a) {
 }
 
 // ---- the rows' weights ----------------------------------------------------------
-// A wave holds 32 keys and goes over all query rows that see any of them, so every
-// key's sum has one owner and one order.
+// S = Q K^T again, with the sums of the rows known (lse): a lane's 16 results are 16
+// query rows of one key, so a key's weight is a sum in one register.  A wave keeps 64
+// keys as operands; query rows pass by in LDS, 64 at a time.  Every key's sum has one
+// owner (or two halves, added in order) and one order.
+// RH = 2 (many rows): eight waves, four on each half of the 64 rows.  RH = 1 (up to
+// 64 rows, staged once): four waves that go on to further keys.
 template <int D>
-__global__ __launch_bounds__(kWaves * 64) void attn_q4_weights_kernel(AttnQ4 a) {
-    const uint32_t head = blockIdx.x % a.heads_kv, kb = blockIdx.x / a.heads_kv;
+struct Wgt {
+    static constexpr int HP = D + 8, R = 64, KS = D / 16;
+    static constexpr size_t kQ = size_t(R) * HP;          // halves of one part of the queries
+    static constexpr size_t lds(int rh) { return 4 * kQ * rh; }  // two buffers where rows pass by
+};
+
+template <int D, int RH>
+__global__ __launch_bounds__(256 * RH) void attn_q4_weights_kernel(AttnQ4 a, uint32_t blocks) {
+    using W = Wgt<D>;
+    constexpr int T = 256 * RH, KS = W::KS;
+    extern __shared__ __align__(16) uint8_t lds[];
+    __shared__ __align__(16) float inv[2][W::R];
+    __shared__ __align__(16) float lse[2][W::R];
+    __shared__ __align__(16) int32_t lim[2][W::R];
+    __shared__ float half[RH == 2 ? 256 : 1];
+    _Float16* qbuf = reinterpret_cast<_Float16*>(lds);
+    const uint32_t head = blockIdx.x % a.heads_kv, first = blockIdx.x / a.heads_kv;
     const Seq x = seq_of(a, head);
     if (!x.live) return;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, g = lane >> 4;
     const uint32_t rows = x.live * a.G, keys = visible(a, x, x.live - 1);
-    const uint32_t key0 = (kb * kWaves + wave) * 32;
-    if (key0 >= keys) return;
+    const uint32_t nb = (keys + 255) / 256;
+    if (first >= nb) return;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l32 = lane & 31, lh = lane >> 5;
+    const int kg = wave & 3, rh = wave >> 2;
     const uint32_t one = code_bits();
-    KTile<D> kt;
-    load_k<D>(kt, a, head, key0, i, g);
-    float w[8];
+    const size_t cap = a.c.capacity;
+    // the rows from r0 on into buffer b
+    auto meta = [&](uint32_t r0, int b) {
+        if (tid < W::R) {
+            const uint32_t r = r0 + tid;
+            const bool ok = r < rows;
+            lse[b][tid] = ok ? a.lse[size_t(head) * a.rows + r] : INFINITY;  // a row past the live ones: weights 0
+            lim[b][tid] = ok ? int32_t(visible(a, x, r / a.G)) : 0;
+        }
+    };
+    QStage<D, T, W::R> qs;
+    for (uint32_t kb = first; kb < nb; kb += blocks) {  // uniform; more than one only with RH = 1
+        const uint32_t key0 = kb * 256 + 64 * kg;
+        const bool mine = key0 < keys;  // uniform in the wave
+        // rows before the first token that sees the block's first key see none of it
+        const uint32_t ta = a.full || kb * 256 < x.len ? 0 : kb * 256 - x.len;
+        const uint32_t ra = ta * a.G / W::R * W::R;
+        if (RH == 2 || kb == first) load_qstage(qs, a, x, ra, tid);
+        h8_t kf[2][KS];
+        if (mine) {
 #pragma unroll
-    for (int k = 0; k < 8; ++k) w[k] = 0.0f;
-    // first token that sees key0
-    const uint32_t ta = a.full || key0 < x.len ? 0 : key0 - x.len;
-    for (uint32_t r0 = ta * a.G / 16 * 16; r0 < rows; r0 += 16) {
-        const uint32_t r = r0 + i;
-        const bool ok = r < rows;
-        h8_t qh[D / 32], ql[D / 32];
-        const float c = load_q<D>(a, x, r, ok, g, qh, ql);
-        const float lse = ok ? a.lse[size_t(head) * a.rows + r] : 0.0f;
-        const uint32_t lim = ok ? visible(a, x, r / a.G) : 0;
-        float s[8];
-        scores<D>(kt, qh, ql, one, s);
+            for (int u = 0; u < 2; ++u) {
+                // the last keys of a block may lie past the capacity: their lanes take the last row's
+                const size_t key = min(size_t(key0) + 32 * u + l32, cap - 1);
+                const uint8_t* p = a.c.k + (size_t(head) * cap + key) * (D / 2) + lh * (D / 4);
+                uint32_t w[KS];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) w[k] += key0 + 8 * g + k < lim ? exp2_(fmaf(s[k], c, -lse)) : 0.0f;
-    }
+                for (int j = 0; j < KS / 4; ++j) {
+                    const uint4 v = reinterpret_cast<const uint4*>(p)[j];
+                    w[4 * j] = v.x;
+                    w[4 * j + 1] = v.y;
+                    w[4 * j + 2] = v.z;
+                    w[4 * j + 3] = v.w;
+                }
 #pragma unroll
-    for (int k = 0; k < 8; ++k) w[k] = group_sum<16>(w[k]);
-    float* dst = a.c.weight + size_t(head) * a.c.capacity + key0 + 8 * g;
-    if (i < 8 && key0 + 8 * g + i < keys) {
-        float v = w[0];
+                for (int j = 0; j < KS / 4; ++j) {
+                    const _Float16 d = __builtin_bit_cast(
+                        _Float16, a.c.k_scale[(size_t(head) * (D / 32) + lh * (KS / 4) + j) * cap + key]);
 #pragma unroll
-        for (int k = 1; k < 8; ++k) v = i == k ? w[k] : v;
-        dst[i] = a.add ? dst[i] + v : v;
+                    for (int i = 0; i < 4; ++i) kf[u][4 * j + i] = dequant8(w[4 * j + i], h2_t{d, d}, one);
+                }
+            }
+        }
+        if (RH == 2 || kb == first) {
+            if (kb != first) __syncthreads();
+            store_qstage(qs, a.scale2, qbuf, qbuf + W::kQ, inv[0], tid);
+            meta(ra, 0);
+            __syncthreads();
+        }
+        float w[2] = {0.0f, 0.0f};
+        int b = 0;
+        for (uint32_t r0 = ra; r0 < rows; r0 += W::R, b ^= 1) {
+            const bool more = RH == 2 && r0 + W::R < rows;
+            if (more) load_qstage(qs, a, x, r0 + W::R, tid);
+            const _Float16* qt = qbuf + size_t(b) * 2 * W::kQ;
+#pragma unroll
+            for (int sub = 0; sub < 2 / RH; ++sub) {
+                const int row0 = 32 * (RH == 2 ? rh : sub);
+                if (!mine || r0 + row0 >= rows) continue;  // uniform in the wave
+                const _Float16* q = qt + (row0 + l32) * W::HP + lh * (D / 2);
+                typedef float acc_t __attribute__((ext_vector_type(16)));
+                acc_t s[2];
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int v = 0; v < 16; ++v) s[u][v] = 0.0f;
+#pragma unroll
+                for (int j = 0; j < KS; ++j) {
+                    const h8_t h = *reinterpret_cast<const h8_t*>(q + 8 * j);
+                    const h8_t l = *reinterpret_cast<const h8_t*>(q + W::kQ + 8 * j);
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        s[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(h, kf[u][j], s[u], 0, 0, 0);
+                        s[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(l, kf[u][j], s[u], 0, 0, 0);
+                    }
+                }
+                // result v of a lane: row 8 (v >> 2) + 4 lh + (v & 3), key l32
+                const bool cut = key0 + 64 > visible(a, x, min(r0 + row0, rows - 1) / a.G);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int at = row0 + 8 * j + 4 * lh;
+                    const float4 c = *reinterpret_cast<const float4*>(&inv[b][at]);
+                    const float4 e = *reinterpret_cast<const float4*>(&lse[b][at]);
+                    const float cc[4] = {c.x, c.y, c.z, c.w}, ee[4] = {e.x, e.y, e.z, e.w};
+                    if (!cut) {
+#pragma unroll
+                        for (int u = 0; u < 2; ++u)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) w[u] += exp2_(fmaf(s[u][4 * j + i], cc[i], -ee[i]));
+                    } else {
+                        const int4 m = *reinterpret_cast<const int4*>(&lim[b][at]);
+                        const int mm[4] = {m.x, m.y, m.z, m.w};
+#pragma unroll
+                        for (int u = 0; u < 2; ++u)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i)
+                                w[u] += int(key0 + 32 * u + l32) < mm[i] ? exp2_(fmaf(s[u][4 * j + i], cc[i], -ee[i])) : 0.0f;
+                    }
+                }
+            }
+            if (more) {  // the other buffer was read last before the previous barrier
+                _Float16* nq = qbuf + size_t(b ^ 1) * 2 * W::kQ;
+                store_qstage(qs, a.scale2, nq, nq + W::kQ, inv[b ^ 1], tid);
+                meta(r0 + W::R, b ^ 1);
+                __syncthreads();
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < 2; ++u) w[u] += __shfl_xor(w[u], 32);
+        float v = lh ? w[1] : w[0];  // lane's key of the wave's 64
+        if constexpr (RH == 2) {
+            if (rh == 1) half[64 * kg + lane] = v;
+            __syncthreads();
+            if (rh == 0) v += half[64 * kg + lane];
+        }
+        if (rh == 0 && key0 + lane < keys) {
+            float* dst = a.c.weight + size_t(head) * cap + key0 + lane;
+            *dst = a.add ? *dst + v : v;
+        }
     }
 }
 
@@ -858,7 +983,10 @@ hipError_t launch_attention_q4(const zq_kv_q4& c, const float* q, float* out, si
     if (flags & ZQ_ATTN_Q4_WEIGHTS) a.lse = reinterpret_cast<float*>(p);
     const size_t tile = a.many ? kTileRows : 16;
     const size_t blocks = size_t(a.heads_kv) * a.splits * ((a.rows + tile - 1) / tile);
-    const size_t key_blocks = size_t(a.heads_kv) * ((c.capacity / 32 + kWaves - 1) / kWaves);
+    // weights: with many rows every 256 keys have a workgroup of their own
+    const bool pass = a.rows > uint32_t(Wgt<64>::R);
+    const size_t all_blocks = (c.capacity + 255) / 256, fill = size_t(device_cu_count()) * 4 / a.heads_kv + 1;
+    const size_t wblocks = pass ? all_blocks : std::min(all_blocks, fill), key_blocks = a.heads_kv * wblocks;
     if (blocks > 0x7fffffffu || key_blocks > 0x7fffffffu) return hipErrorInvalidValue;
 #define ZQ_ATTN_D(KERNEL, GRID, THREADS)                                                                \
     do {                                                                                                \
@@ -881,9 +1009,23 @@ hipError_t launch_attention_q4(const zq_kv_q4& c, const float* q, float* out, si
         ZQ_ATTN_D(attn_q4_few_kernel, blocks, kWaves * 64);
     }
     if (a.splits > 1) ZQ_ATTN_D(attn_q4_combine_kernel, (all + 3) / 4, 256);
-    if (a.lse) ZQ_ATTN_D(attn_q4_weights_kernel, key_blocks, kWaves * 64);
 #undef ZQ_ATTN_D
-    return hipSuccess;
+    if (!a.lse) return hipSuccess;
+#define ZQ_ATTN_W(DD)                                                                                              \
+    do {                                                                                                           \
+        const dim3 grid{uint32_t(key_blocks)};                                                                     \
+        if (pass)                                                                                                  \
+            hipLaunchKernelGGL((attn_q4_weights_kernel<DD, 2>), grid, dim3(512), Wgt<DD>::lds(2), stream, a,       \
+                               uint32_t(wblocks));                                                                 \
+        else                                                                                                       \
+            hipLaunchKernelGGL((attn_q4_weights_kernel<DD, 1>), grid, dim3(256), Wgt<DD>::lds(1), stream, a,       \
+                               uint32_t(wblocks));                                                                 \
+    } while (0)
+    if (c.head_dim == 64) ZQ_ATTN_W(64);
+    else if (c.head_dim == 128) ZQ_ATTN_W(128);
+    else ZQ_ATTN_W(256);
+#undef ZQ_ATTN_W
+    return hipGetLastError();
 }
 
 }  // namespace zq

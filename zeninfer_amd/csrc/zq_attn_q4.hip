@@ -60,10 +60,23 @@ __device__ __forceinline__ uint32_t visible(const AttnQ4& a, const Seq& x, uint3
     return a.full ? x.len : uint32_t(min(uint64_t(x.len) + t + 1, uint64_t(a.c.capacity)));
 }
 
-// A weight as two fp16 parts; the second is rounded by the instruction that forms it.
-__device__ __forceinline__ void split_p(float p, h8_t& h, h8_t& l, int i) {
-    h[i] = _Float16(p);
-    l[i] = _Float16(fmaf(float(h[i]), -1.0f, p));
+// A weight as two fp16 parts.  unit is 1.0f in a register (unit_factor()): with a
+// factor that the compiler does not know, the difference and its rounding are one
+// v_fma_mix instruction.
+__device__ __forceinline__ float unit_factor() {
+    float x = 1.0f;
+    asm("" : "+v"(x));
+    return x;
+}
+// (two at a time: the packed conversion's result is what the differences read)
+__device__ __forceinline__ void split_p2(float p0, float p1, float unit, h8_t& h, h8_t& l, int i) {
+    uint32_t u = __builtin_bit_cast(uint32_t, h2_t{_Float16(p0), _Float16(p1)});
+    asm("" : "+v"(u));
+    const h2_t x = __builtin_bit_cast(h2_t, u);
+    h[i] = x.x;
+    h[i + 1] = x.y;
+    l[i] = _Float16(fmaf(p0, unit, -float(x.x)));
+    l[i + 1] = _Float16(fmaf(p1, unit, -float(x.y)));
 }
 __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ __forceinline__ float max_groups(float v) {  // over the four lanes that share lane & 15
@@ -102,8 +115,8 @@ __device__ __forceinline__ h8_t dequant8(uint32_t w, h2_t d, uint32_t one) {
 
 template <int D>
 struct KTile {  // a wave's part of 32 keys
-    static constexpr int KB = D / 8;   // bytes of a row that a lane takes (2 steps a dword... one a dword)
-    static constexpr int KW = KB / 4;  // dwords, = MFMA steps
+    static constexpr int KB = D / 8;   // bytes of a row that a lane takes
+    static constexpr int KW = KB / 4;  // dwords, one an MFMA step
     static constexpr int NS = KB > 16 ? KB / 16 : 1;  // scales of a lane's part
     uint32_t w[2][KW];
     uint16_t sc[2][NS];
@@ -116,14 +129,17 @@ struct VTile {
     h8_t sc;  // of the 8 keys
 };
 
+// (a base that is one for the wave, and 32-bit offsets of the lane)
 template <int D>
 __device__ __forceinline__ void load_k(KTile<D>& t, const AttnQ4& a, uint32_t head, uint32_t key0, int i, int g) {
     using K = KTile<D>;
     const size_t cap = a.c.capacity;
+    const uint8_t* w = a.c.k + (size_t(head) * cap + key0) * (D / 2);
+    const uint8_t* d = reinterpret_cast<const uint8_t*>(a.c.k_scale + size_t(head) * (D / 32) * cap + key0);
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-        const uint32_t key = key0 + 8 * (i >> 2) + 4 * u + (i & 3);
-        const uint8_t* p = a.c.k + (size_t(head) * cap + key) * (D / 2) + g * K::KB;
+        const uint32_t key = uint32_t(8 * (i >> 2) + 4 * u + (i & 3));
+        const uint8_t* p = w + (key * (D / 2) + uint32_t(g * K::KB));
         if constexpr (K::KB == 8) {
             const uint2 x = *reinterpret_cast<const uint2*>(p);
             t.w[u][0] = x.x;
@@ -140,25 +156,29 @@ __device__ __forceinline__ void load_k(KTile<D>& t, const AttnQ4& a, uint32_t he
         }
 #pragma unroll
         for (int j = 0; j < K::NS; ++j)
-            t.sc[u][j] = a.c.k_scale[(size_t(head) * (D / 32) + (g * K::KB) / 16 + j) * cap + key];
+            t.sc[u][j] = *reinterpret_cast<const uint16_t*>(
+                d + (uint32_t((g * K::KB) / 16 + j) * uint32_t(cap) + key) * 2u);
     }
 }
 template <int D>
 __device__ __forceinline__ void load_v(VTile<D>& t, const AttnQ4& a, uint32_t head, uint32_t key0, int i, int g) {
     using V = VTile<D>;
     const size_t cap = a.c.capacity;
-    const uint8_t* p = a.c.v + (size_t(head) * cap + key0 + 8 * g) * (D / 2) + i * V::VB;
+    const uint8_t* w = a.c.v + (size_t(head) * cap + key0) * (D / 2);
+    const uint8_t* d = reinterpret_cast<const uint8_t*>(a.c.v_scale + size_t(head) * (D / 32) * cap + key0);
+    const uint32_t off = uint32_t(8 * g * (D / 2) + i * V::VB);
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
-        if constexpr (V::VB == 2) t.w[k][0] = *reinterpret_cast<const uint16_t*>(p + k * (D / 2));
-        else if constexpr (V::VB == 4) t.w[k][0] = *reinterpret_cast<const uint32_t*>(p + k * (D / 2));
+        const uint8_t* p = w + off + uint32_t(k * (D / 2));
+        if constexpr (V::VB == 2) t.w[k][0] = *reinterpret_cast<const uint16_t*>(p);
+        else if constexpr (V::VB == 4) t.w[k][0] = *reinterpret_cast<const uint32_t*>(p);
         else {
-            const uint2 x = *reinterpret_cast<const uint2*>(p + k * (D / 2));
+            const uint2 x = *reinterpret_cast<const uint2*>(p);
             t.w[k][0] = x.x;
             t.w[k][1] = x.y;
         }
     }
-    t.sc = *reinterpret_cast<const h8_t*>(a.c.v_scale + (size_t(head) * (D / 32) + (i * V::VB) / 16) * cap + key0 + 8 * g);
+    t.sc = *reinterpret_cast<const h8_t*>(d + (uint32_t((i * V::VB) / 16) * uint32_t(cap) + uint32_t(8 * g)) * 2u);
 }
 // scores of 32 keys and 16 rows: s[4 u + r] = row i, key 8 g + 4 u + r
 template <int D>
@@ -231,7 +251,7 @@ __device__ __forceinline__ Cut cut_of(const AttnQ4& a, const Seq& x, uint32_t r0
 }
 
 template <int D>
-__global__ __launch_bounds__(kWaves * 64) void attn_q4_few_kernel(AttnQ4 a) {
+__global__ __launch_bounds__(kWaves * 64, D == 64 ? 4 : D == 128 ? 3 : 2) void attn_q4_few_kernel(AttnQ4 a) {
     constexpr int NT = D / 16;  // 16-row O^T tiles
     using V = VTile<D>;
     __shared__ float so[kWaves][NT * 4][64];
@@ -244,38 +264,39 @@ __global__ __launch_bounds__(kWaves * 64) void attn_q4_few_kernel(AttnQ4 a) {
     if (r0 >= x.live * a.G) return;
     const Cut cut = cut_of(a, x, r0);
     if (sp >= cut.used) return;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, g = lane >> 4;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane & 15, g = lane >> 4;
     const uint32_t r = r0 + i;
     const bool ok = r < x.live * a.G;
     const uint32_t lim = ok ? visible(a, x, r / a.G) : 0;
     // tiles below it need no mask: every live row sees them
     const uint32_t whole = visible(a, x, r0 / a.G) / 32;
 
+    const uint32_t t1 = min((sp + 1) * cut.per, cut.tiles);
+    uint32_t t = sp * cut.per + wave;
+    // The next tile is loaded as soon as this one's registers are free, K and V apart.
+    // Loads past the last tile repeat it: with a branch around them the compiler would
+    // have to wait for all that are under way.
+    KTile<D> kt;
+    VTile<D> vt;
+    auto key_of = [&](uint32_t tile) { return min(tile, t1 - 1) * 32; };
+    if (t < t1) {
+        load_k<D>(kt, a, head, t * 32, i, g);
+        load_v<D>(vt, a, head, t * 32, i, g);
+    }
     const uint32_t one = code_bits();
+    const float unit = unit_factor();
     h8_t qh[D / 32], ql[D / 32];
     const float c = load_q<D>(a, x, r, ok, g, qh, ql);
     v4f_t o[NT];
 #pragma unroll
     for (int n = 0; n < NT; ++n) o[n] = v4f_t{0, 0, 0, 0};
     float m = -INFINITY, l = 0.0f;
-
-    const uint32_t t1 = min((sp + 1) * cut.per, cut.tiles);
-    uint32_t t = sp * cut.per + wave;
-    KTile<D> kt;
-    VTile<D> vt;
-    if (t < t1) {
-        load_k<D>(kt, a, head, t * 32, i, g);
-        load_v<D>(vt, a, head, t * 32, i, g);
-    }
     for (; t < t1; t += kWaves) {
         float s[8];
         scores<D>(kt, qh, ql, one, s);
-        const VTile<D> vn = vt;
-        if (t + kWaves < t1) {
-            load_k<D>(kt, a, head, (t + kWaves) * 32, i, g);
-            load_v<D>(vt, a, head, (t + kWaves) * 32, i, g);
-        }
-        h8_t vsc = vn.sc;
+        __builtin_amdgcn_sched_barrier(0);
+        load_k<D>(kt, a, head, key_of(t + kWaves), i, g);
+        h8_t vsc = vt.sc;
         if (t >= whole) {
             const uint32_t key = t * 32 + 8 * g;
 #pragma unroll
@@ -296,10 +317,10 @@ __global__ __launch_bounds__(kWaves * 64) void attn_q4_few_kernel(AttnQ4 a) {
         const float ms = (m == -INFINITY ? 0.0f : m) - kShift;
         h8_t ph, pl;
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            const float p = exp2_(fmaf(s[k], c, -ms));
-            l += p;
-            split_p(p, ph, pl, k);
+        for (int k = 0; k < 8; k += 2) {
+            const float p0 = exp2_(fmaf(s[k], c, -ms)), p1 = exp2_(fmaf(s[k + 1], c, -ms));
+            l += p0 + p1;
+            split_p2(p0, p1, unit, ph, pl, k);
         }
         h2_t d[4];
 #pragma unroll
@@ -310,7 +331,7 @@ __global__ __launch_bounds__(kWaves * 64) void attn_q4_few_kernel(AttnQ4 a) {
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
                 const uint32_t sel = 0x0c000c00u | uint32_t((4 + (y & 3)) << 16) | uint32_t(y & 3);
-                const uint32_t u = __builtin_amdgcn_perm(vn.w[2 * k + 1][y / 4], vn.w[2 * k][y / 4], sel);
+                const uint32_t u = __builtin_amdgcn_perm(vt.w[2 * k + 1][y / 4], vt.w[2 * k][y / 4], sel);
                 const h2_t a0 = nibbles2(u, one) * d[k], a1 = nibbles2(u >> 4, one) * d[k];
                 lo[2 * k] = a0.x;
                 lo[2 * k + 1] = a0.y;
@@ -322,6 +343,8 @@ __global__ __launch_bounds__(kWaves * 64) void attn_q4_few_kernel(AttnQ4 a) {
             o[2 * y + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi, ph, o[2 * y + 1], 0, 0, 0);
             o[2 * y + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi, pl, o[2 * y + 1], 0, 0, 0);
         }
+        __builtin_amdgcn_sched_barrier(0);
+        load_v<D>(vt, a, head, key_of(t + kWaves), i, g);
     }
     // ---- the four waves' sums as one ----
     l = sum_groups(l);
@@ -432,8 +455,11 @@ template <int D>
 __device__ __forceinline__ void load_kstage(KStage<D>& r, const AttnQ4& a, uint32_t head, uint32_t key0, int e) {
     const size_t cap = a.c.capacity;
     const int key = e / (D / 32), b = e % (D / 32);
-    r.w = *reinterpret_cast<const uint4*>(a.c.k + (size_t(head) * cap + key0 + key) * (D / 2) + b * 16);
-    r.d = __builtin_bit_cast(_Float16, a.c.k_scale[(size_t(head) * (D / 32) + b) * cap + key0 + key]);
+    // a base that is one for the wave, and 32-bit offsets of the lane
+    const uint8_t* w = a.c.k + (size_t(head) * cap + key0) * (D / 2);
+    const uint8_t* d = reinterpret_cast<const uint8_t*>(a.c.k_scale + size_t(head) * (D / 32) * cap + key0);
+    r.w = *reinterpret_cast<const uint4*>(w + uint32_t(key * (D / 2) + b * 16));
+    r.d = *reinterpret_cast<const _Float16*>(d + (uint32_t(b) * uint32_t(cap) + uint32_t(key)) * 2u);
 }
 template <int D>
 __device__ __forceinline__ void store_kstage(const KStage<D>& r, _Float16* kt, uint32_t one, int e) {
@@ -449,17 +475,20 @@ template <int D>
 __device__ __forceinline__ void load_vstage(VStage<D>& r, const AttnQ4& a, uint32_t head, uint32_t key0, int e) {
     const size_t cap = a.c.capacity;
     const int ch = (e >> 1) % (D / 4), o = (e & 1) + 2 * (e / (D / 2));
-    const uint8_t* p = a.c.v + (size_t(head) * cap + key0 + 8 * o) * (D / 2) + 2 * ch;
+    const uint8_t* w = a.c.v + (size_t(head) * cap + key0) * (D / 2);
+    const uint8_t* d = reinterpret_cast<const uint8_t*>(a.c.v_scale + size_t(head) * (D / 32) * cap + key0);
+    const uint32_t off = uint32_t(8 * o * (D / 2) + 2 * ch);
 #pragma unroll
-    for (int k = 0; k < 8; ++k) r.w[k] = *reinterpret_cast<const uint16_t*>(p + k * (D / 2));
-    r.d = *reinterpret_cast<const h8_t*>(a.c.v_scale + (size_t(head) * (D / 32) + ch / 8) * cap + key0 + 8 * o);
+    for (int k = 0; k < 8; ++k) r.w[k] = *reinterpret_cast<const uint16_t*>(w + off + uint32_t(k * (D / 2)));
+    r.d = *reinterpret_cast<const h8_t*>(d + (uint32_t(ch / 8) * uint32_t(cap) + uint32_t(8 * o)) * 2u);
 }
-// keys: how many of the step hold rows that are seen (the others' scale may be any bits)
-template <int D>
+// MASK: only `keys` of the step's keys hold rows that are seen (the others' scale may be
+// any bits)
+template <int D, bool MASK>
 __device__ __forceinline__ void store_vstage(const VStage<D>& r, _Float16* vt, uint32_t keys, uint32_t one, int e) {
     const int ch = (e >> 1) % (D / 4), o = (e & 1) + 2 * (e / (D / 2));
     h8_t s = r.d;
-    if (keys < uint32_t(Big<D>::TK))
+    if (MASK)
 #pragma unroll
         for (int k = 0; k < 8; ++k) s[k] = uint32_t(8 * o + k) < keys ? s[k] : _Float16(0);
     const int dim = ch / 8 * 32 + 2 * (ch % 8);
@@ -557,7 +586,7 @@ __global__ __launch_bounds__(Big<D>::T) void attn_q4_many_kernel(AttnQ4 a) {
     if (r0 >= rows) return;
     const Cut cut = big_cut(a, x, r0, B::TK);
     if (sp >= cut.used) return;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l32 = lane & 31, lh = lane >> 5;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l32 = lane & 31, lh = lane >> 5;
     const int kg = B::KG == 2 ? wave >> 2 : 0;
     const uint32_t rw = r0 + 32 * (wave & 3), r = rw + l32;
     const bool ok = r < rows;
@@ -572,10 +601,9 @@ __global__ __launch_bounds__(Big<D>::T) void attn_q4_many_kernel(AttnQ4 a) {
     // K by the first 256 threads, V by the others (by the same ones where there are no others)
     const int e = tid & 255;
     const bool kr = (B::KG == 1 || tid < 256) && e < B::kTasks, vr = (B::KG == 1 || tid >= 256) && e < B::kTasks;
+    const int em = min(e, B::kTasks - 1);  // a thread without a task loads the last one's
     const uint32_t one = code_bits();
-    auto put_v = [&](const VStage<D>& s, uint32_t t) {
-        store_vstage<D>(s, vbuf + (t & 1) * B::kV, min(cut.keys - t * B::TK, uint32_t(B::TK)), one, e);
-    };
+    const float unit = unit_factor();
     KStage<D> ks;
     VStage<D> vs;
     if (t0 < t1) {
@@ -611,7 +639,7 @@ __global__ __launch_bounds__(Big<D>::T) void attn_q4_many_kernel(AttnQ4 a) {
                 store_kstage<D>(ks, kbuf + ((t0 + 1) & 1) * B::kK, one, e);
             }
         }
-        if (vr) put_v(vs, t0);
+        if (vr) store_vstage<D, true>(vs, vbuf + (t0 & 1) * B::kV, cut.keys - t0 * B::TK, one, e);
     }
     __syncthreads();
     // this lane's part of a K row: bits 2 and 3 of the row exchanged
@@ -631,55 +659,86 @@ __global__ __launch_bounds__(Big<D>::T) void attn_q4_many_kernel(AttnQ4 a) {
         return y;
     };
     if (t0 < t1) s = product(t0);
-    // Step t: the weights of its scores and, between their instructions, the next
-    // step's scores; then the second product.  K is decoded two steps ahead and V one.
-    for (uint32_t t = t0; t < t1; ++t) {
+    // Step t: the weights of its scores, the next step's scores, the second product and
+    // the decoding of later keys (K two steps ahead, V one) stand in one run of code,
+    // whose vector and matrix instructions the compiler mixes.  Past the last step the
+    // last one is loaded and decoded again, for nothing.
+    auto fetch = [&](uint32_t t, auto k_role, auto v_role) {  // what step t decodes
+        if constexpr (decltype(k_role)::value) load_kstage<D>(ks, a, head, min(t + 2, t1 - 1) * B::TK, em);
+        if constexpr (decltype(v_role)::value) load_vstage<D>(vs, a, head, min(t + 1, t1 - 1) * B::TK, em);
+    };
+    auto step = [&](uint32_t t, auto k_role, auto v_role, auto last) {
         __syncthreads();  // K of t + 1 and V of t are written, K of t and V of t - 1 are read no more
-        if (kr && t + 2 < t1) load_kstage<D>(ks, a, head, (t + 2) * B::TK, e);
-        if (vr && t + 1 < t1) load_vstage<D>(vs, a, head, (t + 1) * B::TK, e);
+        auto decode = [&] {
+            if (B::kTasks == 256 || e < B::kTasks) {
+                if constexpr (decltype(k_role)::value) store_kstage<D>(ks, kbuf + (t & 1) * B::kK, one, e);
+                if constexpr (decltype(v_role)::value)
+                    store_vstage<D, decltype(last)::value>(vs, vbuf + ((t + 1) & 1) * B::kV,
+                                                           cut.keys - min(t + 1, t1 - 1) * B::TK, one, e);
+            }
+            fetch(t + 1, k_role, v_role);
+        };
         const uint32_t key0 = t * B::TK + 32 * kg;
-        if (key0 < most) {  // uniform in the wave, and for no later step where it is not
-            if (key0 + 32 > whole) {
-#pragma unroll
-                for (int v = 0; v < 16; ++v) s[v] = key0 + 16 * (v >> 3) + 8 * lh + (v & 7) < lim ? s[v] : -INFINITY;
-            }
-            float mx = s[0];
-#pragma unroll
-            for (int v = 1; v < 16; ++v) mx = fmaxf(mx, s[v]);
-            mx *= c;
-            if (__any(mx > m + kSlack)) {
-                const float mn = fmaxf(m, fmaxf(mx, __shfl_xor(mx, 32)));
-                const float f = exp2_(m - (mn == -INFINITY ? 0.0f : mn));
-                m = mn;
-                l *= f;
-#pragma unroll
-                for (int n = 0; n < B::NT; ++n)
-#pragma unroll
-                    for (int v = 0; v < 16; ++v) o[n][v] *= f;
-            }
-            const float ms = (m == -INFINITY ? 0.0f : m) - kShift;
-            // (of a step past the last one: what the buffer holds, not used)
-            const v16f_t next = product(t + 1);
-            h8_t ph[2], pl[2];
-#pragma unroll
-            for (int v = 0; v < 16; ++v) {
-                const float p = exp2_(fmaf(s[v], c, -ms));
-                l += p;
-                split_p(p, ph[v >> 3], pl[v >> 3], v & 7);
-            }
-            s = next;
-            const _Float16* vt = vbuf + (t & 1) * B::kV + voff;
-#pragma unroll
-            for (int u = 0; u < 2; ++u)
-#pragma unroll
-                for (int n = 0; n < B::NT; ++n) {
-                    const h8_t v = *reinterpret_cast<const h8_t*>(vt + 32 * n * B::KP + 16 * u);
-                    o[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, ph[u], o[n], 0, 0, 0);
-                    o[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, pl[u], o[n], 0, 0, 0);
-                }
+        if (key0 >= most) {  // uniform in the wave, and so for every later step
+            decode();
+            asm volatile("s_nop 0");  // else the two copies of decode() become one, behind the matrix instructions
+            return;
         }
-        if (kr && t + 2 < t1) store_kstage<D>(ks, kbuf + (t & 1) * B::kK, one, e);
-        if (vr && t + 1 < t1) put_v(vs, t + 1);
+        if (key0 + 32 > whole) {
+#pragma unroll
+            for (int v = 0; v < 16; ++v) s[v] = key0 + 16 * (v >> 3) + 8 * lh + (v & 7) < lim ? s[v] : -INFINITY;
+        }
+        float mx = s[0];
+#pragma unroll
+        for (int v = 1; v < 16; ++v) mx = fmaxf(mx, s[v]);
+        mx *= c;
+        if (__any(mx > m + kSlack)) {
+            const float mn = fmaxf(m, fmaxf(mx, __shfl_xor(mx, 32)));
+            const float f = exp2_(m - (mn == -INFINITY ? 0.0f : mn));
+            m = mn;
+            l *= f;
+#pragma unroll
+            for (int n = 0; n < B::NT; ++n)
+#pragma unroll
+                for (int v = 0; v < 16; ++v) o[n][v] *= f;
+        }
+        const float ms = (m == -INFINITY ? 0.0f : m) - kShift;
+        const v16f_t next = product(t + 1);
+        h8_t ph[2], pl[2];
+#pragma unroll
+        for (int v = 0; v < 16; v += 2) {
+            const float p0 = exp2_(fmaf(s[v], c, -ms)), p1 = exp2_(fmaf(s[v + 1], c, -ms));
+            l += p0 + p1;
+            split_p2(p0, p1, unit, ph[v >> 3], pl[v >> 3], v & 7);
+        }
+        s = next;
+        const _Float16* vt = vbuf + (t & 1) * B::kV + voff;
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int n = 0; n < B::NT; ++n) {
+                const h8_t v = *reinterpret_cast<const h8_t*>(vt + 32 * n * B::KP + 16 * u);
+                o[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, ph[u], o[n], 0, 0, 0);
+                o[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, pl[u], o[n], 0, 0, 0);
+            }
+        // the last two steps' masked decoding stays apart: mixed in, it costs more registers than there are
+        if constexpr (decltype(last)::value) __builtin_amdgcn_sched_barrier(0);
+        decode();
+    };
+    using yes = std::true_type;
+    using no = std::false_type;
+    uint32_t t = t0;
+    if constexpr (B::KG == 1) {
+        if (t < t1) fetch(t, yes{}, yes{});
+        for (; t + 2 < t1; ++t) step(t, yes{}, yes{}, no{});
+        for (; t < t1; ++t) step(t, yes{}, yes{}, yes{});
+    } else if (tid < 256) {
+        if (t < t1) fetch(t, yes{}, no{});
+        for (; t < t1; ++t) step(t, yes{}, no{}, no{});
+    } else {
+        if (t < t1) fetch(t, no{}, yes{});
+        for (; t + 2 < t1; ++t) step(t, no{}, yes{}, no{});
+        for (; t < t1; ++t) step(t, no{}, yes{}, yes{});
     }
     // ---- the two key halves of a row as one ----
     l += __shfl_xor(l, 32);
@@ -730,41 +789,61 @@ __global__ __launch_bounds__(Big<D>::T) void attn_q4_many_kernel(AttnQ4 a) {
                 make_float4(o[n][4 * j] * inv, o[n][4 * j + 1] * inv, o[n][4 * j + 2] * inv, o[n][4 * j + 3] * inv);
 }
 
-// One wave a row: the splits' partial outputs as one.  Splits are few (at most
-// 128), their maxima and sums are held by the lanes.
+// The splits' partial outputs of a row as one, by a workgroup: D / 4 lanes take a
+// split's output, so 1024 / D splits are read at a time.
 template <int D>
 __global__ __launch_bounds__(256) void attn_q4_combine_kernel(AttnQ4 a) {
-    const uint32_t id = blockIdx.x * 4 + (threadIdx.x >> 6);
-    const int lane = threadIdx.x & 63;
-    const uint32_t head = id / a.rows, r = id % a.rows;
-    if (head >= a.heads_kv) return;
+    constexpr int RL = D / 4, P = 256 / RL;
+    __shared__ float wgt[128];
+    __shared__ float4 sum[P][RL];
+    const uint32_t head = blockIdx.x / a.rows, r = blockIdx.x % a.rows;
     const Seq x = seq_of(a, head);
     if (r >= x.live * a.G) return;
     const Cut cut = a.many ? big_cut(a, x, r / kTileRows * kTileRows, Big<D>::TK) : cut_of(a, x, r / 16 * 16);
     if (cut.used == 1) return;  // written by the split itself
+    const int tid = threadIdx.x, lane = tid & 63;
     const size_t row = size_t(head) * a.rows + r;
+    // every wave finds the maximum and the sum of them all (at most 128 splits)
     const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + row * a.splits;
     const float2 none = make_float2(-INFINITY, 0.0f);
     const float2 p0 = uint32_t(lane) < cut.used ? ml[lane] : none;
     const float2 p1 = uint32_t(lane) + 64 < cut.used ? ml[lane + 64] : none;
+    const uint32_t p = uint32_t(tid) / RL, l = uint32_t(tid) % RL;
+    const float4* part = reinterpret_cast<const float4*>(a.part + row * a.splits * D) + l;
+    constexpr int N = 4;  // splits that a lane has on the way
+    float4 v[N];
+#pragma unroll
+    for (int j = 0; j < N; ++j) v[j] = p + j * P < cut.used ? part[size_t(p + j * P) * RL] : make_float4(0, 0, 0, 0);
     const float M = wave_max(fmaxf(p0.x, p1.x)), Ms = M == -INFINITY ? 0.0f : M;
     const float w0 = exp2_(p0.x - Ms), w1 = exp2_(p1.x - Ms);
     const float L = wave_sum(p0.y * w0 + p1.y * w1);
-    constexpr int E = D / 64;
-    const float* part = a.part + row * a.splits * D + lane * E;
-    float acc[E];
+    if (tid < 64) {
+        wgt[lane] = w0;
+        wgt[lane + 64] = w1;
+    }
+    __syncthreads();
+    float4 acc = make_float4(0, 0, 0, 0);
+    for (uint32_t j0 = p; j0 < cut.used; j0 += N * P) {
 #pragma unroll
-    for (int e = 0; e < E; ++e) acc[e] = 0.0f;
-    for (uint32_t j = 0; j < cut.used; ++j) {
-        const float w = j < 64 ? __shfl(w0, int(j)) : __shfl(w1, int(j - 64));
+        for (int j = 0; j < N; ++j) {
+            const float w = j0 + j * P < cut.used ? wgt[j0 + j * P] : 0.0f;
+            acc = make_float4(fmaf(v[j].x, w, acc.x), fmaf(v[j].y, w, acc.y), fmaf(v[j].z, w, acc.z), fmaf(v[j].w, w, acc.w));
+            const uint32_t n = j0 + (N + j) * P;
+            if (n < cut.used) v[j] = part[size_t(n) * RL];
+        }
+    }
+    sum[p][l] = acc;
+    __syncthreads();
+    if (tid >= RL) return;
 #pragma unroll
-        for (int e = 0; e < E; ++e) acc[e] = fmaf(part[size_t(j) * D + e], w, acc[e]);
+    for (int j = 1; j < P; ++j) {
+        const float4 t = sum[j][l];
+        acc = make_float4(acc.x + t.x, acc.y + t.y, acc.z + t.z, acc.w + t.w);
     }
     const float inv = L > 0.0f ? 1.0f / L : (L == 0.0f ? 0.0f : L);
-    float* dst = a.out + ((size_t(x.s) * a.tokens + r / a.G) * a.KH * a.G + x.kh * a.G + r % a.G) * D + lane * E;
-#pragma unroll
-    for (int e = 0; e < E; ++e) dst[e] = acc[e] * inv;
-    if (a.lse && lane == 0) a.lse[row] = M - kShift + log2f(L);
+    reinterpret_cast<float4*>(a.out + ((size_t(x.s) * a.tokens + r / a.G) * a.KH * a.G + x.kh * a.G + r % a.G) * D)[l] =
+        make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+    if (a.lse && tid == 0) a.lse[row] = M - kShift + log2f(L);
 }
 
 // ---- the rows' weights ----------------------------------------------------------
@@ -797,7 +876,7 @@ __global__ __launch_bounds__(256 * RH) void attn_q4_weights_kernel(AttnQ4 a, uin
     const uint32_t rows = x.live * a.G, keys = visible(a, x, x.live - 1);
     const uint32_t nb = (keys + 255) / 256;
     if (first >= nb) return;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l32 = lane & 31, lh = lane >> 5;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l32 = lane & 31, lh = lane >> 5;
     const int kg = wave & 3, rh = wave >> 2;
     const uint32_t one = code_bits();
     const size_t cap = a.c.capacity;
@@ -932,7 +1011,9 @@ Plan plan_of(const zq_kv_q4& c, size_t rows) {
     p.many = rows > 64;
     const size_t tile = p.many ? kTileRows : 16;
     const size_t base = c.seqs * c.kv_heads * ((rows + tile - 1) / tile);
-    const size_t want = (size_t(device_cu_count()) * (p.many ? 1 : 3) + base - 1) / base;
+    // few rows: three workgroups a CU; where there are as many sequences and heads as CUs, six, so that their
+    // lengths even out (64 sequences of up to 8190 rows: 1 split 76, 2 70, 3 60, 4 63, 6 65 us)
+    const size_t cus = size_t(device_cu_count()), want = (cus * (p.many ? 1 : base < cus ? 3 : 6) + base - 1) / base;
     const size_t most = p.many ? (c.capacity + 511) / 512 : (c.capacity / 32 + kWaves - 1) / kWaves;
     p.splits = uint32_t(std::max<size_t>(1, std::min<size_t>({want, most, 128})));
     return p;
@@ -1008,7 +1089,7 @@ hipError_t launch_attention_q4(const zq_kv_q4& c, const float* q, float* out, si
     } else {
         ZQ_ATTN_D(attn_q4_few_kernel, blocks, kWaves * 64);
     }
-    if (a.splits > 1) ZQ_ATTN_D(attn_q4_combine_kernel, (all + 3) / 4, 256);
+    if (a.splits > 1) ZQ_ATTN_D(attn_q4_combine_kernel, all, 256);
 #undef ZQ_ATTN_D
     if (!a.lse) return hipSuccess;
 #define ZQ_ATTN_W(DD)                                                                                              \

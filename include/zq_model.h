@@ -21,6 +21,7 @@
 #include <stdint.h>
 
 #include "zq_gguf.h"
+#include "zq_kv.h"
 
 #ifdef __cplusplus
 extern "C" {
@@ -64,6 +65,25 @@ int zq_model_load_gguf(const zq_gguf* gguf, uint32_t max_positions, zq_model_con
 int zq_model_create_synthetic(const zq_model_config* cfg, uint64_t seed, zq_model** model, char* err, size_t err_cap);
 void zq_model_free(zq_model* model);
 int zq_model_set_prefill_mode(zq_model* model, int mode);
+/* The KV cache's form; the cache starts empty (prefill comes next).  A model is
+ * loaded with ZQ_KV_F32: max_positions rows of fp32 a layer.  No counterpart in
+ * the reference, whose cache is fp32.
+ * ZQ_KV_Q4: rows held as Q4_0 values (zq_kv.h), 4.5 bits an element.  rows == 0:
+ * max_positions rows a layer.  Otherwise the attention weight that rows draw is
+ * added up, and whenever the next tokens do not fit, every layer and kv head
+ * keeps `rows` rows by zq_hip_kv_q4_evict_dev's rule (the `recent` newest
+ * positions, the `first` first ones, then those of the largest weight); the cache
+ * has room for a prefill pass (up to 1024 tokens) beside them, so generation may
+ * run to max_positions on less memory.  first + recent <= rows.  ZQ_KV_F32 takes
+ * rows = recent = first = 0.  On failure (ZQ_ERR_ARG, ZQ_ERR_OOM) the model keeps
+ * the cache it had. */
+#define ZQ_KV_F32 0
+#define ZQ_KV_Q4 1
+int zq_model_set_kv_cache(zq_model* model, int form, uint32_t rows, uint32_t recent, uint32_t first);
+/* One layer's 4-bit cache (seqs = 1; device arrays that the model owns) for the
+ * calls of zq_kv.h, the rows it holds and the positions fed so far.  ZQ_DECLINED
+ * with the fp32 cache (rows and positions are set). */
+int zq_model_kv_cache(const zq_model* model, uint32_t layer, zq_kv_q4* cache, uint32_t* rows, uint32_t* positions);
 /* Prefill `n` tokens from position 0 (the cache is reset).  Logits of the
  * last token to `logits` (vocab floats, may be NULL); greedy id to *next. */
 int zq_model_prefill(zq_model* model, const uint32_t* tokens, size_t n, float* logits, uint32_t* next);

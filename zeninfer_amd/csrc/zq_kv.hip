@@ -67,13 +67,47 @@ __device__ __forceinline__ Q4Block quantize_block(float4 x, bool poison, bool is
     return b;
 }
 
+// Four elements of a row's key and value, by the D / 4 lanes of a row, into `slot`
+// (every lane of the wave takes part; a row with live = false writes nothing).
+template <int D>
+__device__ __forceinline__ void append_row(const zq_kv_q4& c, size_t head, size_t slot, float4 kx, float4 vx, int32_t pos,
+                                           bool live) {
+    constexpr uint32_t RL = D / 4;  // lanes of a row
+    const uint32_t l = threadIdx.x % RL;
+    auto odd = [](float4 x) {  // any exponent of all ones: NaN or infinity
+        const uint32_t e = 0x7f800000u;
+        return (__float_as_uint(x.x) & e) == e || (__float_as_uint(x.y) & e) == e || (__float_as_uint(x.z) & e) == e ||
+               (__float_as_uint(x.w) & e) == e;
+    };
+    const uint64_t bad = __ballot(odd(kx) || odd(vx));
+    const uint32_t row0 = (threadIdx.x & 63u) / RL * RL;  // first lane of this row in the wave
+    const bool poison = ((bad >> row0) & (RL == 64 ? ~uint64_t(0) : (uint64_t(1) << (RL & 63u)) - 1)) != 0;
+    const Q4Block bk = quantize_block(kx, poison, true);
+    const Q4Block bv = quantize_block(vx, poison, false);
+    if (!live) return;
+    const size_t at = head * c.capacity + slot;
+    const uint32_t b = l / 8, l8 = l % 8;
+    if (l8 < 4) {
+        *reinterpret_cast<uint32_t*>(c.k + at * (D / 2) + b * 16 + l8 * 4) = bk.codes;
+        *reinterpret_cast<uint32_t*>(c.v + at * (D / 2) + b * 16 + l8 * 4) = bv.codes;
+    } else if (l8 == 4) {
+        const size_t sc = (head * (D / 32) + b) * c.capacity + slot;
+        c.k_scale[sc] = bk.scale;
+        c.v_scale[sc] = bv.scale;
+    }
+    if (l == 0) {
+        if (c.weight) c.weight[at] = 0.0f;
+        if (c.pos) c.pos[at] = pos;
+    }
+}
+
 template <int D>
 __global__ __launch_bounds__(kT) void kv_q4_append_kernel(const float* __restrict__ k, const float* __restrict__ v,
                                                           zq_kv_q4 c, uint32_t tokens, size_t stride,
                                                           const int32_t* __restrict__ lens,
                                                           const int32_t* __restrict__ counts,
                                                           const int32_t* __restrict__ first_pos, uint32_t rows) {
-    constexpr uint32_t RL = D / 4;  // lanes of a row
+    constexpr uint32_t RL = D / 4;
     const uint32_t KH = uint32_t(c.kv_heads);
     const uint32_t id = blockIdx.x * (kT / RL) + threadIdx.x / RL, l = threadIdx.x % RL;
     const uint32_t row = min(id, rows - 1);  // every lane of a wave takes part in the block's reductions
@@ -86,31 +120,47 @@ __global__ __launch_bounds__(kT) void kv_q4_append_kernel(const float* __restric
     const float4 z = make_float4(0, 0, 0, 0);
     const float4 kx = live ? *reinterpret_cast<const float4*>(k + src) : z;
     const float4 vx = live ? *reinterpret_cast<const float4*>(v + src) : z;
-    auto odd = [](float4 x) {  // any exponent of all ones: NaN or infinity
-        const uint32_t e = 0x7f800000u;
-        return (__float_as_uint(x.x) & e) == e || (__float_as_uint(x.y) & e) == e || (__float_as_uint(x.z) & e) == e ||
-               (__float_as_uint(x.w) & e) == e;
-    };
-    const uint64_t bad = __ballot(odd(kx) || odd(vx));
-    const uint32_t row0 = (threadIdx.x & 63u) / RL * RL;  // first lane of this row in the wave
-    const bool poison = ((bad >> row0) & (RL == 64 ? ~uint64_t(0) : (uint64_t(1) << (RL & 63u)) - 1)) != 0;
-    const Q4Block bk = quantize_block(kx, poison, true);
-    const Q4Block bv = quantize_block(vx, poison, false);
-    if (!live) return;
-    const size_t head = size_t(s) * KH + kh, at = head * c.capacity + slot;
-    const uint32_t b = l / 8, l8 = l % 8;
-    if (l8 < 4) {
-        *reinterpret_cast<uint32_t*>(c.k + at * (D / 2) + b * 16 + l8 * 4) = bk.codes;
-        *reinterpret_cast<uint32_t*>(c.v + at * (D / 2) + b * 16 + l8 * 4) = bv.codes;
-    } else if (l8 == 4) {
-        const size_t sc = (head * (D / 32) + b) * c.capacity + slot;
-        c.k_scale[sc] = bk.scale;
-        c.v_scale[sc] = bv.scale;
+    append_row<D>(c, size_t(s) * KH + kh, slot, kx, vx, (first_pos ? first_pos[s] : len) + int32_t(t), live);
+}
+
+// The decoder's form: rows are the heads of a token, H query heads and then the kv
+// heads.  Pairs (2 i, 2 i + 1) of a float4 rotate by positions' factors; elements past
+// 2 * pairs are left (rope(), :317-328 of the reference runtime).
+template <int D>
+__global__ __launch_bounds__(kT) void rope_kv_q4_kernel(zq_kv_q4 c, const float* q, float* q_out,
+                                                        const float* __restrict__ k, const float* __restrict__ v,
+                                                        const float* __restrict__ cos_tab,
+                                                        const float* __restrict__ sin_tab,
+                                                        const int32_t* __restrict__ len_ptr,
+                                                        const uint32_t* __restrict__ pos_ptr, uint32_t H, uint32_t pairs,
+                                                        uint32_t ldq, uint32_t ldkv, uint32_t rows) {
+    constexpr uint32_t RL = D / 4;
+    const uint32_t heads = H + uint32_t(c.kv_heads);
+    const uint32_t id = blockIdx.x * (kT / RL) + threadIdx.x / RL, l = threadIdx.x % RL;
+    const uint32_t row = min(id, rows - 1), t = row / heads, h = row % heads;
+    const bool is_q = h < H;
+    const uint32_t kh = is_q ? 0 : h - H;
+    const int32_t len = *len_ptr;
+    const uint32_t pos = *pos_ptr + t;
+    const float4 x = is_q ? *reinterpret_cast<const float4*>(q + size_t(t) * ldq + size_t(h) * D + 4 * l)
+                          : *reinterpret_cast<const float4*>(k + size_t(t) * ldkv + size_t(kh) * D + 4 * l);
+    const float4 vx = is_q ? make_float4(0, 0, 0, 0)
+                           : *reinterpret_cast<const float4*>(v + size_t(t) * ldkv + size_t(kh) * D + 4 * l);
+    float4 y = x;
+    const uint32_t i = 2 * l;  // the float4's pairs
+    if (i < pairs) {
+        const float c0 = cos_tab[size_t(pos) * pairs + i], s0 = sin_tab[size_t(pos) * pairs + i];
+        y.x = x.x * c0 - x.y * s0;
+        y.y = x.x * s0 + x.y * c0;
     }
-    if (l == 0) {
-        if (c.weight) c.weight[at] = 0.0f;
-        if (c.pos) c.pos[at] = (first_pos ? first_pos[s] : len) + int32_t(t);
+    if (i + 1 < pairs) {
+        const float c1 = cos_tab[size_t(pos) * pairs + i + 1], s1 = sin_tab[size_t(pos) * pairs + i + 1];
+        y.z = x.z * c1 - x.w * s1;
+        y.w = x.z * s1 + x.w * c1;
     }
+    const bool live = id < rows && !is_q && len >= 0 && size_t(len) + t < c.capacity;
+    append_row<D>(c, kh, live ? size_t(len) + t : 0, y, vx, int32_t(pos), live);
+    if (id < rows && is_q) *reinterpret_cast<float4*>(q_out + (size_t(t) * H + h) * D + 4 * l) = y;
 }
 
 // ---- read ----------------------------------------------------------------------
@@ -345,6 +395,26 @@ hipError_t launch_kv_q4_append(const zq_kv_q4& c, const float* k, const float* v
                        counts, first_pos, rows)
     if (c.head_dim == 64) ZQ_KV(64);
     else if (c.head_dim == 128) ZQ_KV(128);
+    else ZQ_KV(256);
+#undef ZQ_KV
+    return hipGetLastError();
+}
+
+hipError_t launch_rope_kv_q4(const zq_kv_q4& c, const float* q, float* q_out, const float* k, const float* v,
+                             const float* cos_tab, const float* sin_tab, const int32_t* len, const uint32_t* pos,
+                             uint32_t T, uint32_t H, uint32_t pairs, uint32_t ld, hipStream_t stream) {
+    const uint32_t D = uint32_t(c.head_dim), KH = uint32_t(c.kv_heads);
+    auto a16 = [](const void* p) { return p && (reinterpret_cast<uintptr_t>(p) & 15u) == 0; };
+    if (!kv_q4_ok(&c) || c.seqs != 1 || !a16(q) || !a16(q_out) || !a16(k) || !a16(v) || !cos_tab || !sin_tab || !len ||
+        !pos || !T || !H || !pairs || pairs > D / 2 || ld % 4 || (ld && ld < (H + 2 * KH) * D))
+        return hipErrorInvalidValue;
+    const uint32_t rows = T * (H + KH), per = uint32_t(kT) / (D / 4);
+    const dim3 grid((rows + per - 1) / per);
+#define ZQ_KV(DD)                                                                                                  \
+    hipLaunchKernelGGL(rope_kv_q4_kernel<DD>, grid, dim3(kT), 0, stream, c, q, q_out, k, v, cos_tab, sin_tab, len, pos, \
+                       H, pairs, ld ? ld : H * D, ld ? ld : KH * D, rows)
+    if (D == 64) ZQ_KV(64);
+    else if (D == 128) ZQ_KV(128);
     else ZQ_KV(256);
 #undef ZQ_KV
     return hipGetLastError();

@@ -22,6 +22,12 @@ hipError_t launch_kv_q4_read(const zq_kv_q4& c, float* k, float* v, size_t token
 hipError_t launch_kv_q4_evict(const zq_kv_q4& c, const zq_kv_q4& dst, bool in_place, const int32_t* lens, size_t keep,
                               size_t recent, size_t first, const int32_t* next_pos, void* ws, hipStream_t stream);
 size_t kv_q4_evict_bytes(const zq_kv_q4& c, size_t keep);
+// RoPE (adjacent pairs) of T tokens' q into q_out ([T][H * D]) and of their k, then
+// k and v appended to one sequence's cache at slots *len on, positions *pos on.
+// q, k, v: rows ld floats apart (0: dense).
+hipError_t launch_rope_kv_q4(const zq_kv_q4& c, const float* q, float* q_out, const float* k, const float* v,
+                             const float* cos_tab, const float* sin_tab, const int32_t* len, const uint32_t* pos,
+                             uint32_t T, uint32_t H, uint32_t pairs, uint32_t ld, hipStream_t stream);
 // attention: dims of the call, the workspace it needs, the launch
 size_t attention_q4_bytes(const zq_kv_q4& c, size_t tokens, size_t heads, int flags);
 hipError_t launch_attention_q4(const zq_kv_q4& c, const float* q, float* out, size_t tokens, size_t heads, size_t stride,

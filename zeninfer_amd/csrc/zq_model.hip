@@ -23,6 +23,7 @@
 #include "../../include/zq_model.h"
 #include "zq_device.hpp"
 #include "zq_internal.hpp"
+#include "zq_kv.hpp"
 
 #include <hip/hip_runtime.h>
 
@@ -52,8 +53,9 @@ struct Layer {
     Weight q, k, v, o, gate, up, down;
     const float* attn_norm = nullptr;
     const float* ffn_norm = nullptr;
-    float* kc = nullptr;
+    float* kc = nullptr;  // fp32 cache
     float* vc = nullptr;
+    zq_kv_q4 q4{};  // 4-bit cache (k set where it is in use)
 };
 
 }  // namespace
@@ -91,7 +93,18 @@ struct zq_model {
     void* argmax_part = nullptr;
     double* ss = nullptr;  // 2 x zq::kRnSlots sum-of-squares slots of the residual-norm decode
 
-    uint32_t cur_pos = 0;  // positions held in the cache
+    uint32_t cur_pos = 0;  // positions fed so far
+    uint32_t cur_rows = 0;  // rows held in the cache: fewer where rows were evicted
+    // zq_model_set_kv_cache
+    int kv_form = ZQ_KV_F32;
+    void* kv_mem = nullptr;      // the cache's arrays (either form)
+    zq_kv_q4 kv_all{};           // all layers' 4-bit caches as sequences of one
+    uint32_t kv_keep = 0, kv_recent = 0, kv_first = 0;  // kv_keep 0: nothing is evicted
+    int32_t* kv_rows_dev = nullptr;   // [layers] rows held, then [layers] positions fed
+    int32_t* kv_rows_host = nullptr;  // pinned mirror
+    void* kv_ws = nullptr;            // attention and eviction workspace
+    size_t kv_ws_bytes = 0;
+    uint64_t kv_aux_bytes = 0;        // kv_rows_dev and kv_ws, counted as activations
     bool use_graph = true;
     bool fused = false;    // decode step with norms and SiLU folded into the GEMVs
     bool fuse_quant = true;  // prefill norms / SiLU*up also write the int8 activations; K-quant gate|up pair
@@ -111,6 +124,9 @@ struct zq_model {
         if (decode_exec) (void)hipGraphExecDestroy(decode_exec);
         if (decode_graph) (void)hipGraphDestroy(decode_graph);
         for (void* p : allocs) (void)hipFree(p);
+        for (void* p : {kv_mem, static_cast<void*>(kv_rows_dev), kv_ws})
+            if (p) (void)hipFree(p);
+        if (kv_rows_host) (void)hipHostFree(kv_rows_host);
         if (host_small) (void)hipHostFree(host_small);
         if (stream) (void)hipStreamDestroy(stream);
     }
@@ -146,6 +162,100 @@ bool dev_alloc(zq_model& m, void** p, size_t bytes) {
     if (hipMalloc(p, std::max<size_t>(bytes, 1)) != hipSuccess) return false;
     m.allocs.push_back(*p);
     return true;
+}
+
+// The fp32 KV cache: [layer][position][kv_heads * head_dim] for K and V, in place of
+// the cache there is.
+bool set_kv_f32(zq_model& m) {
+    const auto& c = m.cfg;
+    const size_t per = size_t(c.max_positions) * c.kv_heads * c.head_dim * 4;
+    void* kv = nullptr;
+    if (hipMalloc(&kv, 2 * per * c.layers) != hipSuccess) return false;
+    if (m.kv_mem) (void)hipFree(m.kv_mem);
+    m.kv_mem = kv;
+    m.kv_form = ZQ_KV_F32;
+    m.kv_keep = m.kv_recent = m.kv_first = 0;
+    m.cache_bytes = 2 * per * c.layers;
+    for (uint32_t l = 0; l < c.layers; ++l) {
+        m.layers[l].kc = reinterpret_cast<float*>(static_cast<uint8_t*>(kv) + 2 * l * per);
+        m.layers[l].vc = reinterpret_cast<float*>(static_cast<uint8_t*>(kv) + (2 * l + 1) * per);
+        m.layers[l].q4 = zq_kv_q4{};
+    }
+    return true;
+}
+
+// The 4-bit cache.  All layers' rows lie in arrays of one shape, [layer][kv head]...,
+// so that one call evicts from every layer.
+int set_kv_q4(zq_model& m, uint32_t keep, uint32_t recent, uint32_t first) {
+    const auto& c = m.cfg;
+    if (size_t(keep) + kPrefillChunk >= c.max_positions) keep = 0;  // all positions have room: nothing will be evicted
+    const size_t want = keep ? size_t(keep) + kPrefillChunk : c.max_positions;
+    const size_t cap = align_up(want, 32), L = c.layers, heads = L * c.kv_heads, D = c.head_dim;
+    const size_t codes = align_up(heads * cap * D / 2, kAlign), scales = align_up(heads * cap * D / 32 * 2, kAlign);
+    const size_t words = align_up(heads * cap * 4, kAlign);
+    const size_t total = 2 * (codes + scales) + 2 * words;
+    zq_kv_q4 all{};
+    all.seqs = L;
+    all.kv_heads = c.kv_heads;
+    all.head_dim = D;
+    all.capacity = cap;
+    uint8_t* mem = nullptr;
+    int32_t *rows = nullptr, *host = nullptr;
+    void* ws = nullptr;
+    auto fail = [&](int st) {
+        if (mem) (void)hipFree(mem);
+        if (rows) (void)hipFree(rows);
+        if (ws) (void)hipFree(ws);
+        if (host) (void)hipHostFree(host);
+        (void)hipGetLastError();
+        return st;
+    };
+    if (hipMalloc(reinterpret_cast<void**>(&mem), total) != hipSuccess) return fail(ZQ_ERR_OOM);
+    uint8_t* p = mem;
+    all.k = p; p += codes;
+    all.v = p; p += codes;
+    all.k_scale = reinterpret_cast<uint16_t*>(p); p += scales;
+    all.v_scale = reinterpret_cast<uint16_t*>(p); p += scales;
+    all.weight = reinterpret_cast<float*>(p); p += words;
+    all.pos = reinterpret_cast<int32_t*>(p);
+    if (!zq::kv_q4_ok(&all)) return fail(ZQ_ERR_ARG);
+    zq_kv_q4 one = all;
+    one.seqs = 1;
+    size_t need = keep ? zq::kv_q4_evict_bytes(all, keep) : 0;
+    const int flags = keep ? ZQ_ATTN_Q4_WEIGHTS | ZQ_ATTN_Q4_ADD : 0;
+    for (uint32_t T = 1; T <= kPrefillChunk; ++T) need = std::max(need, zq::attention_q4_bytes(one, T, c.heads, flags));
+    if (hipMalloc(reinterpret_cast<void**>(&rows), 2 * L * 4) != hipSuccess ||
+        hipMalloc(&ws, std::max<size_t>(need, 16)) != hipSuccess ||
+        hipHostMalloc(reinterpret_cast<void**>(&host), 2 * L * 4) != hipSuccess)
+        return fail(ZQ_ERR_OOM);
+    for (void* q : {m.kv_mem, static_cast<void*>(m.kv_rows_dev), m.kv_ws})
+        if (q) (void)hipFree(q);
+    if (m.kv_rows_host) (void)hipHostFree(m.kv_rows_host);
+    m.act_bytes += 2 * L * 4 + need - m.kv_aux_bytes;
+    m.kv_aux_bytes = 2 * L * 4 + need;
+    m.kv_mem = mem;
+    m.kv_rows_dev = rows;
+    m.kv_rows_host = host;
+    m.kv_ws = ws;
+    m.kv_ws_bytes = need;
+    m.kv_form = ZQ_KV_Q4;
+    m.kv_all = all;
+    m.kv_keep = keep;
+    m.kv_recent = recent;
+    m.kv_first = first;
+    m.cache_bytes = total;
+    for (size_t l = 0; l < L; ++l) {
+        zq_kv_q4& y = m.layers[l].q4;
+        y = one;
+        y.k += l * c.kv_heads * cap * D / 2;
+        y.v += l * c.kv_heads * cap * D / 2;
+        y.k_scale += l * c.kv_heads * cap * D / 32;
+        y.v_scale += l * c.kv_heads * cap * D / 32;
+        y.weight += l * c.kv_heads * cap;
+        y.pos += l * c.kv_heads * cap;
+        m.layers[l].kc = m.layers[l].vc = nullptr;
+    }
+    return ZQ_OK;
 }
 
 // Activation buffers, GEMM workspace, device scalars, KV cache, RoPE table.
@@ -194,15 +304,7 @@ bool alloc_runtime(zq_model& m, std::string& e) {
     p += kAlign;
     m.tokens_dev = reinterpret_cast<uint32_t*>(p);
 
-    // KV cache: [layer][position][kv_heads * head_dim] for K and V
-    const size_t per = size_t(c.max_positions) * KW * 4;
-    void* kv;
-    if (!dev_alloc(m, &kv, 2 * per * c.layers)) { e = "device allocation failed (KV cache)"; return false; }
-    m.cache_bytes = 2 * per * c.layers;
-    for (uint32_t l = 0; l < c.layers; ++l) {
-        m.layers[l].kc = reinterpret_cast<float*>(static_cast<uint8_t*>(kv) + 2 * l * per);
-        m.layers[l].vc = reinterpret_cast<float*>(static_cast<uint8_t*>(kv) + (2 * l + 1) * per);
-    }
+    if (!set_kv_f32(m)) { e = "device allocation failed (KV cache)"; return false; }
     // RoPE table
     std::vector<float> cs, sn;
     build_rope_table(c.max_positions, c.rope_dim, c.rope_base, 0.0f, cs, sn);
@@ -312,6 +414,49 @@ hipError_t tap(zq_model& m, uint32_t layer, int proj, const Weight& w, uint32_t 
     return hipSuccess;
 }
 
+// The T tokens' q, k and v (rows ld floats apart, 0: dense) into layer l's 4-bit
+// cache and through its attention: m.att gets the result, m.q the rotated queries.
+hipError_t enqueue_attention_q4(zq_model& m, uint32_t l, uint32_t T, const float* q, const float* k, const float* v,
+                                uint32_t ld) {
+    const auto& c = m.cfg;
+    const zq_kv_q4& kv = m.layers[l].q4;
+    HIPCHK(zq::launch_rope_kv_q4(kv, q, m.q, k, v, m.cos_tab, m.sin_tab, m.kv_rows_dev + l, m.pos_dev, T, c.heads, m.pairs,
+                                 ld, m.stream));
+    return zq::launch_attention_q4(kv, m.q, m.att, T, c.heads, size_t(c.heads) * c.head_dim, m.kv_rows_dev + l, nullptr,
+                                   m.attn_scale, m.kv_keep ? ZQ_ATTN_Q4_WEIGHTS | ZQ_ATTN_Q4_ADD : 0, m.kv_ws, m.stream);
+}
+
+// A decode step's attention: RoPE, append and attention of m.q, m.k, m.v into m.att.
+hipError_t enqueue_attention_step(zq_model& m, uint32_t l) {
+    const auto& c = m.cfg;
+    const Layer& L = m.layers[l];
+    if (m.kv_form == ZQ_KV_Q4) return enqueue_attention_q4(m, l, 1, m.q, m.k, m.v, 0);
+    return zq::launch_attention_decode(m.q, m.k, m.v, L.kc, L.vc, m.cos_tab, m.sin_tab, m.attn_part, m.att, m.pos_dev,
+                                       c.heads, c.kv_heads, c.head_dim, m.pairs, c.max_positions, m.attn_scale, m.stream);
+}
+
+// Room in the 4-bit cache for T more tokens, and the device's copy of its length.
+int make_room(zq_model& m, uint32_t T) {
+    if (m.kv_form != ZQ_KV_Q4) return ZQ_OK;
+    const uint32_t L = m.cfg.layers;
+    auto send = [&] {
+        for (uint32_t l = 0; l < L; ++l) {
+            m.kv_rows_host[l] = int32_t(m.cur_rows);
+            m.kv_rows_host[L + l] = int32_t(m.cur_pos);
+        }
+        return hipMemcpyAsync(m.kv_rows_dev, m.kv_rows_host, 2 * L * 4, hipMemcpyHostToDevice, m.stream) == hipSuccess;
+    };
+    if (m.cur_rows + T > m.kv_all.capacity) {
+        if (!m.kv_keep) return ZQ_ERR_ARG;
+        if (!send() || zq::launch_kv_q4_evict(m.kv_all, m.kv_all, true, m.kv_rows_dev, m.kv_keep, m.kv_recent, m.kv_first,
+                                              m.kv_rows_dev + L, m.kv_ws, m.stream) != hipSuccess ||
+            hipStreamSynchronize(m.stream) != hipSuccess)  // the mirror is written again below
+            return ZQ_ERR_HIP;
+        m.cur_rows = std::min(m.cur_rows, m.kv_keep);
+    }
+    return send() ? ZQ_OK : ZQ_ERR_HIP;
+}
+
 // Decoder layers over T tokens at positions pos0 .. pos0+T-1 (pos0 in device
 // memory).  On entry x holds the embeddings; on exit x is the residual stream
 // and h = rmsnorm(x) * output_norm, every residual add fused into the norm
@@ -350,7 +495,7 @@ hipError_t enqueue_layers(zq_model& m, uint32_t T) {
             if (!qz) HIPCHK(quantize_for(m, {&L.q, &L.k, &L.v}, m.h, T, E, qz));
             Weight qkv;
             if (qkv_packed(L, qkv)) {
-                HIPCHK(project(m, qkv, m.h, m.qkv, T, qz, &qkv_splits));
+                HIPCHK(project(m, qkv, m.h, m.qkv, T, qz, m.kv_form == ZQ_KV_F32 ? &qkv_splits : nullptr));
                 HIPCHK(tap(m, l, ZQ_TAP_QKV, qkv, T, qz, m.qkv, qkv_splits));
             } else {
                 HIPCHK(project(m, L.q, m.h, m.q, T, qz));
@@ -362,14 +507,17 @@ hipError_t enqueue_layers(zq_model& m, uint32_t T) {
             }
         }
         if (T == 1) {
-            HIPCHK(zq::launch_attention_decode(m.q, m.k, m.v, L.kc, L.vc, m.cos_tab, m.sin_tab, m.attn_part, m.att,
-                                               m.pos_dev, c.heads, c.kv_heads, c.head_dim, m.pairs, c.max_positions,
-                                               m.attn_scale, m.stream));
+            HIPCHK(enqueue_attention_step(m, l));
             zq::GemvTask t = {L.o.p, m.tmp, E};
             HIPCHK(zq::launch_gemv(L.o.fmt, &t, 1, m.att, QW, m.stream));
         } else {
             Weight qkv;
-            if (qkv_packed(L, qkv)) {
+            if (m.kv_form == ZQ_KV_Q4) {
+                if (qkv_packed(L, qkv))
+                    HIPCHK(enqueue_attention_q4(m, l, T, m.qkv, m.qkv + QW, m.qkv + QW + KW, QW + 2 * KW));
+                else
+                    HIPCHK(enqueue_attention_q4(m, l, T, m.q, m.k, m.v, 0));
+            } else if (qkv_packed(L, qkv)) {
                 const float* base = qkv_splits > 1 ? m.partial : m.qkv;
                 HIPCHK(zq::launch_rope_kv(m.q, base + QW, base + QW + KW, L.kc, L.vc, m.cos_tab, m.sin_tab, m.pos_dev, T,
                                           c.heads, c.kv_heads, c.head_dim, m.pairs, true, m.stream, QW + 2 * KW, base,
@@ -381,9 +529,10 @@ hipError_t enqueue_layers(zq_model& m, uint32_t T) {
             // with int8 o inputs the attention kernel writes them itself when it can
             const bool qo = qin({&L.o});
             bool qz = false;
-            HIPCHK(zq::launch_attention(m.q, L.kc, L.vc, m.att, m.pos_dev, T, c.heads, c.kv_heads, c.head_dim,
-                                        c.max_positions, m.attn_scale, m.stream, qo ? m.xq : nullptr,
-                                        qo ? m.xs : nullptr, &qz));
+            if (m.kv_form == ZQ_KV_F32)
+                HIPCHK(zq::launch_attention(m.q, L.kc, L.vc, m.att, m.pos_dev, T, c.heads, c.kv_heads, c.head_dim,
+                                            c.max_positions, m.attn_scale, m.stream, qo ? m.xq : nullptr,
+                                            qo ? m.xs : nullptr, &qz));
             if (!qz) HIPCHK(quantize_for(m, {&L.o}, m.att, T, QW, qz));
             HIPCHK(project(m, L.o, m.att, m.tmp, T, qz, &o_splits));
             HIPCHK(tap(m, l, ZQ_TAP_O, L.o, T, qz, m.tmp, o_splits));
@@ -464,9 +613,7 @@ hipError_t enqueue_decode_fused(zq_model& m) {
         const zq::XPrologue pq{zq::kAddNorm, r, delta, L.attn_norm, delta ? ralt : nullptr, c.rms_epsilon};
         HIPCHK(zq::launch_gemv_prologue(L.q.fmt, tq, 3, pq, E, m.stream));
         if (delta) std::swap(r, ralt);
-        HIPCHK(zq::launch_attention_decode(m.q, m.k, m.v, L.kc, L.vc, m.cos_tab, m.sin_tab, m.attn_part, m.att,
-                                           m.pos_dev, c.heads, c.kv_heads, c.head_dim, m.pairs, c.max_positions,
-                                           m.attn_scale, m.stream));
+        HIPCHK(enqueue_attention_step(m, l));
         zq::GemvTask to = {L.o.p, m.tmp, E};
         HIPCHK(zq::launch_gemv(L.o.fmt, &to, 1, m.att, QW, m.stream));
         zq::GemvTask tg[2] = {{L.gate.p, m.gate, F}, {L.up.p, m.up, F}};
@@ -517,9 +664,7 @@ hipError_t enqueue_decode_resid(zq_model& m) {
             const zq::ResidNorm rq{B, L.attn_norm, nullptr, nullptr, c.rms_epsilon};
             HIPCHK(zq::launch_gemv_resid(L.q.fmt, zq::kRnNormIn, tq, 3, m.x, E, rq, m.stream));
         }
-        HIPCHK(zq::launch_attention_decode(m.q, m.k, m.v, L.kc, L.vc, m.cos_tab, m.sin_tab, m.attn_part, m.att,
-                                           m.pos_dev, c.heads, c.kv_heads, c.head_dim, m.pairs, c.max_positions,
-                                           m.attn_scale, m.stream));
+        HIPCHK(enqueue_attention_step(m, l));
         const zq::GemvTask to{L.o.p, m.x, E};
         const zq::ResidNorm ro{nullptr, nullptr, A, B, 0.0f};
         HIPCHK(zq::launch_gemv_resid(L.o.fmt, zq::kRnAddOut, &to, 1, m.att, QW, ro, m.stream));
@@ -581,7 +726,7 @@ int prefill(zq_model& m, const uint32_t* tokens, size_t n, float* logits, uint32
     if (!tokens || !n || n > m.cfg.max_positions) return ZQ_ERR_ARG;
     for (size_t i = 0; i < n; ++i)
         if (tokens[i] >= m.cfg.vocab) return ZQ_ERR_ARG;
-    m.cur_pos = 0;
+    m.cur_pos = m.cur_rows = 0;
     m.tap_used = 0;
     m.tap_overflow = false;
     m.tap_recs.clear();
@@ -592,14 +737,16 @@ int prefill(zq_model& m, const uint32_t* tokens, size_t n, float* logits, uint32
         if (hipMemcpyAsync(m.pos_dev, &m.host_small[0], 4, hipMemcpyHostToDevice, m.stream) != hipSuccess ||
             hipMemcpyAsync(m.tokens_dev, &m.host_small[8], size_t(T) * 4, hipMemcpyHostToDevice, m.stream) != hipSuccess)
             return ZQ_ERR_HIP;
+        if (const int st = make_room(m, T); st != ZQ_OK) return st;
         if (zq::launch_embed(m.embd.fmt, m.embd.p, m.tokens_dev, m.cfg.vocab, m.x, m.cfg.embedding, T, m.stream) != hipSuccess ||
             enqueue_layers(m, T) != hipSuccess)
             return ZQ_ERR_HIP;
         if (s + T == n && enqueue_head(m, T - 1) != hipSuccess) return ZQ_ERR_HIP;
         // the staging words are reused by the next chunk: wait for the copies
         if (s + T < n && hipStreamSynchronize(m.stream) != hipSuccess) return ZQ_ERR_HIP;
+        m.cur_pos += T;
+        m.cur_rows += T;
     }
-    m.cur_pos = uint32_t(n);
     return finish_outputs(m, logits, next);
 }
 
@@ -610,6 +757,7 @@ int decode(zq_model& m, uint32_t token, float* logits, uint32_t* next) {
     if (hipMemcpyAsync(m.pos_dev, &m.host_small[0], 4, hipMemcpyHostToDevice, m.stream) != hipSuccess ||
         hipMemcpyAsync(m.tokens_dev, &m.host_small[8], 4, hipMemcpyHostToDevice, m.stream) != hipSuccess)
         return ZQ_ERR_HIP;
+    if (const int st = make_room(m, 1); st != ZQ_OK) return st;
     if (m.use_graph) {
         if (!m.decode_exec) {
             if (hipStreamBeginCapture(m.stream, hipStreamCaptureModeThreadLocal) != hipSuccess) return ZQ_ERR_HIP;
@@ -631,7 +779,10 @@ int decode(zq_model& m, uint32_t token, float* logits, uint32_t* next) {
         return ZQ_ERR_HIP;
     }
     const int st = finish_outputs(m, logits, next);
-    if (st == ZQ_OK) ++m.cur_pos;
+    if (st == ZQ_OK) {
+        ++m.cur_pos;
+        ++m.cur_rows;
+    }
     return st;
 }
 
@@ -860,6 +1011,37 @@ int zq_model_weight(const zq_model* m, uint32_t layer, int which, const void** d
 int zq_model_set_prefill_mode(zq_model* m, int mode) {
     if (!m || (mode != ZQ_PREFILL_INT8 && mode != ZQ_PREFILL_F32)) return ZQ_ERR_ARG;
     m->prefill_mode = mode;
+    return ZQ_OK;
+}
+
+int zq_model_set_kv_cache(zq_model* m, int form, uint32_t rows, uint32_t recent, uint32_t first) {
+    if (!m || (form != ZQ_KV_F32 && form != ZQ_KV_Q4) || (form == ZQ_KV_F32 && rows) || recent > rows ||
+        first > rows - recent)
+        return ZQ_ERR_ARG;
+    if (hipStreamSynchronize(m->stream) != hipSuccess) return ZQ_ERR_HIP;
+    if (form == ZQ_KV_F32) {
+        if (m->kv_form != ZQ_KV_F32 && !set_kv_f32(*m)) {
+            (void)hipGetLastError();
+            return ZQ_ERR_OOM;
+        }
+    } else if (const int st = set_kv_q4(*m, rows, recent, first); st != ZQ_OK) {
+        return st;
+    }
+    m->cur_pos = m->cur_rows = 0;
+    // the captured step holds the old cache's addresses
+    if (m->decode_exec) (void)hipGraphExecDestroy(m->decode_exec);
+    if (m->decode_graph) (void)hipGraphDestroy(m->decode_graph);
+    m->decode_exec = nullptr;
+    m->decode_graph = nullptr;
+    return ZQ_OK;
+}
+
+int zq_model_kv_cache(const zq_model* m, uint32_t layer, zq_kv_q4* cache, uint32_t* rows, uint32_t* positions) {
+    if (!m || layer >= m->layers.size() || !cache) return ZQ_ERR_ARG;
+    if (rows) *rows = m->cur_rows;
+    if (positions) *positions = m->cur_pos;
+    if (m->kv_form != ZQ_KV_Q4) return ZQ_DECLINED;
+    *cache = m->layers[layer].q4;
     return ZQ_OK;
 }
 

@@ -13,6 +13,7 @@ import numpy as np
 from . import zq
 
 PREFILL_INT8, PREFILL_F32 = 0, 1
+KV_F32, KV_Q4 = 0, 1
 GLOBAL = 0xFFFFFFFF
 W_EMBED, W_OUTPUT, W_Q, W_K, W_V, W_O, W_GATE, W_UP, W_DOWN = range(9)
 TAP_QKV, TAP_Q, TAP_K, TAP_V, TAP_O, TAP_GATE, TAP_UP, TAP_DOWN = range(8)
@@ -65,6 +66,21 @@ class Model:
 
     def set_prefill_mode(self, mode):
         zq.check(self._L.zq_model_set_prefill_mode(self._h, mode), "set_prefill_mode")
+
+    def set_kv_cache(self, form, rows=0, recent=0, first=0):
+        """The KV cache's form (zq_model_set_kv_cache): KV_F32, or KV_Q4 with at most `rows` rows kept by the
+        attention weight they draw (0: every position).  The cache starts empty."""
+        zq.check(self._L.zq_model_set_kv_cache(self._h, form, rows, recent, first), "set_kv_cache")
+
+    def kv_cache(self, layer):
+        """(zq.KVQ4 over one layer's 4-bit cache, or None with the fp32 cache; rows held; positions fed)."""
+        c, rows, at = zq.KVCacheQ4(), ctypes.c_uint32(), ctypes.c_uint32()
+        st = self._L.zq_model_kv_cache(self._h, layer, ctypes.byref(c), ctypes.byref(rows), ctypes.byref(at))
+        if st == zq.DECLINED:
+            return None, rows.value, at.value
+        zq.check(st, "kv_cache")
+        return zq.KVQ4(c.k, c.v, c.k_scale, c.v_scale, c.seqs, c.kv_heads, c.head_dim, c.capacity, weight=c.weight,
+                       pos=c.pos), rows.value, at.value
 
     def prefill(self, tokens, logits=True):
         t = np.ascontiguousarray(tokens, dtype=np.uint32)

@@ -34,6 +34,11 @@ struct AttnQ4 {
     float* part;        // partial outputs [head][row][split][D], where splits > 1
     float* part_ml;     // their (max, sum) pairs [head][row][split][2]
     float* lse;         // [head][row], log2 units, where weights are wanted
+    // with many rows as well: the query operands [head][row][2 parts][D], rows padded to
+    // whole tiles, and the factors that take their scale off
+    _Float16* qop;
+    float* qinv;
+    uint32_t rows_pad;
     float scale2;       // scale * log2(e): scores are in log2 units
     uint32_t tokens, G, KH, heads_kv;  // heads_kv = seqs * KH
     uint32_t rows;      // tokens * G
@@ -624,6 +629,17 @@ __global__ __launch_bounds__(Big<D>::T) void attn_q4_many_kernel(AttnQ4 a) {
         qh[j] = *reinterpret_cast<const h8_t*>(kbuf + qrow * B::HP + j * 16 + 8 * lh);
         ql[j] = *reinterpret_cast<const h8_t*>(kbuf + B::kQ + qrow * B::HP + j * 16 + 8 * lh);
     }
+    if (a.qop && sp == 0) {  // the operands once more, for the weights
+        const size_t row = size_t(head) * a.rows_pad + r0;
+        h8_t* dst = reinterpret_cast<h8_t*>(a.qop + row * 2 * D);
+        constexpr int P = D / 8;  // 16-byte parts of a row's one operand
+#pragma unroll 4
+        for (int j = tid; j < int(kTileRows) * 2 * P; j += B::T) {
+            const int rr = j / (2 * P), part = j / P % 2, e8 = j % P;
+            dst[j] = *reinterpret_cast<const h8_t*>(kbuf + part * B::kQ + rr * B::HP + e8 * 8);
+        }
+        if (tid < int(kTileRows)) a.qinv[row + tid] = inv_q[tid];
+    }
     __syncthreads();  // K and V take its place
     v16f_t o[B::NT], s;
 #pragma unroll
@@ -849,155 +865,234 @@ __global__ __launch_bounds__(256) void attn_q4_combine_kernel(AttnQ4 a) {
 // ---- the rows' weights ----------------------------------------------------------
 // S = Q K^T again, with the sums of the rows known (lse): a lane's 16 results are 16
 // query rows of one key, so a key's weight is a sum in one register.  A wave keeps 64
-// keys as operands; query rows pass by in LDS, 64 at a time.  Every key's sum has one
+// keys (D = 256: 32) as operands; query rows pass by in LDS, 64 at a time.  Every key's sum has one
 // owner (or two halves, added in order) and one order.
-// RH = 2 (many rows): eight waves, four on each half of the 64 rows.  RH = 1 (up to
-// 64 rows, staged once): four waves that go on to further keys.
+typedef float acc16_t __attribute__((ext_vector_type(16)));
+constexpr int kWgtRows = 64;
+
 template <int D>
 struct Wgt {
-    static constexpr int HP = D + 8, R = 64, KS = D / 16;
-    static constexpr size_t kQ = size_t(R) * HP;          // halves of one part of the queries
-    static constexpr size_t lds(int rh) { return 4 * kQ * rh; }  // two buffers where rows pass by
+    static constexpr int HP = D + 8, KS = D / 16;
+    static constexpr int KU = D <= 128 ? 2 : 1;           // a wave's keys, by 32: what registers hold
+    static constexpr uint32_t kKeys = 128 * KU;           // a workgroup's
+    static constexpr size_t kQ = size_t(kWgtRows) * HP;   // halves of one part of the queries
 };
+// what a row tile's scores need beside the operands
+struct __align__(16) WgtMeta {
+    float inv[kWgtRows], lse[kWgtRows];
+    int32_t lim[kWgtRows];
+};
+__device__ __forceinline__ void row_meta(WgtMeta& m, const AttnQ4& a, const Seq& x, uint32_t r, int tid) {
+    const bool ok = r < x.live * a.G;
+    m.lse[tid] = ok ? a.lse[size_t(x.head) * a.rows + r] : INFINITY;  // a row past the live ones: weights 0
+    m.lim[tid] = ok ? int32_t(visible(a, x, r / a.G)) : 0;
+}
+// The wave's keys from key0 on as B operands: lane (l32, lh) holds half a row of keys l32
+// and 32 + l32.  The last keys may lie past the capacity: their lanes take its last row.
+template <int D>
+__device__ __forceinline__ void load_keys(h8_t (&kf)[Wgt<D>::KU][D / 16], const AttnQ4& a, uint32_t head, uint32_t key0, int l32,
+                                          int lh, uint32_t one) {
+    constexpr int KS = D / 16, KU = Wgt<D>::KU;
+    const size_t cap = a.c.capacity;
+#pragma unroll
+    for (int u = 0; u < KU; ++u) {
+        const size_t key = min(size_t(key0) + 32 * u + l32, cap - 1);
+        const uint4* p = reinterpret_cast<const uint4*>(a.c.k + (size_t(head) * cap + key) * (D / 2) + lh * (D / 4));
+#pragma unroll
+        for (int j = 0; j < KS / 4; ++j) {
+            const uint4 w = p[j];
+            const _Float16 d =
+                __builtin_bit_cast(_Float16, a.c.k_scale[(size_t(head) * (D / 32) + lh * (KS / 4) + j) * cap + key]);
+            kf[u][4 * j] = dequant8(w.x, h2_t{d, d}, one);
+            kf[u][4 * j + 1] = dequant8(w.y, h2_t{d, d}, one);
+            kf[u][4 * j + 2] = dequant8(w.z, h2_t{d, d}, one);
+            kf[u][4 * j + 3] = dequant8(w.w, h2_t{d, d}, one);
+        }
+    }
+}
+// scores of 32 rows (q: this lane's row and half) and the wave's keys
+template <int D>
+__device__ __forceinline__ void row_scores(const _Float16* q, const h8_t (&kf)[Wgt<D>::KU][D / 16],
+                                           acc16_t (&s)[Wgt<D>::KU]) {
+    constexpr int KU = Wgt<D>::KU;
+#pragma unroll
+    for (int u = 0; u < KU; ++u)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) s[u][v] = 0.0f;
+#pragma unroll
+    for (int j = 0; j < D / 16; ++j) {
+        const h8_t h = *reinterpret_cast<const h8_t*>(q + 8 * j);
+        const h8_t l = *reinterpret_cast<const h8_t*>(q + Wgt<D>::kQ + 8 * j);
+#pragma unroll
+        for (int u = 0; u < KU; ++u) {
+            s[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(h, kf[u][j], s[u], 0, 0, 0);
+            s[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(l, kf[u][j], s[u], 0, 0, 0);
+        }
+    }
+}
+// their softmax weights onto w.  Result v of a lane: row row0 + 8 (v >> 2) + 4 lh + (v & 3),
+// key l32.  CUT: some rows do not see all of the keys.
+template <bool CUT, int KU>
+__device__ __forceinline__ void add_weights(float (&w)[KU], const acc16_t (&s)[KU], const WgtMeta& m, int row0, int key,
+                                            int lh) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const int at = row0 + 8 * j + 4 * lh;
+        const float4 c = *reinterpret_cast<const float4*>(&m.inv[at]);
+        const float4 e = *reinterpret_cast<const float4*>(&m.lse[at]);
+        const float cc[4] = {c.x, c.y, c.z, c.w}, ee[4] = {e.x, e.y, e.z, e.w};
+        int n[4] = {0, 0, 0, 0};
+        if constexpr (CUT) {
+            const int4 t = *reinterpret_cast<const int4*>(&m.lim[at]);
+            n[0] = t.x, n[1] = t.y, n[2] = t.z, n[3] = t.w;
+        }
+#pragma unroll
+        for (int u = 0; u < KU; ++u)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float p = exp2_(fmaf(s[u][4 * j + i], cc[i], -ee[i]));
+                w[u] += !CUT || key + 32 * u < n[i] ? p : 0.0f;
+            }
+    }
+}
 
-template <int D, int RH>
-__global__ __launch_bounds__(256 * RH) void attn_q4_weights_kernel(AttnQ4 a, uint32_t blocks) {
+// the weight of the key that a lane stands for: both lane halves' rows added, lane = key
+template <int KU>
+__device__ __forceinline__ float lane_weight(const float (&w)[KU], int lh) {
+    float v = w[0] + __shfl_xor(w[0], 32);
+    if constexpr (KU == 2) {
+        const float t = w[1] + __shfl_xor(w[1], 32);
+        v = lh ? t : v;
+    }
+    return v;
+}
+
+// Up to 64 rows, staged once: four waves, which go on to further keys.
+template <int D>
+__global__ __launch_bounds__(256) void attn_q4_weights_few_kernel(AttnQ4 a, uint32_t blocks) {
     using W = Wgt<D>;
-    constexpr int T = 256 * RH, KS = W::KS;
     extern __shared__ __align__(16) uint8_t lds[];
-    __shared__ __align__(16) float inv[2][W::R];
-    __shared__ __align__(16) float lse[2][W::R];
-    __shared__ __align__(16) int32_t lim[2][W::R];
-    __shared__ float half[RH == 2 ? 256 : 1];
+    __shared__ WgtMeta meta;
     _Float16* qbuf = reinterpret_cast<_Float16*>(lds);
     const uint32_t head = blockIdx.x % a.heads_kv, first = blockIdx.x / a.heads_kv;
     const Seq x = seq_of(a, head);
     if (!x.live) return;
     const uint32_t rows = x.live * a.G, keys = visible(a, x, x.live - 1);
-    const uint32_t nb = (keys + 255) / 256;
+    const uint32_t nb = (keys + W::kKeys - 1) / W::kKeys;
     if (first >= nb) return;
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l32 = lane & 31, lh = lane >> 5;
-    const int kg = wave & 3, rh = wave >> 2;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l32 = lane & 31,
+              lh = lane >> 5;
     const uint32_t one = code_bits();
-    const size_t cap = a.c.capacity;
-    // the rows from r0 on into buffer b
-    auto meta = [&](uint32_t r0, int b) {
-        if (tid < W::R) {
-            const uint32_t r = r0 + tid;
-            const bool ok = r < rows;
-            lse[b][tid] = ok ? a.lse[size_t(head) * a.rows + r] : INFINITY;  // a row past the live ones: weights 0
-            lim[b][tid] = ok ? int32_t(visible(a, x, r / a.G)) : 0;
+    {
+        QStage<D, 256, kWgtRows> qs;
+        load_qstage(qs, a, x, 0, tid);
+        store_qstage(qs, a.scale2, qbuf, qbuf + W::kQ, meta.inv, tid);
+        if (tid < kWgtRows) row_meta(meta, a, x, tid, tid);
+    }
+    __syncthreads();
+    for (uint32_t kb = first; kb < nb; kb += blocks) {
+        const uint32_t key0 = kb * W::kKeys + 32 * W::KU * wave;
+        if (key0 >= keys) continue;  // uniform in the wave
+        h8_t kf[W::KU][W::KS];
+        load_keys<D>(kf, a, head, key0, l32, lh, one);
+        float w[W::KU] = {};
+        for (uint32_t row0 = 0; row0 < rows; row0 += 32) {
+            acc16_t s[W::KU];
+            row_scores<D>(qbuf + (row0 + l32) * W::HP + lh * (D / 2), kf, s);
+            if (key0 + 32 * W::KU > visible(a, x, row0 / a.G)) add_weights<true>(w, s, meta, int(row0), int(key0 + l32), lh);
+            else add_weights<false>(w, s, meta, int(row0), int(key0 + l32), lh);
         }
-    };
-    QStage<D, T, W::R> qs;
-    for (uint32_t kb = first; kb < nb; kb += blocks) {  // uniform; more than one only with RH = 1
-        const uint32_t key0 = kb * 256 + 64 * kg;
-        const bool mine = key0 < keys;  // uniform in the wave
-        // rows before the first token that sees the block's first key see none of it
-        const uint32_t ta = a.full || kb * 256 < x.len ? 0 : kb * 256 - x.len;
-        const uint32_t ra = ta * a.G / W::R * W::R;
-        if (RH == 2 || kb == first) load_qstage(qs, a, x, ra, tid);
-        h8_t kf[2][KS];
-        if (mine) {
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                // the last keys of a block may lie past the capacity: their lanes take the last row's
-                const size_t key = min(size_t(key0) + 32 * u + l32, cap - 1);
-                const uint8_t* p = a.c.k + (size_t(head) * cap + key) * (D / 2) + lh * (D / 4);
-                uint32_t w[KS];
-#pragma unroll
-                for (int j = 0; j < KS / 4; ++j) {
-                    const uint4 v = reinterpret_cast<const uint4*>(p)[j];
-                    w[4 * j] = v.x;
-                    w[4 * j + 1] = v.y;
-                    w[4 * j + 2] = v.z;
-                    w[4 * j + 3] = v.w;
-                }
-#pragma unroll
-                for (int j = 0; j < KS / 4; ++j) {
-                    const _Float16 d = __builtin_bit_cast(
-                        _Float16, a.c.k_scale[(size_t(head) * (D / 32) + lh * (KS / 4) + j) * cap + key]);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) kf[u][4 * j + i] = dequant8(w[4 * j + i], h2_t{d, d}, one);
-                }
-            }
-        }
-        if (RH == 2 || kb == first) {
-            if (kb != first) __syncthreads();
-            store_qstage(qs, a.scale2, qbuf, qbuf + W::kQ, inv[0], tid);
-            meta(ra, 0);
-            __syncthreads();
-        }
-        float w[2] = {0.0f, 0.0f};
-        int b = 0;
-        for (uint32_t r0 = ra; r0 < rows; r0 += W::R, b ^= 1) {
-            const bool more = RH == 2 && r0 + W::R < rows;
-            if (more) load_qstage(qs, a, x, r0 + W::R, tid);
-            const _Float16* qt = qbuf + size_t(b) * 2 * W::kQ;
-#pragma unroll
-            for (int sub = 0; sub < 2 / RH; ++sub) {
-                const int row0 = 32 * (RH == 2 ? rh : sub);
-                if (!mine || r0 + row0 >= rows) continue;  // uniform in the wave
-                const _Float16* q = qt + (row0 + l32) * W::HP + lh * (D / 2);
-                typedef float acc_t __attribute__((ext_vector_type(16)));
-                acc_t s[2];
-#pragma unroll
-                for (int u = 0; u < 2; ++u)
-#pragma unroll
-                    for (int v = 0; v < 16; ++v) s[u][v] = 0.0f;
-#pragma unroll
-                for (int j = 0; j < KS; ++j) {
-                    const h8_t h = *reinterpret_cast<const h8_t*>(q + 8 * j);
-                    const h8_t l = *reinterpret_cast<const h8_t*>(q + W::kQ + 8 * j);
-#pragma unroll
-                    for (int u = 0; u < 2; ++u) {
-                        s[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(h, kf[u][j], s[u], 0, 0, 0);
-                        s[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(l, kf[u][j], s[u], 0, 0, 0);
-                    }
-                }
-                // result v of a lane: row 8 (v >> 2) + 4 lh + (v & 3), key l32
-                const bool cut = key0 + 64 > visible(a, x, min(r0 + row0, rows - 1) / a.G);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int at = row0 + 8 * j + 4 * lh;
-                    const float4 c = *reinterpret_cast<const float4*>(&inv[b][at]);
-                    const float4 e = *reinterpret_cast<const float4*>(&lse[b][at]);
-                    const float cc[4] = {c.x, c.y, c.z, c.w}, ee[4] = {e.x, e.y, e.z, e.w};
-                    if (!cut) {
-#pragma unroll
-                        for (int u = 0; u < 2; ++u)
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) w[u] += exp2_(fmaf(s[u][4 * j + i], cc[i], -ee[i]));
-                    } else {
-                        const int4 m = *reinterpret_cast<const int4*>(&lim[b][at]);
-                        const int mm[4] = {m.x, m.y, m.z, m.w};
-#pragma unroll
-                        for (int u = 0; u < 2; ++u)
-#pragma unroll
-                            for (int i = 0; i < 4; ++i)
-                                w[u] += int(key0 + 32 * u + l32) < mm[i] ? exp2_(fmaf(s[u][4 * j + i], cc[i], -ee[i])) : 0.0f;
-                    }
-                }
-            }
-            if (more) {  // the other buffer was read last before the previous barrier
-                _Float16* nq = qbuf + size_t(b ^ 1) * 2 * W::kQ;
-                store_qstage(qs, a.scale2, nq, nq + W::kQ, inv[b ^ 1], tid);
-                meta(r0 + W::R, b ^ 1);
-                __syncthreads();
-            }
-        }
-#pragma unroll
-        for (int u = 0; u < 2; ++u) w[u] += __shfl_xor(w[u], 32);
-        float v = lh ? w[1] : w[0];  // lane's key of the wave's 64
-        if constexpr (RH == 2) {
-            if (rh == 1) half[64 * kg + lane] = v;
-            __syncthreads();
-            if (rh == 0) v += half[64 * kg + lane];
-        }
-        if (rh == 0 && key0 + lane < keys) {
-            float* dst = a.c.weight + size_t(head) * cap + key0 + lane;
+        const float v = lane_weight(w, lh);
+        if (lane < 32 * W::KU && key0 + lane < keys) {
+            float* dst = a.c.weight + size_t(head) * a.c.capacity + key0 + lane;
             *dst = a.add ? *dst + v : v;
         }
+    }
+}
+
+// Many rows: eight waves, four on each half of the passing 64
+// rows, whose operands the attention kernel has left in memory.  The next tile's
+// products stand between this one's exponentials; operands are loaded two tiles ahead.
+template <int D>
+__global__ __launch_bounds__(512) void attn_q4_weights_many_kernel(AttnQ4 a) {
+    using W = Wgt<D>;
+    constexpr int P = D / 8, J = kWgtRows * 2 * P / 512;  // 16-byte parts of a row's one operand; parts a thread moves
+    extern __shared__ __align__(16) uint8_t lds[];
+    __shared__ WgtMeta meta[3];
+    __shared__ float half[256];
+    _Float16* qbuf = reinterpret_cast<_Float16*>(lds);
+    const uint32_t head = blockIdx.x % a.heads_kv, kb = blockIdx.x / a.heads_kv;
+    const Seq x = seq_of(a, head);
+    if (!x.live) return;
+    const uint32_t rows = x.live * a.G, keys = visible(a, x, x.live - 1);
+    if (kb * W::kKeys >= keys) return;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l32 = lane & 31,
+              lh = lane >> 5, kg = wave & 3, rh = wave >> 2;
+    const uint32_t one = code_bits(), key0 = kb * W::kKeys + 32 * W::KU * kg;
+    const bool mine = key0 < keys;  // uniform in the wave
+    // rows before the first token that sees the block's first key see none of it
+    const uint32_t ta = a.full || kb * W::kKeys < x.len ? 0 : kb * W::kKeys - x.len;
+    const uint32_t t0 = ta * a.G / kWgtRows, t1 = (rows + kWgtRows - 1) / kWgtRows;
+    h8_t st[J];
+    float st_inv = 0.0f;
+    auto fetch = [&](uint32_t t) {  // tile t (past the last one: that again)
+        const size_t row = size_t(head) * a.rows_pad + min(t, t1 - 1) * kWgtRows;
+        const h8_t* q = reinterpret_cast<const h8_t*>(a.qop + row * 2 * D);
+#pragma unroll
+        for (int j = 0; j < J; ++j) st[j] = q[tid + j * 512];
+        if (tid < kWgtRows) st_inv = a.qinv[row + tid];
+    };
+    auto put = [&](uint32_t t) {
+        _Float16* q = qbuf + (t & 1) * 2 * W::kQ;
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+            const int e = tid + j * 512, r = e / (2 * P), part = e / P % 2, e8 = e % P;
+            *reinterpret_cast<h8_t*>(q + part * W::kQ + r * W::HP + e8 * 8) = st[j];
+        }
+        if (tid < kWgtRows) {
+            WgtMeta& m = meta[t % 3];
+            m.inv[tid] = st_inv;
+            row_meta(m, a, x, t * kWgtRows + tid, tid);
+        }
+    };
+    fetch(t0);
+    h8_t kf[W::KU][W::KS];
+    if (mine) load_keys<D>(kf, a, head, key0, l32, lh, one);
+    put(t0);
+    fetch(t0 + 1);
+    put(t0 + 1);
+    fetch(t0 + 2);
+    __syncthreads();
+    const int row0 = 32 * rh;
+    const _Float16* q = qbuf + (row0 + l32) * W::HP + lh * (D / 2);
+    acc16_t s[W::KU];
+    if (mine) row_scores<D>(q + (t0 & 1) * 2 * W::kQ, kf, s);
+    float w[W::KU] = {};
+    for (uint32_t t = t0; t < t1; ++t) {
+        __syncthreads();  // tile t + 1 is written, the buffer of tile t is read no more
+        if (mine) {
+            acc16_t next[W::KU];
+            const bool cut = key0 + 32 * W::KU > visible(a, x, min(t * kWgtRows + row0, rows - 1) / a.G);
+            if (cut) {
+                add_weights<true>(w, s, meta[t % 3], row0, int(key0 + l32), lh);
+                row_scores<D>(q + ((t + 1) & 1) * 2 * W::kQ, kf, next);
+            } else {
+                row_scores<D>(q + ((t + 1) & 1) * 2 * W::kQ, kf, next);
+                add_weights<false>(w, s, meta[t % 3], row0, int(key0 + l32), lh);
+            }
+#pragma unroll
+            for (int u = 0; u < W::KU; ++u) s[u] = next[u];
+        }
+        put(t + 2);  // (past the last tile: written, read no more)
+        fetch(t + 3);
+    }
+    float v = lane_weight(w, lh);
+    if (rh == 1) half[64 * kg + lane] = v;
+    __syncthreads();
+    if (rh == 0 && lane < 32 * W::KU && key0 + lane < keys) {
+        v += half[64 * kg + lane];
+        float* dst = a.c.weight + size_t(head) * a.c.capacity + key0 + lane;
+        *dst = a.add ? *dst + v : v;
     }
 }
 
@@ -1020,15 +1115,20 @@ Plan plan_of(const zq_kv_q4& c, size_t rows) {
 }
 
 size_t up256(size_t n) { return (n + 255) / 256 * 256; }
+size_t pad_rows(size_t rows) { return (rows + kTileRows - 1) / kTileRows * kTileRows; }
 
 }  // namespace
 
 size_t attention_q4_bytes(const zq_kv_q4& c, size_t tokens, size_t heads, int flags) {
     const size_t rows = tokens * (heads / c.kv_heads), all = c.seqs * c.kv_heads * rows;
-    const size_t splits = plan_of(c, rows).splits;
+    const Plan plan = plan_of(c, rows);
     size_t n = 0;
-    if (splits > 1) n += up256(all * splits * c.head_dim * 4) + up256(all * splits * 8);
-    if (flags & ZQ_ATTN_Q4_WEIGHTS) n += up256(all * 4);
+    if (plan.splits > 1) n += up256(all * plan.splits * c.head_dim * 4) + up256(all * plan.splits * 8);
+    if (flags & ZQ_ATTN_Q4_WEIGHTS) {
+        n += up256(all * 4);
+        const size_t pad = c.seqs * c.kv_heads * pad_rows(rows);
+        if (plan.many) n += up256(pad * c.head_dim * 4) + up256(pad * 4);
+    }
     return n;
 }
 
@@ -1061,13 +1161,22 @@ hipError_t launch_attention_q4(const zq_kv_q4& c, const float* q, float* out, si
         a.part_ml = reinterpret_cast<float*>(p);
         p += up256(all * a.splits * 8);
     }
-    if (flags & ZQ_ATTN_Q4_WEIGHTS) a.lse = reinterpret_cast<float*>(p);
+    if (flags & ZQ_ATTN_Q4_WEIGHTS) {
+        a.lse = reinterpret_cast<float*>(p);
+        p += up256(all * 4);
+        if (a.many) {
+            a.rows_pad = uint32_t(pad_rows(a.rows));
+            const size_t pad = size_t(a.heads_kv) * a.rows_pad;
+            a.qop = reinterpret_cast<_Float16*>(p);
+            p += up256(pad * c.head_dim * 4);
+            a.qinv = reinterpret_cast<float*>(p);
+        }
+    }
     const size_t tile = a.many ? kTileRows : 16;
     const size_t blocks = size_t(a.heads_kv) * a.splits * ((a.rows + tile - 1) / tile);
-    // weights: with many rows every 256 keys have a workgroup of their own
-    const bool pass = a.rows > uint32_t(Wgt<64>::R);
-    const size_t all_blocks = (c.capacity + 255) / 256, fill = size_t(device_cu_count()) * 4 / a.heads_kv + 1;
-    const size_t wblocks = pass ? all_blocks : std::min(all_blocks, fill), key_blocks = a.heads_kv * wblocks;
+    const size_t per_block = c.head_dim == 256 ? Wgt<256>::kKeys : Wgt<128>::kKeys;
+    const size_t all_blocks = (c.capacity + per_block - 1) / per_block, fill = size_t(device_cu_count()) * 4 / a.heads_kv + 1;
+    const size_t wblocks = a.many ? all_blocks : std::min(all_blocks, fill), key_blocks = a.heads_kv * wblocks;
     if (blocks > 0x7fffffffu || key_blocks > 0x7fffffffu) return hipErrorInvalidValue;
 #define ZQ_ATTN_D(KERNEL, GRID, THREADS)                                                                \
     do {                                                                                                \
@@ -1092,15 +1201,14 @@ hipError_t launch_attention_q4(const zq_kv_q4& c, const float* q, float* out, si
     if (a.splits > 1) ZQ_ATTN_D(attn_q4_combine_kernel, all, 256);
 #undef ZQ_ATTN_D
     if (!a.lse) return hipSuccess;
-#define ZQ_ATTN_W(DD)                                                                                              \
-    do {                                                                                                           \
-        const dim3 grid{uint32_t(key_blocks)};                                                                     \
-        if (pass)                                                                                                  \
-            hipLaunchKernelGGL((attn_q4_weights_kernel<DD, 2>), grid, dim3(512), Wgt<DD>::lds(2), stream, a,       \
-                               uint32_t(wblocks));                                                                 \
-        else                                                                                                       \
-            hipLaunchKernelGGL((attn_q4_weights_kernel<DD, 1>), grid, dim3(256), Wgt<DD>::lds(1), stream, a,       \
-                               uint32_t(wblocks));                                                                 \
+#define ZQ_ATTN_W(DD)                                                                                               \
+    do {                                                                                                            \
+        const dim3 grid{uint32_t(key_blocks)};                                                                      \
+        if (a.many)                                                                                                 \
+            hipLaunchKernelGGL(attn_q4_weights_many_kernel<DD>, grid, dim3(512), 8 * Wgt<DD>::kQ, stream, a);       \
+        else                                                                                                        \
+            hipLaunchKernelGGL(attn_q4_weights_few_kernel<DD>, grid, dim3(256), 4 * Wgt<DD>::kQ, stream, a,         \
+                               uint32_t(wblocks));                                                                  \
     } while (0)
     if (c.head_dim == 64) ZQ_ATTN_W(64);
     else if (c.head_dim == 128) ZQ_ATTN_W(128);

@@ -34,7 +34,8 @@ struct AttnQ4 {
     float* part;        // partial outputs [head][row][split][D], where splits > 1
     float* part_ml;     // their (max, sum) pairs [head][row][split][2]
     float* lse;         // [head][row], log2 units, where weights are wanted
-    // with many rows as well: the query operands [head][row][2 parts][D], rows padded to
+    float* sc;          // with at most kScoreRows rows: their scores [head][row][capacity], log2 units
+    // with many rows: the query operands [head][row][2 parts][D], rows padded to
     // whole tiles, and the factors that take their scale off
     _Float16* qop;
     float* qinv;
@@ -309,6 +310,11 @@ __global__ __launch_bounds__(kWaves * 64, D == 64 ? 4 : D == 128 ? 3 : 2) void a
                 s[k] = key + k < lim ? s[k] : -INFINITY;
                 vsc[k] = key + k < cut.keys ? vsc[k] : _Float16(0);  // rows that hold nothing: their scale may be any bits
             }
+        }
+        if (a.sc && ok) {
+            float4* p = reinterpret_cast<float4*>(a.sc + (size_t(head) * a.rows + r) * a.c.capacity + t * 32 + 8 * g);
+            p[0] = make_float4(s[0] * c, s[1] * c, s[2] * c, s[3] * c);
+            p[1] = make_float4(s[4] * c, s[5] * c, s[6] * c, s[7] * c);
         }
         float mx = fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])), fmaxf(fmaxf(s[4], s[5]), fmaxf(s[6], s[7]))) * c;
         if (__any(mx > m + kSlack)) {
@@ -863,7 +869,38 @@ __global__ __launch_bounds__(256) void attn_q4_combine_kernel(AttnQ4 a) {
 }
 
 // ---- the rows' weights ----------------------------------------------------------
-// S = Q K^T again, with the sums of the rows known (lse): a lane's 16 results are 16
+// At most kScoreRows rows (a decode step): the attention kernel has left its scores,
+// 4 bytes a row and key beside the key's 72 to 288, and what is left is their sum.
+constexpr uint32_t kScoreRows = 8;
+__global__ __launch_bounds__(256) void attn_q4_weights_sum_kernel(AttnQ4 a) {
+    const uint32_t head = blockIdx.x % a.heads_kv, key = (blockIdx.x / a.heads_kv * 256 + threadIdx.x) * 4;
+    const Seq x = seq_of(a, head);
+    if (!x.live) return;
+    const uint32_t rows = x.live * a.G, keys = visible(a, x, x.live - 1);
+    if (key >= keys) return;
+    float4 v[kScoreRows];
+    const float* s = a.sc + size_t(head) * a.rows * a.c.capacity + key;
+#pragma unroll
+    for (uint32_t r = 0; r < kScoreRows; ++r)
+        if (r < rows) v[r] = *reinterpret_cast<const float4*>(s + size_t(r) * a.c.capacity);
+    float w[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (uint32_t r = 0; r < kScoreRows; ++r) {
+        if (r < rows) {
+            const float e = a.lse[size_t(head) * a.rows + r];
+            const uint32_t n = visible(a, x, r / a.G);
+            const float t[4] = {v[r].x, v[r].y, v[r].z, v[r].w};
+#pragma unroll
+            for (uint32_t i = 0; i < 4; ++i) w[i] += key + i < n ? exp2_(t[i] - e) : 0.0f;
+        }
+    }
+    float* dst = a.c.weight + size_t(head) * a.c.capacity + key;
+#pragma unroll
+    for (uint32_t i = 0; i < 4; ++i)
+        if (key + i < keys) dst[i] = a.add ? dst[i] + w[i] : w[i];
+}
+
+// More rows: S = Q K^T again, with the sums of the rows known (lse): a lane's 16 results are 16
 // query rows of one key, so a key's weight is a sum in one register.  A wave keeps 64
 // keys (D = 256: 32) as operands; query rows pass by in LDS, 64 at a time.  Every key's sum has one
 // owner (or two halves, added in order) and one order.
@@ -890,25 +927,37 @@ __device__ __forceinline__ void row_meta(WgtMeta& m, const AttnQ4& a, const Seq&
 // The wave's keys from key0 on as B operands: lane (l32, lh) holds half a row of keys l32
 // and 32 + l32.  The last keys may lie past the capacity: their lanes take its last row.
 template <int D>
-__device__ __forceinline__ void load_keys(h8_t (&kf)[Wgt<D>::KU][D / 16], const AttnQ4& a, uint32_t head, uint32_t key0, int l32,
-                                          int lh, uint32_t one) {
-    constexpr int KS = D / 16, KU = Wgt<D>::KU;
+struct KeyCodes {
+    uint4 w[Wgt<D>::KU][D / 64];
+    _Float16 d[Wgt<D>::KU][D / 64];
+};
+template <int D>
+__device__ __forceinline__ void load_keys(KeyCodes<D>& k, const AttnQ4& a, uint32_t head, uint32_t key0, int l32, int lh) {
     const size_t cap = a.c.capacity;
 #pragma unroll
-    for (int u = 0; u < KU; ++u) {
+    for (int u = 0; u < Wgt<D>::KU; ++u) {
         const size_t key = min(size_t(key0) + 32 * u + l32, cap - 1);
         const uint4* p = reinterpret_cast<const uint4*>(a.c.k + (size_t(head) * cap + key) * (D / 2) + lh * (D / 4));
 #pragma unroll
-        for (int j = 0; j < KS / 4; ++j) {
-            const uint4 w = p[j];
-            const _Float16 d =
-                __builtin_bit_cast(_Float16, a.c.k_scale[(size_t(head) * (D / 32) + lh * (KS / 4) + j) * cap + key]);
-            kf[u][4 * j] = dequant8(w.x, h2_t{d, d}, one);
-            kf[u][4 * j + 1] = dequant8(w.y, h2_t{d, d}, one);
-            kf[u][4 * j + 2] = dequant8(w.z, h2_t{d, d}, one);
-            kf[u][4 * j + 3] = dequant8(w.w, h2_t{d, d}, one);
+        for (int j = 0; j < D / 64; ++j) {
+            k.w[u][j] = p[j];
+            k.d[u][j] = __builtin_bit_cast(_Float16, a.c.k_scale[(size_t(head) * (D / 32) + lh * (D / 64) + j) * cap + key]);
         }
     }
+}
+template <int D>
+__device__ __forceinline__ void decode_keys(h8_t (&kf)[Wgt<D>::KU][D / 16], const KeyCodes<D>& k, uint32_t one) {
+#pragma unroll
+    for (int u = 0; u < Wgt<D>::KU; ++u)
+#pragma unroll
+        for (int j = 0; j < D / 64; ++j) {
+            const uint4 w = k.w[u][j];
+            const h2_t d = {k.d[u][j], k.d[u][j]};
+            kf[u][4 * j] = dequant8(w.x, d, one);
+            kf[u][4 * j + 1] = dequant8(w.y, d, one);
+            kf[u][4 * j + 2] = dequant8(w.z, d, one);
+            kf[u][4 * j + 3] = dequant8(w.w, d, one);
+        }
 }
 // scores of 32 rows (q: this lane's row and half) and the wave's keys
 template <int D>
@@ -983,6 +1032,10 @@ __global__ __launch_bounds__(256) void attn_q4_weights_few_kernel(AttnQ4 a, uint
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l32 = lane & 31,
               lh = lane >> 5;
     const uint32_t one = code_bits();
+    // the first keys on their way before the queries, and each next ones before their turn
+    auto key_of = [&](uint32_t kb) { return min(kb, nb - 1) * W::kKeys + 32 * W::KU * wave; };
+    KeyCodes<D> k;
+    load_keys<D>(k, a, head, key_of(first), l32, lh);
     {
         QStage<D, 256, kWgtRows> qs;
         load_qstage(qs, a, x, 0, tid);
@@ -991,10 +1044,11 @@ __global__ __launch_bounds__(256) void attn_q4_weights_few_kernel(AttnQ4 a, uint
     }
     __syncthreads();
     for (uint32_t kb = first; kb < nb; kb += blocks) {
-        const uint32_t key0 = kb * W::kKeys + 32 * W::KU * wave;
-        if (key0 >= keys) continue;  // uniform in the wave
+        const uint32_t key0 = key_of(kb);
+        if (key0 >= keys) break;  // uniform in the wave
         h8_t kf[W::KU][W::KS];
-        load_keys<D>(kf, a, head, key0, l32, lh, one);
+        decode_keys<D>(kf, k, one);
+        load_keys<D>(k, a, head, key_of(kb + blocks), l32, lh);
         float w[W::KU] = {};
         for (uint32_t row0 = 0; row0 < rows; row0 += 32) {
             acc16_t s[W::KU];
@@ -1057,7 +1111,11 @@ __global__ __launch_bounds__(512) void attn_q4_weights_many_kernel(AttnQ4 a) {
     };
     fetch(t0);
     h8_t kf[W::KU][W::KS];
-    if (mine) load_keys<D>(kf, a, head, key0, l32, lh, one);
+    if (mine) {
+        KeyCodes<D> k;
+        load_keys<D>(k, a, head, key0, l32, lh);
+        decode_keys<D>(kf, k, one);
+    }
     put(t0);
     fetch(t0 + 1);
     put(t0 + 1);
@@ -1128,6 +1186,7 @@ size_t attention_q4_bytes(const zq_kv_q4& c, size_t tokens, size_t heads, int fl
         n += up256(all * 4);
         const size_t pad = c.seqs * c.kv_heads * pad_rows(rows);
         if (plan.many) n += up256(pad * c.head_dim * 4) + up256(pad * 4);
+        else if (rows <= kScoreRows) n += up256(all * c.capacity * 4);
     }
     return n;
 }
@@ -1170,6 +1229,8 @@ hipError_t launch_attention_q4(const zq_kv_q4& c, const float* q, float* out, si
             a.qop = reinterpret_cast<_Float16*>(p);
             p += up256(pad * c.head_dim * 4);
             a.qinv = reinterpret_cast<float*>(p);
+        } else if (a.rows <= kScoreRows) {
+            a.sc = reinterpret_cast<float*>(p);
         }
     }
     const size_t tile = a.many ? kTileRows : 16;
@@ -1201,6 +1262,11 @@ hipError_t launch_attention_q4(const zq_kv_q4& c, const float* q, float* out, si
     if (a.splits > 1) ZQ_ATTN_D(attn_q4_combine_kernel, all, 256);
 #undef ZQ_ATTN_D
     if (!a.lse) return hipSuccess;
+    if (a.sc) {
+        const size_t grid = a.heads_kv * ((c.capacity + 1023) / 1024);
+        hipLaunchKernelGGL(attn_q4_weights_sum_kernel, dim3(uint32_t(grid)), dim3(256), 0, stream, a);
+        return hipGetLastError();
+    }
 #define ZQ_ATTN_W(DD)                                                                                               \
     do {                                                                                                            \
         const dim3 grid{uint32_t(key_blocks)};                                                                      \

@@ -811,11 +811,12 @@ __global__ __launch_bounds__(Big<D>::T) void attn_q4_many_kernel(AttnQ4 a) {
                 make_float4(o[n][4 * j] * inv, o[n][4 * j + 1] * inv, o[n][4 * j + 2] * inv, o[n][4 * j + 3] * inv);
 }
 
-// The splits' partial outputs of a row as one, by a workgroup: D / 4 lanes take a
-// split's output, so 1024 / D splits are read at a time.
-template <int D>
-__global__ __launch_bounds__(256) void attn_q4_combine_kernel(AttnQ4 a) {
-    constexpr int RL = D / 4, P = 256 / RL;
+// The splits' partial outputs of a row as one, by a workgroup of one wave (many rows,
+// few splits) or four: D / 4 lanes take a split's output, so WAVES * 256 / D splits are
+// read at a time.
+template <int D, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void attn_q4_combine_kernel(AttnQ4 a) {
+    constexpr int RL = D / 4, P = 64 * WAVES / RL;
     __shared__ float wgt[128];
     __shared__ float4 sum[P][RL];
     const uint32_t head = blockIdx.x / a.rows, r = blockIdx.x % a.rows;
@@ -1259,7 +1260,19 @@ hipError_t launch_attention_q4(const zq_kv_q4& c, const float* q, float* out, si
     } else {
         ZQ_ATTN_D(attn_q4_few_kernel, blocks, kWaves * 64);
     }
-    if (a.splits > 1) ZQ_ATTN_D(attn_q4_combine_kernel, all, 256);
+    if (a.splits > 1) {
+#define ZQ_ATTN_C(DD)                                                                                              \
+    do {                                                                                                           \
+        if (a.many) hipLaunchKernelGGL((attn_q4_combine_kernel<DD, 1>), dim3(uint32_t(all)), dim3(64), 0, stream, a); \
+        else hipLaunchKernelGGL((attn_q4_combine_kernel<DD, 4>), dim3(uint32_t(all)), dim3(256), 0, stream, a);    \
+    } while (0)
+        if (c.head_dim == 64) ZQ_ATTN_C(64);
+        else if (c.head_dim == 128) ZQ_ATTN_C(128);
+        else ZQ_ATTN_C(256);
+#undef ZQ_ATTN_C
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    }
 #undef ZQ_ATTN_D
     if (!a.lse) return hipSuccess;
     if (a.sc) {

@@ -192,13 +192,14 @@ __global__ __launch_bounds__(kT) void kv_q4_read_kernel(zq_kv_q4 c, float* __res
 }
 
 // ---- evict ---------------------------------------------------------------------
-// Two launches.  The first, one workgroup a (sequence, kv head), finds the rows
-// that stay and, for every slot below the new length, the slot its row comes from;
-// it also moves weight and pos, which it alone knows the old values of.  The second
-// copies the rows.  Free slots are filled from above the new length, so what is
-// written and what is read never meet, in place or not, and only evicted slots are
-// written in place.
-constexpr int kEvT = 1024;
+// One workgroup a (sequence, kv head) finds the rows that stay and, for every slot
+// below the new length, the slot its row comes from; it also moves weight and pos.
+// Free slots are filled from above the new length, so what is written and what is read
+// never meet, in place or not, and only evicted slots are written in place.
+// A second launch copies the rows' codes and scales (the one workgroup would take 11 us
+// for 1024 rows of D = 64 where that launch takes 4).
+constexpr int kEvT = 1024, kEvWaves = kEvT / 64;
+constexpr int kEvHeld = 16;  // keys a thread holds: caches up to 16384 rows are read once
 
 // Order of a row: protected ones, then by weight (-0 = +0), a NaN last.
 __device__ __forceinline__ uint32_t evict_key(float w, bool held) {
@@ -208,123 +209,174 @@ __device__ __forceinline__ uint32_t evict_key(float w, bool held) {
     return (u >> 31) ? ~u : (u | 0x80000000u);
 }
 
-struct EvictLists {
-    int32_t* from;   // [keep] the slot that slot j's row comes from
-    int32_t* holes;  // [keep] free slots below the new length, ascending
-    int32_t* above;  // [keep] kept slots from the new length on, ascending
-};
+// Sums of v over the lanes below this one, and of all lanes: DPP shifts within rows of
+// 16 lanes, then the rows' sums on to the rows behind them.
+__device__ __forceinline__ uint32_t wave_before(uint32_t v, uint32_t& all) {
+    auto step = [](uint32_t s, auto ctrl, auto rows) {
+        return s + uint32_t(__builtin_amdgcn_update_dpp(0, int(s), decltype(ctrl)::value, decltype(rows)::value, 0xF, false));
+    };
+    using std::integral_constant;
+    uint32_t s = v;
+    s = step(s, integral_constant<int, 0x111>{}, integral_constant<int, 0xF>{});  // row_shr:1, 2, 4, 8
+    s = step(s, integral_constant<int, 0x112>{}, integral_constant<int, 0xF>{});
+    s = step(s, integral_constant<int, 0x114>{}, integral_constant<int, 0xF>{});
+    s = step(s, integral_constant<int, 0x118>{}, integral_constant<int, 0xF>{});
+    s = step(s, integral_constant<int, 0x142>{}, integral_constant<int, 0xA>{});  // row_bcast:15 into rows 1 and 3
+    s = step(s, integral_constant<int, 0x143>{}, integral_constant<int, 0xC>{});  // row_bcast:31 into rows 2 and 3
+    all = uint32_t(__builtin_amdgcn_readlane(int(s), 63));
+    return s - v;
+}
 
-__global__ __launch_bounds__(kEvT) void kv_q4_evict_select_kernel(zq_kv_q4 c, zq_kv_q4 dst, int in_place,
-                                                                  const int32_t* __restrict__ lens, uint32_t keep,
-                                                                  uint32_t recent, uint32_t first,
-                                                                  const int32_t* __restrict__ next_pos,
-                                                                  int32_t* __restrict__ ws) {
-    __shared__ uint32_t hist[256];
-    __shared__ uint32_t pick[2];  // the byte found, and the rows wanted among those that have it
-    __shared__ uint32_t sums[3][kEvT / 64];
-    const uint32_t head = blockIdx.x, s = head / uint32_t(c.kv_heads);
-    const uint32_t n = uint32_t(clamp_len(lens[s], c.capacity)), kept = min(n, keep);
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+// N: keys a thread holds, for caches of up to N * 1024 rows; N = 16 reads longer ones again
+// for every digit.
+template <int N>
+__device__ __forceinline__ void evict_rows(const zq_kv_q4& c, const zq_kv_q4& dst, int in_place, uint32_t head, uint32_t n,
+                                           uint32_t keep, int64_t newest, uint32_t first, int32_t* __restrict__ ws) {
+    constexpr int kBins = 2048;
+    __shared__ uint32_t hist[2][kBins];
+    __shared__ uint32_t pick[2];           // the digit found, and the rows wanted among those that have it
+    __shared__ uint32_t sums[kEvWaves];
+    __shared__ uint32_t counts[N][kEvWaves];
+    const uint32_t kept = keep;  // n > keep
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const float* w = c.weight + size_t(head) * c.capacity;
     const int32_t* pos = c.pos + size_t(head) * c.capacity;
     float* dw = dst.weight + size_t(head) * dst.capacity;
     int32_t* dp = dst.pos + size_t(head) * dst.capacity;
-    int32_t* from = ws + size_t(head) * 3 * keep;
-    int32_t* holes = from + keep;
-    int32_t* above = holes + keep;
-    if (n <= keep) {  // uniform: everything stays
-        for (uint32_t i = tid; i < n; i += kEvT) {
-            from[i] = int32_t(i);
-            if (!in_place) {
-                dw[i] = w[i];
-                dp[i] = pos[i];
-            }
-        }
-        return;
-    }
-    const int64_t newest = int64_t(next_pos ? next_pos[s] : int32_t(n)) - recent;
+    int32_t* from = ws + size_t(head) * 3 * keep;  // [keep] the slot that slot j's row comes from
+    int32_t* holes = from + keep;                  // free slots below the new length, ascending
+    int32_t* above = holes + keep;                 // kept slots from the new length on, ascending
     auto key = [&](uint32_t i) {
         const int32_t p = pos[i];
         return evict_key(w[i], p >= 0 && (int64_t(p) >= newest || p < int64_t(first)));
     };
-    // the key of rank `kept`, byte by byte from the top: want = rows still to be found among those that share its bytes so far
+    const bool held = N < kEvHeld || n <= uint32_t(kEvHeld * kEvT);  // uniform
+    uint32_t mine[N];
+    // (loads past the end take the last row: no branch between them, all are under way at once)
+    auto load_keys = [&](uint32_t i0) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) mine[j] = key(min(i0 + uint32_t(j * kEvT + tid), n - 1));
+    };
+    if (held) load_keys(0);
+    // the key of rank `kept`, by digits of 11, 11 and 10 bits from the top: want = rows still to be found among
+    // those that share its digits so far.  (A first digit of sign, exponent and two bits spreads weights over
+    // enough bins that the LDS atomics of a wave seldom meet.)
     uint32_t prefix = 0, want = kept;
-    for (int shift = 24; shift >= 0; shift -= 8) {
-        for (int i = tid; i < 256; i += kEvT) hist[i] = 0;
-        __syncthreads();
-        for (uint32_t i = tid; i < n; i += kEvT) {
-            const uint32_t x = key(i);
-            if (shift == 24 || (x >> (shift + 8)) == (prefix >> (shift + 8))) atomicAdd(&hist[(x >> shift) & 255u], 1u);
+    hist[0][tid] = hist[0][tid + kEvT] = 0;
+    __syncthreads();
+    for (int d = 0; d < 3; ++d) {
+        const int shift = d == 0 ? 21 : d == 1 ? 10 : 0, up = d == 0 ? 32 : d == 1 ? 21 : 10;
+        const uint32_t mask = d == 2 ? 1023u : 2047u;
+        uint32_t* bins = hist[d & 1];
+        auto count = [&](uint32_t x) {
+            if (d == 0 || (x >> up) == (prefix >> up)) atomicAdd(&bins[(x >> shift) & mask], 1u);
+        };
+        if (held) {
+#pragma unroll
+            for (int j = 0; j < N; ++j)
+                if (uint32_t(j * kEvT) < n && uint32_t(j * kEvT + tid) < n) count(mine[j]);
+        } else {
+            for (uint32_t i = tid; i < n; i += kEvT) count(key(i));
         }
         __syncthreads();
-        if (wave == 0) {  // lane l holds bins 255 - 4 l down to 252 - 4 l; rows in higher bins than its own by a scan
-            uint32_t h[4], t = 0;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) t += h[j] = hist[255 - 4 * lane - j];
-            uint32_t up = t;
-            for (int o = 1; o < 64; o <<= 1) {
-                const uint32_t x = uint32_t(__shfl_up(int(up), o));
-                if (lane >= o) up += x;
-            }
-            uint32_t before = up - t;  // rows of higher bins
-            if (before < want && want <= up) {
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    if (before < want && want <= before + h[j]) {
-                        pick[0] = uint32_t(255 - 4 * lane - j);
-                        pick[1] = want - before;
-                    }
-                    before += h[j];
-                }
-            }
+        // thread t holds bins 2047 - 2 t and 2046 - 2 t; rows in higher bins than its own by two scans
+        const uint32_t h0 = bins[kBins - 1 - 2 * tid], h1 = bins[kBins - 2 - 2 * tid];
+        hist[(d + 1) & 1][tid] = hist[(d + 1) & 1][tid + kEvT] = 0;  // the next digit's
+        uint32_t all;
+        uint32_t before = wave_before(h0 + h1, all);
+        if (lane == 0) sums[wave] = all;
+        __syncthreads();
+        for (int k = 0; k < kEvWaves; ++k) before += k < wave ? sums[k] : 0u;
+        if (before < want && want <= before + h0) {
+            pick[0] = uint32_t(kBins - 1 - 2 * tid);
+            pick[1] = want - before;
+        } else if (before + h0 < want && want <= before + h0 + h1) {
+            pick[0] = uint32_t(kBins - 2 - 2 * tid);
+            pick[1] = want - before - h0;
         }
         __syncthreads();
         prefix |= pick[0] << shift;
         want = pick[1];
-        __syncthreads();
     }
     // in slot order: a row stays if its key is above the found one, or equal and among the first `want`
-    uint32_t equal = 0, free_n = 0, above_n = 0;  // counts of the chunks before this one
-    for (uint32_t i0 = 0; i0 < n; i0 += kEvT) {
-        const uint32_t i = i0 + tid;
-        const uint32_t x = i < n ? key(i) : 0u;
-        const bool eq = i < n && x == prefix;
-        const uint64_t beq = __ballot(eq), below = (uint64_t(1) << lane) - 1;
-        if (lane == 0) sums[0][wave] = uint32_t(__popcll(beq));
+    const uint64_t below = (uint64_t(1) << lane) - 1;
+    uint32_t equal = 0, free_n = 0, above_n = 0;  // of the 16384 rows' passes before this one
+    for (uint32_t i0 = 0; i0 < n; i0 += N * kEvT) {
+        if (!held) load_keys(i0);
+        // counts of [j][wave], then what stands before each of them in slot order; returns the sum of all
+        constexpr int SW = (N * kEvWaves + 63) / 64;  // waves that scan
+        auto scan_counts = [&] {
+            __syncthreads();
+            if (wave < SW) {
+                uint32_t& at = counts[tid / kEvWaves][tid % kEvWaves];
+                uint32_t all;
+                const uint32_t b = wave_before(tid < N * kEvWaves ? at : 0u, all);
+                if (tid < N * kEvWaves) at = b;
+                if (lane == 0) sums[wave] = all;
+            }
+            __syncthreads();
+            uint32_t all = 0;
+            for (int k = 0; k < SW; ++k) all += sums[k];
+            return all;
+        };
+        auto before = [&](int j) {  // of this wave's part of [j]
+            uint32_t b = counts[j][wave];
+            const int q = j * kEvWaves / 64;  // the scanning wave that part belonged to
+            for (int k = 0; k < q; ++k) b += sums[k];
+            return b;
+        };
         __syncthreads();
-        uint32_t r = equal + uint32_t(__popcll(beq & below)), all = 0;
-        for (int k = 0; k < kEvT / 64; ++k) {
-            const uint32_t t = sums[0][k];
-            r += k < wave ? t : 0u;
-            all += t;
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const uint32_t i = i0 + uint32_t(j * kEvT + tid);
+            uint64_t eq = 0;
+            if (i0 + uint32_t(j * kEvT) < n) eq = __ballot(i < n && mine[j] == prefix);  // uniform
+            if (lane == 0) counts[j][wave] = uint32_t(__popcll(eq));
         }
-        equal += all;
-        const bool stay = i < n && (x > prefix || (eq && r < want));
-        const bool hole = i < kept && !stay, up = i >= kept && stay;
-        const uint64_t bh = __ballot(hole), bu = __ballot(up);
-        if (lane == 0) {
-            sums[1][wave] = uint32_t(__popcll(bh));
-            sums[2][wave] = uint32_t(__popcll(bu));
-        }
-        __syncthreads();
-        uint32_t rh = free_n + uint32_t(__popcll(bh & below)), ru = above_n + uint32_t(__popcll(bu & below));
-        for (int k = 0; k < kEvT / 64; ++k) {
-            const uint32_t a = sums[1][k], b = sums[2][k];
-            rh += k < wave ? a : 0u;
-            ru += k < wave ? b : 0u;
-            free_n += a;
-            above_n += b;
-        }
-        if (hole) holes[rh] = int32_t(i);
-        if (up) above[ru] = int32_t(i);
-        if (i < kept && stay) {
-            from[i] = int32_t(i);
-            if (!in_place) {
-                dw[i] = w[i];
-                dp[i] = pos[i];
+        const uint32_t eq_all = scan_counts();
+        uint32_t stay = 0;  // bit j: row j stays
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const uint32_t i = i0 + uint32_t(j * kEvT + tid);
+            if (i0 + uint32_t(j * kEvT) < n) {  // uniform
+                const bool eq = i < n && mine[j] == prefix;
+                const uint64_t b = __ballot(eq);
+                const uint32_t r = equal + before(j) + uint32_t(__popcll(b & below));
+                if (i < n && (mine[j] > prefix || (eq && r < want))) stay |= 1u << j;
             }
         }
-        // the next chunk writes sums[0] behind this chunk's second barrier, and sums[1], [2] behind its own first
+        equal += eq_all;
+        __syncthreads();  // the counts are read
+        // holes and kept rows above, counted together: 16 bits each (at most 16384 in a pass)
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const uint32_t i = i0 + uint32_t(j * kEvT + tid);
+            const bool st = (stay >> j) & 1u;
+            uint64_t h = 0, u = 0;
+            if (i0 + uint32_t(j * kEvT) < n) h = __ballot(i < kept && !st), u = __ballot(i >= kept && st);
+            if (lane == 0) counts[j][wave] = uint32_t(__popcll(h)) | uint32_t(__popcll(u)) << 16;
+        }
+        const uint32_t both = scan_counts();
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const uint32_t i = i0 + uint32_t(j * kEvT + tid);
+            if (i0 + uint32_t(j * kEvT) < n) {
+                const bool st = (stay >> j) & 1u, hole = i < kept && !st, up = i >= kept && st;
+                const uint64_t h = __ballot(hole), u = __ballot(up);
+                const uint32_t b = before(j);
+                if (hole) holes[free_n + (b & 0xffffu) + uint32_t(__popcll(h & below))] = int32_t(i);
+                if (up) above[above_n + (b >> 16) + uint32_t(__popcll(u & below))] = int32_t(i);
+                if (i < kept && st) {
+                    from[i] = int32_t(i);
+                    if (!in_place) {
+                        dw[i] = w[i];
+                        dp[i] = pos[i];
+                    }
+                }
+            }
+        }
+        free_n += both & 0xffffu;
+        above_n += both >> 16;
     }
     __syncthreads();  // the lists, written by other waves of this workgroup
     for (uint32_t x = tid; x < free_n; x += kEvT) {
@@ -333,43 +385,82 @@ __global__ __launch_bounds__(kEvT) void kv_q4_evict_select_kernel(zq_kv_q4 c, zq
         dw[h] = w[a];
         dp[h] = pos[a];
     }
-    if (!in_place) return;
     __syncthreads();  // every moved weight and pos has been read
-    for (uint32_t i = kept + tid; i < n; i += kEvT) {
-        dw[i] = -INFINITY;
-        dp[i] = -1;
-    }
+    if (in_place)
+        for (uint32_t i = kept + tid; i < n; i += kEvT) {
+            dw[i] = -INFINITY;
+            dp[i] = -1;
+        }
 }
 
-// A workgroup copies 64 rows of one (sequence, kv head): codes in 16-byte parts,
-// scales one by one from their planes.
+__global__ __launch_bounds__(kEvT) void kv_q4_evict_kernel(zq_kv_q4 c, zq_kv_q4 dst, int in_place,
+                                                           const int32_t* __restrict__ lens, uint32_t keep,
+                                                           uint32_t recent, uint32_t first,
+                                                           const int32_t* __restrict__ next_pos,
+                                                           int32_t* __restrict__ ws) {
+    const uint32_t head = blockIdx.x, s = head / uint32_t(c.kv_heads);
+    const uint32_t n = uint32_t(clamp_len(lens[s], c.capacity));
+    if (n <= keep) {  // everything stays
+        int32_t* from = ws + size_t(head) * 3 * keep;
+        const size_t at = size_t(head) * c.capacity, to = size_t(head) * dst.capacity;
+        for (uint32_t i = threadIdx.x; i < n; i += kEvT) {
+            from[i] = int32_t(i);
+            if (!in_place) {
+                dst.weight[to + i] = c.weight[at + i];
+                dst.pos[to + i] = c.pos[at + i];
+            }
+        }
+        return;
+    }
+    const int64_t newest = int64_t(next_pos ? next_pos[s] : int32_t(n)) - recent;
+    if (n <= 2 * kEvT) evict_rows<2>(c, dst, in_place, head, n, keep, newest, first, ws);
+    else evict_rows<kEvHeld>(c, dst, in_place, head, n, keep, newest, first, ws);
+}
+
+// A workgroup copies 64 rows of one (sequence, kv head): codes in 16-byte parts, scales
+// one by one from their planes, all loads before the stores.
 constexpr uint32_t kMoveRows = 64;
+template <int D>
 __global__ __launch_bounds__(kT) void kv_q4_evict_move_kernel(zq_kv_q4 c, zq_kv_q4 dst, int in_place,
                                                               const int32_t* __restrict__ lens, uint32_t keep,
                                                               const int32_t* __restrict__ ws, uint32_t parts) {
-    const uint32_t head = blockIdx.x / parts, j0 = blockIdx.x % parts * kMoveRows;
-    const uint32_t s = head / uint32_t(c.kv_heads), D = uint32_t(c.head_dim);
+    constexpr uint32_t P = D / 32;  // 16-byte parts of a row's codes, and its scales
+    constexpr uint32_t I = (kMoveRows * P + kT - 1) / kT;
+    __shared__ int32_t from[kMoveRows];
+    const uint32_t head = blockIdx.x / parts, j0 = blockIdx.x % parts * kMoveRows, s = head / uint32_t(c.kv_heads);
     const uint32_t kept = min(uint32_t(clamp_len(lens[s], c.capacity)), keep);
     if (j0 >= kept) return;
-    const uint32_t rows = min(kept - j0, kMoveRows);
-    const int32_t* from = ws + size_t(head) * 3 * keep + j0;
-    const uint32_t P = D / 32;  // 16-byte parts of a row's codes, and its scales
+    const uint32_t n = min(kept - j0, kMoveRows), tid = threadIdx.x;
+    if (tid < kMoveRows) from[tid] = ws[size_t(head) * 3 * keep + j0 + min(tid, n - 1)];
+    __syncthreads();
     const size_t src = size_t(head) * c.capacity, to = size_t(head) * dst.capacity + j0;
-    for (uint32_t e = threadIdx.x; e < rows * P; e += kT) {
-        const uint32_t j = e / P, p = e % P;
-        const uint32_t f = uint32_t(from[j]);
-        if (in_place && f == j0 + j) continue;
-        const size_t a = (src + f) * P + p, b = (to + j) * P + p;
-        reinterpret_cast<uint4*>(dst.k)[b] = reinterpret_cast<const uint4*>(c.k)[a];
-        reinterpret_cast<uint4*>(dst.v)[b] = reinterpret_cast<const uint4*>(c.v)[a];
+    uint4 k[I], v[I];
+    uint16_t ks[I], vs[I];
+#pragma unroll
+    for (uint32_t i = 0; i < I; ++i) {  // element e: part e % P of row e / P, and scale e / 64 of row e % 64
+        const uint32_t e = min(tid + i * kT, kMoveRows * P - 1);
+        const size_t a = (src + uint32_t(from[e / P])) * P + e % P;
+        k[i] = reinterpret_cast<const uint4*>(c.k)[a];
+        v[i] = reinterpret_cast<const uint4*>(c.v)[a];
+        const size_t b = (size_t(head) * P + e / kMoveRows) * c.capacity + uint32_t(from[e % kMoveRows]);
+        ks[i] = c.k_scale[b];
+        vs[i] = c.v_scale[b];
     }
-    for (uint32_t e = threadIdx.x; e < rows * P; e += kT) {
-        const uint32_t j = e % rows, p = e / rows;
-        const uint32_t f = uint32_t(from[j]);
-        if (in_place && f == j0 + j) continue;
-        const size_t a = (size_t(head) * P + p) * c.capacity + f, b = (size_t(head) * P + p) * dst.capacity + j0 + j;
-        dst.k_scale[b] = c.k_scale[a];
-        dst.v_scale[b] = c.v_scale[a];
+#pragma unroll
+    for (uint32_t i = 0; i < I; ++i) {
+        const uint32_t e = tid + i * kT;
+        if (e >= kMoveRows * P) break;
+        const uint32_t j = e / P, js = e % kMoveRows;
+        if (j < n && !(in_place && uint32_t(from[j]) == j0 + j)) {
+            const size_t b = (to + j) * P + e % P;
+            reinterpret_cast<uint4*>(dst.k)[b] = k[i];
+            reinterpret_cast<uint4*>(dst.v)[b] = v[i];
+        }
+        if (js < n && !(in_place && uint32_t(from[js]) == j0 + js)) {
+            const size_t b = (size_t(head) * P + e / kMoveRows) * dst.capacity + j0 + js;
+            dst.k_scale[b] = ks[i];
+            dst.v_scale[b] = vs[i];
+        }
     }
 }
 
@@ -441,13 +532,18 @@ size_t kv_q4_evict_bytes(const zq_kv_q4& c, size_t keep) {
 hipError_t launch_kv_q4_evict(const zq_kv_q4& c, const zq_kv_q4& dst, bool in_place, const int32_t* lens, size_t keep,
                               size_t recent, size_t first, const int32_t* next_pos, void* ws, hipStream_t stream) {
     const uint32_t heads = uint32_t(c.seqs * c.kv_heads), kp = uint32_t(keep < c.capacity ? keep : c.capacity);
-    hipLaunchKernelGGL(kv_q4_evict_select_kernel, dim3(heads), dim3(kEvT), 0, stream, c, dst, in_place ? 1 : 0, lens, kp,
+    hipLaunchKernelGGL(kv_q4_evict_kernel, dim3(heads), dim3(kEvT), 0, stream, c, dst, in_place ? 1 : 0, lens, kp,
                        uint32_t(recent), uint32_t(first), next_pos, static_cast<int32_t*>(ws));
-    hipError_t e = hipGetLastError();
+    const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     const uint32_t parts = (kp + kMoveRows - 1) / kMoveRows;
-    hipLaunchKernelGGL(kv_q4_evict_move_kernel, dim3(heads * parts), dim3(kT), 0, stream, c, dst, in_place ? 1 : 0, lens,
-                       kp, static_cast<const int32_t*>(ws), parts);
+#define ZQ_KV(DD)                                                                                                  \
+    hipLaunchKernelGGL(kv_q4_evict_move_kernel<DD>, dim3(heads * parts), dim3(kT), 0, stream, c, dst, in_place ? 1 : 0, \
+                       lens, kp, static_cast<const int32_t*>(ws), parts)
+    if (c.head_dim == 64) ZQ_KV(64);
+    else if (c.head_dim == 128) ZQ_KV(128);
+    else ZQ_KV(256);
+#undef ZQ_KV
     return hipGetLastError();
 }
 

@@ -1160,15 +1160,32 @@ struct Plan {
     bool many;
     uint32_t splits;
 };
-Plan plan_of(const zq_kv_q4& c, size_t rows) {
+// The 16-row kernel reads and decodes the keys for every 16 rows, the 128-row kernel once,
+// but a workgroup of it starts and ends slower (its queries pass through LDS, its sums are
+// merged): it pays from 48 rows on (D = 256: 64) where there are row tiles for half the
+// CUs.  us, 16-row against 128-row kernel:
+//   16 sequences x 8 kv heads, 3000 rows held, D = 128: 48 rows 51 / 53, 64 rows 63 / 54,
+//   128 rows 110 / 70; 16 x 4, D = 64: 28 rows 18 / 24, 56 rows 29 / 27; 16 x 4, D = 256:
+//   64 rows 70 / 76, 100 rows 102 / 90;  1 sequence x 8, 8000 rows, D = 128: 64 rows 21 / 25,
+//   192 rows 33 / 35, 256 rows 40 / 39.
+// (With weights, up to 64 rows and more: the kernels that sum them ask for it.)
+Plan plan_of(const zq_kv_q4& c, size_t rows, bool weights) {
     Plan p;
-    p.many = rows > 64;
+    const size_t heads = c.seqs * c.kv_heads, cus = size_t(device_cu_count());
+    p.many = weights ? rows > size_t(kWgtRows)
+                     : rows > (c.head_dim == 256 ? 64 : 48) && heads * ((rows + 15) / 16) > cus / 2;
     const size_t tile = p.many ? kTileRows : 16;
-    const size_t base = c.seqs * c.kv_heads * ((rows + tile - 1) / tile);
-    // few rows: three workgroups a CU; where there are as many sequences and heads as CUs, six, so that their
-    // lengths even out (64 sequences of up to 8190 rows: 1 split 76, 2 70, 3 60, 4 63, 6 65 us)
-    const size_t cus = size_t(device_cu_count()), want = (cus * (p.many ? 1 : base < cus ? 3 : 6) + base - 1) / base;
-    const size_t most = p.many ? (c.capacity + 511) / 512 : (c.capacity / 32 + kWaves - 1) / kWaves;
+    const size_t base = heads * ((rows + tile - 1) / tile);
+    size_t want, most;
+    if (p.many) {  // one workgroup a CU
+        want = cus / base;
+        most = (c.capacity + 255) / 256;
+    } else {
+        // three workgroups a CU; where there are as many sequences and heads as CUs, six, so that their lengths even
+        // out (64 sequences of up to 8190 rows: 1 split 76, 2 70, 3 60, 4 63, 6 65 us)
+        want = (cus * (base < cus ? 3 : 6) + base - 1) / base;
+        most = (c.capacity / 32 + kWaves - 1) / kWaves;
+    }
     p.splits = uint32_t(std::max<size_t>(1, std::min<size_t>({want, most, 128})));
     return p;
 }
@@ -1180,7 +1197,7 @@ size_t pad_rows(size_t rows) { return (rows + kTileRows - 1) / kTileRows * kTile
 
 size_t attention_q4_bytes(const zq_kv_q4& c, size_t tokens, size_t heads, int flags) {
     const size_t rows = tokens * (heads / c.kv_heads), all = c.seqs * c.kv_heads * rows;
-    const Plan plan = plan_of(c, rows);
+    const Plan plan = plan_of(c, rows, (flags & ZQ_ATTN_Q4_WEIGHTS) != 0);
     size_t n = 0;
     if (plan.splits > 1) n += up256(all * plan.splits * c.head_dim * 4) + up256(all * plan.splits * 8);
     if (flags & ZQ_ATTN_Q4_WEIGHTS) {
@@ -1208,7 +1225,7 @@ hipError_t launch_attention_q4(const zq_kv_q4& c, const float* q, float* out, si
     a.G = uint32_t(heads / c.kv_heads);
     a.heads_kv = uint32_t(c.seqs * c.kv_heads);
     a.rows = uint32_t(tokens) * a.G;
-    const Plan plan = plan_of(c, a.rows);
+    const Plan plan = plan_of(c, a.rows, (flags & ZQ_ATTN_Q4_WEIGHTS) != 0);
     a.splits = plan.splits;
     a.many = plan.many;
     a.full = (flags & ZQ_ATTN_Q4_FULL) != 0;

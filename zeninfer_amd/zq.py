@@ -609,7 +609,7 @@ class KVQ4:
     are checked once, here, and kept alive with the handle."""
 
     def __init__(self, k, v, k_scale, v_scale, seqs, kv_heads, head_dim, capacity, weight=None, pos=None):
-        dev = _device_index()
+        dev = self.dev = _device_index()
         rows = seqs * kv_heads * capacity
         arrays = [(k, rows * (head_dim // 2), "k"), (v, rows * (head_dim // 2), "v"),
                   (k_scale, rows * (head_dim // 32) * 2, "k_scale"), (v_scale, rows * (head_dim // 32) * 2, "v_scale"),
@@ -638,7 +638,7 @@ def _need_rows(t, seqs, tokens, stride, width, what, dev):
 
 def kv_q4_append_dev(cache, k, v, tokens, lens, counts=None, first_pos=None, stride=0, stream=None):
     """New tokens' keys and values [seqs][tokens][stride] into slots lens ... of every sequence."""
-    dev = _device_index()
+    dev = cache.dev
     width = cache.kv_heads * cache.head_dim
     k = _need_rows(k, cache.seqs, tokens, stride, width, "kv_q4_append_dev k", dev)
     v = _need_rows(v, cache.seqs, tokens, stride, width, "kv_q4_append_dev v", dev)
@@ -652,7 +652,7 @@ def kv_q4_append_dev(cache, k, v, tokens, lens, counts=None, first_pos=None, str
 
 def kv_q4_read_dev(cache, k, v, tokens, first, counts=None, stream=None):
     """Rows first ... of every sequence as fp32 [seqs][tokens][kv_heads * head_dim]; k or v may be None."""
-    dev = _device_index()
+    dev = cache.dev
     n = 4 * cache.seqs * tokens * cache.kv_heads * cache.head_dim
     k = _need(k, n, "kv_q4_read_dev k", dev)
     v = _need(v, n, "kv_q4_read_dev v", dev)
@@ -670,7 +670,7 @@ def attention_q4_workspace_bytes(cache, tokens, heads, flags=0):
 def attention_q4_dev(cache, q, out, tokens, heads, lens, scale, counts=None, stride=0, flags=0, workspace=None,
                      workspace_bytes=0, stream=None):
     """Attention of q [seqs][tokens][stride] over the cache into out [seqs][tokens][heads * head_dim]."""
-    dev = _device_index()
+    dev = cache.dev
     width = heads * cache.head_dim
     q = _need_rows(q, cache.seqs, tokens, stride, width, "attention_q4_dev q", dev)
     out = _need(out, 4 * cache.seqs * tokens * width, "attention_q4_dev out", dev)
@@ -689,7 +689,7 @@ def kv_q4_evict_workspace_bytes(cache, keep):
 def kv_q4_evict_dev(cache, lens, keep, recent, first, next_pos=None, dst=None, workspace=None, workspace_bytes=0,
                     stream=None):
     """Keeps the `keep` rows of the most weight (the `recent` newest and `first` first ones always), in place or in dst."""
-    dev = _device_index()
+    dev = cache.dev
     n = 4 * cache.seqs
     lens = _need(lens, n, "kv_q4_evict_dev lens", dev)
     next_pos = _need(next_pos, n, "kv_q4_evict_dev next_pos", dev)

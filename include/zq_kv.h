@@ -29,8 +29,9 @@ extern "C" {
 
 /* The arrays of one cache.  The caller owns them; nothing needs to start at any
  * value: rows past a sequence's length are never used.  capacity is a multiple
- * of 32 (at most 2^24), head_dim 64, 128 or 256; k, v, k_scale and v_scale are
- * 16-byte aligned. */
+ * of 32 (at most 2^24), head_dim 64, 128 or 256, seqs * kv_heads at most 2^20; k, v,
+ * k_scale and v_scale are 16-byte aligned.  One call takes at most 2^25 (sequence,
+ * token, head) rows. */
 typedef struct zq_kv_q4 {
     uint8_t* k;        /* [seqs][kv_heads][capacity][head_dim / 2] codes */
     uint8_t* v;
@@ -56,6 +57,7 @@ size_t zq_kv_q4_bytes(size_t kv_heads, size_t head_dim, size_t capacity);
  * call.  counts [seqs] (NULL: tokens): how many of a sequence's tokens are real;
  * the others, and tokens past the capacity, are not written.  pos gets
  * first_pos[s] + t (NULL: lens[s] + t) and weight 0, where the cache has them.
+ * A sequence of negative length gets nothing, as one that is full.
  * A block's scale is d = fp16(bf16(m / -8)) of its element m of largest
  * magnitude (the first of equals), at most 4096 in magnitude; the code is the
  * nearest to x / d (ties to even) in -8 .. 7, plus 8.  A token whose key or
@@ -77,7 +79,8 @@ int zq_hip_kv_q4_read_dev(const zq_kv_q4* cache, float* k, float* v, size_t toke
  * [tokens][heads * head_dim], 16-byte aligned, not overlapping q.  lens and counts
  * as in the append that came before: query t sees the slots below lens[s] + t +
  * 1, its own token's row the last.  With ZQ_ATTN_Q4_FULL every query sees the
- * lens[s] held rows and no others; where there are none its output is 0.  Outputs
+ * lens[s] held rows and no others; where there are none its output is 0.  A length
+ * below 0 counts as 0, one past the capacity as the capacity.  Outputs
  * of tokens past a sequence's count are left as they were.
  * ZQ_ATTN_Q4_WEIGHTS: weight[s][kv head][p] of every row that a query of the call
  * sees becomes the sum over the queries and the kv head's heads of their softmax
@@ -104,8 +107,10 @@ int zq_hip_attention_q4_dev(const zq_kv_q4* cache, const float* q, float* out, s
  * keep) rows; the caller keeps lens.
  * dst NULL (or of the same arrays): in place, and the slots from the new length to
  * the old get weight -inf and pos -1.  Otherwise the rows go to the same slots of
- * dst (the cache's seqs, kv_heads and head_dim; a capacity of at least keep or the
- * cache's; no array shared) and the cache stays as it is.  Both need weight and pos.
+ * dst (on the same device; the cache's seqs, kv_heads and head_dim; a capacity of at
+ * least keep or the cache's; no array shared) and the cache stays as it is.  Both need
+ * weight and pos.  Lengths count as in the attention.  At most 2^30 kept rows in all
+ * (seqs * kv_heads * keep), else ZQ_ERR_ARG.
  * workspace: zq_hip_kv_q4_evict_workspace_bytes(), 16-byte aligned. */
 size_t zq_hip_kv_q4_evict_workspace_bytes(const zq_kv_q4* cache, size_t keep);
 int zq_hip_kv_q4_evict_dev(const zq_kv_q4* cache, const zq_kv_q4* dst, const int32_t* lens, size_t keep, size_t recent,

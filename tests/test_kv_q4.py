@@ -273,6 +273,36 @@ def test_wrappers_refuse_host_and_short_tensors(monkeypatch):
         zq.kv_q4_evict_dev(c, i32(1), 16, 4, 4, next_pos=i32(0), workspace=u8(1 << 12), workspace_bytes=1 << 12)
 
 
+def test_wrappers_refuse_lengths_of_other_types(monkeypatch):
+    """torch's default integer has 64 bits: its buffer is long enough and would be read as other lengths."""
+    from zeninfer_amd import zq
+    monkeypatch.setattr(zq, "_check_device", lambda t, what: None)
+    c = zq.KVQ4(1 << 20, 2 << 20, 3 << 20, 4 << 20, 1, 2, 64, 64, weight=5 << 20, pos=6 << 20)
+    p, wrong, right = 7 << 20, torch.zeros(4, dtype=torch.int64), torch.zeros(4, dtype=torch.int32)
+    for bad in (wrong, torch.zeros(4), torch.zeros(8, dtype=torch.int16)):
+        for call in (lambda: zq.kv_q4_append_dev(c, p, p, 1, bad), lambda: zq.kv_q4_append_dev(c, p, p, 1, right, counts=bad),
+                     lambda: zq.kv_q4_append_dev(c, p, p, 1, right, first_pos=bad),
+                     lambda: zq.kv_q4_read_dev(c, p, p, 1, bad), lambda: zq.kv_q4_read_dev(c, p, p, 1, right, counts=bad),
+                     lambda: zq.attention_q4_dev(c, p, p, 1, 4, bad, 1.0),
+                     lambda: zq.attention_q4_dev(c, p, p, 1, 4, right, 1.0, counts=bad),
+                     lambda: zq.kv_q4_evict_dev(c, bad, 16, 4, 4), lambda: zq.kv_q4_evict_dev(c, right, 16, 4, 4, next_pos=bad)):
+            with pytest.raises(ValueError, match="needs int32"):
+                call()
+
+
+def test_calls_refuse_launches_past_32_bits():
+    """A launch has fewer than 2^32 threads: 256 for 4 to 16 rows of an append, for 64 kept rows of an eviction, which
+    must not stop between its two launches."""
+    from zeninfer_amd import zq
+    L, p = zq.lib(), 7 << 20
+    c = ctypes.byref(handle(zq, kv_heads=64, seqs=1, capacity=1 << 24))
+    assert L.zq_hip_kv_q4_evict_dev(c, None, p, 1 << 24, 4, 4, None, p, 1 << 62, None) == zq.ERR_ARG
+    assert L.zq_hip_kv_q4_append_dev(c, p, p, (1 << 19) + 1, 0, p, None, None, None) == zq.ERR_ARG
+    assert L.zq_hip_kv_q4_read_dev(c, p, p, (1 << 19) + 1, p, None, None) == zq.ERR_ARG
+    assert L.zq_hip_attention_q4_dev(c, p, p, 1 << 19, 128, 0, p, None, 1.0, 0, p, 1 << 62, None) == zq.ERR_ARG
+    assert L.zq_hip_attention_q4_workspace_bytes(c, 1 << 19, 128, 0) == 0
+
+
 # ---- GPU ------------------------------------------------------------------------
 class Dev:
     """A cache on the GPU beside its plain counterpart.  Everything past what is appended starts as garbage: codes of
@@ -469,6 +499,8 @@ SHAPES = [  # S, KH, G, D, C, lens, T
     (2, 2, 2, 256, 192, [96, 129], 33),
     (1, 2, 4, 128, 224, [0], 200),
     (1, 2, 8, 64, 416, [130], 270),
+    (8, 4, 2, 256, 128, [0, 88, 13, 32, 64, 1, 80, 47], 40),  # many row tiles: the 128-row kernel at its widest
+    (1, 1, 100, 64, 96, [60], 1),
 ]
 
 
@@ -549,7 +581,8 @@ def test_attention_far_scores(zq, T):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("D,T,G", [(64, 1, 8), (128, 2, 4), (256, 1, 1), (64, 20, 8), (128, 40, 4), (256, 70, 1)])
+@pytest.mark.parametrize("D,T,G", [(64, 1, 8), (128, 2, 4), (256, 1, 1), (64, 20, 8), (128, 12, 4),
+                                     (128, 40, 4), (256, 70, 1), (256, 30, 2)])
 def test_attention_of_a_long_cache(zq, D, T, G):
     """Keys split over many workgroups, and the capacity far above the length."""
     r = np.random.default_rng(D)
@@ -558,6 +591,73 @@ def test_attention_of_a_long_cache(zq, D, T, G):
     d.fill([n], 1)
     d.append(tokens(r, 1, T, 1, D), tokens(r, 1, T, 1, D), [n])
     d.check_attention(tokens(r, 1, T, G, D, 1.5), [n], 1 / math.sqrt(D), weights="set")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_many_rows_over_split_keys(zq, D):
+    """Enough rows and heads for the 128-row kernel, and keys split over its workgroups, with lengths that leave some
+    of the splits without keys."""
+    r = np.random.default_rng(D)
+    S, KH, G, T = 2, 8, 2, 70
+    lens = [1400, 300]
+    d = Dev(zq, S, KH, D, 2048)
+    d.fill(lens, 7)
+    d.append(tokens(r, S, T, KH, D), tokens(r, S, T, KH, D), lens)
+    d.check_attention(tokens(r, S, T, KH * G, D, 1.3), lens, 1 / math.sqrt(D))
+    d.check_attention(tokens(r, S, T, KH * G, D, 1.3), lens, 1 / math.sqrt(D), counts=[33, T], full=True, weights="set")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T", [1, 3, 40])
+def test_attention_lengths_that_no_cache_has(zq, T):
+    """Negative lengths count as 0 and those past the capacity as the capacity; counts below 0 as 0."""
+    r = np.random.default_rng(T)
+    S, KH, G, D, C = 6, 2, 4, 64, 96
+    d = Dev(zq, S, KH, D, C)
+    d.fill([C] * S, 3)
+    lens = [-1, -2 ** 31, C, C + 1, 2 ** 31 - 1, C - 1]
+    for counts in (None, [T, T, T, T, T, -5]):
+        q = tokens(r, S, T, KH * G, D)
+        d.check_attention(q, lens, 0.2, counts=counts, weights="set")
+        d.check_attention(q, lens, 0.2, counts=counts, full=True, weights="add")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("seed", range(24))
+def test_random_calls(zq, seed):
+    """Shapes, lengths, idle sequences, strides and flags drawn at random, an append, an attention and an eviction each."""
+    r = np.random.default_rng(1000 + seed)
+    D = int(r.choice([64, 128, 256]))
+    S, KH, G = int(r.integers(1, 6)), int(r.integers(1, 5)), int(r.integers(1, 9))
+    T = int(r.choice([1, 1, 2, 5, 17, 60]))
+    C = 32 * int(r.integers(1 + T // 32 + 1, 16))
+    lens = [int(r.integers(0, C - T + 1)) for _ in range(S)]
+    counts = [int(r.integers(0, T + 1)) if r.random() < 0.5 else T for _ in range(S)]
+    d = Dev(zq, S, KH, D, C)
+    d.fill(lens, seed)
+    d.weight.nan_to_num_(0.0)
+    d.plain.weight[:] = 0
+    at = [int(r.integers(C, 5000)) for _ in range(S)]
+    d.append(tokens(r, S, T, KH, D), tokens(r, S, T, KH, D, 0.6), lens, counts=counts, first_pos=at,
+             stride=KH * D + 4 if r.random() < 0.5 else 0)
+    full = bool(r.random() < 0.3)
+    weights = [None, "set", "add"][int(r.integers(3))]
+    d.check_attention(tokens(r, S, T, KH * G, D, 1.5), lens, float(r.uniform(0.02, 0.3)), counts=counts, full=full,
+                      weights=weights, stride=KH * G * D + 16 if r.random() < 0.5 else 0)
+    now = [n + c for n, c in zip(lens, counts)]
+    d.rows_equal(now)
+    d.plain.weight[:] = d.weight.cpu().numpy()
+    keep = int(r.integers(1, C + 10))
+    recent = int(r.integers(0, keep + 1))
+    first = int(r.integers(0, keep - recent + 1))
+    nxt = [a + c for a, c in zip(at, counts)]
+    n = zq.kv_q4_evict_workspace_bytes(d.c, keep)
+    zq.kv_q4_evict_dev(d.c, d.ints(now), keep, recent, first, next_pos=d.ints(nxt),
+                       workspace=torch.empty(n, dtype=torch.uint8, device="cuda"), workspace_bytes=n)
+    torch.cuda.synchronize()
+    d.plain.evict(now, keep, recent, first, nxt)
+    d.rows_equal([min(x, keep) for x in now])
 
 
 @pytest.mark.gpu
@@ -796,3 +896,19 @@ def test_host_addresses_are_refused(zq):
     lens = torch.zeros(1, dtype=torch.int32, device="cuda")
     with pytest.raises(zq.ZQError, match="status -1"):
         zq.kv_q4_append_dev(c, x, x, 1, lens)
+
+
+@pytest.mark.gpu
+def test_evict_refuses_a_host_destination(zq):
+    """The rows' new cache must lie on the cache's device, as the cache itself."""
+    d = Dev(zq, 1, 1, 64, 64)
+    d.fill([40], 1)
+    buf = np.zeros(1 << 16, np.uint8)
+    p = (buf.ctypes.data + 255) // 256 * 256
+    dst = zq.KVQ4(p, p + 4096, p + 8192, p + 12288, 1, 1, 64, 64, weight=p + 16384, pos=p + 20480)
+    n = zq.kv_q4_evict_workspace_bytes(d.c, 16)
+    ws = torch.empty(n, dtype=torch.uint8, device="cuda")
+    with pytest.raises(zq.ZQError, match="status -1"):
+        zq.kv_q4_evict_dev(d.c, d.ints([40]), 16, 4, 4, dst=dst, workspace=ws, workspace_bytes=n)
+    torch.cuda.synchronize()
+    assert not buf.any()

@@ -1256,7 +1256,7 @@ hipError_t launch_attention_q4(const zq_kv_q4& c, const float* q, float* out, si
     const size_t per_block = c.head_dim == 256 ? Wgt<256>::kKeys : Wgt<128>::kKeys;
     const size_t all_blocks = (c.capacity + per_block - 1) / per_block, fill = size_t(device_cu_count()) * 4 / a.heads_kv + 1;
     const size_t wblocks = a.many ? all_blocks : std::min(all_blocks, fill), key_blocks = a.heads_kv * wblocks;
-    if (blocks > 0x7fffffffu || key_blocks > 0x7fffffffu) return hipErrorInvalidValue;
+    if (a.many && a.lse && key_blocks * 512 > kMaxThreads) return hipErrorInvalidValue;  // over 150 GB of rows
 #define ZQ_ATTN_D(KERNEL, GRID, THREADS)                                                                \
     do {                                                                                                \
         if (c.head_dim == 64) hipLaunchKernelGGL(KERNEL<64>, dim3(uint32_t(GRID)), dim3(THREADS), 0, stream, a);        \

@@ -574,6 +574,7 @@ public:
             st_ = ZQ_ERR_ARG;  // an address of the host: a kernel that used it would fault
             return;
         }
+        dev_ = a.device;
         if (hipGetDevice(&was_) != hipSuccess) st_ = ZQ_ERR_HIP;
         else if (a.device != was_) {
             moved_ = hipSetDevice(a.device) == hipSuccess;
@@ -584,9 +585,18 @@ public:
         if (moved_) (void)hipSetDevice(was_);
     }
     int status() const { return st_; }
+    // p is memory of that device, too
+    bool holds(const void* p) const {
+        hipPointerAttribute_t a;
+        if (hipPointerGetAttributes(&a, p) != hipSuccess) {
+            (void)hipGetLastError();
+            return false;
+        }
+        return (a.type == hipMemoryTypeDevice || a.type == hipMemoryTypeManaged) && a.device == dev_;
+    }
 
 private:
-    int was_ = 0, st_ = ZQ_OK;
+    int was_ = 0, dev_ = 0, st_ = ZQ_OK;
     bool moved_ = false;
 };
 
@@ -683,9 +693,10 @@ int zq_hip_kv_q4_evict_dev(const zq_kv_q4* cache, const zq_kv_q4* dst, const int
     }
     if (workspace_bytes < zq::kv_q4_evict_bytes(*cache, keep)) return ZQ_ERR_ARG;
     const size_t parts = ((keep < cache->capacity ? keep : cache->capacity) + 63) / 64;
-    if (parts * cache->seqs * cache->kv_heads > 0x7fffffffu) return ZQ_ERR_ARG;
+    if (parts * cache->seqs * cache->kv_heads * 256 > zq::kMaxThreads) return ZQ_ERR_ARG;
     const OnDeviceOf dev(cache->k);
     if (dev.status() != ZQ_OK) return dev.status();
+    if (!in_place && !dev.holds(dst->k)) return ZQ_ERR_ARG;
     return status(zq::launch_kv_q4_evict(*cache, *dst, in_place, lens, keep, recent, first, next_pos, workspace,
                                          static_cast<hipStream_t>(stream)));
 }

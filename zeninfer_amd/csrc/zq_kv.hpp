@@ -7,9 +7,10 @@
 
 namespace zq {
 
-// Bounds that keep every index of the kernels in range: rows of one call and
-// grid sizes fit 31 bits, byte offsets are size_t.
-constexpr size_t kKvMaxCapacity = size_t(1) << 24, kKvMaxHeads = size_t(1) << 20, kKvMaxRows = size_t(1) << 27;
+// Bounds that keep every index of the kernels in range: rows of one call fit 31
+// bits, a launch's threads (64 a row at most) 32, as HIP asks; byte offsets are size_t.
+constexpr size_t kKvMaxCapacity = size_t(1) << 24, kKvMaxHeads = size_t(1) << 20, kKvMaxRows = size_t(1) << 25;
+constexpr size_t kMaxThreads = (size_t(1) << 32) - 1;  // of a launch
 
 // Shape, pointers and alignment of a cache, as include/zq_kv.h asks for them.
 bool kv_q4_ok(const zq_kv_q4* c);

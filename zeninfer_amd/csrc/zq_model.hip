@@ -730,20 +730,24 @@ int prefill(zq_model& m, const uint32_t* tokens, size_t n, float* logits, uint32
     m.tap_used = 0;
     m.tap_overflow = false;
     m.tap_recs.clear();
+    auto fail = [&](int st) {  // an empty cache again
+        m.cur_pos = m.cur_rows = 0;
+        return st;
+    };
     for (size_t s = 0; s < n; s += kPrefillChunk) {
         const uint32_t T = uint32_t(std::min<size_t>(kPrefillChunk, n - s));
         m.host_small[0] = uint32_t(s);
         std::memcpy(&m.host_small[8], tokens + s, size_t(T) * 4);
         if (hipMemcpyAsync(m.pos_dev, &m.host_small[0], 4, hipMemcpyHostToDevice, m.stream) != hipSuccess ||
             hipMemcpyAsync(m.tokens_dev, &m.host_small[8], size_t(T) * 4, hipMemcpyHostToDevice, m.stream) != hipSuccess)
-            return ZQ_ERR_HIP;
-        if (const int st = make_room(m, T); st != ZQ_OK) return st;
+            return fail(ZQ_ERR_HIP);
+        if (const int st = make_room(m, T); st != ZQ_OK) return fail(st);
         if (zq::launch_embed(m.embd.fmt, m.embd.p, m.tokens_dev, m.cfg.vocab, m.x, m.cfg.embedding, T, m.stream) != hipSuccess ||
             enqueue_layers(m, T) != hipSuccess)
-            return ZQ_ERR_HIP;
-        if (s + T == n && enqueue_head(m, T - 1) != hipSuccess) return ZQ_ERR_HIP;
+            return fail(ZQ_ERR_HIP);
+        if (s + T == n && enqueue_head(m, T - 1) != hipSuccess) return fail(ZQ_ERR_HIP);
         // the staging words are reused by the next chunk: wait for the copies
-        if (s + T < n && hipStreamSynchronize(m.stream) != hipSuccess) return ZQ_ERR_HIP;
+        if (s + T < n && hipStreamSynchronize(m.stream) != hipSuccess) return fail(ZQ_ERR_HIP);
         m.cur_pos += T;
         m.cur_rows += T;
     }

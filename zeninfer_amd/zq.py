@@ -621,6 +621,13 @@ class KVQ4:
         self.ref = ctypes.byref(self.c)
 
 
+def _need_ints(t, n, what, dev):
+    """Device address of n int32 values (torch's own default, int64, would be read as twice as many)."""
+    if t is not None and not isinstance(t, int) and (t.element_size() != 4 or t.is_floating_point()):
+        raise ValueError(f"{what}: needs int32, got {t.dtype}")
+    return _need(t, 4 * n, what, dev)
+
+
 def _need_rows(t, seqs, tokens, stride, width, what, dev):
     """Device address of [seqs][tokens][stride] fp32 rows of which width floats are used.  With a stride, a view of
     the columns of a wider buffer will do (its storage must hold the last row)."""
@@ -629,8 +636,8 @@ def _need_rows(t, seqs, tokens, stride, width, what, dev):
         return _need(t, n, what, dev)
     _check_device(t, what)
     have = t.untyped_storage().nbytes() - t.storage_offset() * t.element_size()
-    if t.stride(-1) != 1 or t.stride(-2) != stride:
-        raise ValueError(f"{what}: rows must be {stride} floats apart and their elements adjacent")
+    if t.element_size() != 4 or t.stride(-1) != 1 or t.stride(-2) != stride:
+        raise ValueError(f"{what}: rows must be {stride} fp32 values apart and their elements adjacent")
     if have < n:
         raise ValueError(f"{what}: buffer holds {have} bytes, the call needs {n}")
     return t.data_ptr()
@@ -642,10 +649,9 @@ def kv_q4_append_dev(cache, k, v, tokens, lens, counts=None, first_pos=None, str
     width = cache.kv_heads * cache.head_dim
     k = _need_rows(k, cache.seqs, tokens, stride, width, "kv_q4_append_dev k", dev)
     v = _need_rows(v, cache.seqs, tokens, stride, width, "kv_q4_append_dev v", dev)
-    n = 4 * cache.seqs
-    lens = _need(lens, n, "kv_q4_append_dev lens", dev)
-    counts = _need(counts, n, "kv_q4_append_dev counts", dev)
-    first_pos = _need(first_pos, n, "kv_q4_append_dev first_pos", dev)
+    lens = _need_ints(lens, cache.seqs, "kv_q4_append_dev lens", dev)
+    counts = _need_ints(counts, cache.seqs, "kv_q4_append_dev counts", dev)
+    first_pos = _need_ints(first_pos, cache.seqs, "kv_q4_append_dev first_pos", dev)
     return check(lib().zq_hip_kv_q4_append_dev(cache.ref, k, v, tokens, stride, lens, counts, first_pos,
                                                _stream(stream)), "zq_hip_kv_q4_append_dev")
 
@@ -656,9 +662,8 @@ def kv_q4_read_dev(cache, k, v, tokens, first, counts=None, stream=None):
     n = 4 * cache.seqs * tokens * cache.kv_heads * cache.head_dim
     k = _need(k, n, "kv_q4_read_dev k", dev)
     v = _need(v, n, "kv_q4_read_dev v", dev)
-    n = 4 * cache.seqs
-    first = _need(first, n, "kv_q4_read_dev first", dev)
-    counts = _need(counts, n, "kv_q4_read_dev counts", dev)
+    first = _need_ints(first, cache.seqs, "kv_q4_read_dev first", dev)
+    counts = _need_ints(counts, cache.seqs, "kv_q4_read_dev counts", dev)
     return check(lib().zq_hip_kv_q4_read_dev(cache.ref, k, v, tokens, first, counts, _stream(stream)),
                  "zq_hip_kv_q4_read_dev")
 
@@ -674,9 +679,8 @@ def attention_q4_dev(cache, q, out, tokens, heads, lens, scale, counts=None, str
     width = heads * cache.head_dim
     q = _need_rows(q, cache.seqs, tokens, stride, width, "attention_q4_dev q", dev)
     out = _need(out, 4 * cache.seqs * tokens * width, "attention_q4_dev out", dev)
-    n = 4 * cache.seqs
-    lens = _need(lens, n, "attention_q4_dev lens", dev)
-    counts = _need(counts, n, "attention_q4_dev counts", dev)
+    lens = _need_ints(lens, cache.seqs, "attention_q4_dev lens", dev)
+    counts = _need_ints(counts, cache.seqs, "attention_q4_dev counts", dev)
     workspace = _need(workspace, workspace_bytes, "attention_q4_dev workspace", dev)
     return check(lib().zq_hip_attention_q4_dev(cache.ref, q, out, tokens, heads, stride, lens, counts, scale, flags,
                                                workspace, workspace_bytes, _stream(stream)), "zq_hip_attention_q4_dev")
@@ -690,9 +694,8 @@ def kv_q4_evict_dev(cache, lens, keep, recent, first, next_pos=None, dst=None, w
                     stream=None):
     """Keeps the `keep` rows of the most weight (the `recent` newest and `first` first ones always), in place or in dst."""
     dev = cache.dev
-    n = 4 * cache.seqs
-    lens = _need(lens, n, "kv_q4_evict_dev lens", dev)
-    next_pos = _need(next_pos, n, "kv_q4_evict_dev next_pos", dev)
+    lens = _need_ints(lens, cache.seqs, "kv_q4_evict_dev lens", dev)
+    next_pos = _need_ints(next_pos, cache.seqs, "kv_q4_evict_dev next_pos", dev)
     workspace = _need(workspace, workspace_bytes, "kv_q4_evict_dev workspace", dev)
     return check(lib().zq_hip_kv_q4_evict_dev(cache.ref, dst.ref if dst is not None else None, lens, keep, recent, first,
                                               next_pos, workspace, workspace_bytes, _stream(stream)),

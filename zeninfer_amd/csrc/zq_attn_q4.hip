@@ -125,7 +125,7 @@ struct KTile {  // a wave's part of 32 keys
     static constexpr int KW = KB / 4;  // dwords, one an MFMA step
     static constexpr int NS = KB > 16 ? KB / 16 : 1;  // scales of a lane's part
     uint32_t w[2][KW];
-    uint16_t sc[2][NS];
+    uint32_t sc[2][NS];
 };
 template <int D>
 struct VTile {
@@ -196,7 +196,7 @@ __device__ __forceinline__ void scores(const KTile<D>& t, const h8_t (&qh)[D / 3
         v4f_t acc = {0, 0, 0, 0};
 #pragma unroll
         for (int j = 0; j < K::KW; ++j) {
-            const _Float16 d = __builtin_bit_cast(_Float16, t.sc[u][K::NS > 1 ? j / 4 : 0]);
+            const _Float16 d = __builtin_bit_cast(_Float16, uint16_t(t.sc[u][K::NS > 1 ? j / 4 : 0]));
             const h8_t k = dequant8(t.w[u][j], h2_t{d, d}, one);
             acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, qh[j], acc, 0, 0, 0);
             acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, ql[j], acc, 0, 0, 0);

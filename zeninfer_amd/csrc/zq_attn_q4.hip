@@ -107,6 +107,13 @@ __device__ __forceinline__ float sum_groups(float v) {
 // K and V so go from HBM into the operands without LDS, a wave takes whole tiles on
 // its own, and the running maximum is only moved (and the sums rescaled) when a score
 // passes it by 2^8: weights stay below 2^14, within fp16.
+// Bound by the rows' bytes with one row tile and many keys: 64 sequences of up to 8190 rows,
+// 8 kv heads x 4, D = 128: 242 MB in 62.6 us, 3.9 TB/s (a large copy: 5.0).  By latency with
+// one sequence: 24,001 rows 12.3 us (+ 4.2 for joining the splits), 601 rows 6.3 (+ 3.4).  By
+// the decoding, two vector instructions a value, with several row tiles: 16 sequences of up to
+// 3001 rows, 4 kv heads x 7, D = 64, 6 tokens: 15.1 us (+ 5.5).  Tiles two deep on their way
+// cost a wave a SIMD (65 us for the first), two row tiles a workgroup more registers than their
+// shared decoding gives (16.5 for the last).
 constexpr int kWaves = 4;
 constexpr float kShift = 6.0f;  // weights are 2^(s - max + kShift)
 constexpr float kSlack = 8.0f;  // how far a score may pass the running maximum
@@ -430,6 +437,12 @@ __global__ __launch_bounds__(kWaves * 64, D == 64 ? 4 : D == 128 ? 3 : 2) void a
 //  * row rho of the S^T product reads key rho with bits 2 and 3 exchanged, so that a
 //    lane's 16 scores are those of keys 8 h .. 8 h + 7 and 16 + 8 h .. (h = lane >> 5):
 //    the B operands of the second product as they are, and V^T is read in 16-byte runs.
+// Bound by the matrix products, twice those of the formula as both fp32 factors go in as two
+// parts: 1024 tokens behind 7168 rows, 32 heads, D = 128: 258 GF in 275 us, 0.94 PF/s (a
+// large f16 product: 1.1).  A whole prompt of 2048 tokens takes 95 us, 0.73 PF/s: the first
+// tiles see few keys, and a workgroup takes 5 us to stage its queries (D = 256: 11).  D = 256, 4
+// sequences of up to 1777 rows, 333 tokens, 4 heads: 55 us + 6 for joining the splits.  Two
+// workgroups of four waves a CU instead of one of eight: 99 us for the prompt.
 constexpr uint32_t kTileRows = 128;
 typedef float v16f_t __attribute__((ext_vector_type(16)));
 
@@ -813,7 +826,7 @@ __global__ __launch_bounds__(Big<D>::T) void attn_q4_many_kernel(AttnQ4 a) {
 
 // The splits' partial outputs of a row as one, by a workgroup of one wave (many rows,
 // few splits) or four: D / 4 lanes take a split's output, so WAVES * 256 / D splits are
-// read at a time.
+// read at a time.  Bound by latency, 3 to 6 us (one wave a row for all: 29 us at 96 splits).
 template <int D, int WAVES>
 __global__ __launch_bounds__(64 * WAVES) void attn_q4_combine_kernel(AttnQ4 a) {
     constexpr int RL = D / 4, P = 64 * WAVES / RL;
@@ -870,9 +883,14 @@ __global__ __launch_bounds__(64 * WAVES) void attn_q4_combine_kernel(AttnQ4 a) {
 }
 
 // ---- the rows' weights ----------------------------------------------------------
-// At most kScoreRows rows (a decode step): the attention kernel has left its scores,
-// 4 bytes a row and key beside the key's 72 to 288, and what is left is their sum.
-constexpr uint32_t kScoreRows = 8;
+// At most kScoreRows rows, one row tile (a decode step): the attention kernel has left its
+// scores, 4 bytes a row and key beside the key's 72 to 288, and what is left is their sum;
+// bound by reading them.  Whole call with its weights, us, scores stored against the
+// products of the kernel below: 16 sequences x 8 kv heads, 4000 rows held: D = 128, 4 rows
+// 28 / 44, 16 rows 38 / 48, 32 rows (if two row tiles stored theirs) 68 / 68; D = 64, 4 rows
+// 23 / 29, 16 rows 32 / 32, 32 rows 54 / 45; D = 256 (4 kv heads) 16 rows 42 / 62.  1 sequence,
+// 8000 rows, D = 128, 4 rows: 15 / 18.
+constexpr uint32_t kScoreRows = 16;
 __global__ __launch_bounds__(256) void attn_q4_weights_sum_kernel(AttnQ4 a) {
     const uint32_t head = blockIdx.x % a.heads_kv, key = (blockIdx.x / a.heads_kv * 256 + threadIdx.x) * 4;
     const Seq x = seq_of(a, head);
@@ -1017,7 +1035,9 @@ __device__ __forceinline__ float lane_weight(const float (&w)[KU], int lh) {
     return v;
 }
 
-// Up to 64 rows, staged once: four waves, which go on to further keys.
+// Up to 64 rows, staged once: four waves, which go on to further keys.  Bound by the keys'
+// decoding and the exponentials: 16 sequences x 8 kv heads, 4000 rows held, 32 rows, D = 128:
+// a whole call takes 68 us with it, 48 without weights.
 template <int D>
 __global__ __launch_bounds__(256) void attn_q4_weights_few_kernel(AttnQ4 a, uint32_t blocks) {
     using W = Wgt<D>;
@@ -1068,6 +1088,8 @@ __global__ __launch_bounds__(256) void attn_q4_weights_few_kernel(AttnQ4 a, uint
 // Many rows: eight waves, four on each half of the passing 64
 // rows, whose operands the attention kernel has left in memory.  The next tile's
 // products stand between this one's exponentials; operands are loaded two tiles ahead.
+// Bound by the products: 1024 tokens x 32 heads over 8192 rows, D = 128: 129 GF in two parts
+// in 127 to 137 us, 1.0 PF/s (with the operands made here again: 233).
 template <int D>
 __global__ __launch_bounds__(512) void attn_q4_weights_many_kernel(AttnQ4 a) {
     using W = Wgt<D>;
@@ -1168,7 +1190,10 @@ struct Plan {
 //   128 rows 110 / 70; 16 x 4, D = 64: 28 rows 18 / 24, 56 rows 29 / 27; 16 x 4, D = 256:
 //   64 rows 70 / 76, 100 rows 102 / 90;  1 sequence x 8, 8000 rows, D = 128: 64 rows 21 / 25,
 //   192 rows 33 / 35, 256 rows 40 / 39.
-// (With weights, up to 64 rows and more: the kernels that sum them ask for it.)
+// With weights it takes more than 64 rows, whose weights need its operands (the other way
+// holds all rows in LDS).  us, 16-row against 128-row kernel, weights and all: 16 x 8, 4000
+// rows held, D = 128: 32 rows 68 / 105, 64 rows 103 / 111; D = 64: 64 rows 69 / 85; 16 x 4,
+// D = 256: 64 rows 120 / 149.
 Plan plan_of(const zq_kv_q4& c, size_t rows, bool weights) {
     Plan p;
     const size_t heads = c.seqs * c.kv_heads, cus = size_t(device_cu_count());

@@ -1037,7 +1037,7 @@ __device__ __forceinline__ float lane_weight(const float (&w)[KU], int lh) {
 
 // Up to 64 rows, staged once: four waves, which go on to further keys.  Bound by the keys'
 // decoding and the exponentials: 16 sequences x 8 kv heads, 4000 rows held, 32 rows, D = 128:
-// a whole call takes 68 us with it, 48 without weights.
+// 24 us (8.4 GF in two parts: 0.35 PF/s).
 template <int D>
 __global__ __launch_bounds__(256) void attn_q4_weights_few_kernel(AttnQ4 a, uint32_t blocks) {
     using W = Wgt<D>;

@@ -427,10 +427,13 @@ __global__ __launch_bounds__(kWaves * 64, D == 64 ? 4 : D == 128 ? 3 : 2) void a
 
 // ---- many rows: tiles of 128 rows, keys decoded once a tile into LDS ----------------
 // v_mfma_f32_32x32x16_f16, transposed as above.  A workgroup takes 128 rows; its
-// waves stand in four groups of 32 rows, for D <= 128 twice, each half with its 32
-// keys of every staged 64 (their sums are merged at the end), so a SIMD holds two
-// waves whose matrix and vector work overlap.  For D = 256 a wave needs more than 256
-// registers, and four waves take both halves.
+// eight waves stand in four groups of 32 rows, twice, so a SIMD holds two waves whose
+// matrix and vector work overlap.  For D <= 128 each half has its 32 keys of every staged
+// 64, and their sums are merged at the end.  For D = 256 that would take more than the 256
+// registers of a wave: each half has its 128 dimensions of every staged 32 keys, of the
+// queries and of the output, and the two waves of a row group exchange their parts of the
+// scores through LDS (both then compute the weights).  Four waves with the whole dimension
+// each, one a SIMD, took 20 % longer.
 //  * the keys of a step are decoded into LDS as fp16, K row-major with the dwords' own
 //    element order, V transposed, into two buffers each, one barrier a step: decoding
 //    a value takes two vector instructions, which 128 rows share;
@@ -440,8 +443,8 @@ __global__ __launch_bounds__(kWaves * 64, D == 64 ? 4 : D == 128 ? 3 : 2) void a
 // Bound by the matrix products, twice those of the formula as both fp32 factors go in as two
 // parts: 1024 tokens behind 7168 rows, 32 heads, D = 128: 258 GF in 275 us, 0.94 PF/s (a
 // large f16 product: 1.1).  A whole prompt of 2048 tokens takes 95 us, 0.73 PF/s: the first
-// tiles see few keys, and a workgroup takes 5 us to stage its queries (D = 256: 11).  D = 256, 4
-// sequences of up to 1777 rows, 333 tokens, 4 heads: 55 us + 6 for joining the splits.  Two
+// tiles see few keys, and a workgroup takes 5 us to stage its queries.  D = 256, 4
+// sequences of up to 1777 rows, 333 tokens, 4 heads: 44 us + 6 for joining the splits.  Two
 // workgroups of four waves a CU instead of one of eight: 99 us for the prompt.
 constexpr uint32_t kTileRows = 128;
 typedef float v16f_t __attribute__((ext_vector_type(16)));
@@ -449,16 +452,18 @@ typedef float v16f_t __attribute__((ext_vector_type(16)));
 template <int D>
 struct Big {
     static constexpr int KG = D <= 128 ? 2 : 1;  // 32-key parts of a step, each with waves of its own
-    static constexpr int T = 256 * KG;           // threads
+    static constexpr int DG = 2 / KG;            // parts of the head dimension, likewise
+    static constexpr int T = 512;                // threads
     static constexpr int TK = 32 * KG;           // keys of a step
     static constexpr int HP = D + 8;             // halves of a K row in LDS: 16-byte reads of 32 rows, no conflict
     static constexpr int KP = TK + 8;            // halves of a V^T row
-    static constexpr int NT = D / 32, KS = D / 16;
-    static constexpr int kTasks = TK * NT;       // blocks of K, and 8-key column groups of V, of a step: at most 256
+    static constexpr int NT = D / 32 / DG, KS = D / 16 / DG;  // a wave's tiles of O^T, its steps of a score
+    static constexpr int kTasks = TK * D / 32;   // blocks of K, and 8-key column groups of V, of a step: at most 256
     static constexpr size_t kK = size_t(TK) * HP, kV = size_t(D) * KP;  // halves of one buffer of each
     static constexpr size_t kMerge = KG == 2 ? size_t(4) * 64 * (NT * 16 + 2) * 4 : 0;
     static constexpr size_t kQ = size_t(kTileRows) * HP;  // halves of one part of the queries
-    static constexpr size_t kLds = std::max({4 * (kK + kV), 4 * kQ, kMerge});
+    static constexpr size_t kSwap = DG == 2 ? size_t(8) * 16 * 64 : 0;  // floats: the waves' parts of a step's scores
+    static constexpr size_t kLds = std::max({4 * (kK + kV) + 8 * kSwap, 4 * kQ, kMerge});
     static_assert(kTasks <= 256 && kTasks % 64 == 0, "one task a thread, whole waves");
 };
 
@@ -611,7 +616,7 @@ __global__ __launch_bounds__(Big<D>::T) void attn_q4_many_kernel(AttnQ4 a) {
     const Cut cut = big_cut(a, x, r0, B::TK);
     if (sp >= cut.used) return;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l32 = lane & 31, lh = lane >> 5;
-    const int kg = B::KG == 2 ? wave >> 2 : 0;
+    const int kg = B::KG == 2 ? wave >> 2 : 0, dg = B::DG == 2 ? wave >> 2 : 0;
     const uint32_t rw = r0 + 32 * (wave & 3), r = rw + l32;
     const bool ok = r < rows;
     const uint32_t lim = ok ? visible(a, x, r / a.G) : 0;
@@ -622,9 +627,10 @@ __global__ __launch_bounds__(Big<D>::T) void attn_q4_many_kernel(AttnQ4 a) {
     const uint32_t t0 = sp * cut.per, t1 = min(t0 + cut.per, cut.tiles);
     _Float16* kbuf = reinterpret_cast<_Float16*>(lds);
     _Float16* vbuf = kbuf + 2 * B::kK;
-    // K by the first 256 threads, V by the others (by the same ones where there are no others)
+    float* swap = reinterpret_cast<float*>(vbuf + 2 * B::kV) + lane;
+    // K by the first 256 threads, V by the others
     const int e = tid & 255;
-    const bool kr = (B::KG == 1 || tid < 256) && e < B::kTasks, vr = (B::KG == 1 || tid >= 256) && e < B::kTasks;
+    const bool kr = tid < 256 && e < B::kTasks, vr = tid >= 256 && e < B::kTasks;
     const int em = min(e, B::kTasks - 1);  // a thread without a task loads the last one's
     const uint32_t one = code_bits();
     const float unit = unit_factor();
@@ -645,8 +651,8 @@ __global__ __launch_bounds__(Big<D>::T) void attn_q4_many_kernel(AttnQ4 a) {
     const float c = inv_q[qrow];
 #pragma unroll
     for (int j = 0; j < B::KS; ++j) {
-        qh[j] = *reinterpret_cast<const h8_t*>(kbuf + qrow * B::HP + j * 16 + 8 * lh);
-        ql[j] = *reinterpret_cast<const h8_t*>(kbuf + B::kQ + qrow * B::HP + j * 16 + 8 * lh);
+        qh[j] = *reinterpret_cast<const h8_t*>(kbuf + qrow * B::HP + (dg * B::KS + j) * 16 + 8 * lh);
+        ql[j] = *reinterpret_cast<const h8_t*>(kbuf + B::kQ + qrow * B::HP + (dg * B::KS + j) * 16 + 8 * lh);
     }
     if (a.qop && sp == 0) {  // the operands once more, for the weights
         const size_t row = size_t(head) * a.rows_pad + r0;
@@ -678,8 +684,8 @@ __global__ __launch_bounds__(Big<D>::T) void attn_q4_many_kernel(AttnQ4 a) {
     }
     __syncthreads();
     // this lane's part of a K row: bits 2 and 3 of the row exchanged
-    const int krow = 32 * kg + ((l32 & 0x13) | (l32 & 4) << 1 | (l32 & 8) >> 1), koff = krow * B::HP + 8 * lh;
-    const int voff = l32 * B::KP + 32 * kg + 8 * lh;
+    const int krow = 32 * kg + ((l32 & 0x13) | (l32 & 4) << 1 | (l32 & 8) >> 1), koff = krow * B::HP + 16 * B::KS * dg + 8 * lh;
+    const int voff = (32 * B::NT * dg + l32) * B::KP + 32 * kg + 8 * lh;
     auto product = [&](uint32_t t) {
         const _Float16* kt = kbuf + (t & 1) * B::kK + koff;
         v16f_t y;
@@ -693,7 +699,22 @@ __global__ __launch_bounds__(Big<D>::T) void attn_q4_many_kernel(AttnQ4 a) {
         }
         return y;
     };
-    if (t0 < t1) s = product(t0);
+    // DG == 2: a wave's scores are those of its half of the dimension; step t adds the other
+    // wave's, who has left them in one of two places by t (what stood there is read in t - 2)
+    auto give = [&](uint32_t t) {
+        if constexpr (B::DG == 2)
+#pragma unroll
+            for (int v = 0; v < 16; ++v) swap[(t & 1) * B::kSwap + (wave * 16 + v) * 64] = s[v];
+    };
+    auto take = [&](uint32_t t) {
+        if constexpr (B::DG == 2)
+#pragma unroll
+            for (int v = 0; v < 16; ++v) s[v] += swap[(t & 1) * B::kSwap + ((wave ^ 4) * 16 + v) * 64];
+    };
+    if (t0 < t1) {
+        s = product(t0);
+        give(t0);
+    }
     // Step t: the weights of its scores, the next step's scores, the second product and
     // the decoding of later keys (K two steps ahead, V one) stand in one run of code,
     // whose vector and matrix instructions the compiler mixes.  Past the last step the
@@ -719,6 +740,7 @@ __global__ __launch_bounds__(Big<D>::T) void attn_q4_many_kernel(AttnQ4 a) {
             asm volatile("s_nop 0");  // else the two copies of decode() become one, behind the matrix instructions
             return;
         }
+        take(t);
         if (key0 + 32 > whole) {
 #pragma unroll
             for (int v = 0; v < 16; ++v) s[v] = key0 + 16 * (v >> 3) + 8 * lh + (v & 7) < lim ? s[v] : -INFINITY;
@@ -747,6 +769,7 @@ __global__ __launch_bounds__(Big<D>::T) void attn_q4_many_kernel(AttnQ4 a) {
             split_p2(p0, p1, unit, ph[v >> 3], pl[v >> 3], v & 7);
         }
         s = next;
+        give(t + 1);
         const _Float16* vt = vbuf + (t & 1) * B::kV + voff;
 #pragma unroll
         for (int u = 0; u < 2; ++u)
@@ -763,11 +786,7 @@ __global__ __launch_bounds__(Big<D>::T) void attn_q4_many_kernel(AttnQ4 a) {
     using yes = std::true_type;
     using no = std::false_type;
     uint32_t t = t0;
-    if constexpr (B::KG == 1) {
-        if (t < t1) fetch(t, yes{}, yes{});
-        for (; t + 2 < t1; ++t) step(t, yes{}, yes{}, no{});
-        for (; t < t1; ++t) step(t, yes{}, yes{}, yes{});
-    } else if (tid < 256) {
+    if (tid < 256) {
         if (t < t1) fetch(t, yes{}, no{});
         for (; t < t1; ++t) step(t, yes{}, no{}, no{});
     } else {
@@ -804,7 +823,7 @@ __global__ __launch_bounds__(Big<D>::T) void attn_q4_many_kernel(AttnQ4 a) {
     if (!ok) return;
     const bool direct = cut.used == 1;
     const size_t row = size_t(head) * a.rows + r;
-    if (lh == 0) {
+    if (lh == 0 && dg == 0) {
         if (!direct) {
             float* ml = a.part_ml + (row * a.splits + sp) * 2;
             ml[0] = M;
@@ -813,8 +832,8 @@ __global__ __launch_bounds__(Big<D>::T) void attn_q4_many_kernel(AttnQ4 a) {
             a.lse[row] = M - kShift + log2f(L);
         }
     }
-    float* dst = direct ? a.out + ((size_t(x.s) * a.tokens + r / a.G) * a.KH * a.G + x.kh * a.G + r % a.G) * D
-                        : a.part + (row * a.splits + sp) * D;
+    float* dst = (direct ? a.out + ((size_t(x.s) * a.tokens + r / a.G) * a.KH * a.G + x.kh * a.G + r % a.G) * D
+                         : a.part + (row * a.splits + sp) * D) + 32 * B::NT * dg;
     const float inv = direct ? (L > 0.0f ? 1.0f / L : (L == 0.0f ? 0.0f : L)) : 1.0f;
 #pragma unroll
     for (int n = 0; n < B::NT; ++n)
@@ -1184,12 +1203,13 @@ struct Plan {
 };
 // The 16-row kernel reads and decodes the keys for every 16 rows, the 128-row kernel once,
 // but a workgroup of it starts and ends slower (its queries pass through LDS, its sums are
-// merged): it pays from 48 rows on (D = 256: 64) where there are row tiles for half the
-// CUs.  us, 16-row against 128-row kernel:
+// merged): it pays from more than 48 rows on, three row tiles, where there are row tiles for
+// half the CUs.  us, 16-row against 128-row kernel:
 //   16 sequences x 8 kv heads, 3000 rows held, D = 128: 48 rows 51 / 53, 64 rows 63 / 54,
 //   128 rows 110 / 70; 16 x 4, D = 64: 28 rows 18 / 24, 56 rows 29 / 27; 16 x 4, D = 256:
-//   64 rows 70 / 76, 100 rows 102 / 90;  1 sequence x 8, 8000 rows, D = 128: 64 rows 21 / 25,
-//   192 rows 33 / 35, 256 rows 40 / 39.
+//   48 rows 51 / 61, 56 rows 71 / 62;  1 sequence x 8, 8000 rows, D = 128: 64 rows 21 / 25,
+//   192 rows 33 / 35, 256 rows 40 / 39; 4 x 4, 1777 rows, D = 256: 100 rows 37 / 40, 160
+//   rows 46 / 45.
 // With weights it takes more than 64 rows, whose weights need its operands (the other way
 // holds all rows in LDS).  us, 16-row against 128-row kernel, weights and all: 16 x 8, 4000
 // rows held, D = 128: 32 rows 68 / 105, 64 rows 103 / 111; D = 64: 64 rows 69 / 85; 16 x 4,
@@ -1198,7 +1218,7 @@ Plan plan_of(const zq_kv_q4& c, size_t rows, bool weights) {
     Plan p;
     const size_t heads = c.seqs * c.kv_heads, cus = size_t(device_cu_count());
     p.many = weights ? rows > size_t(kWgtRows)
-                     : rows > (c.head_dim == 256 ? 64 : 48) && heads * ((rows + 15) / 16) > cus / 2;
+                     : rows > 48 && heads * ((rows + 15) / 16) > cus / 2;
     const size_t tile = p.many ? kTileRows : 16;
     const size_t base = heads * ((rows + tile - 1) / tile);
     size_t want, most;

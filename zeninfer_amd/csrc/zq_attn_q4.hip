@@ -109,7 +109,7 @@ __device__ __forceinline__ float sum_groups(float v) {
 // passes it by 2^8: weights stay below 2^14, within fp16.
 // Bound by the rows' bytes with one row tile and many keys: 64 sequences of up to 8190 rows,
 // 8 kv heads x 4, D = 128: 242 MB in 62.6 us, 3.9 TB/s (a large copy: 5.0).  By latency with
-// one sequence: 24,001 rows 12.3 us (+ 4.2 for joining the splits), 601 rows 6.3 (+ 3.4).  By
+// one sequence: 24,001 rows 11.8 us (+ 4.0 for joining the splits), 601 rows 6.3 (+ 3.4).  By
 // the decoding, two vector instructions a value, with several row tiles: 16 sequences of up to
 // 3001 rows, 4 kv heads x 7, D = 64, 6 tokens: 15.1 us (+ 5.5).  Tiles two deep on their way
 // cost a wave a SIMD (65 us for the first), two row tiles a workgroup more registers than their
@@ -1226,9 +1226,13 @@ Plan plan_of(const zq_kv_q4& c, size_t rows, bool weights) {
         want = cus / base;
         most = (c.capacity + 255) / 256;
     } else {
-        // three workgroups a CU; where there are as many sequences and heads as CUs, six, so that their lengths even
-        // out (64 sequences of up to 8190 rows: 1 split 76, 2 70, 3 60, 4 63, 6 65 us)
-        want = (cus * (base < cus ? 3 : 6) + base - 1) / base;
+        // Two workgroups a CU, or three where that leaves each less to do (192 row tiles: three splits 25.0 us, four
+        // 23.0; 8 row tiles, 24,000 rows: two workgroups a CU 15.4, three 16.7; 64, 2000 rows: 15.0 / 17.1).  Where
+        // there is a row tile for every CU, three splits even out what sequences of uneven length leave to do (64
+        // sequences x 8 of up to 8190 rows: 1 split 76, 2 70, 3 60, 4 63, 6 65 us; 32 x 8 of 4000 rows each: 3 splits
+        // 40.8, 6 43.6), fewer from two row tiles a CU on.
+        const size_t two = 2 * cus / base, three = 3 * cus / base;
+        want = base < cus ? (3 * two < 2 * three ? three : two) : std::min<size_t>(3, (6 * cus + base - 1) / base);
         most = (c.capacity / 32 + kWaves - 1) / kWaves;
     }
     p.splits = uint32_t(std::max<size_t>(1, std::min<size_t>({want, most, 128})));

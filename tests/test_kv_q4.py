@@ -731,7 +731,8 @@ def random_cache(zq, r, S, KH, D, C, lens):
 @pytest.mark.parametrize("D,C,lens,keep,recent,first", [
     (64, 96, [90, 0, 1, 33], 32, 8, 4), (64, 96, [90, 31, 32, 33], 1, 0, 0), (128, 128, [128, 100], 100, 100, 0),
     (128, 2112, [2100, 1025, 1024], 1000, 300, 16), (256, 96, [96, 64], 95, 0, 95), (64, 5024, [5000], 4999, 2000, 4),
-    (64, 9024, [9001, 2], 64, 10, 10), (128, 64, [64, 50], 500, 100, 4)])
+    (64, 9024, [9001, 2], 64, 10, 10), (128, 64, [64, 50], 500, 100, 4),
+    (64, 12032, [2048, 2049, 8192, 8193], 2000, 100, 4), (64, 26016, [26000, 16385], 7000, 100, 4)])
 def test_evict(zq, D, C, lens, keep, recent, first, in_place):
     r = np.random.default_rng(keep + C)
     S, KH = len(lens), 3

@@ -201,9 +201,9 @@ __global__ __launch_bounds__(kT) void kv_q4_read_kernel(zq_kv_q4 c, float* __res
 // A second launch copies the rows' codes and scales (the one workgroup would take 11 us
 // for 1024 rows of D = 64 where that launch takes 3).
 // Bound by latency: the keys in one read, three digits of an LDS histogram, the ranks.
-// 128 of them with 8192 rows take 24 us, one with 1153 rows 7.
+// 128 of them with 8192 rows take 14 us, one with 1153 rows 7.
 constexpr int kEvT = 1024, kEvWaves = kEvT / 64;
-constexpr int kEvHeld = 16;  // keys a thread holds: caches up to 16384 rows are read once
+constexpr int kEvHeld = 24;  // keys a thread holds at most: caches up to 24576 rows are read once
 
 // Order of a row: protected ones, then by weight (-0 = +0), a NaN last.
 __device__ __forceinline__ uint32_t evict_key(float w, bool held) {
@@ -231,8 +231,10 @@ __device__ __forceinline__ uint32_t wave_before(uint32_t v, uint32_t& all) {
     return s - v;
 }
 
-// N: keys a thread holds, for caches of up to N * 1024 rows; N = 16 reads longer ones again
-// for every digit.
+// N: keys a thread holds, for caches of up to N * 1024 rows; the largest N reads longer ones
+// again for every digit.  A cache takes the smallest N that holds it, as every pass over the
+// keys is N steps: 128 caches of 8192 rows take 14 us with N = 8 (20 from HBM), 23 with 16; 24,000 rows 36
+// with 24, 41 with 32 (registers spilled); 40,000 rows 107.
 template <int N>
 __device__ __forceinline__ void evict_rows(const zq_kv_q4& c, const zq_kv_q4& dst, int in_place, uint32_t head, uint32_t n,
                                            uint32_t keep, int64_t newest, uint32_t first, int32_t* __restrict__ ws) {
@@ -304,7 +306,7 @@ __device__ __forceinline__ void evict_rows(const zq_kv_q4& c, const zq_kv_q4& ds
     }
     // in slot order: a row stays if its key is above the found one, or equal and among the first `want`
     const uint64_t below = (uint64_t(1) << lane) - 1;
-    uint32_t equal = 0, free_n = 0, above_n = 0;  // of the 16384 rows' passes before this one
+    uint32_t equal = 0, free_n = 0, above_n = 0;  // of the passes over N * 1024 rows before this one
     for (uint32_t i0 = 0; i0 < n; i0 += N * kEvT) {
         if (!held) load_keys(i0);
         // counts of [j][wave], then what stands before each of them in slot order; returns the sum of all
@@ -351,7 +353,7 @@ __device__ __forceinline__ void evict_rows(const zq_kv_q4& c, const zq_kv_q4& ds
         }
         equal += eq_all;
         __syncthreads();  // the counts are read
-        // holes and kept rows above, counted together: 16 bits each (at most 16384 in a pass)
+        // holes and kept rows above, counted together: 16 bits each (at most 24576 in a pass)
 #pragma unroll
         for (int j = 0; j < N; ++j) {
             const uint32_t i = i0 + uint32_t(j * kEvT + tid);
@@ -418,6 +420,8 @@ __global__ __launch_bounds__(kEvT) void kv_q4_evict_kernel(zq_kv_q4 c, zq_kv_q4 
     }
     const int64_t newest = int64_t(next_pos ? next_pos[s] : int32_t(n)) - recent;
     if (n <= 2 * kEvT) evict_rows<2>(c, dst, in_place, head, n, keep, newest, first, ws);
+    else if (n <= 8 * kEvT) evict_rows<8>(c, dst, in_place, head, n, keep, newest, first, ws);
+    else if (n <= 16 * kEvT) evict_rows<16>(c, dst, in_place, head, n, keep, newest, first, ws);
     else evict_rows<kEvHeld>(c, dst, in_place, head, n, keep, newest, first, ws);
 }
 

@@ -609,6 +609,31 @@ def test_many_rows_over_split_keys(zq, D):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("D,T,G", [(64, 1, 4), (128, 9, 4), (64, 70, 2), (128, 70, 2), (256, 70, 2)])
+def test_equal_calls_give_equal_bits(zq, D, T, G):
+    """No result depends on the order in which waves or workgroups come to it."""
+    r = np.random.default_rng(D + T)
+    S, KH = 3, 8
+    lens = [900, 410, 0]
+    d = Dev(zq, S, KH, D, 1024)
+    d.fill(lens, 11)
+    d.append(tokens(r, S, T, KH, D), tokens(r, S, T, KH, D), lens)
+    q = torch.from_numpy(tokens(r, S, T, KH * G, D, 1.4)).cuda()
+    n = zq.attention_q4_workspace_bytes(d.c, T, KH * G, zq.ATTN_Q4_WEIGHTS)
+    got = []
+    for i in range(8):
+        ws = torch.full((n,), 0xff if i % 2 else 0, dtype=torch.uint8, device="cuda")
+        out = torch.full((S, T, KH * G, D), math.nan, device="cuda")
+        zq.attention_q4_dev(d.c, q, out, T, KH * G, d.ints(lens), 0.1, flags=zq.ATTN_Q4_WEIGHTS, workspace=ws,
+                            workspace_bytes=n)
+        torch.cuda.synchronize()
+        assert not out.isnan().any()
+        got.append((out, d.weight.clone()))
+    for out, w in got[1:]:
+        assert torch.equal(out, got[0][0]) and torch.equal(w.view(torch.int32), got[0][1].view(torch.int32))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("T", [1, 3, 40])
 def test_attention_lengths_that_no_cache_has(zq, T):
     """Negative lengths count as 0 and those past the capacity as the capacity; counts below 0 as 0."""

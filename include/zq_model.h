@@ -81,8 +81,10 @@ int zq_model_set_prefill_mode(zq_model* model, int mode);
 #define ZQ_KV_Q4 1
 int zq_model_set_kv_cache(zq_model* model, int form, uint32_t rows, uint32_t recent, uint32_t first);
 /* One layer's 4-bit cache (seqs = 1; device arrays that the model owns) for the
- * calls of zq_kv.h, the rows it holds and the positions fed so far.  ZQ_DECLINED
- * with the fp32 cache (rows and positions are set). */
+ * calls of zq_kv.h, the rows it holds and the positions fed so far.  The model
+ * counts its own tokens only: a caller reads and attends to the cache, and leaves
+ * appends and evictions to the model.  ZQ_DECLINED with the fp32 cache (rows and
+ * positions are set). */
 int zq_model_kv_cache(const zq_model* model, uint32_t layer, zq_kv_q4* cache, uint32_t* rows, uint32_t* positions);
 /* Prefill `n` tokens from position 0 (the cache is reset).  Logits of the
  * last token to `logits` (vocab floats, may be NULL); greedy id to *next. */

@@ -1,0 +1,105 @@
+"""The 4-bit KV cache's attention reads nothing outside the cache's arrays.
+
+CPU: every address that the 128-row kernel's threads stage (zq_attn_q4_at.hpp, the
+kernel's own index functions, built for the host), for every step that a capacity
+has.  GPU: arrays of their exact size inside larger ones, which hold NaN scales and
+codes of all ones behind them, give the results of a cache by itself."""
+import ctypes
+import math
+import os
+import subprocess
+
+import numpy as np
+import pytest
+import torch
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+PROGRAM = r"""
+#include "zq_attn_q4_at.hpp"
+#include <stddef.h>
+using namespace zq;
+// Steps of one (sequence, kv head) of `capacity` rows: 0 where every byte lies in its arrays (and a scale in its
+// own plane) and every key below the capacity is read at its own place, else 1 + the first bad key of a step.
+template <int D>
+static long check(uint32_t capacity) {
+    const size_t row = D / 2, planes = D / 32;
+    for (uint32_t key0 = 0; key0 < capacity; key0 += StageShape<D>::TK)
+        for (uint32_t e = 0; e < uint32_t(StageShape<D>::kTasks); ++e) {
+            {
+                const StageAt a = stage_k_at<D>(capacity, key0, e);
+                const uint32_t key = key0 + e / (D / 32), b = e % (D / 32);
+                const size_t code = key0 * row + a.codes, scale = key0 * size_t(2) + a.scales;
+                if (code + 16 > capacity * row || scale + 2 > planes * capacity * 2 || scale / 2 / capacity != b) return 1 + key;
+                if (key < capacity && (code != key * row + b * 16 || scale != (size_t(b) * capacity + key) * 2)) return 1 + key;
+            }
+            {
+                const StageAt a = stage_v_at<D>(capacity, key0, e);
+                const StageV t = stage_v_task<D>(e);
+                const uint32_t key = key0 + 8 * t.o, b = t.ch / 8;
+                const size_t code = key0 * row + a.codes, scale = key0 * size_t(2) + a.scales;
+                if (code + 7 * row + 2 > capacity * row || scale + 16 > planes * capacity * 2 || scale / 2 / capacity != b ||
+                    (scale / 2 + 7) / capacity != b || scale % 16) return 1 + key;
+                if (key < capacity && (code != key * row + 2 * t.ch || scale != (size_t(b) * capacity + key) * 2)) return 1 + key;
+            }
+        }
+    return 0;
+}
+extern "C" long check_stage(int D, uint32_t capacity) {
+    return D == 64 ? check<64>(capacity) : D == 128 ? check<128>(capacity) : check<256>(capacity);
+}
+"""
+
+
+@pytest.fixture(scope="module")
+def check_stage(tmp_path_factory):
+    tmp = tmp_path_factory.mktemp("stage")
+    (tmp / "stage.cpp").write_text(PROGRAM)
+    subprocess.run(["g++", "-O1", "-std=c++17", "-Wall", "-Werror", "-shared", "-fPIC", "-I",
+                    os.path.join(ROOT, "zeninfer_amd", "csrc"), "-o", str(tmp / "stage.so"), str(tmp / "stage.cpp")],
+                   check=True)
+    f = ctypes.CDLL(str(tmp / "stage.so")).check_stage
+    f.restype, f.argtypes = ctypes.c_long, [ctypes.c_int, ctypes.c_uint32]
+    return f
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_staged_keys_lie_in_the_arrays(check_stage, D):
+    bad = {C: check_stage(D, C) for C in [*range(32, 2049, 32), 40000, 65504, 99968]}
+    assert not {C: n - 1 for C, n in bad.items() if n}
+
+
+def inside(t):
+    """A copy of t in a larger array: 64 KiB of ones before and behind it (codes of all ones, NaN scales and weights)."""
+    pad = 1 << 16
+    raw = t.contiguous().view(torch.uint8).flatten()
+    buf = torch.full((raw.numel() + 2 * pad,), 0xff, dtype=torch.uint8, device="cuda")
+    buf[pad:pad + raw.numel()] = raw
+    return buf, buf[pad:pad + raw.numel()].view(t.dtype).view(t.shape)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("weights", [None, "set"])
+@pytest.mark.parametrize("full", [False, True])
+@pytest.mark.parametrize("S,KH,G,D,C,lens,T", [
+    (4, 8, 4, 128, 96, [56, 1, 40, 50], 40), (2, 8, 8, 64, 416, [386, 200], 30), (1, 8, 4, 128, 224, [24], 200),
+    (1, 1, 8, 64, 32, [2], 30), (4, 4, 4, 256, 160, [120, 3, 90, 60], 40), (3, 2, 4, 128, 160, [159, 0, 70], 1)])
+def test_rows_behind_the_arrays_are_nothing_to_it(zq, S, KH, G, D, C, lens, T, full, weights):
+    from tests.test_kv_q4 import Dev, tokens
+    r = np.random.default_rng(C + T)
+    d = Dev(zq, S, KH, D, C)
+    d.fill(lens, 3)
+    if not full:
+        d.append(tokens(r, S, T, KH, D), tokens(r, S, T, KH, D, 0.7), lens)
+    if full:  # every slot but the last sequence's is seen
+        d.fill([C] * S, 4)
+        lens = [C] * (S - 1) + lens[-1:] if S > 1 else [C]
+    bufs = []
+    for name in ("k", "v", "ks", "vs", "weight", "pos"):
+        buf, view = inside(getattr(d, name))
+        setattr(d, name, view)
+        bufs.append(buf)
+    d.c = zq.KVQ4(d.k, d.v, d.ks, d.vs, S, KH, D, C, weight=d.weight, pos=d.pos)
+    d.check_attention(tokens(r, S, T, KH * G, D, 1.4), lens, 1 / math.sqrt(D), full=full, weights=weights)
+    for b in bufs:
+        assert (b[:1 << 16] == 0xff).all() and (b[-(1 << 16):] == 0xff).all()

@@ -12,6 +12,7 @@
 // operands of the f16 MFMA; queries and softmax weights are fp32 and go in as two
 // fp16 parts h + l (22 bits), accumulated in fp32.
 #include "../../include/zq_hip.h"
+#include "zq_attn_q4_at.hpp"
 #include "zq_internal.hpp"
 #include "zq_kv.hpp"
 
@@ -454,17 +455,17 @@ struct Big {
     static constexpr int KG = D <= 128 ? 2 : 1;  // 32-key parts of a step, each with waves of its own
     static constexpr int DG = 2 / KG;            // parts of the head dimension, likewise
     static constexpr int T = 512;                // threads
-    static constexpr int TK = 32 * KG;           // keys of a step
+    static constexpr int TK = StageShape<D>::TK;  // keys of a step
     static constexpr int HP = D + 8;             // halves of a K row in LDS: 16-byte reads of 32 rows, no conflict
     static constexpr int KP = TK + 8;            // halves of a V^T row
     static constexpr int NT = D / 32 / DG, KS = D / 16 / DG;  // a wave's tiles of O^T, its steps of a score
-    static constexpr int kTasks = TK * D / 32;   // blocks of K, and 8-key column groups of V, of a step: at most 256
+    static constexpr int kTasks = StageShape<D>::kTasks;  // blocks of K, and 8-key column groups of V, of a step
     static constexpr size_t kK = size_t(TK) * HP, kV = size_t(D) * KP;  // halves of one buffer of each
     static constexpr size_t kMerge = KG == 2 ? size_t(4) * 64 * (NT * 16 + 2) * 4 : 0;
     static constexpr size_t kQ = size_t(kTileRows) * HP;  // halves of one part of the queries
     static constexpr size_t kSwap = DG == 2 ? size_t(8) * 16 * 64 : 0;  // floats: the waves' parts of a step's scores
     static constexpr size_t kLds = std::max({4 * (kK + kV) + 8 * kSwap, 4 * kQ, kMerge});
-    static_assert(kTasks <= 256 && kTasks % 64 == 0, "one task a thread, whole waves");
+    static_assert(TK == 32 * KG && kTasks <= 256 && kTasks % 64 == 0, "one task a thread, whole waves");
 };
 
 // Task e of K: key e / (D / 32), block e % (D / 32).  Task e of V: 8 keys, two bytes
@@ -483,12 +484,12 @@ struct VStage {
 template <int D>
 __device__ __forceinline__ void load_kstage(KStage<D>& r, const AttnQ4& a, uint32_t head, uint32_t key0, int e) {
     const size_t cap = a.c.capacity;
-    const int key = e / (D / 32), b = e % (D / 32);
+    const StageAt at = stage_k_at<D>(uint32_t(cap), key0, uint32_t(e));
     // a base that is one for the wave, and 32-bit offsets of the lane
     const uint8_t* w = a.c.k + (size_t(head) * cap + key0) * (D / 2);
     const uint8_t* d = reinterpret_cast<const uint8_t*>(a.c.k_scale + size_t(head) * (D / 32) * cap + key0);
-    r.w = *reinterpret_cast<const uint4*>(w + uint32_t(key * (D / 2) + b * 16));
-    r.d = *reinterpret_cast<const _Float16*>(d + (uint32_t(b) * uint32_t(cap) + uint32_t(key)) * 2u);
+    r.w = *reinterpret_cast<const uint4*>(w + at.codes);
+    r.d = *reinterpret_cast<const _Float16*>(d + at.scales);
 }
 template <int D>
 __device__ __forceinline__ void store_kstage(const KStage<D>& r, _Float16* kt, uint32_t one, int e) {
@@ -503,19 +504,19 @@ __device__ __forceinline__ void store_kstage(const KStage<D>& r, _Float16* kt, u
 template <int D>
 __device__ __forceinline__ void load_vstage(VStage<D>& r, const AttnQ4& a, uint32_t head, uint32_t key0, int e) {
     const size_t cap = a.c.capacity;
-    const int ch = (e >> 1) % (D / 4), o = (e & 1) + 2 * (e / (D / 2));
+    const StageAt at = stage_v_at<D>(uint32_t(cap), key0, uint32_t(e));
     const uint8_t* w = a.c.v + (size_t(head) * cap + key0) * (D / 2);
     const uint8_t* d = reinterpret_cast<const uint8_t*>(a.c.v_scale + size_t(head) * (D / 32) * cap + key0);
-    const uint32_t off = uint32_t(8 * o * (D / 2) + 2 * ch);
 #pragma unroll
-    for (int k = 0; k < 8; ++k) r.w[k] = *reinterpret_cast<const uint16_t*>(w + off + uint32_t(k * (D / 2)));
-    r.d = *reinterpret_cast<const h8_t*>(d + (uint32_t(ch / 8) * uint32_t(cap) + uint32_t(8 * o)) * 2u);
+    for (int k = 0; k < 8; ++k) r.w[k] = *reinterpret_cast<const uint16_t*>(w + at.codes + uint32_t(k * (D / 2)));
+    r.d = *reinterpret_cast<const h8_t*>(d + at.scales);
 }
 // MASK: only `keys` of the step's keys hold rows that are seen (the others' scale may be
 // any bits)
 template <int D, bool MASK>
 __device__ __forceinline__ void store_vstage(const VStage<D>& r, _Float16* vt, uint32_t keys, uint32_t one, int e) {
-    const int ch = (e >> 1) % (D / 4), o = (e & 1) + 2 * (e / (D / 2));
+    const StageV task = stage_v_task<D>(uint32_t(e));
+    const int ch = int(task.ch), o = int(task.o);
     h8_t s = r.d;
     if (MASK)
 #pragma unroll

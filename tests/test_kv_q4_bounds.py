@@ -63,6 +63,54 @@ def check_stage(tmp_path_factory):
     return f
 
 
+def views():
+    """(name, view of a [2][8][512] buffer's rows of 128 floats, seqs, tokens, row stride, whether rows are in place)."""
+    buf = torch.arange(2 * 8 * 512, dtype=torch.float32).reshape(2, 8, 512)
+    flat = buf.reshape(16, 512)
+    return [
+        ("all tokens", buf[:, :, 128:256], 2, 8, 512, True),
+        ("flattened", flat[:, 128:256], 2, 8, 512, True),
+        ("heads apart", buf[:, :, 128:256].unflatten(-1, (2, 64)), 2, 8, 512, True),
+        ("heads apart, flattened", flat[:, 128:256].unflatten(-1, (2, 64)), 2, 8, 512, True),
+        ("one sequence", buf[1:, :3, :128], 1, 3, 512, True),
+        ("one sequence without its dimension", buf[1, :3, 64:192], 1, 3, 512, True),
+        ("one token", buf[:1, 4:5, :128], 1, 1, 512, True),
+        ("more rows than asked", flat[:, :128], 2, 3, 512, True),
+        ("wider rows than asked", buf[:, :, 128:300], 2, 8, 512, True),
+        ("a token of each sequence", buf[:, 5, :128], 2, 1, 8 * 512, True),
+        ("a token of each sequence, dimension kept", buf[:, 5:6, :128], 2, 1, 8 * 512, True),
+        ("some tokens of each sequence", buf[:, :3, :128], 2, 3, 512, False),
+        ("sequences in place, tokens not asked for", buf[:, :, :128], 2, 3, 512, False),
+        ("a token of each sequence, by the tokens' stride", buf[:, 5, :128], 2, 1, 512, False),
+        ("every other token", buf[:, ::2, :128], 2, 4, 512, False),
+        ("another stride", buf[:, :, :128], 2, 8, 256, False),
+        ("too few columns", flat[:4, 128:252], 1, 4, 512, False),
+        ("every other column", flat[:4, ::4], 1, 4, 512, False),
+        ("heads apart that are not adjacent", flat[:4].unflatten(-1, (4, 128))[:, ::2, :64], 1, 4, 512, False),
+        ("sequences and tokens exchanged", buf.transpose(0, 1)[:, :, :128], 8, 2, 512, False),
+        ("too few rows", flat[:4, :128], 1, 6, 512, False),
+        ("one row", flat[3, ::4], 1, 1, 512, False),
+    ]
+
+
+@pytest.mark.parametrize("name,view,seqs,tokens,stride,right", views(), ids=lambda x: x if isinstance(x, str) else "")
+def test_strided_views_are_the_rows_that_the_kernels_read(monkeypatch, name, view, seqs, tokens, stride, right):
+    """What a view passes as is what the kernels read: row (s, t) at (s * tokens + t) * stride of its address."""
+    from zeninfer_amd import zq
+    monkeypatch.setattr(zq, "_check_device", lambda t, what: None)
+    call = lambda: zq._need_rows(view, seqs, tokens, stride, 128, "rows", 0)
+    if not right:
+        with pytest.raises(ValueError, match="rows: (rows must be|buffer holds)"):
+            call()
+        return
+    assert call() == view.data_ptr()
+    read = torch.as_strided(view, (seqs, tokens, 128), (tokens * stride, stride, 1), view.storage_offset())
+    rows = view.flatten(-2) if view.shape[-1] == 64 else view
+    if rows.dim() == 2:
+        rows = rows[:seqs * tokens].unflatten(0, (seqs, tokens))
+    assert torch.equal(read, rows[:seqs, :tokens, :128])
+
+
 @pytest.mark.parametrize("D", [64, 128, 256])
 def test_staged_keys_lie_in_the_arrays(check_stage, D):
     bad = {C: check_stage(D, C) for C in [*range(32, 2049, 32), 40000, 65504, 99968]}

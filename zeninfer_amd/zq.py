@@ -630,16 +630,24 @@ def _need_ints(t, n, what, dev):
 
 def _need_rows(t, seqs, tokens, stride, width, what, dev):
     """Device address of [seqs][tokens][stride] fp32 rows of which width floats are used.  With a stride, a view of
-    the columns of a wider buffer will do (its storage must hold the last row)."""
+    the columns of a wider buffer will do, as [seqs][tokens][...] or [seqs * tokens][...] whose rows lie where the
+    kernels look for them (and whose storage holds the last one)."""
     n = 4 * ((seqs * tokens - 1) * (stride or width) + width)
     if t is None or isinstance(t, int) or not stride or t.is_contiguous():
         return _need(t, n, what, dev)
     _check_device(t, what)
     have = t.untyped_storage().nbytes() - t.storage_offset() * t.element_size()
-    if t.element_size() != 4 or t.stride(-1) != 1 or t.stride(-2) != stride:
-        raise ValueError(f"{what}: rows must be {stride} fp32 values apart and their elements adjacent")
     if have < n:
         raise ValueError(f"{what}: buffer holds {have} bytes, the call needs {n}")
+    # the last dimensions are a row's elements, side by side; those before them count rows
+    dims, row = [(a, b) for a, b in zip(t.shape, t.stride())], 1
+    while dims and row < width and (dims[-1][0] == 1 or dims[-1][1] == row):
+        row *= dims.pop()[0]
+    need = [(seqs * tokens, stride)] if len(dims) == 1 else [(seqs, tokens * stride), (tokens, stride)]
+    if t.element_size() != 4 or row < width or len(dims) != len(need) or any(
+            size < count or (count > 1 and at != step) for (size, at), (count, step) in zip(dims, need)):
+        raise ValueError(f"{what}: rows must be {stride} fp32 values apart, [{seqs}][{tokens}] of them, and their {width} "
+                         f"elements adjacent; got a view of shape {tuple(t.shape)}, strides {tuple(t.stride())}")
     return t.data_ptr()
 
 

@@ -111,6 +111,41 @@ def test_strided_views_are_the_rows_that_the_kernels_read(monkeypatch, name, vie
     assert torch.equal(read, rows[:seqs, :tokens, :128])
 
 
+def test_wrappers_refuse_other_types(monkeypatch):
+    """Buffers of other types are long enough, and would be read as other values."""
+    from zeninfer_amd import zq
+    monkeypatch.setattr(zq, "_check_device", lambda t, what: None)
+    c = zq.KVQ4(1 << 20, 2 << 20, 3 << 20, 4 << 20, 1, 2, 64, 64, weight=5 << 20, pos=6 << 20)
+    p, lens = 7 << 20, torch.zeros(1, dtype=torch.int32)
+    for dtype in (torch.float64, torch.float16, torch.bfloat16, torch.int32, torch.int64, torch.complex64):
+        x = torch.zeros(4096, dtype=dtype)
+        wide = torch.zeros(4, 512, dtype=dtype)[:, :256]
+        for call in (lambda: zq.kv_q4_append_dev(c, x, p, 1, lens), lambda: zq.kv_q4_append_dev(c, p, x, 1, lens),
+                     lambda: zq.kv_q4_append_dev(c, wide, p, 4, lens, stride=512), lambda: zq.kv_q4_read_dev(c, x, p, 1, lens),
+                     lambda: zq.kv_q4_read_dev(c, None, x, 1, lens), lambda: zq.attention_q4_dev(c, x, p, 1, 4, lens, 1.0),
+                     lambda: zq.attention_q4_dev(c, wide, p, 4, 4, lens, 1.0, stride=512),
+                     lambda: zq.attention_q4_dev(c, p, x, 1, 4, lens, 1.0)):
+            with pytest.raises(ValueError, match="needs float32, got torch"):
+                call()
+    z = lambda n, dtype: torch.zeros(n, dtype=dtype)
+    right = dict(k=torch.uint8, v=torch.uint8, k_scale=torch.float16, v_scale=torch.float16, weight=torch.float32,
+                 pos=torch.int32)
+    wrong = dict(k=(torch.float16, torch.float32), v=(torch.bfloat16, torch.float32), k_scale=(torch.bfloat16, torch.float32),
+                 v_scale=(torch.bfloat16, torch.float64), weight=(torch.float64, torch.float16, torch.int32),
+                 pos=(torch.int64, torch.float32, torch.int16))
+    for name, types in wrong.items():
+        for dtype in types:
+            with pytest.raises(ValueError, match=f"KVQ4 {name}: needs "):
+                zq.KVQ4(seqs=1, kv_heads=2, head_dim=64, capacity=64, **{n: z(8192, dtype if n == name else t) for n, t in right.items()})
+    # the types they have, their bits, and their bytes: what is too short is what is left to refuse
+    for over in ({}, {n: torch.uint8 for n in right}, dict(k_scale=torch.int16, v_scale=torch.uint8)):
+        with pytest.raises(ValueError, match="KVQ4 k: buffer holds"):
+            zq.KVQ4(seqs=1, kv_heads=2, head_dim=64, capacity=64, **{n: z(8, over.get(n, t)) for n, t in right.items()})
+    for x in (z(8, torch.float32), z(8, torch.uint8)):
+        with pytest.raises(ValueError, match="k: buffer holds"):
+            zq.kv_q4_append_dev(c, x, p, 1, lens)
+
+
 @pytest.mark.parametrize("D", [64, 128, 256])
 def test_staged_keys_lie_in_the_arrays(check_stage, D):
     bad = {C: check_stage(D, C) for C in [*range(32, 2049, 32), 40000, 65504, 99968]}

@@ -602,6 +602,28 @@ def kv_q4_bytes(kv_heads, head_dim, capacity):
     return lib().zq_kv_q4_bytes(kv_heads, head_dim, capacity)
 
 
+_KINDS = {"float32": set(), "float16": set(), "int32": set(), "int": set()}  # torch's types found to be of a kind
+
+
+def _need_kind(t, kind, what):
+    """A tensor holds values of the kind, or their bytes (a part of a uint8 buffer).  Others' buffers may be long
+    enough, and would be read as other values."""
+    if t is None or isinstance(t, int) or t.dtype in _KINDS[kind]:
+        return
+    size, floating = t.element_size(), t.is_floating_point()
+    integer = not floating and not t.is_complex()
+    if not (integer and size == 1 or {"float32": floating and size == 4, "int32": integer and size == 4, "int": integer,
+                                      "float16": integer or str(t.dtype) == "torch.float16"}[kind]):
+        raise ValueError(f"{what}: needs {kind}, got {t.dtype}")
+    _KINDS[kind].add(t.dtype)
+
+
+def _need_f32(t, n, what, dev):
+    """Device address of n fp32 values."""
+    _need_kind(t, "float32", what)
+    return _need(t, 4 * n, what, dev)
+
+
 class KVQ4:
     """A 4-bit KV cache over the caller's device arrays (zq_kv_q4): codes k and v
     [seqs][kv_heads][capacity][head_dim / 2], scales [seqs][kv_heads][head_dim / 32]
@@ -614,6 +636,8 @@ class KVQ4:
         arrays = [(k, rows * (head_dim // 2), "k"), (v, rows * (head_dim // 2), "v"),
                   (k_scale, rows * (head_dim // 32) * 2, "k_scale"), (v_scale, rows * (head_dim // 32) * 2, "v_scale"),
                   (weight, rows * 4, "weight"), (pos, rows * 4, "pos")]
+        for (t, _, name), kind in zip(arrays, ("int", "int", "float16", "float16", "float32", "int32")):
+            _need_kind(t, kind, f"KVQ4 {name}")
         self.c = KVCacheQ4(*[_need(t, n, f"KVQ4 {name}", dev) for t, n, name in arrays], seqs, kv_heads, head_dim,
                            capacity)
         self.arrays = [t for t, _, _ in arrays]
@@ -633,6 +657,7 @@ def _need_rows(t, seqs, tokens, stride, width, what, dev):
     the columns of a wider buffer will do, as [seqs][tokens][...] or [seqs * tokens][...] whose rows lie where the
     kernels look for them (and whose storage holds the last one)."""
     n = 4 * ((seqs * tokens - 1) * (stride or width) + width)
+    _need_kind(t, "float32", what)
     if t is None or isinstance(t, int) or not stride or t.is_contiguous():
         return _need(t, n, what, dev)
     _check_device(t, what)
@@ -667,9 +692,9 @@ def kv_q4_append_dev(cache, k, v, tokens, lens, counts=None, first_pos=None, str
 def kv_q4_read_dev(cache, k, v, tokens, first, counts=None, stream=None):
     """Rows first ... of every sequence as fp32 [seqs][tokens][kv_heads * head_dim]; k or v may be None."""
     dev = cache.dev
-    n = 4 * cache.seqs * tokens * cache.kv_heads * cache.head_dim
-    k = _need(k, n, "kv_q4_read_dev k", dev)
-    v = _need(v, n, "kv_q4_read_dev v", dev)
+    n = cache.seqs * tokens * cache.kv_heads * cache.head_dim
+    k = _need_f32(k, n, "kv_q4_read_dev k", dev)
+    v = _need_f32(v, n, "kv_q4_read_dev v", dev)
     first = _need_ints(first, cache.seqs, "kv_q4_read_dev first", dev)
     counts = _need_ints(counts, cache.seqs, "kv_q4_read_dev counts", dev)
     return check(lib().zq_hip_kv_q4_read_dev(cache.ref, k, v, tokens, first, counts, _stream(stream)),
@@ -686,7 +711,7 @@ def attention_q4_dev(cache, q, out, tokens, heads, lens, scale, counts=None, str
     dev = cache.dev
     width = heads * cache.head_dim
     q = _need_rows(q, cache.seqs, tokens, stride, width, "attention_q4_dev q", dev)
-    out = _need(out, 4 * cache.seqs * tokens * width, "attention_q4_dev out", dev)
+    out = _need_f32(out, cache.seqs * tokens * width, "attention_q4_dev out", dev)
     lens = _need_ints(lens, cache.seqs, "attention_q4_dev lens", dev)
     counts = _need_ints(counts, cache.seqs, "attention_q4_dev counts", dev)
     workspace = _need(workspace, workspace_bytes, "attention_q4_dev workspace", dev)

@@ -146,6 +146,32 @@ def test_wrappers_refuse_other_types(monkeypatch):
             zq.kv_q4_append_dev(c, x, p, 1, lens)
 
 
+def test_wrappers_refuse_sizes_below_zero(monkeypatch):
+    """A size_t takes -1 as the largest number: any workspace would be long enough, and everything would be kept."""
+    from zeninfer_amd import zq
+    monkeypatch.setattr(zq, "_check_device", lambda t, what: None)
+    c = zq.KVQ4(1 << 20, 2 << 20, 3 << 20, 4 << 20, 1, 2, 64, 64, weight=5 << 20, pos=6 << 20)
+    p, lens, ws = 7 << 20, torch.zeros(1, dtype=torch.int32), torch.zeros(16, dtype=torch.uint8)
+    for w in (ws, p):
+        with pytest.raises(ValueError, match="attention_q4_dev workspace: a size below zero"):
+            zq.attention_q4_dev(c, p, p, 1, 4, lens, 1.0, flags=zq.ATTN_Q4_WEIGHTS, workspace=w, workspace_bytes=-1)
+        with pytest.raises(ValueError, match="kv_q4_evict_dev workspace: a size below zero"):
+            zq.kv_q4_evict_dev(c, lens, 16, 4, 4, workspace=w, workspace_bytes=-16)
+    for bad in ((-1, 4, 4), (16, -1, 4), (16, 4, -1)):
+        with pytest.raises(ValueError, match="a number of rows below zero"):
+            zq.kv_q4_evict_dev(c, lens, *bad, workspace=ws, workspace_bytes=16)
+    for bad in (dict(seqs=-1), dict(kv_heads=-2), dict(capacity=-64)):
+        with pytest.raises(ValueError, match="KVQ4 k: a size below zero"):
+            zq.KVQ4(1 << 20, 2 << 20, 3 << 20, 4 << 20, **{**dict(seqs=1, kv_heads=2, head_dim=64, capacity=64), **bad})
+    for tokens in (-1, -3):
+        with pytest.raises(ValueError, match="a size below zero"):
+            zq.kv_q4_append_dev(c, p, p, tokens, lens)
+        with pytest.raises(ValueError, match="a size below zero"):
+            zq.kv_q4_read_dev(c, p, p, tokens, lens)
+        with pytest.raises(ValueError, match="a size below zero"):
+            zq.attention_q4_dev(c, p, p, tokens, 4, lens, 1.0)
+
+
 @pytest.mark.parametrize("D", [64, 128, 256])
 def test_staged_keys_lie_in_the_arrays(check_stage, D):
     bad = {C: check_stage(D, C) for C in [*range(32, 2049, 32), 40000, 65504, 99968]}

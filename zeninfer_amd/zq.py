@@ -255,7 +255,10 @@ def _need(t, nbytes, what, dev=None):
     and hold at least nbytes: the kernels index it from the sizes alone, so a
     short buffer would be read or written past its end, and the address of a
     host tensor handed to a kernel faults the GPU.  Raw addresses are the
-    caller's responsibility.  dev: _device_index(), where the caller has it."""
+    caller's responsibility.  dev: _device_index(), where the caller has it.
+    A negative size is refused: the library would take it for a huge one."""
+    if nbytes < 0:
+        raise ValueError(f"{what}: a size below zero ({nbytes} bytes)")
     if t is None or isinstance(t, int):
         return t
     # one pass of cheap queries where all is well (this runs for every buffer
@@ -727,6 +730,8 @@ def kv_q4_evict_dev(cache, lens, keep, recent, first, next_pos=None, dst=None, w
                     stream=None):
     """Keeps the `keep` rows of the most weight (the `recent` newest and `first` first ones always), in place or in dst."""
     dev = cache.dev
+    if min(keep, recent, first) < 0:
+        raise ValueError(f"kv_q4_evict_dev: a number of rows below zero (keep {keep}, recent {recent}, first {first})")
     lens = _need_ints(lens, cache.seqs, "kv_q4_evict_dev lens", dev)
     next_pos = _need_ints(next_pos, cache.seqs, "kv_q4_evict_dev next_pos", dev)
     workspace = _need(workspace, workspace_bytes, "kv_q4_evict_dev workspace", dev)

@@ -172,6 +172,66 @@ def test_wrappers_refuse_sizes_below_zero(monkeypatch):
             zq.attention_q4_dev(c, p, p, tokens, 4, lens, 1.0)
 
 
+class FakeLibrary:
+    """The decoder's entry points that Model.kv_cache meets, over made-up addresses."""
+
+    def __init__(self, zq):
+        self.zq, self.freed, self.status = zq, 0, zq.OK
+
+    def zq_model_kv_cache(self, h, layer, cache, rows, positions):
+        c = cache._obj
+        c.k, c.v, c.k_scale, c.v_scale, c.weight, c.pos = [(i + 1) << 20 for i in range(6)]
+        c.seqs, c.kv_heads, c.head_dim, c.capacity = 1, 2, 64, 64
+        return self.zq.OK
+
+    def zq_model_set_kv_cache(self, h, form, rows, recent, first):
+        return self.status
+
+    def zq_model_free(self, h):
+        self.freed += 1
+
+
+def test_a_models_cache_ends_with_its_arrays(monkeypatch):
+    """The handle of a model's cache keeps the model alive, and is refused once the model has freed the arrays."""
+    import gc
+    from zeninfer_amd import model, zq
+    fake = FakeLibrary(zq)
+    with monkeypatch.context() as mp:
+        mp.setattr(zq, "lib", lambda: fake)
+        m = model.Model(1, zq.ModelConfig())
+    lens = torch.zeros(1, dtype=torch.int32)
+    monkeypatch.setattr(zq, "_check_device", lambda t, what: None)
+
+    def uses(c):
+        own = zq.KVQ4(*[i << 20 for i in range(11, 15)], 1, 2, 64, 64, weight=15 << 20, pos=16 << 20)
+        return [lambda: zq.kv_q4_append_dev(c, 1 << 24, 1 << 24, 1, lens), lambda: zq.kv_q4_read_dev(c, 1 << 24, None, 1, lens),
+                lambda: zq.attention_q4_dev(c, 1 << 24, 1 << 24, 1, 4, lens, 1.0),
+                lambda: zq.attention_q4_workspace_bytes(c, 1, 4), lambda: zq.kv_q4_evict_workspace_bytes(c, 4),
+                lambda: zq.kv_q4_evict_dev(c, lens, 4, 1, 1), lambda: zq.kv_q4_evict_dev(own, lens, 4, 1, 1, dst=c)]
+
+    def refused(c):
+        for use in uses(c):
+            with pytest.raises(ValueError, match="has freed this 4-bit cache"):
+                use()
+    c = m.kv_cache(0)[0]
+    assert isinstance(c, zq.KVQ4) and zq.kv_q4_evict_workspace_bytes(c, 4) == 2 * 3 * 4 * 4
+    fake.status = zq.ERR_OOM  # the model keeps the cache it had
+    with pytest.raises(zq.ZQError):
+        m.set_kv_cache(model.KV_Q4)
+    assert zq.kv_q4_evict_workspace_bytes(c, 4)
+    fake.status = zq.OK
+    m.set_kv_cache(model.KV_Q4)
+    refused(c)
+    c = m.kv_cache(1)[0]
+    assert zq.attention_q4_workspace_bytes(c, 1, 4, zq.ATTN_Q4_WEIGHTS)
+    del m
+    gc.collect()
+    assert fake.freed == 0 and zq.kv_q4_evict_workspace_bytes(c, 4)
+    c._model.close()
+    assert fake.freed == 1
+    refused(c)
+
+
 @pytest.mark.parametrize("D", [64, 128, 256])
 def test_staged_keys_lie_in_the_arrays(check_stage, D):
     bad = {C: check_stage(D, C) for C in [*range(32, 2049, 32), 40000, 65504, 99968]}

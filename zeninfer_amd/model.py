@@ -23,10 +23,31 @@ class ModelError(RuntimeError):
     pass
 
 
+class ModelKVQ4(zq.KVQ4):
+    """One layer's 4-bit cache of a model (Model.kv_cache): it keeps the model alive, and every call of it is refused
+    once the model has freed its arrays (set_kv_cache, close)."""
+
+    def __init__(self, model, c):
+        self._model, self._arrays = model, model._arrays
+        super().__init__(c.k, c.v, c.k_scale, c.v_scale, c.seqs, c.kv_heads, c.head_dim, c.capacity, weight=c.weight,
+                         pos=c.pos)
+
+    @property
+    def ref(self):
+        if self._model._arrays is not self._arrays:
+            raise ValueError("the model has freed this 4-bit cache (set_kv_cache or close): ask it for the present one")
+        return self._ref
+
+    @ref.setter
+    def ref(self, ref):
+        self._ref = ref
+
+
 class Model:
     def __init__(self, handle, cfg):
         self._L = zq.lib()
         self._h = handle
+        self._arrays = object()  # stands for the KV cache's arrays: another one when they are freed
         self.config = {n: getattr(cfg, n) for n, _ in cfg._fields_}
 
     @classmethod
@@ -55,6 +76,7 @@ class Model:
 
     def close(self):
         if self._h:
+            self._arrays = None
             self._L.zq_model_free(self._h)
             self._h = None
 
@@ -69,18 +91,20 @@ class Model:
 
     def set_kv_cache(self, form, rows=0, recent=0, first=0):
         """The KV cache's form (zq_model_set_kv_cache): KV_F32, or KV_Q4 with at most `rows` rows kept by the
-        attention weight they draw (0: every position).  The cache starts empty."""
+        attention weight they draw (0: every position).  The cache starts empty; handles of the one before
+        (kv_cache) are refused from here on."""
         zq.check(self._L.zq_model_set_kv_cache(self._h, form, rows, recent, first), "set_kv_cache")
+        self._arrays = object()
 
     def kv_cache(self, layer):
-        """(zq.KVQ4 over one layer's 4-bit cache, or None with the fp32 cache; rows held; positions fed)."""
+        """(ModelKVQ4 over one layer's 4-bit cache, or None with the fp32 cache; rows held; positions fed).  The cache may
+        be used until the next set_kv_cache or close."""
         c, rows, at = zq.KVCacheQ4(), ctypes.c_uint32(), ctypes.c_uint32()
         st = self._L.zq_model_kv_cache(self._h, layer, ctypes.byref(c), ctypes.byref(rows), ctypes.byref(at))
         if st == zq.DECLINED:
             return None, rows.value, at.value
         zq.check(st, "kv_cache")
-        return zq.KVQ4(c.k, c.v, c.k_scale, c.v_scale, c.seqs, c.kv_heads, c.head_dim, c.capacity, weight=c.weight,
-                       pos=c.pos), rows.value, at.value
+        return ModelKVQ4(self, c), rows.value, at.value
 
     def prefill(self, tokens, logits=True):
         t = np.ascontiguousarray(tokens, dtype=np.uint32)

@@ -245,3 +245,28 @@ def test_eviction_keeps_the_rule(zq):
             assert set(range(1500 + room - recent, at)) <= set(kept) and set(range(first)) <= set(kept)
             assert len(set(kept)) == n
     m.close()
+
+
+def test_switching_back_frees_what_the_4_bit_form_took(zq):
+    """An fp32 model is charged for no 4-bit workspace, however often the form changes, and the memory is given back."""
+    import torch
+    from zeninfer_amd.model import KV_F32, KV_Q4
+    m = build(zq)
+    start = m.memory()
+    m.set_kv_cache(KV_F32)
+    assert m.memory() == start
+    free = []
+    for i in range(3):
+        m.set_kv_cache(KV_Q4, 64, 8, 4)
+        four = m.memory()
+        assert four["activations"] > start["activations"] and four["kv_cache"] < start["kv_cache"]
+        m.set_kv_cache(KV_Q4)
+        m.prefill(list(range(20)))
+        m.set_kv_cache(KV_F32)
+        assert m.memory() == start
+        with pytest.raises(zq.ZQError):
+            m.set_kv_cache(KV_F32, 16)
+        m.prefill(list(range(20)))
+        free.append(torch.cuda.mem_get_info()[0])
+    assert free[2] >= free[0]
+    m.close()

@@ -105,6 +105,19 @@ struct zq_model {
     void* kv_ws = nullptr;            // attention and eviction workspace
     size_t kv_ws_bytes = 0;
     uint64_t kv_aux_bytes = 0;        // kv_rows_dev and kv_ws, counted as activations
+
+    // The cache's arrays, and the 4-bit form's lengths and workspace.
+    void free_kv() {
+        for (void* p : {kv_mem, static_cast<void*>(kv_rows_dev), kv_ws})
+            if (p) (void)hipFree(p);
+        if (kv_rows_host) (void)hipHostFree(kv_rows_host);
+        kv_mem = kv_ws = nullptr;
+        kv_rows_dev = kv_rows_host = nullptr;
+        kv_ws_bytes = 0;
+        kv_all = zq_kv_q4{};
+        act_bytes -= kv_aux_bytes;
+        kv_aux_bytes = 0;
+    }
     bool use_graph = true;
     bool fused = false;    // decode step with norms and SiLU folded into the GEMVs
     bool fuse_quant = true;  // prefill norms / SiLU*up also write the int8 activations; K-quant gate|up pair
@@ -124,9 +137,7 @@ struct zq_model {
         if (decode_exec) (void)hipGraphExecDestroy(decode_exec);
         if (decode_graph) (void)hipGraphDestroy(decode_graph);
         for (void* p : allocs) (void)hipFree(p);
-        for (void* p : {kv_mem, static_cast<void*>(kv_rows_dev), kv_ws})
-            if (p) (void)hipFree(p);
-        if (kv_rows_host) (void)hipHostFree(kv_rows_host);
+        free_kv();
         if (host_small) (void)hipHostFree(host_small);
         if (stream) (void)hipStreamDestroy(stream);
     }
@@ -171,7 +182,7 @@ bool set_kv_f32(zq_model& m) {
     const size_t per = size_t(c.max_positions) * c.kv_heads * c.head_dim * 4;
     void* kv = nullptr;
     if (hipMalloc(&kv, 2 * per * c.layers) != hipSuccess) return false;
-    if (m.kv_mem) (void)hipFree(m.kv_mem);
+    m.free_kv();
     m.kv_mem = kv;
     m.kv_form = ZQ_KV_F32;
     m.kv_keep = m.kv_recent = m.kv_first = 0;
@@ -228,11 +239,9 @@ int set_kv_q4(zq_model& m, uint32_t keep, uint32_t recent, uint32_t first) {
         hipMalloc(&ws, std::max<size_t>(need, 16)) != hipSuccess ||
         hipHostMalloc(reinterpret_cast<void**>(&host), 2 * L * 4) != hipSuccess)
         return fail(ZQ_ERR_OOM);
-    for (void* q : {m.kv_mem, static_cast<void*>(m.kv_rows_dev), m.kv_ws})
-        if (q) (void)hipFree(q);
-    if (m.kv_rows_host) (void)hipHostFree(m.kv_rows_host);
-    m.act_bytes += 2 * L * 4 + need - m.kv_aux_bytes;
+    m.free_kv();
     m.kv_aux_bytes = 2 * L * 4 + need;
+    m.act_bytes += m.kv_aux_bytes;
     m.kv_mem = mem;
     m.kv_rows_dev = rows;
     m.kv_rows_host = host;

@@ -938,3 +938,108 @@ def test_evict_refuses_a_host_destination(zq):
         zq.kv_q4_evict_dev(d.c, d.ints([40]), 16, 4, 4, dst=dst, workspace=ws, workspace_bytes=n)
     torch.cuda.synchronize()
     assert not buf.any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("to_other", [False, True])
+def test_graph_replays_evict_what_the_replay_finds(zq, to_other):
+    """A captured append, attention with weights and eviction, replayed while the lengths rise past `keep`: every replay
+    drops the rows that the rule says, of the weights that the replay before has left, and equals the eager calls."""
+    r = np.random.default_rng(21)
+    S, KH, G, D, C, keep, recent, first, T = 3, 2, 4, 64, 512, 300, 32, 4, 5
+    lens0, at0 = [298, 77, 299], [298, 77, 299]
+    eager, graph = Dev(zq, S, KH, D, C), Dev(zq, S, KH, D, C)
+    for d in (eager, graph):
+        d.fill(lens0, 4)
+    other = [Dev(zq, S, KH, D, 320) for _ in range(2)]
+    k, v, q = (torch.zeros(S, T, h, D, device="cuda") for h in (KH, KH, KH * G))
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")
+    lens, counts, at = i32(lens0), i32([T] * S), i32(at0)
+    held, nxt = i32([0] * S), i32([0] * S)
+    flags = zq.ATTN_Q4_WEIGHTS | zq.ATTN_Q4_ADD
+    n = -(-zq.attention_q4_workspace_bytes(eager.c, T, KH * G, flags) // 16) * 16
+    m = zq.kv_q4_evict_workspace_bytes(eager.c, keep)
+
+    def step_of(d, ws, out, stream):
+        zq.kv_q4_append_dev(d.c, k, v, T, lens, counts=counts, first_pos=at, stream=stream)
+        zq.attention_q4_dev(d.c, q, out, T, KH * G, lens, 0.11, counts=counts, flags=flags, workspace=ws[:n],
+                            workspace_bytes=n, stream=stream)
+
+    def evict(d, to, ws, stream):
+        zq.kv_q4_evict_dev(d.c, held, keep, recent, first, next_pos=nxt, dst=to.c if to_other else None, workspace=ws[n:],
+                           workspace_bytes=m, stream=stream)
+
+    wa, wb = (torch.full((n + m,), 0xff, dtype=torch.uint8, device="cuda") for _ in range(2))
+    oa, ob = (torch.zeros(S, T, KH * G, D, device="cuda") for _ in range(2))
+    torch.cuda.synchronize()
+    g, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with torch.cuda.graph(g, stream=side):
+        step_of(graph, wb, ob, torch.cuda.current_stream())
+        evict(graph, other[1], wb, torch.cuda.current_stream())
+    now, pos, dropped = list(lens0), list(at0), 0
+    for step in range(4):
+        for x in (k, v, q):
+            x.copy_(torch.from_numpy(r.standard_normal(tuple(x.shape)).astype(np.float32) * 1.3))
+        new = [T, step % 3, T - step]
+        after, end = [a + b for a, b in zip(now, new)], [a + b for a, b in zip(pos, new)]
+        for t, x in ((lens, now), (counts, new), (at, pos), (held, after), (nxt, end)):
+            t.copy_(i32(x))
+        torch.cuda.synchronize()
+        plain = eager.plain
+        plain.append(k.cpu().numpy(), v.cpu().numpy(), now, new, pos)
+        step_of(eager, wa, oa, None)
+        torch.cuda.synchronize()
+        plain.weight[:] = eager.weight.cpu().numpy()  # the device's own sums: ranks are compared exactly
+        evict(eager, other[0], wa, None)
+        torch.cuda.synchronize()
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(oa, ob)
+        for a, b in ((eager, graph), other):
+            for x in ("k", "v", "ks", "vs", "weight", "pos"):
+                assert torch.equal(getattr(a, x).view(torch.uint8), getattr(b, x).view(torch.uint8)), (step, x)
+        to = other[0] if to_other else eager
+        plain.evict(after, keep, recent, first, end, to=to.plain if to_other else None)
+        kept = [min(x, keep) for x in after]
+        to.rows_equal(kept)
+        for s in range(S):
+            assert np.array_equal(to.weight[s, :, :kept[s]].cpu().numpy(), to.plain.weight[s, :, :kept[s]].astype(np.float32))
+            assert to_other or (eager.pos[s, :, kept[s]:after[s]] == -1).all()
+        dropped += sum(after) - sum(kept)
+        now, pos = after if to_other else kept, end
+    assert dropped >= 16
+
+
+@pytest.mark.gpu
+def test_two_streams_at_once_draw_the_same_weights(zq):
+    """Two caches on two streams, each with its own workspace: outputs and accumulated weights of one after the other."""
+    KH, G, D, C, n, T = 2, 4, 128, 2048, 1900, 4
+    flags = zq.ATTN_Q4_WEIGHTS | zq.ATTN_Q4_ADD
+    r = np.random.default_rng(5)
+    ds, alone = ([Dev(zq, 1, KH, D, C) for _ in range(2)] for _ in range(2))
+    for i in range(2):
+        for d in (ds[i], alone[i]):
+            d.fill([n + T], i)
+    q = [torch.from_numpy(tokens(r, 1, T, KH * G, D)).cuda() for _ in ds]
+    lens = torch.tensor([n], dtype=torch.int32, device="cuda")
+    need = zq.attention_q4_workspace_bytes(ds[0].c, T, KH * G, flags)
+    outs = [[torch.zeros(1, T, KH * G, D, device="cuda") for _ in range(6)] for _ in ds]
+    ws = [torch.empty(need, dtype=torch.uint8, device="cuda") for _ in ds]
+    streams = [torch.cuda.Stream() for _ in ds]
+    call = lambda d, i, out, stream: zq.attention_q4_dev(d.c, q[i], out, T, KH * G, lens, 0.1, flags=flags, workspace=ws[i],
+                                                         workspace_bytes=need, stream=stream)
+    torch.cuda.synchronize()
+    for j in range(6):
+        for i, d in enumerate(ds):
+            call(d, i, outs[i][j], streams[i])
+    torch.cuda.synchronize()
+    for i, d in enumerate(alone):
+        for j in range(6):
+            one = torch.zeros(1, T, KH * G, D, device="cuda")
+            call(d, i, one, None)
+            torch.cuda.synchronize()
+            assert torch.equal(outs[i][j], one)
+        assert torch.equal(ds[i].weight.view(torch.int32), d.weight.view(torch.int32))
+        # every head's weights of a query sum to 1: sums of n fp32 terms, 6 calls' T * G of them a kv head
+        total = d.weight[0, :, :n + T].double().sum(-1)
+        assert ((total - 6 * T * G).abs() <= 6 * T * G * (n + T) * 2 * U).all()

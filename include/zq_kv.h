@@ -74,9 +74,16 @@ int zq_hip_kv_q4_read_dev(const zq_kv_q4* cache, float* k, float* v, size_t toke
 
 /* ---- attention -----------------------------------------------------------
  * out[s][t][h] = sum_p softmax_p(scale * q . k_p) v_p, h of kv head h / (heads /
- * kv_heads), to fp32 accuracy of the held values.  q: [seqs][tokens][stride] fp32,
- * heads * head_dim used (stride as above, 0 = heads * head_dim); out: [seqs]
- * [tokens][heads * head_dim], 16-byte aligned, not overlapping q.  lens and counts
+ * kv_heads).  The held values are exact operands, q has 22 bits, scores, exponentials
+ * and sums are fp32: over n rows an output is off by at most (n / 2 + 128) * 2^-24 of
+ * the largest |v|, and by what 2^-21 of the largest sum of |scale q k| moves the
+ * softmax.  Nearly all calls are far below the first term: it needs rows of equal
+ * weight, and so many queries that the rows are not split over workgroups (1,000,003
+ * equal rows: 4e-4 of the largest |v| with 512 tokens of 4 heads a kv head at head_dim
+ * 64, 1.2e-3 with 2048 tokens at 256, 2e-7 with one token; of unequal weight: 7e-7 at
+ * most).  q: [seqs][tokens]
+ * [stride] fp32, heads * head_dim used (stride as above, 0 = heads * head_dim); out:
+ * [seqs][tokens][heads * head_dim], 16-byte aligned, not overlapping q.  lens and counts
  * as in the append that came before: query t sees the slots below lens[s] + t +
  * 1, its own token's row the last.  With ZQ_ATTN_Q4_FULL every query sees the
  * lens[s] held rows and no others; where there are none its output is 0.  A length

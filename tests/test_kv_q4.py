@@ -1043,3 +1043,50 @@ def test_two_streams_at_once_draw_the_same_weights(zq):
         # every head's weights of a query sum to 1: sums of n fp32 terms, 6 calls' T * G of them a kv head
         total = d.weight[0, :, :n + T].double().sum(-1)
         assert ((total - 6 * T * G).abs() <= 6 * T * G * (n + T) * 2 * U).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D,T,G", [(64, 1, 4), (64, 512, 4), (128, 512, 4), (256, 2048, 2), (256, 3, 3)])
+def test_equal_rows_of_a_long_cache(zq, D, T, G):
+    """zq_kv.h's bound where sums round the same way again and again: one row, and 300,002 others that are equal.
+    A lane's running sum takes 8 additions of a pair of weights for 32 (D = 256) or 64 keys, its outputs 4 rounded
+    products: 12 / 32 n at most, and the products' own sums, the two halves of a weight, the merges and the quotient are
+    within 128 roundings.  A score here is one product: 2^-21 of itself, and as much for the exponential."""
+    n, KH = 300003, 8 if T > 1 else 2
+    C = -(-n // 32) * 32
+    cuda = dict(device="cuda")
+    k, v = (torch.empty((1, KH, C, D // 2), dtype=torch.uint8, **cuda) for _ in range(2))
+    ks, vs = (torch.empty((1, KH, D // 32, C), dtype=torch.float16, **cuda) for _ in range(2))
+    w = torch.zeros((1, KH, C), **cuda)
+    c = zq.KVQ4(k, v, ks, vs, 1, KH, D, C, weight=w)
+    r = np.random.default_rng(D)
+    new_k = torch.zeros(1, 2, KH, D, **cuda)
+    new_k[0, 0, :, 0], new_k[0, 1, :, 0] = 1.0, 0.3
+    new_v = torch.from_numpy((r.random((1, 2, KH, D)) + 1).astype(np.float32)).cuda()
+    zero = torch.zeros(1, dtype=torch.int32, **cuda)
+    zq.kv_q4_append_dev(c, new_k, new_v, 2, zero)
+    hk, hv = torch.empty_like(new_k), torch.empty_like(new_v)
+    zq.kv_q4_read_dev(c, hk, hv, 2, zero)
+    for t in (k, v):
+        t[:, :, 2:] = t[:, :, 1:2]
+    for t in (ks, vs):
+        t[..., 2:] = t[..., 1:2]
+    q = torch.zeros(1, T, KH * G, D, **cuda)
+    q[..., 0] = torch.from_numpy(r.uniform(0.5, 3, (1, T, KH * G)).astype(np.float32)).cuda()
+    flags = zq.ATTN_Q4_FULL | zq.ATTN_Q4_WEIGHTS
+    need = zq.attention_q4_workspace_bytes(c, T, KH * G, flags)
+    ws, out = torch.empty(need, dtype=torch.uint8, **cuda), torch.empty_like(q)
+    zq.attention_q4_dev(c, q, out, T, KH * G, torch.tensor([n], dtype=torch.int32, **cuda), 1.0, flags=flags, workspace=ws,
+                        workspace_bytes=need)
+    torch.cuda.synchronize()
+    s = q[0, :, :, 0].double()[..., None] * hk[0, :, :, 0].double().T.repeat_interleave(G, 0)[None]  # [T][H][2 rows]
+    e = torch.exp(s - s.amax(-1, keepdim=True)) * torch.tensor([1.0, n - 1.0], dtype=torch.float64, **cuda)
+    p = e / e.sum(-1, keepdim=True)
+    vv = hv[0].double().repeat_interleave(G, 1)  # [2][H][D]
+    want = p[..., :1] * vv[0] + p[..., 1:] * vv[1]
+    tol = (n / 2 + 128) * U + 2 * (s.abs().max().item() + 1) * 2.0 ** -21
+    assert ((out[0].double() - want).abs().max() <= tol * vv.abs().max()).item()
+    drawn = p.sum(0).reshape(KH, G, 2).sum(1)  # of row 0, and of the others together
+    for i, at in ((0, 0), (1, 1), (1, n - 1)):
+        each = drawn[:, i] / (1 if i == 0 else n - 1)
+        assert ((w[0, :, at].double() - each).abs() <= (tol + T * G * U) * each).all()

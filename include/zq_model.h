@@ -74,7 +74,9 @@ int zq_model_set_prefill_mode(zq_model* model, int mode);
  * keeps `rows` rows by zq_hip_kv_q4_evict_dev's rule (the `recent` newest
  * positions, the `first` first ones, then those of the largest weight); the cache
  * has room for a prefill pass (up to 1024 tokens) beside them, so generation may
- * run to max_positions on less memory.  first + recent <= rows.  ZQ_KV_F32 takes
+ * run to max_positions on less memory.  first + recent <= rows.  Where rows and a
+ * prefill pass together reach max_positions nothing would ever be evicted: the call
+ * is that of rows == 0, and no weight is added up.  ZQ_KV_F32 takes
  * rows = recent = first = 0.  On failure (ZQ_ERR_ARG, ZQ_ERR_OOM) the model keeps
  * the cache it had. */
 #define ZQ_KV_F32 0
@@ -82,8 +84,10 @@ int zq_model_set_prefill_mode(zq_model* model, int mode);
 int zq_model_set_kv_cache(zq_model* model, int form, uint32_t rows, uint32_t recent, uint32_t first);
 /* One layer's 4-bit cache (seqs = 1; device arrays that the model owns) for the
  * calls of zq_kv.h, the rows it holds and the positions fed so far.  The model
- * counts its own tokens only: a caller reads and attends to the cache, and leaves
- * appends and evictions to the model.  ZQ_DECLINED with the fp32 cache (rows and
+ * counts its own tokens only: a caller reads and attends to the cache (without
+ * ZQ_ATTN_Q4_WEIGHTS, as the model evicts by the weights), done before the model's
+ * next call, and leaves appends and evictions to the model; the arrays are freed by
+ * zq_model_set_kv_cache and zq_model_free.  ZQ_DECLINED with the fp32 cache (rows and
  * positions are set). */
 int zq_model_kv_cache(const zq_model* model, uint32_t layer, zq_kv_q4* cache, uint32_t* rows, uint32_t* positions);
 /* Prefill `n` tokens from position 0 (the cache is reset).  Logits of the

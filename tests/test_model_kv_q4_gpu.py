@@ -270,3 +270,25 @@ def test_switching_back_frees_what_the_4_bit_form_took(zq):
         free.append(torch.cuda.mem_get_info()[0])
     assert free[2] >= free[0]
     m.close()
+
+
+def test_a_bound_that_is_never_reached_is_none(zq):
+    """Rows and a prefill pass (1024 tokens) together reach max_positions: the cache of rows == 0, without weights; one
+    row fewer and they are drawn."""
+    from zeninfer_amd.model import KV_Q4
+    hip = ctypes.CDLL("libamdhip64.so")
+    for max_positions, rows, bounded in ((1100, 76, False), (1100, 75, True)):
+        m = build(zq, max_positions=max_positions)
+        m.set_kv_cache(KV_Q4)
+        whole = m.memory()
+        m.set_kv_cache(KV_Q4, rows, 5, 2)
+        assert (m.memory() == whole) == (not bounded)
+        m.prefill(list(range(60)))
+        m.decode(3)
+        cache, n, _ = m.kv_cache(1)
+        w = np.empty(cache.kv_heads * cache.capacity, np.float32)
+        assert hip.hipMemcpy(w.ctypes.data_as(ctypes.c_void_p), ctypes.c_void_p(cache.c.weight), ctypes.c_size_t(w.nbytes), 2) == 0
+        w = w.reshape(cache.kv_heads, -1)[:, :n]
+        # 61 queries of 4 heads a kv head, whose weights each sum to 1
+        assert np.allclose(w.astype(np.float64).sum(-1), 61 * 4 if bounded else 0, rtol=61 * 4 * 2.0 ** -22)
+        m.close()

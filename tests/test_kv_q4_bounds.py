@@ -172,6 +172,29 @@ def test_wrappers_refuse_sizes_below_zero(monkeypatch):
             zq.attention_q4_dev(c, p, p, tokens, 4, lens, 1.0)
 
 
+def test_evict_refuses_a_destination_that_meets_the_cache():
+    """An array of the destination inside any array of the cache, of whatever role, or ending in it: its rows would be
+    overwritten while they are read.  Next to each other they may lie (that call gets as far as the device)."""
+    from tests.test_kv_q4 import handle
+    from zeninfer_amd import zq
+    L, p, need = zq.lib(), 7 << 20, 1 << 20
+    c = dict(k=1 << 20, v=2 << 20, k_scale=3 << 20, v_scale=4 << 20, weight=5 << 20, pos=6 << 20)
+    size = dict(k=2 * 2 * 64 * 32, v=2 * 2 * 64 * 32, k_scale=2 * 2 * 64 * 4, v_scale=2 * 2 * 64 * 4, weight=2 * 2 * 64 * 4,
+                pos=2 * 2 * 64 * 4)  # of the cache; half of it with 32 slots
+    far = {n: a + (16 << 20) for n, a in c.items()}
+    evict = lambda d: L.zq_hip_kv_q4_evict_dev(ctypes.byref(handle(zq)), ctypes.byref(handle(zq, capacity=32, **d)), p, 16, 4,
+                                               4, None, p, need, None)
+    for mine, a in c.items():
+        for theirs in far:
+            for at in (a, a + 16, a + size[mine] - 16, a - size[theirs] // 2 + 16):
+                assert evict({**far, theirs: at}) == zq.ERR_ARG, (mine, theirs, at - a)
+    if not torch.cuda.is_available():
+        for mine, a in c.items():
+            for theirs in far:
+                for at in (a + size[mine], a - size[theirs] // 2):
+                    assert evict({**far, theirs: at}) == zq.ERR_NO_DEVICE, (mine, theirs, at - a)
+
+
 class FakeLibrary:
     """The decoder's entry points that Model.kv_cache meets, over made-up addresses."""
 

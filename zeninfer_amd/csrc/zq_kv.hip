@@ -610,6 +610,27 @@ private:
     bool moved_ = false;
 };
 
+// Some array of b meets some array of a.
+bool arrays_meet(const zq_kv_q4& a, const zq_kv_q4& b) {
+    struct Range {
+        uintptr_t at;
+        size_t bytes;
+    };
+    auto ranges = [](const zq_kv_q4& c, Range (&r)[6]) {
+        const size_t rows = c.seqs * c.kv_heads * c.capacity, codes = rows * (c.head_dim / 2), scales = rows * (c.head_dim / 16);
+        const void* p[6] = {c.k, c.v, c.k_scale, c.v_scale, c.weight, c.pos};
+        const size_t n[6] = {codes, codes, scales, scales, rows * 4, rows * 4};
+        for (int i = 0; i < 6; ++i) r[i] = {reinterpret_cast<uintptr_t>(p[i]), n[i]};
+    };
+    Range x[6], y[6];
+    ranges(a, x);
+    ranges(b, y);
+    for (const Range& i : x)
+        for (const Range& j : y)
+            if (i.at < j.at + j.bytes && j.at < i.at + i.bytes) return true;
+    return false;
+}
+
 bool tokens_ok(const zq_kv_q4& c, size_t tokens, size_t heads) {
     return tokens && tokens <= zq::kKvMaxRows && heads <= zq::kKvMaxHeads && c.seqs * heads <= zq::kKvMaxRows / tokens;
 }
@@ -696,9 +717,7 @@ int zq_hip_kv_q4_evict_dev(const zq_kv_q4* cache, const zq_kv_q4* dst, const int
             return ZQ_ERR_ARG;
     } else if (!zq::kv_q4_ok(dst) || !dst->weight || !dst->pos || dst->seqs != cache->seqs ||
                dst->kv_heads != cache->kv_heads || dst->head_dim != cache->head_dim ||
-               dst->capacity < (keep < cache->capacity ? keep : cache->capacity) || dst->v == cache->v ||
-               dst->k_scale == cache->k_scale || dst->v_scale == cache->v_scale || dst->weight == cache->weight ||
-               dst->pos == cache->pos) {
+               dst->capacity < (keep < cache->capacity ? keep : cache->capacity) || arrays_meet(*cache, *dst)) {
         return ZQ_ERR_ARG;
     }
     if (workspace_bytes < zq::kv_q4_evict_bytes(*cache, keep)) return ZQ_ERR_ARG;

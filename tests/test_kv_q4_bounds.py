@@ -255,6 +255,18 @@ def test_a_models_cache_ends_with_its_arrays(monkeypatch):
     refused(c)
 
 
+def test_a_models_row_budget_is_not_below_zero(monkeypatch):
+    """A uint32_t takes -1 as 4,294,967,295: a cache without a bound."""
+    from zeninfer_amd import model, zq
+    with monkeypatch.context() as mp:
+        mp.setattr(zq, "lib", lambda: FakeLibrary(zq))
+        m = model.Model(1, zq.ModelConfig())
+    for bad in (dict(rows=-1), dict(rows=64, recent=-1), dict(rows=64, first=-4)):
+        with pytest.raises(ValueError, match="a number of rows below zero"):
+            m.set_kv_cache(model.KV_Q4, **bad)
+    m.set_kv_cache(model.KV_Q4, 64, 8, 4)
+
+
 @pytest.mark.parametrize("D", [64, 128, 256])
 def test_staged_keys_lie_in_the_arrays(check_stage, D):
     bad = {C: check_stage(D, C) for C in [*range(32, 2049, 32), 40000, 65504, 99968]}

@@ -93,6 +93,8 @@ class Model:
         """The KV cache's form (zq_model_set_kv_cache): KV_F32, or KV_Q4 with at most `rows` rows kept by the
         attention weight they draw (0: every position).  The cache starts empty; handles of the one before
         (kv_cache) are refused from here on."""
+        if min(rows, recent, first) < 0:
+            raise ValueError(f"set_kv_cache: a number of rows below zero (rows {rows}, recent {recent}, first {first})")
         zq.check(self._L.zq_model_set_kv_cache(self._h, form, rows, recent, first), "set_kv_cache")
         self._arrays = object()
 

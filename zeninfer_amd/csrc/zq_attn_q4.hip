@@ -109,12 +109,14 @@ __device__ __forceinline__ float sum_groups(float v) {
 // its own, and the running maximum is only moved (and the sums rescaled) when a score
 // passes it by 2^8: weights stay below 2^14, within fp16.
 // Bound by the rows' bytes with one row tile and many keys: 64 sequences of up to 8190 rows,
-// 8 kv heads x 4, D = 128: 242 MB in 62.6 us, 3.9 TB/s (a large copy: 5.0).  By latency with
-// one sequence: 24,001 rows 11.8 us (+ 4.0 for joining the splits), 601 rows 6.3 (+ 3.4).  By
-// the decoding, two vector instructions a value, with several row tiles: 16 sequences of up to
-// 3001 rows, 4 kv heads x 7, D = 64, 6 tokens: 15.1 us (+ 5.5).  Tiles two deep on their way
-// cost a wave a SIMD (65 us for the first), two row tiles a workgroup more registers than their
-// shared decoding gives (16.5 for the last).
+// 8 kv heads x 4, D = 128: 242 MB in 58.3 us, 4.1 TB/s (a large copy: 4.9), with vector
+// instructions on 52 % of the issue slots.  By latency with one sequence: 24,001 rows 11.8 us
+// (+ 3.9 for joining the splits), 601 rows 6.3 (+ 3.6).  By latency, and by the longest
+// sequence, with several row tiles and uneven lengths: 16 sequences of up to 3001 rows, 4 kv heads
+// x 7, D = 64, 6 tokens: 14.5 us (+ 5.3), 19 % of the issue slots and the matrix cores busy 4 %
+// of the time.  Against the times of their step, tiles two deep on their way cost a wave a SIMD
+// (65 for 60 us for the first), two row tiles a workgroup more registers than their shared
+// decoding gives (16.5 for 15.2 for the last).
 constexpr int kWaves = 4;
 constexpr float kShift = 6.0f;  // weights are 2^(s - max + kShift)
 constexpr float kSlack = 8.0f;  // how far a score may pass the running maximum
@@ -442,11 +444,12 @@ __global__ __launch_bounds__(kWaves * 64, D == 64 ? 4 : D == 128 ? 3 : 2) void a
 //    lane's 16 scores are those of keys 8 h .. 8 h + 7 and 16 + 8 h .. (h = lane >> 5):
 //    the B operands of the second product as they are, and V^T is read in 16-byte runs.
 // Bound by the matrix products, twice those of the formula as both fp32 factors go in as two
-// parts: 1024 tokens behind 7168 rows, 32 heads, D = 128: 258 GF in 275 us, 0.94 PF/s (a
-// large f16 product: 1.1).  A whole prompt of 2048 tokens takes 95 us, 0.73 PF/s: the first
-// tiles see few keys, and a workgroup takes 5 us to stage its queries.  D = 256, 4
-// sequences of up to 1777 rows, 333 tokens, 4 heads: 44 us + 6 for joining the splits.  Two
-// workgroups of four waves a CU instead of one of eight: 99 us for the prompt.
+// parts: 1024 tokens behind 7168 rows, 32 heads, D = 128: 258 GF in 250 us, 1.03 PF/s (a
+// large f16 product: 1.34), the matrix cores busy 45 % of the time.  A whole prompt of 2048
+// tokens takes 83 us, 0.83 PF/s: the first tiles see few keys, and a workgroup takes 5 us to
+// stage its queries.  D = 256, 4 sequences of up to 1777 rows, 333 tokens, 4 heads: 41 us + 6
+// for joining the splits: one workgroup a CU, of unequal lengths.  Two workgroups of four waves
+// a CU instead of one of eight: 99 for 94 us for the prompt, at the clocks of that step.
 constexpr uint32_t kTileRows = 128;
 typedef float v16f_t __attribute__((ext_vector_type(16)));
 
@@ -456,7 +459,9 @@ struct Big {
     static constexpr int DG = 2 / KG;            // parts of the head dimension, likewise
     static constexpr int T = 512;                // threads
     static constexpr int TK = StageShape<D>::TK;  // keys of a step
-    static constexpr int HP = D + 8;             // halves of a K row in LDS: 16-byte reads of 32 rows, no conflict
+    // halves of a K row in LDS: the 16-byte parts of 16 rows lie on banks of their own (counted all the same, over
+    // all of the kernel: conflicts are 14 % of the LDS cycles, 24 % at D = 256)
+    static constexpr int HP = D + 8;
     static constexpr int KP = TK + 8;            // halves of a V^T row
     static constexpr int NT = D / 32 / DG, KS = D / 16 / DG;  // a wave's tiles of O^T, its steps of a score
     static constexpr int kTasks = StageShape<D>::kTasks;  // blocks of K, and 8-key column groups of V, of a step
@@ -1109,7 +1114,8 @@ __global__ __launch_bounds__(256) void attn_q4_weights_few_kernel(AttnQ4 a, uint
 // rows, whose operands the attention kernel has left in memory.  The next tile's
 // products stand between this one's exponentials; operands are loaded two tiles ahead.
 // Bound by the products: 1024 tokens x 32 heads over 8192 rows, D = 128: 129 GF in two parts
-// in 127 to 137 us, 1.0 PF/s (with the operands made here again: 233).
+// in 118 us, 1.09 PF/s (a large f16 product: 1.34; with the operands made here again the
+// kernel took 233 for 139 us at that step).
 template <int D>
 __global__ __launch_bounds__(512) void attn_q4_weights_many_kernel(AttnQ4 a) {
     using W = Wgt<D>;

@@ -15,9 +15,9 @@ constexpr int kT = 256;
 // ---- append ------------------------------------------------------------------
 // One lane takes four consecutive elements of a row's key and of its value, so 8
 // lanes hold a block and D / 4 lanes a row; a wave takes 256 / D rows (one row =
-// one token of one kv head).  Bound by the fp32 rows it reads, 8 D bytes a row
-// against D + D / 8 written, and by its launch: 1024 tokens of 8 kv heads, D = 128,
-// take 6.3 us, 3.0 TB/s.
+// one token of one kv head).  Bound by its launch and two dependent round trips to
+// memory, then by the fp32 rows it reads, 8 D bytes a row against D + D / 8 written: 1024
+// tokens of 8 kv heads, D = 128, 9.6 MB, take 6.2 us, 1.5 TB/s; 26 tokens 3.7 us.
 // The block's scale is an eighth of its element of largest magnitude, negated,
 // so that this element gets code 0 and all 16 codes are in use.  m / -8 is exact;
 // rounding it to bf16 leaves (code - 8) * d with at most 11 significant bits,
@@ -126,7 +126,8 @@ __global__ __launch_bounds__(kT) void kv_q4_append_kernel(const float* __restric
 
 // The decoder's form: rows are the heads of a token, H query heads and then the kv
 // heads.  Pairs (2 i, 2 i + 1) of a float4 rotate by positions' factors; elements past
-// 2 * pairs are left (rope(), :317-328 of the reference runtime).
+// 2 * pairs are left (rope(), :317-328 of the reference runtime).  Bound as the append:
+// 32 + 8 heads of D = 128, one token 3.8 us, 1024 tokens (43 MB, most of it q) 16.4, 2.6 TB/s.
 template <int D>
 __global__ __launch_bounds__(kT) void rope_kv_q4_kernel(zq_kv_q4 c, const float* q, float* q_out,
                                                         const float* __restrict__ k, const float* __restrict__ v,
@@ -167,7 +168,7 @@ __global__ __launch_bounds__(kT) void rope_kv_q4_kernel(zq_kv_q4 c, const float*
 // ---- read ----------------------------------------------------------------------
 // A lane gives four elements (the low or the high nibbles of four bytes), so a
 // row's stores are as wide as its fp32 elements allow: bound by those.  262,144 rows,
-// D = 128: 54 us, 5.7 TB/s; 8192 rows 4.9 us.
+// D = 128: 54 us, 5.7 TB/s; 8192 rows 4.8 us.
 template <int D>
 __global__ __launch_bounds__(kT) void kv_q4_read_kernel(zq_kv_q4 c, float* __restrict__ k, float* __restrict__ v,
                                                         uint32_t tokens, const int32_t* __restrict__ first,
@@ -201,7 +202,8 @@ __global__ __launch_bounds__(kT) void kv_q4_read_kernel(zq_kv_q4 c, float* __res
 // A second launch copies the rows' codes and scales (the one workgroup would take 11 us
 // for 1024 rows of D = 64 where that launch takes 3).
 // Bound by latency: the keys in one read, three digits of an LDS histogram, the ranks.
-// 128 of them with 8192 rows take 14 us, one with 1153 rows 7.
+// 128 of them with 8192 rows take 19 us (14 where an L2 holds their weights), 8 with 1153
+// rows 7; a decoder's 256, 1024 rows more than the 2048 that stay, 15.
 constexpr int kEvT = 1024, kEvWaves = kEvT / 64;
 constexpr int kEvHeld = 24;  // keys a thread holds at most: caches up to 24576 rows are read once
 
@@ -428,7 +430,8 @@ __global__ __launch_bounds__(kEvT) void kv_q4_evict_kernel(zq_kv_q4 c, zq_kv_q4 
 // A workgroup copies 64 rows of one (sequence, kv head): codes in 16-byte parts, scales
 // one by one from their planes, all loads before the stores.  Kept rows lie anywhere, so a
 // row's 64 bytes of codes bring a line of 128 and a scale one of its own: 262,144 rows,
-// D = 128, another cache: 32 us for 75 MB that are used.
+// D = 128, another cache: 32 us for 75 MB that are used; in place, 256 caches that keep 2048
+// rows each: 26 us.
 constexpr uint32_t kMoveRows = 64;
 template <int D>
 __global__ __launch_bounds__(kT) void kv_q4_evict_move_kernel(zq_kv_q4 c, zq_kv_q4 dst, int in_place,

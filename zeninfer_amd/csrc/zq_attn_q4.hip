@@ -110,7 +110,7 @@ __device__ __forceinline__ float sum_groups(float v) {
 // passes it by 2^8: weights stay below 2^14, within fp16.
 // Bound by the rows' bytes with one row tile and many keys: 64 sequences of up to 8190 rows,
 // 8 kv heads x 4, D = 128: 242 MB in 58.3 us, 4.1 TB/s (a large copy: 4.9), with vector
-// instructions on 52 % of the issue slots.  By latency with one sequence: 24,001 rows 11.8 us
+// instructions on 53 % of the issue slots.  By latency with one sequence: 24,001 rows 11.8 us
 // (+ 3.9 for joining the splits), 601 rows 6.3 (+ 3.6).  By latency, and by the longest
 // sequence, with several row tiles and uneven lengths: 16 sequences of up to 3001 rows, 4 kv heads
 // x 7, D = 64, 6 tokens: 14.5 us (+ 5.3), 19 % of the issue slots and the matrix cores busy 4 %

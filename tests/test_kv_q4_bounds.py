@@ -146,6 +146,21 @@ def test_wrappers_refuse_other_types(monkeypatch):
             zq.kv_q4_append_dev(c, x, p, 1, lens)
 
 
+def test_wrappers_refuse_what_is_no_tensor():
+    """Arrays of the host and lists are refused as such, for every buffer."""
+    from zeninfer_amd import zq
+    c = zq.KVQ4(1 << 20, 2 << 20, 3 << 20, 4 << 20, 1, 2, 64, 64, weight=5 << 20, pos=6 << 20)
+    p = 7 << 20
+    for bad in (np.zeros(4096, np.float32), np.zeros(4096, np.int32), [0.0] * 4096):
+        for call in (lambda: zq.kv_q4_append_dev(c, bad, p, 1, p), lambda: zq.kv_q4_append_dev(c, p, bad, 1, p, stride=256),
+                     lambda: zq.kv_q4_append_dev(c, p, p, 1, bad), lambda: zq.kv_q4_read_dev(c, bad, None, 1, p),
+                     lambda: zq.attention_q4_dev(c, bad, p, 1, 4, p, 1.0), lambda: zq.attention_q4_dev(c, p, bad, 1, 4, p, 1.0),
+                     lambda: zq.attention_q4_dev(c, p, p, 1, 4, p, 1.0, counts=bad),
+                     lambda: zq.kv_q4_evict_dev(c, bad, 16, 4, 4), lambda: zq.KVQ4(p, p, bad, p, 1, 2, 64, 64)):
+            with pytest.raises(ValueError, match="tensor must be on the GPU"):
+                call()
+
+
 def test_wrappers_refuse_sizes_below_zero(monkeypatch):
     """A size_t takes -1 as the largest number: any workspace would be long enough, and everything would be kept."""
     from zeninfer_amd import zq

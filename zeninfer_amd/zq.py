@@ -611,8 +611,10 @@ _KINDS = {"float32": set(), "float16": set(), "int32": set(), "int": set()}  # t
 def _need_kind(t, kind, what):
     """A tensor holds values of the kind, or their bytes (a part of a uint8 buffer).  Others' buffers may be long
     enough, and would be read as other values."""
-    if t is None or isinstance(t, int) or t.dtype in _KINDS[kind]:
+    if t is None or isinstance(t, int) or getattr(t, "dtype", None) in _KINDS[kind]:
         return
+    if not hasattr(t, "element_size"):  # no tensor
+        return _check_device(t, what)
     size, floating = t.element_size(), t.is_floating_point()
     integer = not floating and not t.is_complex()
     if not (integer and size == 1 or {"float32": floating and size == 4, "int32": integer and size == 4, "int": integer,
@@ -650,7 +652,8 @@ class KVQ4:
 
 def _need_ints(t, n, what, dev):
     """Device address of n int32 values (torch's own default, int64, would be read as twice as many)."""
-    if t is not None and not isinstance(t, int) and (t.element_size() != 4 or t.is_floating_point()):
+    if t is not None and not isinstance(t, int) and hasattr(t, "element_size") and (
+            t.element_size() != 4 or t.is_floating_point()):
         raise ValueError(f"{what}: needs int32, got {t.dtype}")
     return _need(t, 4 * n, what, dev)
 

@@ -79,6 +79,9 @@ def views():
         ("wider rows than asked", buf[:, :, 128:300], 2, 8, 512, True),
         ("a token of each sequence", buf[:, 5, :128], 2, 1, 8 * 512, True),
         ("a token of each sequence, dimension kept", buf[:, 5:6, :128], 2, 1, 8 * 512, True),
+        ("a row", flat[3:4, 128:256], 1, 1, 512, True),
+        ("tokens before a batch of one", flat[:6, None, 128:256], 1, 6, 512, True),
+        ("tokens before a batch of one, heads apart", flat[:6, 128:256].unflatten(-1, (2, 64))[:, None], 1, 6, 512, True),
         ("some tokens of each sequence", buf[:, :3, :128], 2, 3, 512, False),
         ("sequences in place, tokens not asked for", buf[:, :, :128], 2, 3, 512, False),
         ("a token of each sequence, by the tokens' stride", buf[:, 5, :128], 2, 1, 512, False),
@@ -106,8 +109,8 @@ def test_strided_views_are_the_rows_that_the_kernels_read(monkeypatch, name, vie
     assert call() == view.data_ptr()
     read = torch.as_strided(view, (seqs, tokens, 128), (tokens * stride, stride, 1), view.storage_offset())
     rows = view.flatten(-2) if view.shape[-1] == 64 else view
-    if rows.dim() == 2:
-        rows = rows[:seqs * tokens].unflatten(0, (seqs, tokens))
+    if rows.dim() == 2 or rows.shape[1] < tokens:
+        rows = rows.reshape(-1, rows.shape[-1])[:seqs * tokens].unflatten(0, (seqs, tokens))
     assert torch.equal(read, rows[:seqs, :tokens, :128])
 
 

@@ -674,6 +674,7 @@ def _need_rows(t, seqs, tokens, stride, width, what, dev):
     dims, row = [(a, b) for a, b in zip(t.shape, t.stride())], 1
     while dims and row < width and (dims[-1][0] == 1 or dims[-1][1] == row):
         row *= dims.pop()[0]
+    dims = [d for d in dims if d[0] != 1] or [(1, 0)]
     need = [(seqs * tokens, stride)] if len(dims) == 1 else [(seqs, tokens * stride), (tokens, stride)]
     if t.element_size() != 4 or row < width or len(dims) != len(need) or any(
             size < count or (count > 1 and at != step) for (size, at), (count, step) in zip(dims, need)):

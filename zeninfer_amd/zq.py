@@ -23,6 +23,8 @@ ERR_ARG, ERR_NO_DEVICE, ERR_OOM, ERR_HIP, ERR_TOO_LARGE = -1, -2, -3, -4, -5
 WEIGHT_TAIL_PAD = 64
 MAX_BATCH = 8
 ATTN_Q4_FULL, ATTN_Q4_WEIGHTS, ATTN_Q4_ADD = 1, 2, 4
+KV_F32, KV_F16, KV_BF16 = 0, 1, 2
+ATTN_PAGED_FULL = 1
 
 _P = ctypes.c_void_p
 _S = ctypes.c_size_t
@@ -150,6 +152,32 @@ KV_SIGNATURES = {
 }
 
 
+class PageTablesC(ctypes.Structure):
+    """zq_page_tables (include/zq_paged.h)."""
+    _fields_ = [("table", _P), ("free_pages", _P), ("seqs", _S), ("width", _S), ("pages", _S), ("page_size", _S)]
+
+
+class KVCachePaged(ctypes.Structure):
+    """zq_kv_paged (include/zq_paged.h)."""
+    _fields_ = [(n, _P) for n in ("k", "v", "bounds", "bounds_exp")] + [
+        (n, _S) for n in ("pages", "kv_heads", "head_dim", "page_size")] + [("type", ctypes.c_int)]
+
+
+# Every symbol include/zq_paged.h declares.
+_PT, _PG = ctypes.POINTER(PageTablesC), ctypes.POINTER(KVCachePaged)
+PAGED_SIGNATURES = {
+    "zq_hip_page_tables_step_dev": (ctypes.c_int, [_PT, _P, _P, _P, _P, _P, _P, _P, _P, _P, _S, _P]),
+    "zq_hip_page_tables_release_dev": (ctypes.c_int, [_PT, _P, _P, _P, _P, _P]),
+    "zq_hip_kv_paged_append_dev": (ctypes.c_int, [_PG, _P, _P, _S, _S, _P, _P]),
+    "zq_hip_attention_paged_workspace_bytes": (_S, [_PG, _PT, _S, _S]),
+    "zq_hip_attention_paged_dev": (ctypes.c_int, [_PG, _PT, _P, _P, _S, _S, _S, _P, _P, _P, _P, _S, ctypes.c_float,
+                                                  ctypes.c_int, _P, _S, _P]),
+    "zq_hip_page_select_workspace_bytes": (_S, [_PG, _PT, _S, _S, _S]),
+    "zq_hip_page_select_dev": (ctypes.c_int, [_PG, _PT, _P, _P, _S, _S, _S, _P, _P, _P, _S, _S, _S, ctypes.c_int, _P, _S,
+                                              _P]),
+}
+
+
 class ModelConfig(ctypes.Structure):
     _fields_ = [(n, ctypes.c_uint32) for n in ("embedding", "layers", "heads", "kv_heads", "head_dim", "ffn", "vocab",
                                                "context", "max_positions", "rope_dim")] + [
@@ -200,7 +228,8 @@ def lib():
             raise RuntimeError(f"{path} is missing: build it with `python -m zeninfer_amd.build` "
                                "(there is no CPU fallback for this path)")
         L = ctypes.CDLL(path)
-        for name, (res, args) in {**SIGNATURES, **GGUF_SIGNATURES, **KV_SIGNATURES, **MODEL_SIGNATURES}.items():
+        for name, (res, args) in {**SIGNATURES, **GGUF_SIGNATURES, **KV_SIGNATURES, **PAGED_SIGNATURES,
+                                  **MODEL_SIGNATURES}.items():
             fn = getattr(L, name)
             fn.restype = res
             fn.argtypes = args
@@ -742,3 +771,149 @@ def kv_q4_evict_dev(cache, lens, keep, recent, first, next_pos=None, dst=None, w
     return check(lib().zq_hip_kv_q4_evict_dev(cache.ref, dst.ref if dst is not None else None, lens, keep, recent, first,
                                               next_pos, workspace, workspace_bytes, _stream(stream)),
                  "zq_hip_kv_q4_evict_dev")
+
+
+# ---- paged KV cache (include/zq_paged.h) -----------------------------------
+_PAGED_TYPES = {"torch.float32": (KV_F32, 4), "torch.float16": (KV_F16, 2), "torch.bfloat16": (KV_BF16, 2)}
+
+
+def _need_long(t, n, what, dev):
+    """Device address of n int64 values."""
+    if t is not None and not isinstance(t, int) and hasattr(t, "element_size") and (
+            t.element_size() != 8 or t.is_floating_point()):
+        raise ValueError(f"{what}: needs int64, got {t.dtype}")
+    return _need(t, 8 * n, what, dev)
+
+
+class PageTables:
+    """Which pages sequences have (zq_page_tables), over the caller's device arrays: table [seqs][width] and the stack
+    of free pages free_pages [pages] (None where only attention and selection use it), int32.  The arrays are checked
+    once, here, and kept alive with the handle."""
+
+    def __init__(self, table, free_pages, seqs, width, pages, page_size):
+        if min(seqs, width, pages, page_size) < 0:
+            raise ValueError(f"PageTables: a size below zero (seqs {seqs}, width {width}, pages {pages}, page_size {page_size})")
+        dev = self.dev = _device_index()
+        self.c = PageTablesC(_need_ints(table, seqs * width, "PageTables table", dev),
+                             _need_ints(free_pages, pages, "PageTables free_pages", dev), seqs, width, pages, page_size)
+        self.arrays = [table, free_pages]
+        self.seqs, self.width, self.pages, self.page_size = seqs, width, pages, page_size
+        self.ref = ctypes.byref(self.c)
+
+
+class KVPaged:
+    """A paged KV cache over the caller's device arrays (zq_kv_paged): k and v [pages][kv_heads][page_size][head_dim]
+    of one of the types float32, float16 and bfloat16 (raw addresses: `type`, a KV_* number), and optionally bounds
+    [pages][kv_heads][2][head_dim] and bounds_exp [pages][kv_heads], int8.  Checked once, here, and kept alive."""
+
+    def __init__(self, k, v, pages, kv_heads, head_dim, page_size, bounds=None, bounds_exp=None, type=None):
+        if min(pages, kv_heads, head_dim, page_size) < 0:
+            raise ValueError(f"KVPaged: a size below zero (pages {pages}, kv_heads {kv_heads}, head_dim {head_dim}, "
+                             f"page_size {page_size})")
+        dev = self.dev = _device_index()
+        for t, name in ((k, "k"), (v, "v")):
+            if t is None or isinstance(t, int):
+                continue
+            if str(getattr(t, "dtype", None)) not in _PAGED_TYPES:
+                raise ValueError(f"KVPaged {name}: needs float32, float16 or bfloat16, got {getattr(t, 'dtype', t)}")
+            kind = _PAGED_TYPES[str(t.dtype)][0]
+            if type is not None and kind != type:
+                raise ValueError(f"KVPaged {name}: is {t.dtype}, not of the cache's type")
+            type = kind
+        if type not in (KV_F32, KV_F16, KV_BF16):
+            raise ValueError(f"KVPaged: no type of a cache: {type}")
+        for t, name in ((bounds, "bounds"), (bounds_exp, "bounds_exp")):
+            if t is not None and not isinstance(t, int) and hasattr(t, "dtype") and str(t.dtype) != "torch.int8":
+                raise ValueError(f"KVPaged {name}: needs int8, got {t.dtype}")
+        heads = pages * kv_heads
+        n = heads * page_size * head_dim * (4 if type == KV_F32 else 2)
+        self.c = KVCachePaged(_need(k, n, "KVPaged k", dev), _need(v, n, "KVPaged v", dev),
+                              _need(bounds, heads * 2 * head_dim, "KVPaged bounds", dev),
+                              _need(bounds_exp, heads, "KVPaged bounds_exp", dev), pages, kv_heads, head_dim, page_size,
+                              type)
+        self.arrays = [k, v, bounds, bounds_exp]
+        self.pages, self.kv_heads, self.head_dim, self.page_size, self.type = pages, kv_heads, head_dim, page_size, type
+        self.ref = ctypes.byref(self.c)
+
+
+def page_tables_step_dev(tables, lens, counts, free_count, free_left, granted, start, slots, positions, seq_of, tokens,
+                         stream=None):
+    """Pages for counts [seqs] new tokens behind lens [seqs] held ones; slots, positions and seq_of [tokens] of the
+    packed new tokens (positions and seq_of may be None), start [seqs + 1], granted [seqs]."""
+    dev, n = tables.dev, tables.seqs
+    lens = _need_ints(lens, n, "page_tables_step_dev lens", dev)
+    counts = _need_ints(counts, n, "page_tables_step_dev counts", dev)
+    free_count = _need_ints(free_count, 1, "page_tables_step_dev free_count", dev)
+    free_left = _need_ints(free_left, 1, "page_tables_step_dev free_left", dev)
+    granted = _need_ints(granted, n, "page_tables_step_dev granted", dev)
+    start = _need_ints(start, n + 1, "page_tables_step_dev start", dev)
+    slots = _need_long(slots, tokens, "page_tables_step_dev slots", dev)
+    positions = _need_ints(positions, tokens, "page_tables_step_dev positions", dev)
+    seq_of = _need_ints(seq_of, tokens, "page_tables_step_dev seq_of", dev)
+    return check(lib().zq_hip_page_tables_step_dev(tables.ref, lens, counts, free_count, free_left, granted, start, slots,
+                                                   positions, seq_of, tokens, _stream(stream)),
+                 "zq_hip_page_tables_step_dev")
+
+
+def page_tables_release_dev(tables, lens, keep, free_count, free_left, stream=None):
+    """Gives back the pages that sequences of lens [seqs] tokens do not need for their first keep [seqs]."""
+    dev, n = tables.dev, tables.seqs
+    lens = _need_ints(lens, n, "page_tables_release_dev lens", dev)
+    keep = _need_ints(keep, n, "page_tables_release_dev keep", dev)
+    free_count = _need_ints(free_count, 1, "page_tables_release_dev free_count", dev)
+    free_left = _need_ints(free_left, 1, "page_tables_release_dev free_left", dev)
+    return check(lib().zq_hip_page_tables_release_dev(tables.ref, lens, keep, free_count, free_left, _stream(stream)),
+                 "zq_hip_page_tables_release_dev")
+
+
+def kv_paged_append_dev(cache, k, v, tokens, slots, stride=0, stream=None):
+    """Keys and values [tokens][stride] fp32 into slots [tokens] (int64)."""
+    dev, width = cache.dev, cache.kv_heads * cache.head_dim
+    k = _need_rows(k, 1, tokens, stride, width, "kv_paged_append_dev k", dev)
+    v = _need_rows(v, 1, tokens, stride, width, "kv_paged_append_dev v", dev)
+    slots = _need_long(slots, tokens, "kv_paged_append_dev slots", dev)
+    return check(lib().zq_hip_kv_paged_append_dev(cache.ref, k, v, tokens, stride, slots, _stream(stream)),
+                 "zq_hip_kv_paged_append_dev")
+
+
+def attention_paged_workspace_bytes(cache, tables, queries, heads):
+    return lib().zq_hip_attention_paged_workspace_bytes(cache.ref, tables.ref, queries, heads)
+
+
+def attention_paged_dev(cache, tables, q, out, queries, heads, lens, scale, counts=None, seq_of=None, select=None, keep=0,
+                        stride=0, flags=0, workspace=None, workspace_bytes=0, stream=None):
+    """Attention of q [queries][stride] over the pages of their sequences (of select [queries][kv_heads][keep] only) into
+    out [queries][heads * head_dim]."""
+    dev, width = cache.dev, heads * cache.head_dim
+    q = _need_rows(q, 1, queries, stride, width, "attention_paged_dev q", dev)
+    out = _need_f32(out, queries * width, "attention_paged_dev out", dev)
+    lens = _need_ints(lens, queries, "attention_paged_dev lens", dev)
+    counts = _need_ints(counts, queries, "attention_paged_dev counts", dev)
+    seq_of = _need_ints(seq_of, queries, "attention_paged_dev seq_of", dev)
+    select = _need_ints(select, queries * cache.kv_heads * keep, "attention_paged_dev select", dev)
+    workspace = _need(workspace, workspace_bytes, "attention_paged_dev workspace", dev)
+    return check(lib().zq_hip_attention_paged_dev(cache.ref, tables.ref, q, out, queries, heads, stride, seq_of, lens,
+                                                  counts, select, keep, scale, flags, workspace, workspace_bytes,
+                                                  _stream(stream)), "zq_hip_attention_paged_dev")
+
+
+def page_select_workspace_bytes(cache, tables, queries, heads, keep):
+    return lib().zq_hip_page_select_workspace_bytes(cache.ref, tables.ref, queries, heads, keep)
+
+
+def page_select_dev(cache, tables, q, select, queries, heads, lens, keep, recent=0, first=0, counts=None, seq_of=None,
+                    stride=0, flags=0, workspace=None, workspace_bytes=0, stream=None):
+    """The `keep` pages of every query and kv head with the largest bound on q . k, the `first` first and `recent` last
+    ones among them, into select [queries][kv_heads][keep]."""
+    dev = cache.dev
+    if min(keep, recent, first) < 0:
+        raise ValueError(f"page_select_dev: a number of pages below zero (keep {keep}, recent {recent}, first {first})")
+    q = _need_rows(q, 1, queries, stride, heads * cache.head_dim, "page_select_dev q", dev)
+    select = _need_ints(select, queries * cache.kv_heads * keep, "page_select_dev select", dev)
+    lens = _need_ints(lens, queries, "page_select_dev lens", dev)
+    counts = _need_ints(counts, queries, "page_select_dev counts", dev)
+    seq_of = _need_ints(seq_of, queries, "page_select_dev seq_of", dev)
+    workspace = _need(workspace, workspace_bytes, "page_select_dev workspace", dev)
+    return check(lib().zq_hip_page_select_dev(cache.ref, tables.ref, q, select, queries, heads, stride, seq_of, lens, counts,
+                                              keep, recent, first, flags, workspace, workspace_bytes, _stream(stream)),
+                 "zq_hip_page_select_dev")

@@ -559,6 +559,39 @@ def test_attention_nan_and_infinity_reach_only_those_who_see_them(zq, kind):
 
 
 @gpu
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("value", [math.nan, math.inf])
+def test_a_value_that_is_no_number_reaches_only_the_drafted_tokens_that_see_it(zq, kind, value):
+    """Queries of one sequence share products; each of them sees one row more."""
+    pool = Pool(zq, kind, [70], 2, 64, 16, seed=13)
+    pool.v[pool.table[0, 4], 1, 1, 9] = value      # row 65 of kv head 1
+    pool.v[pool.table[0, 3], 0, 15, 63] = -value   # row 63 of kv head 0
+    pool.upload(zq)
+    lens = list(range(58, 70))
+    got = run_attention(zq, pool, queries(pool.rng, 12, 6, 64), lens, 0.125, seq_of=[0] * 12)
+    bad = np.zeros((12, 6, 64), bool)
+    for i, n in enumerate(lens):
+        bad[i, 3:, 9] = n >= 65
+        bad[i, :3, 63] = n >= 63
+    assert (np.isfinite(got) == ~bad).all()
+
+
+@gpu
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("G", [1, 2, 3, 5, 8, 9])
+def test_attention_of_drafted_tokens(zq, kind, G):
+    """Runs of queries of one sequence, of all lengths, in any order of lengths, idle ones among them."""
+    pool = Pool(zq, kind, [400, 40, 17, 1], 2, 64, 16, seed=G)
+    seq_of = [0] * 21 + [1] * 3 + [2] + [0] + [3] + [1] * 9 + [-1] + [1] * 2
+    lens = [int(pool.rng.integers(0, pool.lens[max(s, 0)])) for s in seq_of]
+    counts = [int(pool.rng.integers(0, 3)) for _ in seq_of]
+    for c in (None, counts):
+        if c is not None:
+            lens = [min(n, pool.lens[max(s, 0)] - x) for n, s, x in zip(lens, seq_of, c)]
+        check_attention(zq, pool, queries(pool.rng, len(lens), 2 * G, 64), lens, 0.125, seq_of=seq_of, counts=c)
+
+
+@gpu
 def test_attention_of_infinite_scores_and_a_spread_of_sizes(zq):
     """Keys so large that the scores of the reference are past fp32's range in exp only: the largest takes all."""
     pool = Pool(zq, "bf16", [90], 1, 64, 16, seed=11, fill=1e4)

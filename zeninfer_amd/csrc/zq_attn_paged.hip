@@ -20,6 +20,10 @@ typedef __bf16 b8_t __attribute__((ext_vector_type(8)));
 typedef uint32_t v4u_t __attribute__((ext_vector_type(4)));
 typedef uint32_t v2u_t __attribute__((ext_vector_type(2)));
 
+struct Cut {
+    uint32_t query, kh, rows, parts;  // parts 0: none
+    uint64_t slot;                    // of the first part; part j > 0 has slot 2 (w + j)
+};
 struct AttnPaged {
     const uint8_t* k;
     const uint8_t* v;
@@ -27,12 +31,14 @@ struct AttnPaged {
     const int32_t* select;
     const float* q;
     float* out;
-    float* part;     // partial outputs [2 W][G][D]
-    float* part_ml;  // their (max, sum) [2 W][G][2]
+    float* part;     // partial outputs [2 W][RS][D]
+    float* part_ml;  // their (max, sum) [2 W][RS][2]
+    Cut* cut;        // [W] the pair that a share's end cuts, if the share has its start
     Queries see;
     size_t stride;   // floats between queries
     float scale2;    // scale * log2(e): scores are in log2 units
     uint32_t width, pages, KH, G, keep, lp;
+    uint32_t P, RS, RL;  // queries of a group at most, rows of a partial and of a workgroup
 };
 
 // ---- work of a workgroup ---------------------------------------------------------
@@ -51,14 +57,41 @@ __device__ __forceinline__ uint32_t entries_of(const AttnPaged& a, uint32_t rows
     const uint32_t pages = (rows + (1u << a.lp) - 1) >> a.lp;
     return a.select ? min(pages, a.keep) : pages;
 }
-template <int TYPE>
+// Queries of one sequence that lie next to each other, as drafted tokens and prompts do,
+// share a product where their heads fit 16 rows (GROUP; not with selected pages): the
+// first one of every P (by number) and of every sequence stands for those behind it.
+struct Group {
+    Seen first;
+    uint32_t queries, most, least;  // rows that they see
+};
+template <bool GROUP>
+__device__ __forceinline__ Group group_of(const AttnPaged& a, uint32_t i) {
+    Group x{seen_by(a.see, i), 1, 0, 0};
+    x.most = x.least = x.first.rows;
+    if constexpr (GROUP) {
+        for (uint32_t j = i + 1; x.first.seq >= 0 && j < a.see.n && j % a.P; ++j) {
+            const Seen y = seen_by(a.see, j);
+            if (y.seq != x.first.seq) break;
+            ++x.queries;
+            x.most = max(x.most, y.rows);
+            x.least = min(x.least, y.rows);
+        }
+    }
+    return x;
+}
+template <int TYPE, bool GROUP>
 __device__ __forceinline__ uint32_t units_of(const AttnPaged& a, uint32_t i) {
-    const Seen x = seen_by(a.see, i);
-    if (x.seq < 0) return 0;
-    const uint32_t rows = a.select ? entries_of(a, x.rows) << a.lp : x.rows;
+    const Group x = group_of<GROUP>(a, i);
+    if (x.first.seq < 0) return 0;
+    if (GROUP && i % a.P && seen_by(a.see, i - 1).seq == x.first.seq) return 0;
+    const uint32_t rows = a.select ? entries_of(a, x.most) << a.lp : x.most;
     return max((rows + Tile<TYPE>::kUnit - 1) / Tile<TYPE>::kUnit, 1u);  // no rows: a unit that writes zeros
 }
 
+// Where row r (query, head) of a group goes; without groups r is a head, G of them and no more.
+__device__ __forceinline__ size_t out_row(const AttnPaged& a, uint32_t query, uint32_t kh, uint32_t r) {
+    return size_t(query + r / a.G) * a.KH * a.G + size_t(kh) * a.G + r % a.G;
+}
 __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ __forceinline__ float max_groups(float v) {  // over the four lanes that share lane & 15
     v = fmaxf(v, __shfl_xor(v, 16));
@@ -114,6 +147,74 @@ __device__ __forceinline__ v4f_t mma(v4u_t held, v4u_t part, v4f_t c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8_t, held), __builtin_bit_cast(b8_t, part), c, 0, 0, 0);
 }
 
+template <int TYPE, int D>
+struct Shape {
+    static constexpr int ES = TYPE == ZQ_KV_F32 ? 4 : 2;
+    static constexpr int H = Tile<TYPE>::H;
+    static constexpr int KC = D * ES / 64;                          // 16-byte loads of a key
+    static constexpr int VE = TYPE == ZQ_KV_F32 ? 4 : D == 64 ? 4 : 8;  // elements of a V load
+    static constexpr int VC = D / (16 * VE);                        // V loads of a row
+    static constexpr int VW = VE * ES / 4;                          // dwords of one
+    static constexpr int VR = 4 * H;                                // rows whose V a lane loads
+    static constexpr int NP = TYPE == ZQ_KV_F32 ? 1 : TYPE == ZQ_KV_F16 ? 2 : 3;
+    static constexpr bool kQInLds = true;
+};
+
+// The softmax weights of a lane's rows as operands, and what they add to one tile of O^T.
+template <int TYPE, int VR>
+struct Weights {
+    Parts<TYPE> x;
+    __device__ __forceinline__ explicit Weights(const float (&p)[VR]) {
+#pragma unroll
+        for (int r = 0; r < VR; r += 2) x.set2(r, p[r], p[r + 1]);
+    }
+};
+template <int VR>
+struct Weights<ZQ_KV_F32, VR> {
+    float x[VR];
+    __device__ __forceinline__ explicit Weights(const float (&p)[VR]) {
+#pragma unroll
+        for (int r = 0; r < VR; ++r) x[r] = p[r];
+    }
+};
+template <int TYPE, int VR, int VC, int VW, int PARTS = Shape<TYPE, 128>::NP>
+__device__ __forceinline__ v4f_t add_pv(const uint32_t (&v)[VR][VC][VW], const Weights<TYPE, VR>& p, int n, int e, v4f_t o) {
+    if constexpr (TYPE == ZQ_KV_F32) {
+#pragma unroll
+        for (int r = 0; r < VR; ++r) o = __builtin_amdgcn_mfma_f32_16x16x4f32(bits_f(v[r][n][e]), p.x[r], o, 0, 0, 0);
+    } else {
+        v4u_t w;
+#pragma unroll
+        for (int z = 0; z < 4; ++z)
+            w[z] = __builtin_amdgcn_perm(v[2 * z + 1][n][e / 2], v[2 * z][n][e / 2], e & 1 ? 0x07060302u : 0x05040100u);
+#pragma unroll
+        for (int y = PARTS - 1; y >= 0; --y) o = mma<TYPE>(w, p.x.bits(y), o);
+    }
+    return o;
+}
+// Infinities and NaN of a dword's values: ones in their places, and zeros in the dword.
+template <int TYPE>
+__device__ __forceinline__ uint32_t take_odd(uint32_t& w) {
+    constexpr uint32_t m = TYPE == ZQ_KV_F32 ? 0x7f800000u : TYPE == ZQ_KV_F16 ? 0x7c00u : 0x7f80u;
+    constexpr uint32_t one = TYPE == ZQ_KV_F32 ? 0x3f800000u : TYPE == ZQ_KV_F16 ? 0x3c00u : 0x3f80u;
+    constexpr uint32_t all = TYPE == ZQ_KV_F32 ? 0xffffffffu : 0xffffu;
+    uint32_t gone = (w & m) == m ? all : 0u, ones = gone & one;
+    if constexpr (TYPE != ZQ_KV_F32) {
+        const bool hi = (w & m << 16) == m << 16;
+        gone |= hi ? all << 16 : 0u;
+        ones |= hi ? one << 16 : 0u;
+    }
+    w &= ~gone;
+    return ones;
+}
+// Whether there are any.
+template <int TYPE>
+__device__ __forceinline__ bool not_finite(uint32_t w) {
+    if (TYPE == ZQ_KV_F32) return (w & 0x7f800000u) == 0x7f800000u;
+    const uint32_t m = TYPE == ZQ_KV_F16 ? 0x7c00u : 0x7f80u;
+    return (w & m) == m || (w >> 16 & m) == m;
+}
+
 // ---- the kernel ------------------------------------------------------------------
 // Both products are computed transposed (S^T = K Q^T, O^T = V^T P^T) on 16x16 tiles,
 // so that nothing crosses lanes between them.  With lane (i = lane & 15, g = lane >> 4):
@@ -129,20 +230,7 @@ __device__ __forceinline__ v4f_t mma(v4u_t held, v4u_t part, v4f_t c) {
 // in one page: its place is one readlane of the table entries that the wave loaded, 64
 // parts at once.  The next tile's K is asked for when this one's scores are there, the
 // next V when this one is used.
-template <int TYPE, int D>
-struct Shape {
-    static constexpr int ES = TYPE == ZQ_KV_F32 ? 4 : 2;
-    static constexpr int H = Tile<TYPE>::H;
-    static constexpr int KC = D * ES / 64;                          // 16-byte loads of a key
-    static constexpr int VE = TYPE == ZQ_KV_F32 ? 4 : D == 64 ? 4 : 8;  // elements of a V load
-    static constexpr int VC = D / (16 * VE);                        // V loads of a row
-    static constexpr int VW = VE * ES / 4;                          // dwords of one
-    static constexpr int VR = 4 * H;                                // rows whose V a lane loads
-    static constexpr int NP = TYPE == ZQ_KV_F32 ? 1 : TYPE == ZQ_KV_F16 ? 2 : 3;
-    static constexpr bool kQInLds = true;
-};
-
-template <int TYPE, int D>
+template <int TYPE, int D, bool GROUP>
 __global__ __launch_bounds__(kT, D == 64 ? 4 : D == 128 ? 3 : 2) void attn_paged_kernel(AttnPaged a) {
     using S = Shape<TYPE, D>;
     constexpr int H = S::H, KC = S::KC, VE = S::VE, VC = S::VC, VW = S::VW, VR = S::VR, NP = S::NP;
@@ -151,14 +239,15 @@ __global__ __launch_bounds__(kT, D == 64 ? 4 : D == 128 ? 3 : 2) void attn_paged
     __shared__ float sm[kWaves][16], sl[kWaves][16];
     const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const uint32_t row0 = blockIdx.y * 16, R = min(a.G - row0, 16u);  // rows of this workgroup
-    const auto units = [&](uint32_t n) { return units_of<TYPE>(a, n); };
+    const uint32_t row0 = GROUP ? 0u : blockIdx.y * 16;  // the first head of this workgroup's
+    const auto units = [&](uint32_t n) { return units_of<TYPE, GROUP>(a, n); };
     uint32_t mine, own;
     const Shares sh = scan_units(a.see.n, a.KH, gridDim.x, units, scan, mine, own);
+    if (threadIdx.x == 0 && blockIdx.y == 0) a.cut[blockIdx.x].parts = 0;
     if (blockIdx.x >= sh.used) return;
     const uint64_t begin = share_start(sh, blockIdx.x), end = share_start(sh, blockIdx.x + 1);
-    find_query(a.see.n, a.KH, units, scan, begin, mine, own);
-    uint32_t qi = scan.query, before = scan.before;
+    const Found at_begin = find_query(a.see.n, a.KH, units, scan, begin, mine, own);
+    uint32_t qi = at_begin.query, before = at_begin.before;
     uint64_t pos = begin;
     const size_t head_rows = size_t(1) << a.lp;
     while (pos < end) {
@@ -170,17 +259,20 @@ __global__ __launch_bounds__(kT, D == 64 ? 4 : D == 128 ? 3 : 2) void attn_paged
         }
         const uint32_t rel = uint32_t(pos - uint64_t(before) * a.KH), kh = rel / u, u0 = rel % u;
         const uint32_t u1 = uint32_t(min(uint64_t(u), u0 + (end - pos)));
-        const Seen x = seen_by(a.see, qi);
-        const uint32_t entries = entries_of(a, x.rows);
-        const uint32_t parts = a.select ? entries << (a.lp - 4) : (x.rows + 15) >> 4;  // 16-key parts of the pair
+        const Group x = group_of<GROUP>(a, qi);
+        const uint32_t R = GROUP ? x.queries * a.G : min(a.G - row0, 16u);  // rows: query, head
+        const uint32_t entries = entries_of(a, x.most);
+        const uint32_t parts = a.select ? entries << (a.lp - 4) : (x.most + 15) >> 4;  // 16-key parts of the pair
         const uint32_t tiles = (parts + H - 1) / H;
         const uint32_t t0 = u0 * kWaves + wave, t1 = min(u1 * kWaves, tiles);
         const uint32_t nt = t0 < t1 ? (t1 - t0 + kWaves - 1) / kWaves : 0;  // tiles of this wave
-        const int32_t* table = a.table + size_t(x.seq) * a.width;
+        const int32_t* table = a.table + size_t(x.first.seq) * a.width;
         const int32_t* select = a.select ? a.select + (size_t(qi) * a.KH + kh) * a.keep : nullptr;
 
         // ---- the queries as operands ----
-        const float* qrow = a.q + qi * a.stride + (size_t(kh) * a.G + row0 + min(uint32_t(i), R - 1)) * D;
+        const uint32_t row = min(uint32_t(i), R - 1), member = GROUP ? row / a.G : 0u;
+        const float* qrow = a.q + (qi + member) * a.stride + (size_t(kh) * a.G + row0 + row - member * a.G) * D;
+        const uint32_t my_rows = GROUP ? seen_by(a.see, qi + member).rows : 0u;  // that this lane's query sees
         v4u_t qop[S::kQInLds ? 1 : KC][NP];
         float c = a.scale2;  // takes a score into log2 units
         {
@@ -220,7 +312,7 @@ __global__ __launch_bounds__(kT, D == 64 ? 4 : D == 128 ? 3 : 2) void attn_paged
                     for (int n = 0; n < NP; ++n) op[n] = p.bits(n);
                 }
                 if constexpr (S::kQInLds) {
-                    v4u_t* at = reinterpret_cast<v4u_t*>(dyn + kWaves * R * (D + 4));
+                    v4u_t* at = reinterpret_cast<v4u_t*>(dyn + kWaves * a.RL * (D + 4));
                     if (k % kWaves == wave)
 #pragma unroll
                         for (int n = 0; n < NP; ++n) at[(k * NP + n) * 64 + lane] = op[n];
@@ -256,10 +348,10 @@ __global__ __launch_bounds__(kT, D == 64 ? 4 : D == 128 ? 3 : 2) void attn_paged
                 place = 0;
                 if (j < nt && e < entries) {
                     const uint32_t y = select ? uint32_t(select[e]) : e;  // place in the sequence
-                    if (y < a.width && (y << a.lp) < x.rows) {
+                    if (y < a.width && (y << a.lp) < x.most) {
                         const uint32_t page = uint32_t(table[y]);
                         const uint32_t first = (y << a.lp) + ((part << 4) & (uint32_t(head_rows) - 1));
-                        if (page < a.pages && first < x.rows) place = page | min(x.rows - first, 16u) << 24;
+                        if (page < a.pages && first < x.most) place = page | min(x.most - first, 16u) << 24;
                     }
                 }
             }
@@ -307,7 +399,7 @@ __global__ __launch_bounds__(kT, D == 64 ? 4 : D == 128 ? 3 : 2) void attn_paged
 #pragma unroll
                     for (int n = 0; n < NP; ++n) {
                         if constexpr (S::kQInLds)
-                            op[n] = reinterpret_cast<const v4u_t*>(dyn + kWaves * R * (D + 4))[(k * NP + n) * 64 + lane];
+                            op[n] = reinterpret_cast<const v4u_t*>(dyn + kWaves * a.RL * (D + 4))[(k * NP + n) * 64 + lane];
                         else
                             op[n] = qop[k][n];
                     }
@@ -329,16 +421,20 @@ __global__ __launch_bounds__(kT, D == 64 ? 4 : D == 128 ? 3 : 2) void attn_paged
                 for (int h = 0; h < H; ++h) {
                     rows[h] = rows_at(j * H + h);
                     cut |= rows[h] < 16;
+                    if (GROUP) cut |= (((t0 + (b + j) * kWaves) * H + h) << 4) + 16 > x.least;
                 }
                 if constexpr (!decltype(last)::value) load_k(j + 1);
 #pragma unroll
                 for (int h = 0; h < H; ++h) s[h] *= c;
                 if (cut) {  // uniform
 #pragma unroll
-                    for (int h = 0; h < H; ++h)
+                    for (int h = 0; h < H; ++h) {
+                        uint32_t n = rows[h];
+                        if (GROUP) n = min(n, uint32_t(max(int32_t(my_rows - (((t0 + (b + j) * kWaves) * H + h) << 4)), 0)));
 #pragma unroll
                         for (int r = 0; r < 4; ++r)
-                            if (uint32_t(4 * g + r) >= rows[h]) s[h][r] = -INFINITY;
+                            if (uint32_t(4 * g + r) >= n) s[h][r] = -INFINITY;
+                    }
                 }
                 float most = -INFINITY;
 #pragma unroll
@@ -375,31 +471,46 @@ __global__ __launch_bounds__(kT, D == 64 ? 4 : D == 128 ? 3 : 2) void attn_paged
 #pragma unroll
                                     for (int z = 0; z < VW; ++z) vt[h * 4 + r][n][z] = 0;
                 }
-                if constexpr (TYPE == ZQ_KV_F32) {
+                const Weights<TYPE, VR> pw(p);
+                if (GROUP && cut && x.least < x.most) {
+                    // a value that is no number must not reach (0 times it) the queries that do not see its row
+                    bool odd = false;
 #pragma unroll
-                    for (int n = 0; n < VC; ++n)
+                    for (int r = 0; r < VR; ++r)
 #pragma unroll
-                        for (int e = 0; e < VE; ++e)
+                        for (int n = 0; n < VC; ++n)
 #pragma unroll
-                            for (int r = 0; r < 4; ++r)
-                                o[n][e] = __builtin_amdgcn_mfma_f32_16x16x4f32(bits_f(vt[r][n][e]), p[r], o[n][e], 0, 0, 0);
-                } else {
-                    Parts<TYPE> pp;
+                            for (int z = 0; z < VW; ++z) odd |= not_finite<TYPE>(vt[r][n][z]);
+                    if (__any(odd)) {
+                        // per element: how many such values a query sees; more than none gives NaN
+                        float sees[VR];
 #pragma unroll
-                    for (int r = 0; r < VR; r += 2) pp.set2(r, p[r], p[r + 1]);
+                        for (int r = 0; r < VR; ++r)
+                            sees[r] = (((t0 + (b + j) * kWaves) * H + r / 4) << 4) + 4 * g + r % 4 < my_rows ? 1.0f : 0.0f;
+                        const Weights<TYPE, VR> ps(sees);
 #pragma unroll
-                    for (int n = 0; n < VC; ++n)
+                        for (int n = 0; n < VC; ++n)
 #pragma unroll
-                        for (int e = 0; e < VE; ++e) {
-                            v4u_t w;
+                            for (int z = 0; z < VW; ++z) {
+                                uint32_t w[VR][1][1];
 #pragma unroll
-                            for (int z = 0; z < 4; ++z)
-                                w[z] = __builtin_amdgcn_perm(vt[2 * z + 1][n][e / 2], vt[2 * z][n][e / 2],
-                                                             e & 1 ? 0x07060302u : 0x05040100u);
+                                for (int r = 0; r < VR; ++r) {
+                                    w[r][0][0] = take_odd<TYPE>(vt[r][n][z]);
+                                }
 #pragma unroll
-                            for (int y = NP - 1; y >= 0; --y) o[n][e] = mma<TYPE>(w, pp.bits(y), o[n][e]);
-                        }
+                                for (int e = 0; e < VE / VW; ++e) {
+                                    const v4f_t y = add_pv<TYPE, VR, 1, 1, 1>(w, ps, 0, e, v4f_t{0.0f, 0.0f, 0.0f, 0.0f});
+                                    v4f_t& to = o[n][z * (VE / VW) + e];
+#pragma unroll
+                                    for (int k = 0; k < 4; ++k) to[k] = y[k] > 0.0f ? NAN : to[k];
+                                }
+                            }
+                    }
                 }
+#pragma unroll
+                for (int n = 0; n < VC; ++n)
+#pragma unroll
+                    for (int e = 0; e < VE; ++e) o[n][e] = add_pv<TYPE, VR, VC, VW>(vt, pw, n, e, o[n][e]);
                 if constexpr (!decltype(last)::value) load_v(j + 1);
             };
             for (uint32_t j = 0; j + 1 < count; ++j) step(j, std::false_type{});
@@ -407,26 +518,33 @@ __global__ __launch_bounds__(kT, D == 64 ? 4 : D == 128 ? 3 : 2) void attn_paged
         }
 
         // ---- the four waves' sums as one ----
+        uint32_t ln = threadIdx.x;
+        asm volatile("" : "+v"(ln));  // the addresses below are made here, not held through the tiles
+        const uint32_t mi = ln & 15, mg = (ln >> 4) & 3;
         l = sum_groups(l);
-        if (g == 0) {
-            sm[wave][i] = m;
-            sl[wave][i] = l;
+        if (mg == 0) {
+            sm[wave][mi] = m;
+            sl[wave][mi] = l;
         }
-        if (uint32_t(i) < R) {
-            float* to = dyn + (size_t(wave) * R + i) * (D + 4);
+        if (mi < R) {
+            float* to = dyn + (size_t(wave) * a.RL + mi) * (D + 4);
 #pragma unroll
             for (int n = 0; n < VC; ++n)
 #pragma unroll
                 for (int r = 0; r < 4; ++r)
 #pragma unroll
                     for (int e = 0; e < VE; e += 4)
-                        *reinterpret_cast<float4*>(to + n * 16 * VE + VE * (4 * g + r) + e) =
+                        *reinterpret_cast<float4*>(to + n * 16 * VE + VE * (4 * mg + r) + e) =
                             make_float4(o[n][e][r], o[n][e + 1][r], o[n][e + 2][r], o[n][e + 3][r]);
         }
         __syncthreads();
         const bool whole = u0 == 0 && u1 == u;
-        const size_t slot = (size_t(blockIdx.x) * 2 + (pos != begin)) * a.G + row0;
-        float* out = whole ? a.out + (size_t(qi) * a.KH * a.G + size_t(kh) * a.G + row0) * D : a.part + slot * D;
+        const size_t at = size_t(blockIdx.x) * 2 + (pos != begin), slot = at * a.RS + row0;
+        if (u0 == 0 && u1 < u && threadIdx.x == 0 && blockIdx.y == 0) {
+            // shares with a part of the pair: up to the last one that starts below its end
+            const uint64_t last = ((pos + u) * sh.used + sh.all - 1) / sh.all - 1;
+            a.cut[blockIdx.x] = {qi, kh, GROUP ? R : a.G, uint32_t(last - blockIdx.x + 1), at};
+        }
         for (uint32_t z = threadIdx.x; z < R * (D / 4); z += kT) {
             const uint32_t r = z / (D / 4), d = z % (D / 4) * 4;
             float M = sm[0][r];
@@ -438,7 +556,7 @@ __global__ __launch_bounds__(kT, D == 64 ? 4 : D == 128 ? 3 : 2) void attn_paged
 #pragma unroll
             for (int w = 0; w < kWaves; ++w) {
                 const float f = exp2_(sm[w][r] - Ms);
-                const float4 t = *reinterpret_cast<const float4*>(dyn + (w * R + r) * (D + 4) + d);
+                const float4 t = *reinterpret_cast<const float4*>(dyn + (w * a.RL + r) * (D + 4) + d);
                 L += sl[w][r] * f;
                 y.x += t.x * f, y.y += t.y * f, y.z += t.z * f, y.w += t.w * f;
             }
@@ -449,7 +567,8 @@ __global__ __launch_bounds__(kT, D == 64 ? 4 : D == 128 ? 3 : 2) void attn_paged
                 a.part_ml[(slot + r) * 2] = M;
                 a.part_ml[(slot + r) * 2 + 1] = L;
             }
-            *reinterpret_cast<float4*>(out + size_t(r) * D + d) = y;
+            float* to = whole ? out_row(a, qi, kh, row0 + r) * D + a.out : a.part + (slot + r) * D;
+            *reinterpret_cast<float4*>(to + d) = y;
         }
         __syncthreads();
         pos += u1 - u0;
@@ -457,44 +576,28 @@ __global__ __launch_bounds__(kT, D == 64 ? 4 : D == 128 ? 3 : 2) void attn_paged
 }
 
 // ---- join ------------------------------------------------------------------------
-// Workgroup (b, r) puts row r of the pair together that the end of share b cuts, if
-// it is the first share's end in that pair.
-template <int TYPE, int D>
-__global__ __launch_bounds__(kT) void attn_paged_join_kernel(AttnPaged a, uint32_t W) {
+// Workgroup (w, r) puts row r of the pair together that the end of share w cuts.
+template <int D>
+__global__ __launch_bounds__(kT) void attn_paged_join_kernel(AttnPaged a) {
     constexpr int E = D / 64;  // elements of a lane
-    __shared__ ShareScan scan;
     __shared__ float acc[kWaves][D];
     __shared__ float wm[kWaves], wl[kWaves];
-    const auto units = [&](uint32_t n) { return units_of<TYPE>(a, n); };
-    uint32_t mine, own;
-    const Shares sh = scan_units(a.see.n, a.KH, W, units, scan, mine, own);
-    const uint32_t b = blockIdx.x + 1;
-    if (b >= sh.used) return;
-    const uint64_t x = share_start(sh, b), x0 = share_start(sh, b - 1);
-    find_query(a.see.n, a.KH, units, scan, x, mine, own);
-    const uint32_t qi = scan.query, u = units(qi);
-    const uint64_t base = uint64_t(scan.before) * a.KH;
-    const uint32_t kh = uint32_t(x - base) / u;
-    const uint64_t first = base + uint64_t(kh) * u;  // the pair's units: first .. first + u
-    if (x == first || x0 > first) return;
-    // partials: of share b - 1, then of shares b, b + 1, ... that start below the pair's end
-    const uint32_t r = blockIdx.y;
+    const uint32_t w = blockIdx.x, r = blockIdx.y;
+    const Cut c = a.cut[w];
+    if (r >= c.rows || c.parts == 0) return;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    auto slot = [&](uint32_t w) { return (size_t(w) * 2 + (w == b - 1 && x0 != first)) * a.G + r; };
-    uint32_t n = uint32_t(((first + u) * sh.used - 1) / sh.all) - (b - 1) + 1;  // shares with a part of it
-    while (share_start(sh, b - 1 + n) < first + u) ++n;
-    while (n > 1 && share_start(sh, b - 1 + n - 1) >= first + u) --n;
+    auto slot = [&](uint32_t j) { return (j ? size_t(w + j) * 2 : size_t(c.slot)) * a.RS + r; };
     float M = -INFINITY;
-    for (uint32_t j = threadIdx.x; j < n; j += kT) M = fmaxf(M, a.part_ml[slot(b - 1 + j) * 2]);
+    for (uint32_t j = threadIdx.x; j < c.parts; j += kT) M = fmaxf(M, a.part_ml[slot(j) * 2]);
     M = wave_max(M);
     if (lane == 0) wm[wave] = M;
     __syncthreads();
     M = fmaxf(fmaxf(wm[0], wm[1]), fmaxf(wm[2], wm[3]));
     const float Ms = M == -INFINITY ? 0.0f : M;
     float L = 0.0f, y[E] = {};
-#pragma unroll 4
-    for (uint32_t j = wave; j < n; j += kWaves) {
-        const size_t at = slot(b - 1 + j);
+#pragma unroll 8
+    for (uint32_t j = wave; j < c.parts; j += kWaves) {
+        const size_t at = slot(j);
         const float f = exp2_(a.part_ml[at * 2] - Ms);
         L += a.part_ml[at * 2 + 1] * f;
 #pragma unroll
@@ -506,8 +609,8 @@ __global__ __launch_bounds__(kT) void attn_paged_join_kernel(AttnPaged a, uint32
     __syncthreads();
     L = (wl[0] + wl[1]) + (wl[2] + wl[3]);
     const float inv = L > 0.0f ? 1.0f / L : (L == 0.0f ? 0.0f : L);
-    for (uint32_t d = threadIdx.x; d < D; d += kT)
-        a.out[(size_t(qi) * a.KH * a.G + size_t(kh) * a.G + r) * D + d] = ((acc[0][d] + acc[1][d]) + (acc[2][d] + acc[3][d])) * inv;
+    float* out = a.out + out_row(a, c.query, c.kh, r) * D;
+    for (uint32_t d = threadIdx.x; d < D; d += kT) out[d] = ((acc[0][d] + acc[1][d]) + (acc[2][d] + acc[3][d])) * inv;
 }
 
 // Workgroups for a call: three a CU are resident (two with D = 256), and as many as
@@ -519,31 +622,38 @@ uint32_t shares_of(const zq_kv_paged& c, const zq_page_tables& t, size_t queries
     return uint32_t(most < want ? most : want);
 }
 
-template <int TYPE, int D>
+// Queries of a group at most, and rows of a partial, for G heads of a kv head.
+uint32_t group_most(size_t G) { return G <= 8 ? uint32_t(16 / G) : 1; }
+size_t part_rows(size_t G) { return G * group_most(G); }
+
+template <int TYPE, int D, bool GROUP>
 hipError_t run_attention(const AttnPaged& a, uint32_t W, hipStream_t stream) {
     using S = Shape<TYPE, D>;
-    const uint32_t R = a.G < 16 ? a.G : 16;
-    const size_t lds = size_t(kWaves) * R * (D + 4) * 4 + (S::kQInLds ? size_t(S::KC) * S::NP * 64 * 16 : 0);
+    const size_t lds = size_t(kWaves) * a.RL * (D + 4) * 4 + size_t(S::KC) * S::NP * 64 * 16;
     if (lds > 64 * 1024) {
-        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&attn_paged_kernel<TYPE, D>),
+        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&attn_paged_kernel<TYPE, D, GROUP>),
                                                  hipFuncAttributeMaxDynamicSharedMemorySize, int(lds));
         if (e != hipSuccess) return e;
     }
-    hipLaunchKernelGGL((attn_paged_kernel<TYPE, D>), dim3(W, (a.G + 15) / 16), dim3(kT), lds, stream, a);
+    hipLaunchKernelGGL((attn_paged_kernel<TYPE, D, GROUP>), dim3(W, GROUP ? 1 : (a.G + 15) / 16), dim3(kT), lds, stream, a);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || W == 1) return e;
-    hipLaunchKernelGGL((attn_paged_join_kernel<TYPE, D>), dim3(W - 1, a.G), dim3(kT), 0, stream, a, W);
+    hipLaunchKernelGGL(attn_paged_join_kernel<D>, dim3(W - 1, a.RS), dim3(kT), 0, stream, a);
     return hipGetLastError();
 }
-template <int TYPE>
+template <int TYPE, bool GROUP>
 hipError_t run_attention(const AttnPaged& a, uint32_t W, size_t D, hipStream_t stream) {
-    return D == 64 ? run_attention<TYPE, 64>(a, W, stream)
-                   : D == 128 ? run_attention<TYPE, 128>(a, W, stream) : run_attention<TYPE, 256>(a, W, stream);
+    return D == 64 ? run_attention<TYPE, 64, GROUP>(a, W, stream)
+                   : D == 128 ? run_attention<TYPE, 128, GROUP>(a, W, stream) : run_attention<TYPE, 256, GROUP>(a, W, stream);
+}
+template <int TYPE>
+hipError_t run_attention(const AttnPaged& a, uint32_t W, size_t D, bool group, hipStream_t stream) {
+    return group ? run_attention<TYPE, true>(a, W, D, stream) : run_attention<TYPE, false>(a, W, D, stream);
 }
 
 size_t workspace(const zq_kv_paged& c, const zq_page_tables& t, size_t queries, size_t heads) {
-    const size_t rows = size_t(shares_of(c, t, queries)) * 2 * (heads / c.kv_heads);
-    return (rows * (c.head_dim + 2) * 4 + 255) / 256 * 256;
+    const size_t W = shares_of(c, t, queries), rows = W * 2 * part_rows(heads / c.kv_heads);
+    return (W * sizeof(Cut) + rows * (c.head_dim + 2) * 4 + 255) / 256 * 256;
 }
 
 }  // namespace
@@ -583,8 +693,13 @@ int zq_hip_attention_paged_dev(const zq_kv_paged* cache, const zq_page_tables* t
     a.select = select;
     a.q = q;
     a.out = out;
+    const bool group = seq_of && !select && zq::group_most(G) > 1;
+    a.P = group ? zq::group_most(G) : 1;
+    a.RS = a.P * G;
+    a.RL = a.RS < 16 ? a.RS : 16;
     a.part = static_cast<float*>(workspace);
-    a.part_ml = a.part + size_t(W) * 2 * G * cache->head_dim;
+    a.cut = reinterpret_cast<zq::Cut*>(a.part + size_t(W) * 2 * a.RS * cache->head_dim);
+    a.part_ml = reinterpret_cast<float*>(a.cut + W);
     a.see = {seq_of, lens, counts, uint32_t(queries), uint32_t(tables->seqs), uint32_t(tables->width * tables->page_size),
              flags & ZQ_ATTN_PAGED_FULL};
     a.stride = stride;
@@ -596,9 +711,9 @@ int zq_hip_attention_paged_dev(const zq_kv_paged* cache, const zq_page_tables* t
     a.keep = uint32_t(keep);
     a.lp = zq::log2_of(tables->page_size);
     const hipStream_t st = static_cast<hipStream_t>(stream);
-    return zq::status(cache->type == ZQ_KV_F32   ? zq::run_attention<ZQ_KV_F32>(a, W, cache->head_dim, st)
-                      : cache->type == ZQ_KV_F16 ? zq::run_attention<ZQ_KV_F16>(a, W, cache->head_dim, st)
-                                                 : zq::run_attention<ZQ_KV_BF16>(a, W, cache->head_dim, st));
+    return zq::status(cache->type == ZQ_KV_F32   ? zq::run_attention<ZQ_KV_F32>(a, W, cache->head_dim, group, st)
+                      : cache->type == ZQ_KV_F16 ? zq::run_attention<ZQ_KV_F16>(a, W, cache->head_dim, group, st)
+                                                 : zq::run_attention<ZQ_KV_BF16>(a, W, cache->head_dim, group, st));
 }
 
 }  // extern "C"

@@ -58,8 +58,8 @@ __global__ __launch_bounds__(kShareT) void page_score_kernel(SelectArgs a) {
     if (blockIdx.x >= sh.used) return;
     uint64_t pos = share_start(sh, blockIdx.x);
     const uint64_t end = share_start(sh, blockIdx.x + 1);
-    find_query(a.see.n, a.KH, units, scan, pos, mine, own);
-    uint32_t qi = scan.query, before = scan.before;
+    const Found at = find_query(a.see.n, a.KH, units, scan, pos, mine, own);
+    uint32_t qi = at.query, before = at.before;
     const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     while (pos < end) {

@@ -13,14 +13,14 @@ namespace {
 // A step in numbers: sequence s fits with c_s new tokens, lacks need_s pages; P, C the
 // sums of need and c up to and with s.  It is served where P and C are within the free
 // pages and the rows; both only grow, so those served come first, and their sums are
-// the last served one's.  A workgroup takes all the sums by itself (8 sequences a
-// thread at most) into LDS; then every packed row finds its sequence by bisection and
-// its page without any other row: the page of a new one is as far below the top of the
-// stack as P says.  With few rows one workgroup does it all; with many, each of a grid
-// repeats the sums, and a second launch writes what the first one still reads (the
-// counts may be the granted ones' array, the free pages' number its own successor).
-constexpr int kTabT = 1024, kTabWaves = kTabT / 64;
+// the last served one's.  A workgroup takes all the sums by itself (N sequences a
+// thread) into LDS; then every packed row finds its sequence by bisection and its page
+// without any other row: the page of a new one is as far below the top of the stack as
+// P says.  Every workgroup of a grid repeats the sums, so that one launch will do; where
+// an output is an input too (the granted ones' array the counts', the number of free
+// pages its own successor) and one workgroup is too few, a second launch writes them.
 constexpr uint32_t kExpand = 1, kCommit = 2;
+constexpr size_t kOneTable = 4096;  // rows up to which one workgroup does it all then
 
 struct StepArgs {
     int32_t* table;
@@ -37,11 +37,12 @@ struct StepArgs {
     uint32_t seqs, width, pages, lp, tokens;
 };
 
-// Sums before a thread's own value over the workgroup (v: two values), and their totals.
+// Sums before a thread's own values over a workgroup of W waves, and their totals.
 struct Sums2 {
     uint32_t a, b;
 };
-__device__ __forceinline__ Sums2 block_before2(Sums2 v, uint32_t (&part)[2][kTabWaves], Sums2& all) {
+template <int W>
+__device__ __forceinline__ Sums2 block_before2(Sums2 v, uint32_t (&part)[2][W], Sums2& all) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     uint32_t wa, wb;
     Sums2 x{wave_before_sat(v.a, wa), wave_before_sat(v.b, wb)};
@@ -51,7 +52,8 @@ __device__ __forceinline__ Sums2 block_before2(Sums2 v, uint32_t (&part)[2][kTab
     }
     __syncthreads();
     all = {0, 0};
-    for (int w = 0; w < kTabWaves; ++w) {
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
         if (w == wave) {
             x.a = add_sat31(x.a, all.a);
             x.b = add_sat31(x.b, all.b);
@@ -59,79 +61,107 @@ __device__ __forceinline__ Sums2 block_before2(Sums2 v, uint32_t (&part)[2][kTab
         all.a = add_sat31(all.a, part[0][w]);
         all.b = add_sat31(all.b, part[1][w]);
     }
-    __syncthreads();
     return x;
 }
 __device__ __forceinline__ uint32_t pages_of(uint32_t tokens, uint32_t lp) { return (tokens + (1u << lp) - 1) >> lp; }
 
-__global__ __launch_bounds__(kTabT) void page_step_kernel(StepArgs a, uint32_t role) {
-    __shared__ uint32_t end[kPgMaxSeqs];   // granted tokens up to and with a sequence
-    __shared__ uint32_t taken[kPgMaxSeqs]; // pages taken before it
-    __shared__ uint32_t part[2][kTabWaves];
-    __shared__ uint32_t total[2];
-    const uint32_t tid = threadIdx.x, each = (a.seqs + kTabT - 1) / kTabT, s0 = tid * each, s1 = min(s0 + each, a.seqs);
-    const uint32_t cap = a.width << a.lp, fc = uint32_t(min(max(a.free_count[0], 0), int32_t(a.pages)));
+template <int T, int N>
+__global__ __launch_bounds__(T) void page_step_kernel(StepArgs a, uint32_t role) {
+    __shared__ uint32_t end[T * N];    // granted tokens up to and with a sequence
+    __shared__ uint32_t taken[T * N];  // pages taken before it
+    __shared__ uint32_t part[2][T / 64];
+    __shared__ uint32_t total[3];
+    const uint32_t tid = threadIdx.x, cap = a.width << a.lp;
+    const uint32_t fc = uint32_t(min(max(a.free_count[0], 0), int32_t(a.pages)));
     auto len_of = [&](uint32_t s) { return uint32_t(min(max(a.lens[s], 0), int32_t(cap))); };
-    struct Want {
-        uint32_t tokens, pages;
-        bool fits;
-    };
-    auto want = [&](uint32_t s) {
-        const uint32_t n = len_of(s), c = uint32_t(max(a.counts[s], 0));
-        if (c > cap - n) return Want{0, 0, false};
-        return Want{c, pages_of(n + c, a.lp) - pages_of(n, a.lp), true};
-    };
-    Sums2 own{0, 0}, all;
-    for (uint32_t s = s0; s < s1; ++s) {
-        const Want w = want(s);
-        own.a = add_sat31(own.a, w.tokens);
-        own.b = add_sat31(own.b, w.pages);
+    uint32_t n[N], c[N], need[N];
+    bool fits[N];
+    if (tid < 3) total[tid] = 0;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+        const uint32_t s = tid * N + j, at = min(s, a.seqs - 1);
+        n[j] = len_of(at);
+        c[j] = s < a.seqs ? uint32_t(max(a.counts[at], 0)) : 0u;
     }
-    if (tid < 2) total[tid] = 0;
-    Sums2 at = block_before2(own, part, all);
+    Sums2 own{0, 0}, all;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+        fits[j] = c[j] <= cap - n[j];
+        if (!fits[j]) c[j] = 0;
+        need[j] = pages_of(n[j] + c[j], a.lp) - pages_of(n[j], a.lp);
+        own.a = add_sat31(own.a, c[j]);
+        own.b = add_sat31(own.b, need[j]);
+    }
+    // (the page that the first new token of this thread's sequence continues, if it does: asked for before the sums)
+    const uint32_t row_n = n[0] & ((1u << a.lp) - 1);
+    int32_t last_page = -1;
+    if (N == 1 && tid < a.seqs && c[0] && row_n) last_page = a.table[size_t(tid) * a.width + (n[0] >> a.lp)];
+    Sums2 at = block_before2<T / 64>(own, part, all);
     uint32_t tok = 0, pg = 0;  // the sums of the last one served
-    for (uint32_t s = s0; s < s1; ++s) {
-        const Want w = want(s);
-        taken[s] = at.b;
-        at.a = add_sat31(at.a, w.tokens);
-        at.b = add_sat31(at.b, w.pages);
-        end[s] = at.a;
-        if (w.fits && at.a <= a.tokens && at.b <= fc) tok = at.a, pg = at.b;
+    const Sums2 first = at;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+        taken[tid * N + j] = at.b;
+        at.a = add_sat31(at.a, c[j]);
+        at.b = add_sat31(at.b, need[j]);
+        end[tid * N + j] = at.a;
+        if (fits[j] && at.a <= a.tokens && at.b <= fc) tok = at.a, pg = at.b;
     }
     if (tok) atomicMax(&total[0], tok);
     if (pg) atomicMax(&total[1], pg);
+    if (N == 1 && c[0] > 1) total[2] = 1;
     __syncthreads();
     const uint32_t served = total[0], taken_all = total[1];
     if (role & kExpand) {
-        for (uint32_t r = blockIdx.x * kTabT + tid; r < a.tokens; r += gridDim.x * kTabT) {
-            int64_t slot = -1;
-            int32_t pos = -1, seq = -1;
-            if (r < served) {
-                uint32_t lo = 0, hi = a.seqs - 1;  // the first sequence whose end is past r
-                while (lo < hi) {
-                    const uint32_t mid = (lo + hi) >> 1;
-                    if (end[mid] > r) hi = mid;
-                    else lo = mid + 1;
-                }
-                const uint32_t n = len_of(lo), p = n + r - (lo ? end[lo - 1] : 0u), j = p >> a.lp, old = pages_of(n, a.lp);
-                const uint32_t page = uint32_t(j < old ? a.table[size_t(lo) * a.width + j]
-                                                       : a.free_pages[fc - 1 - (taken[lo] + j - old)]);
-                const uint32_t row = p & ((1u << a.lp) - 1);
-                if (row == 0) a.table[size_t(lo) * a.width + j] = int32_t(page);  // a new page's first token is a new one
-                if (page < a.pages) slot = (int64_t(page) << a.lp) + row;
-                pos = int32_t(p);
-                seq = int32_t(lo);
-            }
+        auto put = [&](uint32_t r, int64_t slot, int32_t pos, int32_t seq) {
             a.slots[r] = slot;
             if (a.positions) a.positions[r] = pos;
             if (a.seq_of) a.seq_of[r] = seq;
+        };
+        if (N == 1 && !total[2]) {  // a decode step: a thread's sequence has one row at most
+            if (blockIdx.x == 0 && c[0] && at.a <= served) {
+                uint32_t page = uint32_t(last_page);
+                if (!row_n) {
+                    page = uint32_t(a.free_pages[fc - 1 - first.b]);
+                    a.table[size_t(tid) * a.width + (n[0] >> a.lp)] = int32_t(page);
+                }
+                put(first.a, page < a.pages ? (int64_t(page) << a.lp) + row_n : -1, int32_t(n[0]), int32_t(tid));
+            }
+            for (uint32_t r = served + blockIdx.x * T + tid; r < a.tokens; r += gridDim.x * T) put(r, -1, -1, -1);
+        } else {
+            for (uint32_t r = blockIdx.x * T + tid; r < a.tokens; r += gridDim.x * T) {
+                int64_t slot = -1;
+                int32_t pos = -1, seq = -1;
+                if (r < served) {
+                    uint32_t lo = 0, hi = a.seqs - 1;  // the first sequence whose end is past r
+                    while (lo < hi) {
+                        const uint32_t mid = (lo + hi) >> 1;
+                        if (end[mid] > r) hi = mid;
+                        else lo = mid + 1;
+                    }
+                    const uint32_t len = len_of(lo), p = len + r - (lo ? end[lo - 1] : 0u), j = p >> a.lp;
+                    const uint32_t old = pages_of(len, a.lp), row = p & ((1u << a.lp) - 1);
+                    const uint32_t page = uint32_t(j < old ? a.table[size_t(lo) * a.width + j]
+                                                           : a.free_pages[fc - 1 - (taken[lo] + j - old)]);
+                    if (row == 0) a.table[size_t(lo) * a.width + j] = int32_t(page);  // a new page's first token is a new one
+                    if (page < a.pages) slot = (int64_t(page) << a.lp) + row;
+                    pos = int32_t(p);
+                    seq = int32_t(lo);
+                }
+                put(r, slot, pos, seq);
+            }
         }
     }
-    if (role & kCommit) {
-        for (uint32_t s = tid; s < a.seqs; s += kTabT) {
-            const uint32_t e = min(end[s], served), b = s ? min(end[s - 1], served) : 0u;
-            a.start[s] = int32_t(b);
-            a.granted[s] = int32_t(e - b);
+    if ((role & kCommit) && blockIdx.x == 0) {
+        uint32_t b = min(first.a, served);
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const uint32_t s = tid * N + j, e = min(end[s], served);
+            if (s < a.seqs) {
+                a.start[s] = int32_t(b);
+                a.granted[s] = int32_t(e - b);
+            }
+            b = e;
         }
         if (tid == 0) {
             a.start[a.seqs] = int32_t(served);
@@ -151,48 +181,75 @@ struct ReleaseArgs {
     int32_t* free_left;
     uint32_t seqs, width, pages, lp;
 };
-__global__ __launch_bounds__(kTabT) void page_release_kernel(ReleaseArgs a, uint32_t role) {
-    __shared__ uint32_t end[kPgMaxSeqs];
-    __shared__ uint32_t part[2][kTabWaves];
-    const uint32_t tid = threadIdx.x, each = (a.seqs + kTabT - 1) / kTabT, s0 = tid * each, s1 = min(s0 + each, a.seqs);
-    const uint32_t cap = a.width << a.lp, fc = uint32_t(min(max(a.free_count[0], 0), int32_t(a.pages)));
-    struct Span {
-        uint32_t from, to;
-    };
-    auto span = [&](uint32_t s) {
-        const uint32_t n = uint32_t(min(max(a.lens[s], 0), int32_t(cap)));
-        const uint32_t k = min(uint32_t(max(a.keep[s], 0)), n);
-        return Span{pages_of(k, a.lp), pages_of(n, a.lp)};
-    };
+template <int T, int N>
+__global__ __launch_bounds__(T) void page_release_kernel(ReleaseArgs a, uint32_t role) {
+    __shared__ uint32_t end[T * N];
+    __shared__ uint32_t from[T * N];  // the first page of a sequence that goes back
+    __shared__ uint32_t part[2][T / 64];
+    const uint32_t tid = threadIdx.x, cap = a.width << a.lp;
+    const uint32_t fc = uint32_t(min(max(a.free_count[0], 0), int32_t(a.pages)));
+    uint32_t back[N];
     Sums2 own{0, 0}, all;
-    for (uint32_t s = s0; s < s1; ++s) {
-        const Span x = span(s);
-        own.a = add_sat31(own.a, x.to - x.from);
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+        const uint32_t s = min(tid * N + j, a.seqs - 1), n = uint32_t(min(max(a.lens[s], 0), int32_t(cap)));
+        const uint32_t k = pages_of(min(uint32_t(max(a.keep[s], 0)), n), a.lp);
+        from[tid * N + j] = k;
+        back[j] = tid * N + j < a.seqs ? pages_of(n, a.lp) - k : 0u;
+        own.a = add_sat31(own.a, back[j]);
     }
-    Sums2 at = block_before2(own, part, all);
-    for (uint32_t s = s0; s < s1; ++s) {
-        const Span x = span(s);
-        end[s] = at.a = add_sat31(at.a, x.to - x.from);
-    }
+    Sums2 at = block_before2<T / 64>(own, part, all);
+#pragma unroll
+    for (int j = 0; j < N; ++j) end[tid * N + j] = at.a = add_sat31(at.a, back[j]);
     __syncthreads();
     const uint32_t n = all.a;
     if (role & kExpand) {
-        for (uint32_t x = blockIdx.x * kTabT + tid; x < n; x += gridDim.x * kTabT) {
+        for (uint32_t x = blockIdx.x * T + tid; x < n; x += gridDim.x * T) {
             uint32_t lo = 0, hi = a.seqs - 1;
             while (lo < hi) {
                 const uint32_t mid = (lo + hi) >> 1;
                 if (end[mid] > x) hi = mid;
                 else lo = mid + 1;
             }
-            const uint32_t j = span(lo).from + x - (lo ? end[lo - 1] : 0u), to = fc + (n - 1 - x);
+            const uint32_t j = from[lo] + x - (lo ? end[lo - 1] : 0u), to = fc + (n - 1 - x);
             if (to < a.pages) a.free_pages[to] = a.table[size_t(lo) * a.width + j];
         }
     }
-    if ((role & kCommit) && tid == 0) a.free_left[0] = int32_t(min(fc + n, a.pages));
+    if ((role & kCommit) && blockIdx.x == 0 && tid == 0) a.free_left[0] = int32_t(min(fc + n, a.pages));
 }
 
-// Rows up to which one workgroup does it all.
-constexpr size_t kOneTable = 4096;
+// Workgroups of T threads for `rows` rows; where what one writes is what others read, one workgroup or two launches.
+template <class F>
+void expand_and_commit(size_t rows, int T, bool overlap, F launch) {
+    const size_t blocks = (rows + T - 1) / T, most = 1024;
+    const uint32_t g = uint32_t(blocks < most ? blocks : most);
+    if (!overlap) return launch(g, kExpand | kCommit);
+    if (rows <= kOneTable) return launch(1u, kExpand | kCommit);
+    launch(g, kExpand);
+    launch(1u, kCommit);
+}
+void run_step(const StepArgs& a, hipStream_t stream) {
+    const bool overlap = a.granted == a.counts || a.free_left == a.free_count;
+    auto run = [&](auto kernel, int T) {
+        expand_and_commit(a.tokens, T, overlap, [&](uint32_t g, uint32_t role) {
+            hipLaunchKernelGGL(kernel, dim3(g), dim3(T), 0, stream, a, role);
+        });
+    };
+    if (a.seqs <= 256) run(page_step_kernel<256, 1>, 256);
+    else if (a.seqs <= 1024) run(page_step_kernel<256, 4>, 256);
+    else run(page_step_kernel<1024, 8>, 1024);
+}
+void run_release(const ReleaseArgs& a, hipStream_t stream) {
+    const size_t all = size_t(a.seqs) * a.width;
+    auto run = [&](auto kernel, int T) {
+        expand_and_commit(all < a.pages ? all : a.pages, T, a.free_left == a.free_count, [&](uint32_t g, uint32_t role) {
+            hipLaunchKernelGGL(kernel, dim3(g), dim3(T), 0, stream, a, role);
+        });
+    };
+    if (a.seqs <= 256) run(page_release_kernel<256, 1>, 256);
+    else if (a.seqs <= 1024) run(page_release_kernel<256, 4>, 256);
+    else run(page_release_kernel<1024, 8>, 1024);
+}
 
 // ---- append ----------------------------------------------------------------------
 template <int TYPE>
@@ -248,72 +305,122 @@ __global__ __launch_bounds__(256) void paged_append_kernel(AppendArgs a) {
     *reinterpret_cast<vec*>(a.v + to * sizeof(T)) = v;
 }
 
-// Bounds of the pages that got rows: a wave for every (token, kv head), which goes on
-// where the token is the last of its page in this call.
+// The same with the bounds of the pages that get rows.  The rows of one page in a call
+// are neighbours: a wave takes such a run for one kv head, writes its rows, reads the
+// page's rows before them, and has the bounds without reading the new ones back.  A
+// workgroup looks for the runs that end in its B tokens and shares them out over its
+// waves: B is 4 where there are few tokens (a decode step: a wave a token) and 64 where
+// there are many.
 template <int TYPE, int D>
-__global__ __launch_bounds__(256) void paged_bounds_kernel(AppendArgs a) {
+__global__ __launch_bounds__(256) void paged_append_bounds_kernel(AppendArgs a, uint32_t tokens, uint32_t B) {
     typedef typename Held<TYPE>::type T;
     constexpr int E = 16 / sizeof(T), L = D / E, R = 64 / L;  // elements a lane, lanes a row, rows at once
-    const uint32_t row = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + threadIdx.x / 64);
-    const int lane = threadIdx.x & 63, l = lane % L;
-    if (row >= a.rows) return;
-    const uint32_t t = row / a.KH, h = row % a.KH;
-    const int64_t slot = a.slots[t], ps = int64_t(1) << a.lp;
-    if (slot < 0 || slot >= a.all_slots) return;
-    const int last = int(slot & (ps - 1));
-    if ((row / a.KH + 1) * a.KH < a.rows && last + 1 < ps && a.slots[t + 1] == slot + 1) return;
-    const size_t head = size_t(slot >> a.lp) * a.KH + h;
-    const T* p = reinterpret_cast<const T*>(a.k) + (head << a.lp) * D + l * E;
-    float lo[E], hi[E];
-#pragma unroll
-    for (int i = 0; i < E; ++i) lo[i] = INFINITY, hi[i] = -INFINITY;
     typedef T vec __attribute__((ext_vector_type(E)));
-    for (int r = lane / L; r <= last; r += R) {
-        const vec x = *reinterpret_cast<const vec*>(p + size_t(r) * D);
+    const int lane = threadIdx.x & 63, l = lane % L, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t h = blockIdx.y, t0 = blockIdx.x * B;
+    const int64_t ps = int64_t(1) << a.lp;
+    bool ends = false;
+    int64_t mine = -1;
+    if (uint32_t(lane) < B && t0 + lane < tokens) {
+        mine = a.slots[t0 + lane];
+        const int64_t next = t0 + lane + 1 < tokens ? a.slots[t0 + lane + 1] : -1;
+        ends = mine >= 0 && mine < a.all_slots && !(next == mine + 1 && (next & (ps - 1)) != 0);
+    }
+    uint64_t runs = __ballot(ends);
+    for (int z = 0; runs; ++z) {
+        const int at = __builtin_ctzll(runs);
+        runs &= runs - 1;
+        if (z % 4 != wave) continue;
+        const uint32_t t = t0 + uint32_t(at);  // the run's last token
+        const uint64_t slot = uint64_t(uint32_t(__builtin_amdgcn_readlane(int(mine), at))) |
+                              uint64_t(uint32_t(__builtin_amdgcn_readlane(int(mine >> 32), at))) << 32;
+        const int last = int(slot & uint64_t(ps - 1));
+        int n = 0;  // rows of the run
+        for (bool more = true; more; n += 64) {  // ends: at token 0, at the page's first row, or before
+            const int64_t back = int64_t(n) + lane;
+            const bool same = back <= last && back <= int64_t(t) && a.slots[int64_t(t) - back] == int64_t(slot) - back;
+            const uint64_t m = ~__ballot(same);
+            if (m) {
+                n += __builtin_ctzll(m) - 64;
+                more = false;
+            }
+        }
+        const size_t head = size_t(slot >> a.lp) * a.KH + h;
+        const size_t base = (head << a.lp) * D + l * E;
+        T* pk = reinterpret_cast<T*>(a.k) + base;
+        T* pv = reinterpret_cast<T*>(a.v) + base;
+        float lo[E], hi[E];
+#pragma unroll
+        for (int i = 0; i < E; ++i) lo[i] = INFINITY, hi[i] = -INFINITY;
+        auto take = [&](const vec& x) {
+#pragma unroll
+            for (int i = 0; i < E; ++i) {
+                lo[i] = fminf(lo[i], float(x[i]));
+                hi[i] = fmaxf(hi[i], float(x[i]));
+            }
+        };
+        const int first = last + 1 - n;
+#pragma unroll 2
+        for (int r = lane / L; r < first; r += R) take(*reinterpret_cast<const vec*>(pk + size_t(r) * D));
+        const size_t src = size_t(t - uint32_t(n - 1)) * a.stride + h * D + l * E;
+#pragma unroll 2
+        for (int r = lane / L; r < n; r += R) {
+            vec k, v;
+#pragma unroll
+            for (int i = 0; i < E; i += 4) {
+                const float4 x = *reinterpret_cast<const float4*>(a.src_k + src + r * a.stride + i);
+                const float4 y = *reinterpret_cast<const float4*>(a.src_v + src + r * a.stride + i);
+                k[i] = T(x.x), k[i + 1] = T(x.y), k[i + 2] = T(x.z), k[i + 3] = T(x.w);
+                v[i] = T(y.x), v[i + 1] = T(y.y), v[i + 2] = T(y.z), v[i + 3] = T(y.w);
+            }
+            *reinterpret_cast<vec*>(pk + size_t(first + r) * D) = k;
+            *reinterpret_cast<vec*>(pv + size_t(first + r) * D) = v;
+            take(k);
+        }
+        float most = 0.0f;
 #pragma unroll
         for (int i = 0; i < E; ++i) {
-            lo[i] = fminf(lo[i], float(x[i]));
-            hi[i] = fmaxf(hi[i], float(x[i]));
+#pragma unroll
+            for (int m = L; m < 64; m *= 2) {
+                lo[i] = fminf(lo[i], __shfl_xor(lo[i], m));
+                hi[i] = fmaxf(hi[i], __shfl_xor(hi[i], m));
+            }
+            if (lo[i] > hi[i]) lo[i] = hi[i] = 0.0f;  // NaN only
+            most = fmaxf(most, fmaxf(fabsf(lo[i]), fabsf(hi[i])));
         }
-    }
-    float most = 0.0f;
 #pragma unroll
-    for (int i = 0; i < E; ++i) {
+        for (int m = 1; m < L; m *= 2) most = fmaxf(most, __shfl_xor(most, m));
+        const int e = bound_exp(most);
+        uint32_t w[2][E / 4] = {};
 #pragma unroll
-        for (int m = L; m < 64; m *= 2) {
-            lo[i] = fminf(lo[i], __shfl_xor(lo[i], m));
-            hi[i] = fmaxf(hi[i], __shfl_xor(hi[i], m));
+        for (int i = 0; i < E; ++i) {
+            const int c0 = bound_code(floorf(ldexpf(lo[i], -e))), c1 = bound_code(ceilf(ldexpf(hi[i], -e)));
+            w[0][i / 4] |= uint32_t(c0 & 255) << (8 * (i % 4));
+            w[1][i / 4] |= uint32_t(c1 & 255) << (8 * (i % 4));
         }
-        if (lo[i] > hi[i]) lo[i] = hi[i] = 0.0f;  // NaN only
-        most = fmaxf(most, fmaxf(fabsf(lo[i]), fabsf(hi[i])));
-    }
+        if (lane < L) {
+            int8_t* b = a.bounds + head * 2 * D + l * E;
 #pragma unroll
-    for (int m = 1; m < L; m *= 2) most = fmaxf(most, __shfl_xor(most, m));
-    const int e = bound_exp(most);
-    uint32_t w[2][(E + 3) / 4] = {};
-#pragma unroll
-    for (int i = 0; i < E; ++i) {
-        const int c0 = bound_code(floorf(ldexpf(lo[i], -e))), c1 = bound_code(ceilf(ldexpf(hi[i], -e)));
-        w[0][i / 4] |= uint32_t(c0 & 255) << (8 * (i % 4));
-        w[1][i / 4] |= uint32_t(c1 & 255) << (8 * (i % 4));
-    }
-    if (lane < L) {
-        int8_t* b = a.bounds + head * 2 * D + l * E;
-#pragma unroll
-        for (int i = 0; i < E / 4; ++i) {
-            reinterpret_cast<uint32_t*>(b)[i] = w[0][i];
-            reinterpret_cast<uint32_t*>(b + D)[i] = w[1][i];
+            for (int i = 0; i < E / 4; ++i) {
+                reinterpret_cast<uint32_t*>(b)[i] = w[0][i];
+                reinterpret_cast<uint32_t*>(b + D)[i] = w[1][i];
+            }
+            if (lane == 0) a.bounds_exp[head] = int8_t(e);
         }
-        if (lane == 0) a.bounds_exp[head] = int8_t(e);
     }
 }
+constexpr uint32_t kManyTokens = 1024;
 
 template <int TYPE, int D>
 void run_append(const AppendArgs& a, hipStream_t stream) {
+    if (a.bounds) {
+        const uint32_t tokens = a.rows / a.KH, B = tokens < kManyTokens ? 4 : 64;
+        hipLaunchKernelGGL((paged_append_bounds_kernel<TYPE, D>), dim3((tokens + B - 1) / B, a.KH), dim3(256), 0, stream, a,
+                           tokens, B);
+        return;
+    }
     constexpr uint32_t per = 256 / (D * sizeof(typename Held<TYPE>::type) / 16);
     hipLaunchKernelGGL((paged_append_kernel<TYPE, D>), dim3((a.rows + per - 1) / per), dim3(256), 0, stream, a);
-    if (a.bounds)
-        hipLaunchKernelGGL((paged_bounds_kernel<TYPE, D>), dim3((a.rows + 3) / 4), dim3(256), 0, stream, a);
 }
 template <int TYPE>
 void run_append(const AppendArgs& a, size_t D, hipStream_t stream) {
@@ -365,15 +472,7 @@ int zq_hip_page_tables_step_dev(const zq_page_tables* tables, const int32_t* len
     const zq::StepArgs a{tables->table, tables->free_pages, lens, counts, free_count, free_left, granted, start, slots,
                          positions, seq_of, uint32_t(tables->seqs), uint32_t(tables->width), uint32_t(tables->pages),
                          zq::log2_of(tables->page_size), uint32_t(tokens)};
-    const hipStream_t st = static_cast<hipStream_t>(stream);
-    if (tokens <= zq::kOneTable) {
-        hipLaunchKernelGGL(zq::page_step_kernel, dim3(1), dim3(zq::kTabT), 0, st, a, zq::kExpand | zq::kCommit);
-    } else {
-        const size_t blocks = (tokens + zq::kTabT - 1) / zq::kTabT;
-        hipLaunchKernelGGL(zq::page_step_kernel, dim3(uint32_t(blocks < 512 ? blocks : 512)), dim3(zq::kTabT), 0, st, a,
-                           zq::kExpand);
-        hipLaunchKernelGGL(zq::page_step_kernel, dim3(1), dim3(zq::kTabT), 0, st, a, zq::kCommit);
-    }
+    zq::run_step(a, static_cast<hipStream_t>(stream));
     return zq::status(hipGetLastError());
 }
 
@@ -386,16 +485,7 @@ int zq_hip_page_tables_release_dev(const zq_page_tables* tables, const int32_t* 
     if (dev.status() != ZQ_OK) return dev.status();
     const zq::ReleaseArgs a{tables->table, tables->free_pages, lens, keep, free_count, free_left, uint32_t(tables->seqs),
                             uint32_t(tables->width), uint32_t(tables->pages), zq::log2_of(tables->page_size)};
-    const hipStream_t st = static_cast<hipStream_t>(stream);
-    const size_t most = tables->seqs * tables->width < tables->pages ? tables->seqs * tables->width : tables->pages;
-    if (most <= zq::kOneTable) {
-        hipLaunchKernelGGL(zq::page_release_kernel, dim3(1), dim3(zq::kTabT), 0, st, a, zq::kExpand | zq::kCommit);
-    } else {
-        const size_t blocks = (most + zq::kTabT - 1) / zq::kTabT;
-        hipLaunchKernelGGL(zq::page_release_kernel, dim3(uint32_t(blocks < 256 ? blocks : 256)), dim3(zq::kTabT), 0, st, a,
-                           zq::kExpand);
-        hipLaunchKernelGGL(zq::page_release_kernel, dim3(1), dim3(zq::kTabT), 0, st, a, zq::kCommit);
-    }
+    zq::run_release(a, static_cast<hipStream_t>(stream));
     return zq::status(hipGetLastError());
 }
 

@@ -103,14 +103,18 @@ __device__ __forceinline__ Shares scan_units(uint32_t n, uint32_t mult, uint32_t
         if (w == wave) mine += s.units;
         s.units += sh.part[w];
     }
+    s.units = uint32_t(__builtin_amdgcn_readfirstlane(int(s.units)));  // one for the workgroup
     s.all = uint64_t(s.units) * mult;
     s.used = uint32_t(min(uint64_t(W), s.all));
     return s;
 }
 // The query that has unit x (< all) of all kv heads, and the units of one kv head before it.
+struct Found {
+    uint32_t query, before;
+};
 template <class F>
-__device__ __forceinline__ void find_query(uint32_t n, uint32_t mult, F units, ShareScan& sh, uint64_t x, uint32_t mine,
-                                           uint32_t own) {
+__device__ __forceinline__ Found find_query(uint32_t n, uint32_t mult, F units, ShareScan& sh, uint64_t x, uint32_t mine,
+                                            uint32_t own) {
     if (x >= uint64_t(mine) * mult && x < uint64_t(mine + own) * mult) {
         uint32_t i = threadIdx.x * ((n + kShareT - 1) / kShareT), before = mine;
         for (;;) {  // ends: the unit is one of this thread's queries
@@ -123,6 +127,7 @@ __device__ __forceinline__ void find_query(uint32_t n, uint32_t mult, F units, S
         sh.before = before;
     }
     __syncthreads();
+    return {uint32_t(__builtin_amdgcn_readfirstlane(int(sh.query))), uint32_t(__builtin_amdgcn_readfirstlane(int(sh.before)))};
 }
 #endif
 

@@ -44,8 +44,10 @@ struct AttnPaged {
 // ---- work of a workgroup ---------------------------------------------------------
 // The rows of a (query, kv head) pair are cut into units of kUnit keys, and these are
 // shared out evenly (zq_paged.hpp).  A pair that a share's end cuts is put together by
-// the join kernel.
+// the join kernel.  Starting on a pair and writing its outputs takes as long as kStart
+// units more, which count as units without keys at its start.
 constexpr int kT = kShareT, kWaves = kShareWaves;
+constexpr uint32_t kStart = 2;
 template <int TYPE>
 struct Tile {
     static constexpr int kKeys = TYPE == ZQ_KV_F32 ? 16 : 32;  // keys of a wave's tile
@@ -65,12 +67,12 @@ struct Group {
     uint32_t queries, most, least;  // rows that they see
 };
 template <bool GROUP>
-__device__ __forceinline__ Group group_of(const AttnPaged& a, uint32_t i) {
-    Group x{seen_by(a.see, i), 1, 0, 0};
+__device__ __forceinline__ Group group_of(const AttnPaged& a, const ShareScan& sh, uint32_t i) {
+    Group x{seen_held(a.see, sh, i), 1, 0, 0};
     x.most = x.least = x.first.rows;
     if constexpr (GROUP) {
         for (uint32_t j = i + 1; x.first.seq >= 0 && j < a.see.n && j % a.P; ++j) {
-            const Seen y = seen_by(a.see, j);
+            const Seen y = seen_held(a.see, sh, j);
             if (y.seq != x.first.seq) break;
             ++x.queries;
             x.most = max(x.most, y.rows);
@@ -80,12 +82,12 @@ __device__ __forceinline__ Group group_of(const AttnPaged& a, uint32_t i) {
     return x;
 }
 template <int TYPE, bool GROUP>
-__device__ __forceinline__ uint32_t units_of(const AttnPaged& a, uint32_t i) {
-    const Group x = group_of<GROUP>(a, i);
+__device__ __forceinline__ uint32_t units_of(const AttnPaged& a, const ShareScan& sh, uint32_t i) {
+    const Group x = group_of<GROUP>(a, sh, i);
     if (x.first.seq < 0) return 0;
-    if (GROUP && i % a.P && seen_by(a.see, i - 1).seq == x.first.seq) return 0;
+    if (GROUP && i % a.P && seen_held(a.see, sh, i - 1).seq == x.first.seq) return 0;
     const uint32_t rows = a.select ? entries_of(a, x.most) << a.lp : x.most;
-    return max((rows + Tile<TYPE>::kUnit - 1) / Tile<TYPE>::kUnit, 1u);  // no rows: a unit that writes zeros
+    return kStart + max((rows + Tile<TYPE>::kUnit - 1) / Tile<TYPE>::kUnit, 1u);  // no rows: a unit that writes zeros
 }
 
 // Where row r (query, head) of a group goes; without groups r is a head, G of them and no more.
@@ -157,7 +159,6 @@ struct Shape {
     static constexpr int VW = VE * ES / 4;                          // dwords of one
     static constexpr int VR = 4 * H;                                // rows whose V a lane loads
     static constexpr int NP = TYPE == ZQ_KV_F32 ? 1 : TYPE == ZQ_KV_F16 ? 2 : 3;
-    static constexpr bool kQInLds = true;
 };
 
 // The softmax weights of a lane's rows as operands, and what they add to one tile of O^T.
@@ -215,6 +216,12 @@ __device__ __forceinline__ bool not_finite(uint32_t w) {
     return (w & m) == m || (w >> 16 & m) == m;
 }
 
+// A held row's bytes: read by one workgroup alone, or (GROUP) by those of other queries of its sequence too.
+template <bool GROUP, class V>
+__device__ __forceinline__ V load_held(const uint8_t* p) {
+    return GROUP ? *reinterpret_cast<const V*>(p) : load_once<V>(p);
+}
+
 // ---- the kernel ------------------------------------------------------------------
 // Both products are computed transposed (S^T = K Q^T, O^T = V^T P^T) on 16x16 tiles,
 // so that nothing crosses lanes between them.  With lane (i = lane & 15, g = lane >> 4):
@@ -234,13 +241,14 @@ template <int TYPE, int D, bool GROUP>
 __global__ __launch_bounds__(kT, D == 64 ? 4 : D == 128 ? 3 : 2) void attn_paged_kernel(AttnPaged a) {
     using S = Shape<TYPE, D>;
     constexpr int H = S::H, KC = S::KC, VE = S::VE, VC = S::VC, VW = S::VW, VR = S::VR, NP = S::NP;
-    extern __shared__ float dyn[];  // [4 waves][rows][D + 4], then q's operands where they are kept here
+    extern __shared__ float dyn[];  // [4 waves][rows][D + 4], then q's operands
     __shared__ ShareScan scan;
     __shared__ float sm[kWaves][16], sl[kWaves][16];
     const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t row0 = GROUP ? 0u : blockIdx.y * 16;  // the first head of this workgroup's
-    const auto units = [&](uint32_t n) { return units_of<TYPE, GROUP>(a, n); };
+    const auto units = [&](uint32_t n) { return units_of<TYPE, GROUP>(a, scan, n); };
+    hold_seen(a.see, scan);
     uint32_t mine, own;
     const Shares sh = scan_units(a.see.n, a.KH, gridDim.x, units, scan, mine, own);
     if (threadIdx.x == 0 && blockIdx.y == 0) a.cut[blockIdx.x].parts = 0;
@@ -250,16 +258,24 @@ __global__ __launch_bounds__(kT, D == 64 ? 4 : D == 128 ? 3 : 2) void attn_paged
     uint32_t qi = at_begin.query, before = at_begin.before;
     uint64_t pos = begin;
     const size_t head_rows = size_t(1) << a.lp;
+    v4u_t* held_q = reinterpret_cast<v4u_t*>(dyn + kWaves * a.RL * (D + 4));  // q's operands [KC][NP][64]
     while (pos < end) {
-        const uint32_t u = units(qi);
+        const uint32_t u = uniform(units(qi));
         if (pos >= uint64_t(before + u) * a.KH) {
             before += u;
             ++qi;
             continue;
         }
-        const uint32_t rel = uint32_t(pos - uint64_t(before) * a.KH), kh = rel / u, u0 = rel % u;
-        const uint32_t u1 = uint32_t(min(uint64_t(u), u0 + (end - pos)));
-        const Group x = group_of<GROUP>(a, qi);
+        const uint32_t rel = uint32_t(pos - uint64_t(before) * a.KH), kh = rel / u, v0 = rel % u;
+        const uint32_t v1 = uint32_t(min(uint64_t(u), v0 + (end - pos)));
+        const uint32_t u0 = v0 > kStart ? v0 - kStart : 0u, u1 = v1 > kStart ? v1 - kStart : 0u;  // with keys
+        if (u1 == 0) {
+            pos += v1 - v0;
+            continue;
+        }
+        Group x = group_of<GROUP>(a, scan, qi);
+        x.first.seq = int32_t(uniform(uint32_t(x.first.seq)));
+        x.queries = uniform(x.queries), x.most = uniform(x.most), x.least = uniform(x.least);
         const uint32_t R = GROUP ? x.queries * a.G : min(a.G - row0, 16u);  // rows: query, head
         const uint32_t entries = entries_of(a, x.most);
         const uint32_t parts = a.select ? entries << (a.lp - 4) : (x.most + 15) >> 4;  // 16-key parts of the pair
@@ -269,70 +285,9 @@ __global__ __launch_bounds__(kT, D == 64 ? 4 : D == 128 ? 3 : 2) void attn_paged
         const int32_t* table = a.table + size_t(x.first.seq) * a.width;
         const int32_t* select = a.select ? a.select + (size_t(qi) * a.KH + kh) * a.keep : nullptr;
 
-        // ---- the queries as operands ----
-        const uint32_t row = min(uint32_t(i), R - 1), member = GROUP ? row / a.G : 0u;
-        const float* qrow = a.q + (qi + member) * a.stride + (size_t(kh) * a.G + row0 + row - member * a.G) * D;
-        const uint32_t my_rows = GROUP ? seen_by(a.see, qi + member).rows : 0u;  // that this lane's query sees
-        v4u_t qop[S::kQInLds ? 1 : KC][NP];
-        float c = a.scale2;  // takes a score into log2 units
-        {
-            float4 x0[KC][TYPE == ZQ_KV_F32 ? 1 : 2];
-            float most = 0.0f;
-#pragma unroll
-            for (int k = 0; k < KC; ++k)
-#pragma unroll
-                for (int j = 0; j < (TYPE == ZQ_KV_F32 ? 1 : 2); ++j) {
-                    float4 y = *reinterpret_cast<const float4*>(qrow + (4 * k + g) * (TYPE == ZQ_KV_F32 ? 4 : 8) + 4 * j);
-                    if (uint32_t(i) >= R) y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                    x0[k][j] = y;
-                    most = fmaxf(most, fmaxf(fmaxf(fabsf(y.x), fabsf(y.y)), fmaxf(fabsf(y.z), fabsf(y.w))));
-                }
-            float up = 1.0f;
-            if constexpr (TYPE == ZQ_KV_F16) {  // the row's largest element to 2^14 .. 2^15
-                most = max_groups(most);
-                if (most > 0.0f) {
-                    const int e = min(max(15 - __builtin_amdgcn_frexp_expf(most), -113), 126);
-                    up = pow2f(e);
-                    c *= pow2f(-e);
-                }
-            }
-#pragma unroll
-            for (int k = 0; k < KC; ++k) {
-                v4u_t op[NP];
-                if constexpr (TYPE == ZQ_KV_F32) {
-                    op[0] = v4u_t{f_bits(x0[k][0].x), f_bits(x0[k][0].y), f_bits(x0[k][0].z), f_bits(x0[k][0].w)};
-                } else {
-                    Parts<TYPE> p;
-#pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        p.set2(4 * j, x0[k][j].x * up, x0[k][j].y * up);
-                        p.set2(4 * j + 2, x0[k][j].z * up, x0[k][j].w * up);
-                    }
-#pragma unroll
-                    for (int n = 0; n < NP; ++n) op[n] = p.bits(n);
-                }
-                if constexpr (S::kQInLds) {
-                    v4u_t* at = reinterpret_cast<v4u_t*>(dyn + kWaves * a.RL * (D + 4));
-                    if (k % kWaves == wave)
-#pragma unroll
-                        for (int n = 0; n < NP; ++n) at[(k * NP + n) * 64 + lane] = op[n];
-                } else {
-#pragma unroll
-                    for (int n = 0; n < NP; ++n) qop[k][n] = op[n];
-                }
-            }
-        }
-        if constexpr (S::kQInLds) __syncthreads();
-
         // ---- the wave's tiles ----
         v4u_t kt[H][KC];
         uint32_t vt[VR][VC][VW];
-        v4f_t o[VC][VE];
-#pragma unroll
-        for (int n = 0; n < VC; ++n)
-#pragma unroll
-            for (int e = 0; e < VE; ++e) o[n][e] = v4f_t{0.0f, 0.0f, 0.0f, 0.0f};
-        float m = -INFINITY, l = 0.0f;
         uint32_t place = 0;  // lane p: page | rows there << 24 of the p-th part that the wave has ahead
         // byte offset of the wave's part p (of 64) from the cache's start
         auto part_at = [&](uint32_t p, uint32_t part) {
@@ -342,179 +297,236 @@ __global__ __launch_bounds__(kT, D == 64 ? 4 : D == 128 ? 3 : 2) void attn_paged
         };
         auto rows_at = [&](uint32_t p) { return uint32_t(__builtin_amdgcn_readlane(int(place), int(p))) >> 24; };
         constexpr uint32_t kBatch = 64 / H;  // tiles whose places a wave holds
-        for (uint32_t b = 0; b < nt; b += kBatch) {
-            {
-                const uint32_t j = b + lane / H, part = (t0 + j * kWaves) * H + lane % H, e = part >> (a.lp - 4);
-                place = 0;
-                if (j < nt && e < entries) {
-                    const uint32_t y = select ? uint32_t(select[e]) : e;  // place in the sequence
-                    if (y < a.width && (y << a.lp) < x.most) {
-                        const uint32_t page = uint32_t(table[y]);
-                        const uint32_t first = (y << a.lp) + ((part << 4) & (uint32_t(head_rows) - 1));
-                        if (page < a.pages && first < x.most) place = page | min(x.most - first, 16u) << 24;
+        uint32_t b = 0;  // the first tile of the batch
+        auto load_places = [&] {
+            const uint32_t j = b + lane / H, part = (t0 + j * kWaves) * H + lane % H, e = part >> (a.lp - 4);
+            place = 0;
+            if (j < nt && e < entries) {
+                const uint32_t y = select ? uint32_t(select[e]) : e;  // place in the sequence
+                if (y < a.width && (y << a.lp) < x.most) {
+                    const uint32_t page = uint32_t(table[y]);
+                    const uint32_t first = (y << a.lp) + ((part << 4) & (uint32_t(head_rows) - 1));
+                    if (page < a.pages && first < x.most) place = page | min(x.most - first, 16u) << 24;
+                }
+            }
+        };
+        auto load_k = [&](uint32_t j) {
+#pragma unroll
+            for (int h = 0; h < H; ++h) {
+                const uint8_t* p = a.k + part_at(j * H + h, (t0 + (b + j) * kWaves) * H + h);
+#pragma unroll
+                for (int k = 0; k < KC; ++k)
+                    kt[h][k] = load_held<GROUP, v4u_t>(p + uint32_t(i * D * S::ES + k * 64 + g * 16));
+            }
+        };
+        auto load_v = [&](uint32_t j) {
+#pragma unroll
+            for (int h = 0; h < H; ++h) {
+                const uint8_t* p = a.v + part_at(j * H + h, (t0 + (b + j) * kWaves) * H + h);
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+#pragma unroll
+                    for (int n = 0; n < VC; ++n) {
+                        const uint8_t* at = p + uint32_t((4 * g + r) * D * S::ES + (n * 16 + i) * VE * S::ES);
+                        if constexpr (VW == 4) {
+                            const v4u_t w = load_held<GROUP, v4u_t>(at);
+#pragma unroll
+                            for (int z = 0; z < 4; ++z) vt[h * 4 + r][n][z] = w[z];
+                        } else {
+                            const v2u_t w = load_held<GROUP, v2u_t>(at);
+                            vt[h * 4 + r][n][0] = w[0];
+                            vt[h * 4 + r][n][1] = w[1];
+                        }
+                    }
+            }
+        };
+        load_places();
+
+        // ---- the queries as operands ----
+        const uint32_t row = min(uint32_t(i), R - 1), member = GROUP ? row / a.G : 0u;
+        const float* qrow = a.q + (qi + member) * a.stride + (size_t(kh) * a.G + row0 + row - member * a.G) * D;
+        const uint32_t my_rows = GROUP ? seen_held(a.see, scan, qi + member).rows : 0u;  // that this lane's query sees
+        float c = a.scale2;  // takes a score into log2 units
+        float4 x0[KC][TYPE == ZQ_KV_F32 ? 1 : 2];
+        float most = 0.0f;
+#pragma unroll
+        for (int k = 0; k < KC; ++k)
+#pragma unroll
+            for (int j = 0; j < (TYPE == ZQ_KV_F32 ? 1 : 2); ++j) {
+                float4 y = *reinterpret_cast<const float4*>(qrow + (4 * k + g) * (TYPE == ZQ_KV_F32 ? 4 : 8) + 4 * j);
+                if (uint32_t(i) >= R) y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                x0[k][j] = y;
+                most = fmaxf(most, fmaxf(fmaxf(fabsf(y.x), fabsf(y.y)), fmaxf(fabsf(y.z), fabsf(y.w))));
+            }
+        // (asked for behind the queries, which are waited for first; a wave without tiles reads rows of page 0)
+        load_k(0);
+        load_v(0);
+        float up = 1.0f;
+        if constexpr (TYPE == ZQ_KV_F16) {  // the row's largest element to 2^14 .. 2^15
+            most = max_groups(most);
+            if (most > 0.0f) {
+                const int e = min(max(15 - __builtin_amdgcn_frexp_expf(most), -113), 126);
+                up = pow2f(e);
+                c *= pow2f(-e);
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < KC; ++k) {
+            v4u_t op[NP];
+            if constexpr (TYPE == ZQ_KV_F32) {
+                op[0] = v4u_t{f_bits(x0[k][0].x), f_bits(x0[k][0].y), f_bits(x0[k][0].z), f_bits(x0[k][0].w)};
+            } else {
+                Parts<TYPE> p;
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    p.set2(4 * j, x0[k][j].x * up, x0[k][j].y * up);
+                    p.set2(4 * j + 2, x0[k][j].z * up, x0[k][j].w * up);
+                }
+#pragma unroll
+                for (int n = 0; n < NP; ++n) op[n] = p.bits(n);
+            }
+            if (k % kWaves == wave)
+#pragma unroll
+                for (int n = 0; n < NP; ++n) held_q[(k * NP + n) * 64 + lane] = op[n];
+        }
+        __syncthreads();
+
+        v4f_t o[VC][VE];
+#pragma unroll
+        for (int n = 0; n < VC; ++n)
+#pragma unroll
+            for (int e = 0; e < VE; ++e) o[n][e] = v4f_t{0.0f, 0.0f, 0.0f, 0.0f};
+        float m = -INFINITY, l = 0.0f;
+        auto step = [&](uint32_t j, auto last) {
+            v4f_t s[H];
+#pragma unroll
+            for (int h = 0; h < H; ++h) s[h] = v4f_t{0.0f, 0.0f, 0.0f, 0.0f};
+            asm volatile("" ::: "memory");  // q is read again, not held
+#pragma unroll
+            for (int k = 0; k < KC; ++k) {
+                v4u_t op[NP];
+#pragma unroll
+                for (int n = 0; n < NP; ++n) op[n] = held_q[(k * NP + n) * 64 + lane];
+#pragma unroll
+                for (int h = 0; h < H; ++h) {
+                    if constexpr (TYPE == ZQ_KV_F32) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            s[h] = __builtin_amdgcn_mfma_f32_16x16x4f32(bits_f(kt[h][k][e]), bits_f(op[0][e]), s[h], 0, 0, 0);
+                    } else {
+#pragma unroll
+                        for (int n = NP - 1; n >= 0; --n) s[h] = mma<TYPE>(kt[h][k], op[n], s[h]);
                     }
                 }
             }
-            const uint32_t count = min(nt - b, kBatch);
-            auto load_k = [&](uint32_t j) {
+            uint32_t rows[H];
+            bool cut = false;
+#pragma unroll
+            for (int h = 0; h < H; ++h) {
+                rows[h] = rows_at(j * H + h);
+                cut |= rows[h] < 16;
+                if (GROUP) cut |= (((t0 + (b + j) * kWaves) * H + h) << 4) + 16 > x.least;
+            }
+            if constexpr (!decltype(last)::value) load_k(j + 1);
+#pragma unroll
+            for (int h = 0; h < H; ++h) s[h] *= c;
+            if (cut) {  // uniform
 #pragma unroll
                 for (int h = 0; h < H; ++h) {
-                    const uint8_t* p = a.k + part_at(j * H + h, (t0 + (b + j) * kWaves) * H + h);
-#pragma unroll
-                    for (int k = 0; k < KC; ++k)
-                        kt[h][k] = *reinterpret_cast<const v4u_t*>(p + uint32_t(i * D * S::ES + k * 64 + g * 16));
-                }
-            };
-            auto load_v = [&](uint32_t j) {
-#pragma unroll
-                for (int h = 0; h < H; ++h) {
-                    const uint8_t* p = a.v + part_at(j * H + h, (t0 + (b + j) * kWaves) * H + h);
+                    uint32_t n = rows[h];
+                    if (GROUP) n = min(n, uint32_t(max(int32_t(my_rows - (((t0 + (b + j) * kWaves) * H + h) << 4)), 0)));
 #pragma unroll
                     for (int r = 0; r < 4; ++r)
-#pragma unroll
-                        for (int n = 0; n < VC; ++n) {
-                            const uint8_t* at = p + uint32_t((4 * g + r) * D * S::ES + (n * 16 + i) * VE * S::ES);
-                            if constexpr (VW == 4) {
-                                const v4u_t w = *reinterpret_cast<const v4u_t*>(at);
-#pragma unroll
-                                for (int z = 0; z < 4; ++z) vt[h * 4 + r][n][z] = w[z];
-                            } else {
-                                const v2u_t w = *reinterpret_cast<const v2u_t*>(at);
-                                vt[h * 4 + r][n][0] = w[0];
-                                vt[h * 4 + r][n][1] = w[1];
-                            }
-                        }
+                        if (uint32_t(4 * g + r) >= n) s[h][r] = -INFINITY;
                 }
-            };
-            load_k(0);
-            load_v(0);
-            auto step = [&](uint32_t j, auto last) {
-                v4f_t s[H];
+            }
+            float most = -INFINITY;
 #pragma unroll
-                for (int h = 0; h < H; ++h) s[h] = v4f_t{0.0f, 0.0f, 0.0f, 0.0f};
-                if constexpr (S::kQInLds) asm volatile("" ::: "memory");  // q is read again, not held
+            for (int h = 0; h < H; ++h)
 #pragma unroll
-                for (int k = 0; k < KC; ++k) {
-                    v4u_t op[NP];
-#pragma unroll
-                    for (int n = 0; n < NP; ++n) {
-                        if constexpr (S::kQInLds)
-                            op[n] = reinterpret_cast<const v4u_t*>(dyn + kWaves * a.RL * (D + 4))[(k * NP + n) * 64 + lane];
-                        else
-                            op[n] = qop[k][n];
-                    }
-#pragma unroll
-                    for (int h = 0; h < H; ++h) {
-                        if constexpr (TYPE == ZQ_KV_F32) {
-#pragma unroll
-                            for (int e = 0; e < 4; ++e)
-                                s[h] = __builtin_amdgcn_mfma_f32_16x16x4f32(bits_f(kt[h][k][e]), bits_f(op[0][e]), s[h], 0, 0, 0);
-                        } else {
-#pragma unroll
-                            for (int n = NP - 1; n >= 0; --n) s[h] = mma<TYPE>(kt[h][k], op[n], s[h]);
-                        }
-                    }
-                }
-                uint32_t rows[H];
-                bool cut = false;
-#pragma unroll
-                for (int h = 0; h < H; ++h) {
-                    rows[h] = rows_at(j * H + h);
-                    cut |= rows[h] < 16;
-                    if (GROUP) cut |= (((t0 + (b + j) * kWaves) * H + h) << 4) + 16 > x.least;
-                }
-                if constexpr (!decltype(last)::value) load_k(j + 1);
-#pragma unroll
-                for (int h = 0; h < H; ++h) s[h] *= c;
-                if (cut) {  // uniform
-#pragma unroll
-                    for (int h = 0; h < H; ++h) {
-                        uint32_t n = rows[h];
-                        if (GROUP) n = min(n, uint32_t(max(int32_t(my_rows - (((t0 + (b + j) * kWaves) * H + h) << 4)), 0)));
-#pragma unroll
-                        for (int r = 0; r < 4; ++r)
-                            if (uint32_t(4 * g + r) >= n) s[h][r] = -INFINITY;
-                    }
-                }
-                float most = -INFINITY;
-#pragma unroll
-                for (int h = 0; h < H; ++h)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) most = fmaxf(most, s[h][r]);
-                if (__any(most > m + kSlack)) {
-                    const float to = fmaxf(m, max_groups(most));
-                    const float f = to == -INFINITY ? 1.0f : exp2_(m - to);
-                    m = to;
-                    l *= f;
-#pragma unroll
-                    for (int n = 0; n < VC; ++n)
-#pragma unroll
-                        for (int e = 0; e < VE; ++e) o[n][e] *= f;
-                }
-                const float ms = (m == -INFINITY ? 0.0f : m) - kShift;
-                float p[VR];
-#pragma unroll
-                for (int h = 0; h < H; ++h)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        p[h * 4 + r] = exp2_(s[h][r] - ms);
-                        l += p[h * 4 + r];
-                    }
-                if (cut) {
-#pragma unroll
-                    for (int h = 0; h < H; ++h)
-#pragma unroll
-                        for (int r = 0; r < 4; ++r)
-                            if (uint32_t(4 * g + r) >= rows[h])
-#pragma unroll
-                                for (int n = 0; n < VC; ++n)
-#pragma unroll
-                                    for (int z = 0; z < VW; ++z) vt[h * 4 + r][n][z] = 0;
-                }
-                const Weights<TYPE, VR> pw(p);
-                if (GROUP && cut && x.least < x.most) {
-                    // a value that is no number must not reach (0 times it) the queries that do not see its row
-                    bool odd = false;
-#pragma unroll
-                    for (int r = 0; r < VR; ++r)
-#pragma unroll
-                        for (int n = 0; n < VC; ++n)
-#pragma unroll
-                            for (int z = 0; z < VW; ++z) odd |= not_finite<TYPE>(vt[r][n][z]);
-                    if (__any(odd)) {
-                        // per element: how many such values a query sees; more than none gives NaN
-                        float sees[VR];
-#pragma unroll
-                        for (int r = 0; r < VR; ++r)
-                            sees[r] = (((t0 + (b + j) * kWaves) * H + r / 4) << 4) + 4 * g + r % 4 < my_rows ? 1.0f : 0.0f;
-                        const Weights<TYPE, VR> ps(sees);
-#pragma unroll
-                        for (int n = 0; n < VC; ++n)
-#pragma unroll
-                            for (int z = 0; z < VW; ++z) {
-                                uint32_t w[VR][1][1];
-#pragma unroll
-                                for (int r = 0; r < VR; ++r) {
-                                    w[r][0][0] = take_odd<TYPE>(vt[r][n][z]);
-                                }
-#pragma unroll
-                                for (int e = 0; e < VE / VW; ++e) {
-                                    const v4f_t y = add_pv<TYPE, VR, 1, 1, 1>(w, ps, 0, e, v4f_t{0.0f, 0.0f, 0.0f, 0.0f});
-                                    v4f_t& to = o[n][z * (VE / VW) + e];
-#pragma unroll
-                                    for (int k = 0; k < 4; ++k) to[k] = y[k] > 0.0f ? NAN : to[k];
-                                }
-                            }
-                    }
-                }
+                for (int r = 0; r < 4; ++r) most = fmaxf(most, s[h][r]);
+            if (__any(most > m + kSlack)) {
+                const float to = fmaxf(m, max_groups(most));
+                const float f = to == -INFINITY ? 1.0f : exp2_(m - to);
+                m = to;
+                l *= f;
 #pragma unroll
                 for (int n = 0; n < VC; ++n)
 #pragma unroll
-                    for (int e = 0; e < VE; ++e) o[n][e] = add_pv<TYPE, VR, VC, VW>(vt, pw, n, e, o[n][e]);
-                if constexpr (!decltype(last)::value) load_v(j + 1);
-            };
+                    for (int e = 0; e < VE; ++e) o[n][e] *= f;
+            }
+            const float ms = (m == -INFINITY ? 0.0f : m) - kShift;
+            float p[VR];
+#pragma unroll
+            for (int h = 0; h < H; ++h)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    p[h * 4 + r] = exp2_(s[h][r] - ms);
+                    l += p[h * 4 + r];
+                }
+            if (cut) {
+#pragma unroll
+                for (int h = 0; h < H; ++h)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (uint32_t(4 * g + r) >= rows[h])
+#pragma unroll
+                            for (int n = 0; n < VC; ++n)
+#pragma unroll
+                                for (int z = 0; z < VW; ++z) vt[h * 4 + r][n][z] = 0;
+            }
+            const Weights<TYPE, VR> pw(p);
+            if (GROUP && cut && x.least < x.most) {
+                // a value that is no number must not reach (0 times it) the queries that do not see its row
+                bool odd = false;
+#pragma unroll
+                for (int r = 0; r < VR; ++r)
+#pragma unroll
+                    for (int n = 0; n < VC; ++n)
+#pragma unroll
+                        for (int z = 0; z < VW; ++z) odd |= not_finite<TYPE>(vt[r][n][z]);
+                if (__any(odd)) {
+                    // per element: how many such values a query sees; more than none gives NaN
+                    float sees[VR];
+#pragma unroll
+                    for (int r = 0; r < VR; ++r)
+                        sees[r] = (((t0 + (b + j) * kWaves) * H + r / 4) << 4) + 4 * g + r % 4 < my_rows ? 1.0f : 0.0f;
+                    const Weights<TYPE, VR> ps(sees);
+#pragma unroll
+                    for (int n = 0; n < VC; ++n)
+#pragma unroll
+                        for (int z = 0; z < VW; ++z) {
+                            uint32_t w[VR][1][1];
+#pragma unroll
+                            for (int r = 0; r < VR; ++r) {
+                                w[r][0][0] = take_odd<TYPE>(vt[r][n][z]);
+                            }
+#pragma unroll
+                            for (int e = 0; e < VE / VW; ++e) {
+                                const v4f_t y = add_pv<TYPE, VR, 1, 1, 1>(w, ps, 0, e, v4f_t{0.0f, 0.0f, 0.0f, 0.0f});
+                                v4f_t& to = o[n][z * (VE / VW) + e];
+#pragma unroll
+                                for (int k = 0; k < 4; ++k) to[k] = y[k] > 0.0f ? NAN : to[k];
+                            }
+                        }
+                }
+            }
+#pragma unroll
+            for (int n = 0; n < VC; ++n)
+#pragma unroll
+                for (int e = 0; e < VE; ++e) o[n][e] = add_pv<TYPE, VR, VC, VW>(vt, pw, n, e, o[n][e]);
+            if constexpr (!decltype(last)::value) load_v(j + 1);
+        };
+        while (b < nt) {
+            const uint32_t count = min(nt - b, kBatch);
             for (uint32_t j = 0; j + 1 < count; ++j) step(j, std::false_type{});
             step(count - 1, std::true_type{});
+            b += kBatch;
+            if (b < nt) {
+                load_places();
+                load_k(0);
+                load_v(0);
+            }
         }
 
         // ---- the four waves' sums as one ----
@@ -538,11 +550,11 @@ __global__ __launch_bounds__(kT, D == 64 ? 4 : D == 128 ? 3 : 2) void attn_paged
                             make_float4(o[n][e][r], o[n][e + 1][r], o[n][e + 2][r], o[n][e + 3][r]);
         }
         __syncthreads();
-        const bool whole = u0 == 0 && u1 == u;
+        const bool whole = u0 == 0 && v1 == u;
         const size_t at = size_t(blockIdx.x) * 2 + (pos != begin), slot = at * a.RS + row0;
-        if (u0 == 0 && u1 < u && threadIdx.x == 0 && blockIdx.y == 0) {
+        if (u0 == 0 && v1 < u && threadIdx.x == 0 && blockIdx.y == 0) {
             // shares with a part of the pair: up to the last one that starts below its end
-            const uint64_t last = ((pos + u) * sh.used + sh.all - 1) / sh.all - 1;
+            const uint64_t last = ((pos - v0 + u) * sh.used + sh.all - 1) / sh.all - 1;
             a.cut[blockIdx.x] = {qi, kh, GROUP ? R : a.G, uint32_t(last - blockIdx.x + 1), at};
         }
         for (uint32_t z = threadIdx.x; z < R * (D / 4); z += kT) {
@@ -571,7 +583,7 @@ __global__ __launch_bounds__(kT, D == 64 ? 4 : D == 128 ? 3 : 2) void attn_paged
             *reinterpret_cast<float4*>(to + d) = y;
         }
         __syncthreads();
-        pos += u1 - u0;
+        pos += v1 - v0;
     }
 }
 
@@ -613,12 +625,14 @@ __global__ __launch_bounds__(kT) void attn_paged_join_kernel(AttnPaged a) {
     for (uint32_t d = threadIdx.x; d < D; d += kT) out[d] = ((acc[0][d] + acc[1][d]) + (acc[2][d] + acc[3][d])) * inv;
 }
 
-// Workgroups for a call: three a CU are resident (two with D = 256), and as many as
-// there are units at most.
+// Workgroups for a call, as many as there are units at most: two a CU, and a third (all that are resident) where there
+// are so many pairs that every one starts on several of them; with D = 256 one.  (512, 768, 1536 workgroups, us: 64
+// sequences of up to 8190 rows, 512 pairs: 175, 177, 182; 512 of up to 400, 4096 pairs: 114, 110, 104; 131,072 rows of
+// one: 89, 91, 100; 32 of up to 8000, bf16, D = 256, with 256, 512 and 1024: 97, 110, 131.)
 uint32_t shares_of(const zq_kv_paged& c, const zq_page_tables& t, size_t queries) {
-    const size_t unit = c.type == ZQ_KV_F32 ? 64 : 128;
-    const size_t most = queries * c.kv_heads * ((t.width * t.page_size + unit - 1) / unit);
-    const size_t want = 256 * (c.head_dim == 256 ? 2 : 3);
+    const size_t unit = c.type == ZQ_KV_F32 ? 64 : 128, pairs = queries * c.kv_heads;
+    const size_t most = pairs * ((t.width * t.page_size + unit - 1) / unit + kStart);
+    const size_t want = 256 * (c.head_dim == 256 ? 1 : pairs < 2048 ? 2 : 3);
     return uint32_t(most < want ? most : want);
 }
 

@@ -24,10 +24,10 @@ struct SelectArgs {
     const int32_t* table;
     const float* q;
     int32_t* select;
-    float* score;  // [queries][KH][width]
+    float* score;  // [queries][KH][pitch]
     Queries see;
     size_t stride;
-    uint32_t width, pages, KH, G, lp, keep, recent, first;
+    uint32_t width, pitch, pages, KH, G, lp, keep, recent, first;  // pitch: width in whole groups of 4
 };
 __device__ __forceinline__ uint32_t pages_seen(const SelectArgs& a, const Seen& x) {
     return (x.rows + (1u << a.lp) - 1) >> a.lp;
@@ -48,8 +48,9 @@ template <int D>
 __global__ __launch_bounds__(kShareT) void page_score_kernel(SelectArgs a) {
     using S = ScoreShape<D>;
     __shared__ ShareScan scan;
+    hold_seen(a.see, scan);
     const auto units = [&](uint32_t i) {
-        const Seen x = seen_by(a.see, i);
+        const Seen x = seen_held(a.see, scan, i);
         const uint32_t n = x.seq < 0 ? 0u : pages_seen(a, x);
         return n > a.keep ? (n + S::kUnit - 1) / S::kUnit : 0u;
     };
@@ -63,7 +64,7 @@ __global__ __launch_bounds__(kShareT) void page_score_kernel(SelectArgs a) {
     const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     while (pos < end) {
-        const uint32_t u = units(qi);
+        const uint32_t u = uniform(units(qi));
         if (pos >= uint64_t(before + u) * a.KH) {
             before += u;
             ++qi;
@@ -71,10 +72,11 @@ __global__ __launch_bounds__(kShareT) void page_score_kernel(SelectArgs a) {
         }
         const uint32_t rel = uint32_t(pos - uint64_t(before) * a.KH), kh = rel / u, u0 = rel % u;
         const uint32_t u1 = uint32_t(min(uint64_t(u), u0 + (end - pos)));
-        const Seen x = seen_by(a.see, qi);
-        const uint32_t n = pages_seen(a, x);
+        Seen x = seen_held(a.see, scan, qi);
+        x.seq = int32_t(uniform(uint32_t(x.seq)));
+        const uint32_t n = uniform(pages_seen(a, x));
         const int32_t* table = a.table + size_t(x.seq) * a.width;
-        float* score = a.score + (size_t(qi) * a.KH + kh) * a.width;
+        float* score = a.score + (size_t(qi) * a.KH + kh) * a.pitch;
         for (uint32_t h0 = 0; h0 < a.G; h0 += 16) {  // 16 heads at once
             // codes of head h0 + i: elements 16 g .. of every 64
             const uint32_t R = min(a.G - h0, 16u);
@@ -127,7 +129,7 @@ __global__ __launch_bounds__(kShareT) void page_score_kernel(SelectArgs a) {
                     const uint32_t pg = uint32_t(__shfl(int(page), w * 16 + i));
                     const int8_t* at = a.bounds + (size_t(pg) * a.KH + kh) * 2 * D + g * 16;
 #pragma unroll
-                    for (int k = 0; k < S::KC; ++k) b[w][k] = *reinterpret_cast<const v4i_t*>(at + k * 64);
+                    for (int k = 0; k < S::KC; ++k) b[w][k] = load_once<v4i_t>(at + k * 64);
                 }
                 float mine_s = 0.0f;
 #pragma unroll
@@ -160,9 +162,10 @@ __global__ __launch_bounds__(kShareT) void page_score_kernel(SelectArgs a) {
 
 // ---- the largest ---------------------------------------------------------------------
 // A workgroup for every (query, kv head).  Thread t holds pages t N .. t N + N - 1 (of
-// every N * 1024).  The score of rank `want` is found by digits of 11 bits from the top bit
-// in which any two differ, counted in LDS; one scan of (pages above it, pages at it) then
-// gives every page that stays its place.
+// every N * 1024), as whole numbers in the order of the scores, from the least one on.
+// The score of rank `want` is found by digits of 11 bits from the highest bit there is,
+// counted in LDS, until all that share its digits stay; one scan of (pages above it,
+// pages at it) then gives every page that stays its place.
 constexpr int kTopT = 1024, kTopWaves = kTopT / 64, kBins = 2048;
 
 __device__ __forceinline__ uint32_t score_key(float f) {
@@ -171,22 +174,27 @@ __device__ __forceinline__ uint32_t score_key(float f) {
 }
 
 template <int N>
-__device__ __forceinline__ void top_pages(const SelectArgs& a, const float* score, int32_t* to, uint32_t n) {
-    __shared__ uint32_t hist[2][kBins];
-    __shared__ uint32_t pick[2];
-    __shared__ uint32_t part[2][kTopWaves];
+__device__ __forceinline__ void top_pages(const SelectArgs& a, const float* score, int32_t* to, uint32_t n,
+                                          uint32_t (&hist)[2][kBins], uint32_t (&pick)[3], uint32_t (&part)[2][kTopWaves]) {
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint32_t lo = a.first, hi = n - a.recent;  // the others stay; n > keep >= first + recent
     const bool held = n <= uint32_t(N * kTopT);
-    uint32_t key[N];
-    auto load = [&](uint32_t i0) {  // 0 for those that are no candidates
+    uint32_t key[N], least = 0;
+    auto load = [&](uint32_t i0) {
+        const uint32_t p = i0 + uint32_t(tid * N);
+        if constexpr (N % 4 == 0) {  // (within the pitch; what lies behind the scores is not looked at)
 #pragma unroll
-        for (int j = 0; j < N; ++j) {
-            const uint32_t p = i0 + uint32_t(tid * N + j);
-            key[j] = score_key(score[min(p, n - 1)]);
+            for (int j = 0; j < N; j += 4) {
+                const float4 x = *reinterpret_cast<const float4*>(score + min(p + j, a.pitch - 4));
+                key[j] = score_key(x.x) - least, key[j + 1] = score_key(x.y) - least;
+                key[j + 2] = score_key(x.z) - least, key[j + 3] = score_key(x.w) - least;
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < N; ++j) key[j] = score_key(score[min(p + j, n - 1)]) - least;
         }
     };
-    auto each = [&](auto f) {  // f(key, page) of every candidate
+    auto each = [&](auto f) {  // f(key) of every candidate
         for (uint32_t i0 = 0; i0 < n; i0 += N * kTopT) {
             if (!held) load(i0);
 #pragma unroll
@@ -197,25 +205,32 @@ __device__ __forceinline__ void top_pages(const SelectArgs& a, const float* scor
         }
     };
     if (held) load(0);
-    uint32_t want = a.keep - a.first - a.recent, above = 0xffffffffu;  // above: keys past it stay
+    // of the candidates, those from `top` on stay, and the first `want` of those from `at` on below it
+    uint32_t want = a.keep - a.first - a.recent, at = 0xffffffffu, top = 0xffffffffu;
     if (want) {
-        uint32_t least = 0xffffffffu, most = 0;
+        uint32_t low = 0xffffffffu, most = 0;
         each([&](uint32_t k) {
-            least = min(least, k);
+            low = min(low, k);
             most = max(most, k);
         });
 #pragma unroll
         for (int m = 1; m < 64; m *= 2) {
-            least = min(least, uint32_t(__shfl_xor(int(least), m)));
+            low = min(low, uint32_t(__shfl_xor(int(low), m)));
             most = max(most, uint32_t(__shfl_xor(int(most), m)));
         }
-        if (lane == 0) part[0][wave] = least, part[1][wave] = most;
+        if (lane == 0) part[0][wave] = low, part[1][wave] = most;
         hist[0][tid] = hist[0][tid + kTopT] = 0;
         __syncthreads();
-        for (int w = 0; w < kTopWaves; ++w) least = min(least, part[0][w]), most = max(most, part[1][w]);
-        int bits = 32 - __clz(int(least ^ most));  // that differ (0: all are equal)
-        uint32_t prefix = bits < 32 ? (most >> bits) << bits : 0u;
-        for (int d = 0; bits > 0; ++d) {
+#pragma unroll
+        for (int w = 0; w < kTopWaves; ++w) low = min(low, part[0][w]), most = max(most, part[1][w]);
+        least = low;
+        if (held)
+#pragma unroll
+            for (int j = 0; j < N; ++j) key[j] -= least;
+        int bits = 32 - __clz(int(most - low));  // of the largest key (0: all are equal)
+        uint32_t prefix = 0;
+        bool all_stay = false;
+        for (int d = 0; bits > 0 && !all_stay; ++d) {
             const int shift = max(bits - 11, 0);
             uint32_t* bins = hist[d & 1];
             const uint64_t up = uint64_t(prefix) >> bits;
@@ -230,41 +245,47 @@ __device__ __forceinline__ void top_pages(const SelectArgs& a, const float* scor
             uint32_t before = wave_before_sat(h0 + h1, all);
             if (lane == 0) part[0][wave] = all;
             __syncthreads();
-            for (int w = 0; w < wave; ++w) before += part[0][w];
+#pragma unroll
+            for (int w = 0; w < kTopWaves; ++w) before += w < wave ? part[0][w] : 0u;
             if (before < want && want <= before + h0) {
                 pick[0] = uint32_t(kBins - 1 - 2 * tid);
                 pick[1] = want - before;
+                pick[2] = h0;
             } else if (before + h0 < want && want <= before + h0 + h1) {
                 pick[0] = uint32_t(kBins - 2 - 2 * tid);
                 pick[1] = want - before - h0;
+                pick[2] = h1;
             }
             __syncthreads();
             prefix |= pick[0] << shift;
             want = pick[1];
+            all_stay = pick[2] == want;
             bits = shift;
         }
-        above = prefix;
+        at = prefix;
+        top = all_stay ? prefix : prefix + 1;  // (a key is below 2^32 - 1: the largest score's is)
     }
     // pages that stay, in order: those held anyway, those above, and the first `want` at it
     uint32_t done = 0, equal = 0;
     for (uint32_t i0 = 0; i0 < n; i0 += N * kTopT) {
         if (!held) load(i0);
-        uint32_t sure = 0, at = 0;
+        uint32_t sure = 0, some = 0;
 #pragma unroll
         for (int j = 0; j < N; ++j) {
             const uint32_t p = i0 + uint32_t(tid * N + j);
             if (p < n) {
                 const bool must = p < lo || p >= hi;
-                sure += must || key[j] > above;
-                at += !must && key[j] == above;
+                sure += must || key[j] >= top;
+                some += !must && key[j] >= at && key[j] < top;
             }
         }
         uint32_t all_s, all_e;
-        uint32_t bs = wave_before_sat(sure, all_s), be = wave_before_sat(at, all_e);
+        uint32_t bs = wave_before_sat(sure, all_s), be = wave_before_sat(some, all_e);
         __syncthreads();
         if (lane == 0) part[0][wave] = all_s, part[1][wave] = all_e;
         __syncthreads();
         uint32_t ts = 0, te = 0;
+#pragma unroll
         for (int w = 0; w < kTopWaves; ++w) {
             if (w == wave) bs += ts, be += te;
             ts += part[0][w];
@@ -276,10 +297,9 @@ __device__ __forceinline__ void top_pages(const SelectArgs& a, const float* scor
         for (int j = 0; j < N; ++j) {
             const uint32_t p = i0 + uint32_t(tid * N + j);
             if (p < n) {
-                const bool must = p < lo || p >= hi, eq = !must && key[j] == above;
-                const uint32_t place = bs + min(be, want);
-                if (must || key[j] > above || (eq && be < want)) to[place] = int32_t(p);
-                bs += must || key[j] > above;
+                const bool must = p < lo || p >= hi, yes = must || key[j] >= top, eq = !yes && key[j] >= at;
+                if (yes || (eq && be < want)) to[bs + min(be, want)] = int32_t(p);
+                bs += yes;
                 be += eq;
             }
         }
@@ -298,10 +318,13 @@ __global__ __launch_bounds__(kTopT) void page_top_kernel(SelectArgs a) {
         for (uint32_t j = threadIdx.x; j < a.keep; j += kTopT) to[j] = j < n ? int32_t(j) : -1;
         return;
     }
-    const float* score = a.score + size_t(pair) * a.width;
-    if (n <= kTopT) top_pages<1>(a, score, to, n);
-    else if (n <= 4 * kTopT) top_pages<4>(a, score, to, n);
-    else top_pages<8>(a, score, to, n);
+    const float* score = a.score + size_t(pair) * a.pitch;
+    __shared__ uint32_t hist[2][kBins];
+    __shared__ uint32_t pick[3];
+    __shared__ uint32_t part[2][kTopWaves];
+    if (n <= kTopT) top_pages<1>(a, score, to, n, hist, pick, part);
+    else if (n <= 4 * kTopT) top_pages<4>(a, score, to, n, hist, pick, part);
+    else top_pages<8>(a, score, to, n, hist, pick, part);
 }
 
 uint32_t score_shares(const zq_kv_paged& c, const zq_page_tables& t, size_t queries) {
@@ -310,8 +333,9 @@ uint32_t score_shares(const zq_kv_paged& c, const zq_page_tables& t, size_t quer
     return uint32_t(most < 1024 ? most : 1024);
 }
 
+uint32_t pitch_of(const zq_page_tables& t) { return uint32_t(t.width + 3) / 4 * 4; }
 size_t select_bytes(const zq_kv_paged& c, const zq_page_tables& t, size_t queries) {
-    return (queries * c.kv_heads * t.width * 4 + 255) / 256 * 256;
+    return (queries * c.kv_heads * pitch_of(t) * 4 + 255) / 256 * 256;
 }
 
 template <int D>
@@ -360,6 +384,7 @@ int zq_hip_page_select_dev(const zq_kv_paged* cache, const zq_page_tables* table
              flags & ZQ_ATTN_PAGED_FULL};
     a.stride = stride;
     a.width = uint32_t(tables->width);
+    a.pitch = zq::pitch_of(*tables);
     a.pages = uint32_t(tables->pages);
     a.KH = uint32_t(cache->kv_heads);
     a.G = uint32_t(heads / cache->kv_heads);

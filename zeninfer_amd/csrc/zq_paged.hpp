@@ -74,18 +74,35 @@ __device__ __forceinline__ int bound_code(float x) { return int(fminf(fmaxf(x, -
 // ---- even shares of uneven work ------------------------------------------------
 // Query i has units(i) units of work for each of `mult` kv heads (0 where it is idle);
 // the units of all, one behind the other, are cut into equal shares, one a workgroup,
-// whatever the lengths are.  Every workgroup of 256 takes the sums by itself.
+// whatever the lengths are.  Every workgroup of 256 takes the sums by itself, and holds
+// what the queries see in LDS where they are few: what follows then waits for no memory.
 constexpr int kShareT = 256, kShareWaves = kShareT / 64;
+constexpr uint32_t kSeenHeld = 1024;
+struct ShareScan {
+    int32_t seq[kSeenHeld];
+    uint32_t rows[kSeenHeld];
+    uint32_t part[kShareWaves];
+    uint32_t query, before;
+};
 struct Shares {
     uint32_t units;  // of all queries, for one kv head
     uint64_t all;    // of all kv heads
     uint32_t used;   // workgroups that have a share
 };
 __device__ __forceinline__ uint64_t share_start(const Shares& s, uint32_t w) { return uint64_t(w) * s.all / s.used; }
-struct ShareScan {
-    uint32_t part[kShareWaves];
-    uint32_t query, before;
-};
+__device__ __forceinline__ void hold_seen(const Queries& a, ShareScan& sh) {
+    if (a.n > kSeenHeld) return;
+    for (uint32_t i = threadIdx.x; i < a.n; i += kShareT) {
+        const Seen x = seen_by(a, i);
+        sh.seq[i] = x.seq;
+        sh.rows[i] = x.rows;
+    }
+    __syncthreads();
+}
+__device__ __forceinline__ Seen seen_held(const Queries& a, const ShareScan& sh, uint32_t i) {
+    if (a.n > kSeenHeld) return seen_by(a, i);
+    return {sh.seq[i], sh.rows[i]};
+}
 // The sums; mine: before this thread's queries (t * each ...), own: of them.
 template <class F>
 __device__ __forceinline__ Shares scan_units(uint32_t n, uint32_t mult, uint32_t W, F units, ShareScan& sh, uint32_t& mine,
@@ -105,7 +122,10 @@ __device__ __forceinline__ Shares scan_units(uint32_t n, uint32_t mult, uint32_t
     }
     s.units = uint32_t(__builtin_amdgcn_readfirstlane(int(s.units)));  // one for the workgroup
     s.all = uint64_t(s.units) * mult;
-    s.used = uint32_t(min(uint64_t(W), s.all));
+    // few units: a workgroup a CU, and more of them only where each has kFew units to itself (a share's start and what
+    // it leaves to be joined cost as much as several units; 100,000 rows of one kv head: 23 us so, 37 with a unit each)
+    constexpr uint32_t kFew = 6, kCUs = 256;
+    s.used = uint32_t(min(min(uint64_t(W), s.all), max(uint64_t(kCUs), s.all / kFew)));
     return s;
 }
 // The query that has unit x (< all) of all kv heads, and the units of one kv head before it.
@@ -129,6 +149,12 @@ __device__ __forceinline__ Found find_query(uint32_t n, uint32_t mult, F units, 
     __syncthreads();
     return {uint32_t(__builtin_amdgcn_readfirstlane(int(sh.query))), uint32_t(__builtin_amdgcn_readfirstlane(int(sh.before)))};
 }
+// A read of bytes that no other workgroup reads: they need not stay in a cache.
+template <class V>
+__device__ __forceinline__ V load_once(const void* p) {
+    return __builtin_nontemporal_load(reinterpret_cast<const V*>(p));
+}
+__device__ __forceinline__ uint32_t uniform(uint32_t x) { return uint32_t(__builtin_amdgcn_readfirstlane(int(x))); }
 #endif
 
 }  // namespace zq

@@ -634,7 +634,7 @@ def kv_q4_bytes(kv_heads, head_dim, capacity):
     return lib().zq_kv_q4_bytes(kv_heads, head_dim, capacity)
 
 
-_KINDS = {"float32": set(), "float16": set(), "int32": set(), "int": set()}  # torch's types found to be of a kind
+_KINDS = {"float32": set(), "float16": set(), "int32": set(), "int": set(), "int64": set()}  # torch's types found to be of a kind
 
 
 def _need_kind(t, kind, what):
@@ -647,7 +647,8 @@ def _need_kind(t, kind, what):
     size, floating = t.element_size(), t.is_floating_point()
     integer = not floating and not t.is_complex()
     if not (integer and size == 1 or {"float32": floating and size == 4, "int32": integer and size == 4, "int": integer,
-                                      "float16": integer or str(t.dtype) == "torch.float16"}[kind]):
+                                      "float16": integer or str(t.dtype) == "torch.float16",
+                                      "int64": integer and size == 8}[kind]):
         raise ValueError(f"{what}: needs {kind}, got {t.dtype}")
     _KINDS[kind].add(t.dtype)
 
@@ -777,12 +778,27 @@ def kv_q4_evict_dev(cache, lens, keep, recent, first, next_pos=None, dst=None, w
 _PAGED_TYPES = {"torch.float32": (KV_F32, 4), "torch.float16": (KV_F16, 2), "torch.bfloat16": (KV_BF16, 2)}
 
 
-def _need_long(t, n, what, dev):
-    """Device address of n int64 values."""
-    if t is not None and not isinstance(t, int) and hasattr(t, "element_size") and (
-            t.element_size() != 8 or t.is_floating_point()):
-        raise ValueError(f"{what}: needs int64, got {t.dtype}")
-    return _need(t, 8 * n, what, dev)
+_SIZES = {"float32": 4, "int32": 4, "int64": 8}
+
+
+def _need_of(t, n, kind, what, dev):
+    """Device address of n values of the kind.  One pass of cheap queries where all is well: at decode sizes these calls
+    take as long as the kernels that they launch."""
+    if t is None:
+        return None
+    nbytes = n * _SIZES[kind]
+    try:
+        if t.dtype in _KINDS[kind] and t.get_device() == dev and 0 <= nbytes <= t.nbytes and t.is_contiguous():
+            return t.data_ptr()
+    except AttributeError:  # an address, or no tensor
+        pass
+    _need_kind(t, kind, what)
+    return _need(t, nbytes, what, dev)
+
+
+def _need_queries(t, rows, stride, width, what, dev):
+    """Device address of [rows][stride] fp32, a view of columns with a stride (as _need_rows)."""
+    return _need_rows(t, 1, rows, stride, width, what, dev) if stride else _need_of(t, rows * width, "float32", what, dev)
 
 
 class PageTables:
@@ -794,8 +810,8 @@ class PageTables:
         if min(seqs, width, pages, page_size) < 0:
             raise ValueError(f"PageTables: a size below zero (seqs {seqs}, width {width}, pages {pages}, page_size {page_size})")
         dev = self.dev = _device_index()
-        self.c = PageTablesC(_need_ints(table, seqs * width, "PageTables table", dev),
-                             _need_ints(free_pages, pages, "PageTables free_pages", dev), seqs, width, pages, page_size)
+        self.c = PageTablesC(_need_of(table, seqs * width, "int32", "PageTables table", dev),
+                             _need_of(free_pages, pages, "int32", "PageTables free_pages", dev), seqs, width, pages, page_size)
         self.arrays = [table, free_pages]
         self.seqs, self.width, self.pages, self.page_size = seqs, width, pages, page_size
         self.ref = ctypes.byref(self.c)
@@ -841,15 +857,15 @@ def page_tables_step_dev(tables, lens, counts, free_count, free_left, granted, s
     """Pages for counts [seqs] new tokens behind lens [seqs] held ones; slots, positions and seq_of [tokens] of the
     packed new tokens (positions and seq_of may be None), start [seqs + 1], granted [seqs]."""
     dev, n = tables.dev, tables.seqs
-    lens = _need_ints(lens, n, "page_tables_step_dev lens", dev)
-    counts = _need_ints(counts, n, "page_tables_step_dev counts", dev)
-    free_count = _need_ints(free_count, 1, "page_tables_step_dev free_count", dev)
-    free_left = _need_ints(free_left, 1, "page_tables_step_dev free_left", dev)
-    granted = _need_ints(granted, n, "page_tables_step_dev granted", dev)
-    start = _need_ints(start, n + 1, "page_tables_step_dev start", dev)
-    slots = _need_long(slots, tokens, "page_tables_step_dev slots", dev)
-    positions = _need_ints(positions, tokens, "page_tables_step_dev positions", dev)
-    seq_of = _need_ints(seq_of, tokens, "page_tables_step_dev seq_of", dev)
+    lens = _need_of(lens, n, "int32", "page_tables_step_dev lens", dev)
+    counts = _need_of(counts, n, "int32", "page_tables_step_dev counts", dev)
+    free_count = _need_of(free_count, 1, "int32", "page_tables_step_dev free_count", dev)
+    free_left = _need_of(free_left, 1, "int32", "page_tables_step_dev free_left", dev)
+    granted = _need_of(granted, n, "int32", "page_tables_step_dev granted", dev)
+    start = _need_of(start, n + 1, "int32", "page_tables_step_dev start", dev)
+    slots = _need_of(slots, tokens, "int64", "page_tables_step_dev slots", dev)
+    positions = _need_of(positions, tokens, "int32", "page_tables_step_dev positions", dev)
+    seq_of = _need_of(seq_of, tokens, "int32", "page_tables_step_dev seq_of", dev)
     return check(lib().zq_hip_page_tables_step_dev(tables.ref, lens, counts, free_count, free_left, granted, start, slots,
                                                    positions, seq_of, tokens, _stream(stream)),
                  "zq_hip_page_tables_step_dev")
@@ -858,10 +874,10 @@ def page_tables_step_dev(tables, lens, counts, free_count, free_left, granted, s
 def page_tables_release_dev(tables, lens, keep, free_count, free_left, stream=None):
     """Gives back the pages that sequences of lens [seqs] tokens do not need for their first keep [seqs]."""
     dev, n = tables.dev, tables.seqs
-    lens = _need_ints(lens, n, "page_tables_release_dev lens", dev)
-    keep = _need_ints(keep, n, "page_tables_release_dev keep", dev)
-    free_count = _need_ints(free_count, 1, "page_tables_release_dev free_count", dev)
-    free_left = _need_ints(free_left, 1, "page_tables_release_dev free_left", dev)
+    lens = _need_of(lens, n, "int32", "page_tables_release_dev lens", dev)
+    keep = _need_of(keep, n, "int32", "page_tables_release_dev keep", dev)
+    free_count = _need_of(free_count, 1, "int32", "page_tables_release_dev free_count", dev)
+    free_left = _need_of(free_left, 1, "int32", "page_tables_release_dev free_left", dev)
     return check(lib().zq_hip_page_tables_release_dev(tables.ref, lens, keep, free_count, free_left, _stream(stream)),
                  "zq_hip_page_tables_release_dev")
 
@@ -869,9 +885,9 @@ def page_tables_release_dev(tables, lens, keep, free_count, free_left, stream=No
 def kv_paged_append_dev(cache, k, v, tokens, slots, stride=0, stream=None):
     """Keys and values [tokens][stride] fp32 into slots [tokens] (int64)."""
     dev, width = cache.dev, cache.kv_heads * cache.head_dim
-    k = _need_rows(k, 1, tokens, stride, width, "kv_paged_append_dev k", dev)
-    v = _need_rows(v, 1, tokens, stride, width, "kv_paged_append_dev v", dev)
-    slots = _need_long(slots, tokens, "kv_paged_append_dev slots", dev)
+    k = _need_queries(k, tokens, stride, width, "kv_paged_append_dev k", dev)
+    v = _need_queries(v, tokens, stride, width, "kv_paged_append_dev v", dev)
+    slots = _need_of(slots, tokens, "int64", "kv_paged_append_dev slots", dev)
     return check(lib().zq_hip_kv_paged_append_dev(cache.ref, k, v, tokens, stride, slots, _stream(stream)),
                  "zq_hip_kv_paged_append_dev")
 
@@ -885,12 +901,12 @@ def attention_paged_dev(cache, tables, q, out, queries, heads, lens, scale, coun
     """Attention of q [queries][stride] over the pages of their sequences (of select [queries][kv_heads][keep] only) into
     out [queries][heads * head_dim]."""
     dev, width = cache.dev, heads * cache.head_dim
-    q = _need_rows(q, 1, queries, stride, width, "attention_paged_dev q", dev)
-    out = _need_f32(out, queries * width, "attention_paged_dev out", dev)
-    lens = _need_ints(lens, queries, "attention_paged_dev lens", dev)
-    counts = _need_ints(counts, queries, "attention_paged_dev counts", dev)
-    seq_of = _need_ints(seq_of, queries, "attention_paged_dev seq_of", dev)
-    select = _need_ints(select, queries * cache.kv_heads * keep, "attention_paged_dev select", dev)
+    q = _need_queries(q, queries, stride, width, "attention_paged_dev q", dev)
+    out = _need_of(out, queries * width, "float32", "attention_paged_dev out", dev)
+    lens = _need_of(lens, queries, "int32", "attention_paged_dev lens", dev)
+    counts = _need_of(counts, queries, "int32", "attention_paged_dev counts", dev)
+    seq_of = _need_of(seq_of, queries, "int32", "attention_paged_dev seq_of", dev)
+    select = _need_of(select, queries * cache.kv_heads * keep, "int32", "attention_paged_dev select", dev)
     workspace = _need(workspace, workspace_bytes, "attention_paged_dev workspace", dev)
     return check(lib().zq_hip_attention_paged_dev(cache.ref, tables.ref, q, out, queries, heads, stride, seq_of, lens,
                                                   counts, select, keep, scale, flags, workspace, workspace_bytes,
@@ -908,11 +924,11 @@ def page_select_dev(cache, tables, q, select, queries, heads, lens, keep, recent
     dev = cache.dev
     if min(keep, recent, first) < 0:
         raise ValueError(f"page_select_dev: a number of pages below zero (keep {keep}, recent {recent}, first {first})")
-    q = _need_rows(q, 1, queries, stride, heads * cache.head_dim, "page_select_dev q", dev)
-    select = _need_ints(select, queries * cache.kv_heads * keep, "page_select_dev select", dev)
-    lens = _need_ints(lens, queries, "page_select_dev lens", dev)
-    counts = _need_ints(counts, queries, "page_select_dev counts", dev)
-    seq_of = _need_ints(seq_of, queries, "page_select_dev seq_of", dev)
+    q = _need_queries(q, queries, stride, heads * cache.head_dim, "page_select_dev q", dev)
+    select = _need_of(select, queries * cache.kv_heads * keep, "int32", "page_select_dev select", dev)
+    lens = _need_of(lens, queries, "int32", "page_select_dev lens", dev)
+    counts = _need_of(counts, queries, "int32", "page_select_dev counts", dev)
+    seq_of = _need_of(seq_of, queries, "int32", "page_select_dev seq_of", dev)
     workspace = _need(workspace, workspace_bytes, "page_select_dev workspace", dev)
     return check(lib().zq_hip_page_select_dev(cache.ref, tables.ref, q, select, queries, heads, stride, seq_of, lens, counts,
                                               keep, recent, first, flags, workspace, workspace_bytes, _stream(stream)),

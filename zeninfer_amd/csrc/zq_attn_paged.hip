@@ -48,6 +48,9 @@ struct AttnPaged {
 // units more, which count as units without keys at its start.
 constexpr int kT = kShareT, kWaves = kShareWaves;
 constexpr uint32_t kStart = 2;
+// More workgroups than CUs only where each has this many units: 100,000 rows of one kv head take 23 us so, 37 with a unit
+// each (768 partials to join).
+constexpr uint32_t kFew = 6;
 template <int TYPE>
 struct Tile {
     static constexpr int kKeys = TYPE == ZQ_KV_F32 ? 16 : 32;  // keys of a wave's tile
@@ -237,28 +240,337 @@ __device__ __forceinline__ V load_held(const uint8_t* p) {
 // in one page: its place is one readlane of the table entries that the wave loaded, 64
 // parts at once.  The next tile's K is asked for when this one's scores are there, the
 // next V when this one is used.
-template <int TYPE, int D, bool GROUP>
-__global__ __launch_bounds__(kT, D == 64 ? 4 : D == 128 ? 3 : 2) void attn_paged_kernel(AttnPaged a) {
+// One (query or group, kv head) pair, or the units u0 .. u1 of it, by a workgroup.
+// whole: straight into the output; else into partial `slot`.
+template <int TYPE, int D, bool GROUP, class F>
+__device__ __forceinline__ void attend(const AttnPaged& a, float* dyn, float (&sm)[kWaves][16], float (&sl)[kWaves][16], uint32_t qi,
+                                       uint32_t kh, const Group& x, uint32_t row0, uint32_t u0, uint32_t u1, bool whole,
+                                       size_t slot, F rows_of) {
     using S = Shape<TYPE, D>;
     constexpr int H = S::H, KC = S::KC, VE = S::VE, VC = S::VC, VW = S::VW, VR = S::VR, NP = S::NP;
-    extern __shared__ float dyn[];  // [4 waves][rows][D + 4], then q's operands
-    __shared__ ShareScan scan;
-    __shared__ float sm[kWaves][16], sl[kWaves][16];
     const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const size_t head_rows = size_t(1) << a.lp;
+    v4u_t* held_q = reinterpret_cast<v4u_t*>(dyn + kWaves * a.RL * (D + 4));  // q's operands [KC][NP][64]
+    const uint32_t R = GROUP ? x.queries * a.G : min(a.G - row0, 16u);  // rows: query, head
+    const uint32_t entries = entries_of(a, x.most);
+    const uint32_t parts = a.select ? entries << (a.lp - 4) : (x.most + 15) >> 4;  // 16-key parts of the pair
+    const uint32_t tiles = (parts + H - 1) / H;
+    const uint32_t t0 = u0 * kWaves + wave, t1 = min(u1 * kWaves, tiles);
+    const uint32_t nt = t0 < t1 ? (t1 - t0 + kWaves - 1) / kWaves : 0;  // tiles of this wave
+    const int32_t* table = a.table + size_t(x.first.seq) * a.width;
+    const int32_t* select = a.select ? a.select + (size_t(qi) * a.KH + kh) * a.keep : nullptr;
+
+    // ---- the wave's tiles ----
+    v4u_t kt[H][KC];
+    uint32_t vt[VR][VC][VW];
+    uint32_t place = 0;  // lane p: page | rows there << 24 of the p-th part that the wave has ahead
+    // byte offset of the wave's part p (of 64) from the cache's start
+    auto part_at = [&](uint32_t p, uint32_t part) {
+        const uint32_t page = uint32_t(__builtin_amdgcn_readlane(int(place), int(p))) & 0xffffffu;
+        const uint32_t in = (part << 4) & (uint32_t(head_rows) - 1);
+        return ((size_t(page) * a.KH + kh) * head_rows + in) * (D * S::ES);
+    };
+    auto rows_at = [&](uint32_t p) { return uint32_t(__builtin_amdgcn_readlane(int(place), int(p))) >> 24; };
+    constexpr uint32_t kBatch = 64 / H;  // tiles whose places a wave holds
+    uint32_t b = 0;  // the first tile of the batch
+    auto load_places = [&] {
+        const uint32_t j = b + lane / H, part = (t0 + j * kWaves) * H + lane % H, e = part >> (a.lp - 4);
+        place = 0;
+        if (j < nt && e < entries) {
+            const uint32_t y = select ? uint32_t(select[e]) : e;  // place in the sequence
+            if (y < a.width && (y << a.lp) < x.most) {
+                const uint32_t page = uint32_t(table[y]);
+                const uint32_t first = (y << a.lp) + ((part << 4) & (uint32_t(head_rows) - 1));
+                if (page < a.pages && first < x.most) place = page | min(x.most - first, 16u) << 24;
+            }
+        }
+    };
+    auto load_k = [&](uint32_t j) {
+#pragma unroll
+        for (int h = 0; h < H; ++h) {
+            const uint8_t* p = a.k + part_at(j * H + h, (t0 + (b + j) * kWaves) * H + h);
+#pragma unroll
+            for (int k = 0; k < KC; ++k)
+                kt[h][k] = load_held<GROUP, v4u_t>(p + uint32_t(i * D * S::ES + k * 64 + g * 16));
+        }
+    };
+    auto load_v = [&](uint32_t j) {
+#pragma unroll
+        for (int h = 0; h < H; ++h) {
+            const uint8_t* p = a.v + part_at(j * H + h, (t0 + (b + j) * kWaves) * H + h);
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+#pragma unroll
+                for (int n = 0; n < VC; ++n) {
+                    const uint8_t* at = p + uint32_t((4 * g + r) * D * S::ES + (n * 16 + i) * VE * S::ES);
+                    if constexpr (VW == 4) {
+                        const v4u_t w = load_held<GROUP, v4u_t>(at);
+#pragma unroll
+                        for (int z = 0; z < 4; ++z) vt[h * 4 + r][n][z] = w[z];
+                    } else {
+                        const v2u_t w = load_held<GROUP, v2u_t>(at);
+                        vt[h * 4 + r][n][0] = w[0];
+                        vt[h * 4 + r][n][1] = w[1];
+                    }
+                }
+        }
+    };
+    load_places();
+
+    // ---- the queries as operands ----
+    const uint32_t row = min(uint32_t(i), R - 1), member = GROUP ? row / a.G : 0u;
+    const float* qrow = a.q + (qi + member) * a.stride + (size_t(kh) * a.G + row0 + row - member * a.G) * D;
+    const uint32_t my_rows = GROUP ? rows_of(qi + member) : 0u;  // that this lane's query sees
+    float c = a.scale2;  // takes a score into log2 units
+    float4 x0[KC][TYPE == ZQ_KV_F32 ? 1 : 2];
+    float most = 0.0f;
+#pragma unroll
+    for (int k = 0; k < KC; ++k)
+#pragma unroll
+        for (int j = 0; j < (TYPE == ZQ_KV_F32 ? 1 : 2); ++j) {
+            float4 y = *reinterpret_cast<const float4*>(qrow + (4 * k + g) * (TYPE == ZQ_KV_F32 ? 4 : 8) + 4 * j);
+            if (uint32_t(i) >= R) y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            x0[k][j] = y;
+            most = fmaxf(most, fmaxf(fmaxf(fabsf(y.x), fabsf(y.y)), fmaxf(fabsf(y.z), fabsf(y.w))));
+        }
+    // (asked for behind the queries, which are waited for first; a wave without tiles reads rows of page 0)
+    load_k(0);
+    load_v(0);
+    float up = 1.0f;
+    if constexpr (TYPE == ZQ_KV_F16) {  // the row's largest element to 2^14 .. 2^15
+        most = max_groups(most);
+        if (most > 0.0f) {
+            const int e = min(max(15 - __builtin_amdgcn_frexp_expf(most), -113), 126);
+            up = pow2f(e);
+            c *= pow2f(-e);
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < KC; ++k) {
+        v4u_t op[NP];
+        if constexpr (TYPE == ZQ_KV_F32) {
+            op[0] = v4u_t{f_bits(x0[k][0].x), f_bits(x0[k][0].y), f_bits(x0[k][0].z), f_bits(x0[k][0].w)};
+        } else {
+            Parts<TYPE> p;
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                p.set2(4 * j, x0[k][j].x * up, x0[k][j].y * up);
+                p.set2(4 * j + 2, x0[k][j].z * up, x0[k][j].w * up);
+            }
+#pragma unroll
+            for (int n = 0; n < NP; ++n) op[n] = p.bits(n);
+        }
+        if (k % kWaves == wave)
+#pragma unroll
+            for (int n = 0; n < NP; ++n) held_q[(k * NP + n) * 64 + lane] = op[n];
+    }
+    __syncthreads();
+
+    v4f_t o[VC][VE];
+#pragma unroll
+    for (int n = 0; n < VC; ++n)
+#pragma unroll
+        for (int e = 0; e < VE; ++e) o[n][e] = v4f_t{0.0f, 0.0f, 0.0f, 0.0f};
+    float m = -INFINITY, l = 0.0f;
+    auto step = [&](uint32_t j, auto last) {
+        v4f_t s[H];
+#pragma unroll
+        for (int h = 0; h < H; ++h) s[h] = v4f_t{0.0f, 0.0f, 0.0f, 0.0f};
+        asm volatile("" ::: "memory");  // q is read again, not held
+#pragma unroll
+        for (int k = 0; k < KC; ++k) {
+            v4u_t op[NP];
+#pragma unroll
+            for (int n = 0; n < NP; ++n) op[n] = held_q[(k * NP + n) * 64 + lane];
+#pragma unroll
+            for (int h = 0; h < H; ++h) {
+                if constexpr (TYPE == ZQ_KV_F32) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        s[h] = __builtin_amdgcn_mfma_f32_16x16x4f32(bits_f(kt[h][k][e]), bits_f(op[0][e]), s[h], 0, 0, 0);
+                } else {
+#pragma unroll
+                    for (int n = NP - 1; n >= 0; --n) s[h] = mma<TYPE>(kt[h][k], op[n], s[h]);
+                }
+            }
+        }
+        uint32_t rows[H];
+        bool cut = false;
+#pragma unroll
+        for (int h = 0; h < H; ++h) {
+            rows[h] = rows_at(j * H + h);
+            cut |= rows[h] < 16;
+            if (GROUP) cut |= (((t0 + (b + j) * kWaves) * H + h) << 4) + 16 > x.least;
+        }
+        if constexpr (!decltype(last)::value) load_k(j + 1);
+#pragma unroll
+        for (int h = 0; h < H; ++h) s[h] *= c;
+        if (cut) {  // uniform
+#pragma unroll
+            for (int h = 0; h < H; ++h) {
+                uint32_t n = rows[h];
+                if (GROUP) n = min(n, uint32_t(max(int32_t(my_rows - (((t0 + (b + j) * kWaves) * H + h) << 4)), 0)));
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    if (uint32_t(4 * g + r) >= n) s[h][r] = -INFINITY;
+            }
+        }
+        float most = -INFINITY;
+#pragma unroll
+        for (int h = 0; h < H; ++h)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) most = fmaxf(most, s[h][r]);
+        if (__any(most > m + kSlack)) {
+            const float to = fmaxf(m, max_groups(most));
+            const float f = to == -INFINITY ? 1.0f : exp2_(m - to);
+            m = to;
+            l *= f;
+#pragma unroll
+            for (int n = 0; n < VC; ++n)
+#pragma unroll
+                for (int e = 0; e < VE; ++e) o[n][e] *= f;
+        }
+        const float ms = (m == -INFINITY ? 0.0f : m) - kShift;
+        float p[VR];
+#pragma unroll
+        for (int h = 0; h < H; ++h)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                p[h * 4 + r] = exp2_(s[h][r] - ms);
+                l += p[h * 4 + r];
+            }
+        if (cut) {
+#pragma unroll
+            for (int h = 0; h < H; ++h)
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    if (uint32_t(4 * g + r) >= rows[h])
+#pragma unroll
+                        for (int n = 0; n < VC; ++n)
+#pragma unroll
+                            for (int z = 0; z < VW; ++z) vt[h * 4 + r][n][z] = 0;
+        }
+        const Weights<TYPE, VR> pw(p);
+        if (GROUP && cut && x.least < x.most) {
+            // a value that is no number must not reach (0 times it) the queries that do not see its row
+            bool odd = false;
+#pragma unroll
+            for (int r = 0; r < VR; ++r)
+#pragma unroll
+                for (int n = 0; n < VC; ++n)
+#pragma unroll
+                    for (int z = 0; z < VW; ++z) odd |= not_finite<TYPE>(vt[r][n][z]);
+            if (__any(odd)) {
+                // per element: how many such values a query sees; more than none gives NaN
+                float sees[VR];
+#pragma unroll
+                for (int r = 0; r < VR; ++r)
+                    sees[r] = (((t0 + (b + j) * kWaves) * H + r / 4) << 4) + 4 * g + r % 4 < my_rows ? 1.0f : 0.0f;
+                const Weights<TYPE, VR> ps(sees);
+#pragma unroll
+                for (int n = 0; n < VC; ++n)
+#pragma unroll
+                    for (int z = 0; z < VW; ++z) {
+                        uint32_t w[VR][1][1];
+#pragma unroll
+                        for (int r = 0; r < VR; ++r) {
+                            w[r][0][0] = take_odd<TYPE>(vt[r][n][z]);
+                        }
+#pragma unroll
+                        for (int e = 0; e < VE / VW; ++e) {
+                            const v4f_t y = add_pv<TYPE, VR, 1, 1, 1>(w, ps, 0, e, v4f_t{0.0f, 0.0f, 0.0f, 0.0f});
+                            v4f_t& to = o[n][z * (VE / VW) + e];
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) to[k] = y[k] > 0.0f ? NAN : to[k];
+                        }
+                    }
+            }
+        }
+#pragma unroll
+        for (int n = 0; n < VC; ++n)
+#pragma unroll
+            for (int e = 0; e < VE; ++e) o[n][e] = add_pv<TYPE, VR, VC, VW>(vt, pw, n, e, o[n][e]);
+        if constexpr (!decltype(last)::value) load_v(j + 1);
+    };
+    while (b < nt) {
+        const uint32_t count = min(nt - b, kBatch);
+        for (uint32_t j = 0; j + 1 < count; ++j) step(j, std::false_type{});
+        step(count - 1, std::true_type{});
+        b += kBatch;
+        if (b < nt) {
+            load_places();
+            load_k(0);
+            load_v(0);
+        }
+    }
+
+    // ---- the four waves' sums as one ----
+    uint32_t ln = threadIdx.x;
+    asm volatile("" : "+v"(ln));  // the addresses below are made here, not held through the tiles
+    const uint32_t mi = ln & 15, mg = (ln >> 4) & 3;
+    l = sum_groups(l);
+    if (mg == 0) {
+        sm[wave][mi] = m;
+        sl[wave][mi] = l;
+    }
+    if (mi < R) {
+        float* to = dyn + (size_t(wave) * a.RL + mi) * (D + 4);
+#pragma unroll
+        for (int n = 0; n < VC; ++n)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+#pragma unroll
+                for (int e = 0; e < VE; e += 4)
+                    *reinterpret_cast<float4*>(to + n * 16 * VE + VE * (4 * mg + r) + e) =
+                        make_float4(o[n][e][r], o[n][e + 1][r], o[n][e + 2][r], o[n][e + 3][r]);
+    }
+    __syncthreads();
+    for (uint32_t z = threadIdx.x; z < R * (D / 4); z += kT) {
+        const uint32_t r = z / (D / 4), d = z % (D / 4) * 4;
+        float M = sm[0][r];
+#pragma unroll
+        for (int w = 1; w < kWaves; ++w) M = fmaxf(M, sm[w][r]);
+        const float Ms = M == -INFINITY ? 0.0f : M;
+        float L = 0.0f;
+        float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) {
+            const float f = exp2_(sm[w][r] - Ms);
+            const float4 t = *reinterpret_cast<const float4*>(dyn + (w * a.RL + r) * (D + 4) + d);
+            L += sl[w][r] * f;
+            y.x += t.x * f, y.y += t.y * f, y.z += t.z * f, y.w += t.w * f;
+        }
+        if (whole) {
+            const float inv = L > 0.0f ? 1.0f / L : (L == 0.0f ? 0.0f : L);  // no row: 0; NaN stays
+            y.x *= inv, y.y *= inv, y.z *= inv, y.w *= inv;
+        } else if (d == 0) {
+            a.part_ml[(slot + r) * 2] = M;
+            a.part_ml[(slot + r) * 2 + 1] = L;
+        }
+        float* to = whole ? out_row(a, qi, kh, row0 + r) * D + a.out : a.part + (slot + r) * D;
+        *reinterpret_cast<float4*>(to + d) = y;
+    }
+    __syncthreads();
+}
+
+// Shares of all pairs' units, as they come.
+template <int TYPE, int D, bool GROUP>
+__global__ __launch_bounds__(kT, D == 64 ? 4 : D == 128 ? 3 : 2) void attn_paged_kernel(AttnPaged a) {
+    extern __shared__ float dyn[];  // [waves][rows][D + 4], then q's operands
+    __shared__ ShareScan scan;
+    __shared__ float sm[kWaves][16], sl[kWaves][16];
     const uint32_t row0 = GROUP ? 0u : blockIdx.y * 16;  // the first head of this workgroup's
     const auto units = [&](uint32_t n) { return units_of<TYPE, GROUP>(a, scan, n); };
     hold_seen(a.see, scan);
     uint32_t mine, own;
-    const Shares sh = scan_units(a.see.n, a.KH, gridDim.x, units, scan, mine, own);
+    const Shares sh = scan_units(a.see.n, a.KH, gridDim.x, kFew, units, scan, mine, own);
     if (threadIdx.x == 0 && blockIdx.y == 0) a.cut[blockIdx.x].parts = 0;
     if (blockIdx.x >= sh.used) return;
     const uint64_t begin = share_start(sh, blockIdx.x), end = share_start(sh, blockIdx.x + 1);
     const Found at_begin = find_query(a.see.n, a.KH, units, scan, begin, mine, own);
     uint32_t qi = at_begin.query, before = at_begin.before;
     uint64_t pos = begin;
-    const size_t head_rows = size_t(1) << a.lp;
-    v4u_t* held_q = reinterpret_cast<v4u_t*>(dyn + kWaves * a.RL * (D + 4));  // q's operands [KC][NP][64]
     while (pos < end) {
         const uint32_t u = uniform(units(qi));
         if (pos >= uint64_t(before + u) * a.KH) {
@@ -276,315 +588,30 @@ __global__ __launch_bounds__(kT, D == 64 ? 4 : D == 128 ? 3 : 2) void attn_paged
         Group x = group_of<GROUP>(a, scan, qi);
         x.first.seq = int32_t(uniform(uint32_t(x.first.seq)));
         x.queries = uniform(x.queries), x.most = uniform(x.most), x.least = uniform(x.least);
-        const uint32_t R = GROUP ? x.queries * a.G : min(a.G - row0, 16u);  // rows: query, head
-        const uint32_t entries = entries_of(a, x.most);
-        const uint32_t parts = a.select ? entries << (a.lp - 4) : (x.most + 15) >> 4;  // 16-key parts of the pair
-        const uint32_t tiles = (parts + H - 1) / H;
-        const uint32_t t0 = u0 * kWaves + wave, t1 = min(u1 * kWaves, tiles);
-        const uint32_t nt = t0 < t1 ? (t1 - t0 + kWaves - 1) / kWaves : 0;  // tiles of this wave
-        const int32_t* table = a.table + size_t(x.first.seq) * a.width;
-        const int32_t* select = a.select ? a.select + (size_t(qi) * a.KH + kh) * a.keep : nullptr;
-
-        // ---- the wave's tiles ----
-        v4u_t kt[H][KC];
-        uint32_t vt[VR][VC][VW];
-        uint32_t place = 0;  // lane p: page | rows there << 24 of the p-th part that the wave has ahead
-        // byte offset of the wave's part p (of 64) from the cache's start
-        auto part_at = [&](uint32_t p, uint32_t part) {
-            const uint32_t page = uint32_t(__builtin_amdgcn_readlane(int(place), int(p))) & 0xffffffu;
-            const uint32_t in = (part << 4) & (uint32_t(head_rows) - 1);
-            return ((size_t(page) * a.KH + kh) * head_rows + in) * (D * S::ES);
-        };
-        auto rows_at = [&](uint32_t p) { return uint32_t(__builtin_amdgcn_readlane(int(place), int(p))) >> 24; };
-        constexpr uint32_t kBatch = 64 / H;  // tiles whose places a wave holds
-        uint32_t b = 0;  // the first tile of the batch
-        auto load_places = [&] {
-            const uint32_t j = b + lane / H, part = (t0 + j * kWaves) * H + lane % H, e = part >> (a.lp - 4);
-            place = 0;
-            if (j < nt && e < entries) {
-                const uint32_t y = select ? uint32_t(select[e]) : e;  // place in the sequence
-                if (y < a.width && (y << a.lp) < x.most) {
-                    const uint32_t page = uint32_t(table[y]);
-                    const uint32_t first = (y << a.lp) + ((part << 4) & (uint32_t(head_rows) - 1));
-                    if (page < a.pages && first < x.most) place = page | min(x.most - first, 16u) << 24;
-                }
-            }
-        };
-        auto load_k = [&](uint32_t j) {
-#pragma unroll
-            for (int h = 0; h < H; ++h) {
-                const uint8_t* p = a.k + part_at(j * H + h, (t0 + (b + j) * kWaves) * H + h);
-#pragma unroll
-                for (int k = 0; k < KC; ++k)
-                    kt[h][k] = load_held<GROUP, v4u_t>(p + uint32_t(i * D * S::ES + k * 64 + g * 16));
-            }
-        };
-        auto load_v = [&](uint32_t j) {
-#pragma unroll
-            for (int h = 0; h < H; ++h) {
-                const uint8_t* p = a.v + part_at(j * H + h, (t0 + (b + j) * kWaves) * H + h);
-#pragma unroll
-                for (int r = 0; r < 4; ++r)
-#pragma unroll
-                    for (int n = 0; n < VC; ++n) {
-                        const uint8_t* at = p + uint32_t((4 * g + r) * D * S::ES + (n * 16 + i) * VE * S::ES);
-                        if constexpr (VW == 4) {
-                            const v4u_t w = load_held<GROUP, v4u_t>(at);
-#pragma unroll
-                            for (int z = 0; z < 4; ++z) vt[h * 4 + r][n][z] = w[z];
-                        } else {
-                            const v2u_t w = load_held<GROUP, v2u_t>(at);
-                            vt[h * 4 + r][n][0] = w[0];
-                            vt[h * 4 + r][n][1] = w[1];
-                        }
-                    }
-            }
-        };
-        load_places();
-
-        // ---- the queries as operands ----
-        const uint32_t row = min(uint32_t(i), R - 1), member = GROUP ? row / a.G : 0u;
-        const float* qrow = a.q + (qi + member) * a.stride + (size_t(kh) * a.G + row0 + row - member * a.G) * D;
-        const uint32_t my_rows = GROUP ? seen_held(a.see, scan, qi + member).rows : 0u;  // that this lane's query sees
-        float c = a.scale2;  // takes a score into log2 units
-        float4 x0[KC][TYPE == ZQ_KV_F32 ? 1 : 2];
-        float most = 0.0f;
-#pragma unroll
-        for (int k = 0; k < KC; ++k)
-#pragma unroll
-            for (int j = 0; j < (TYPE == ZQ_KV_F32 ? 1 : 2); ++j) {
-                float4 y = *reinterpret_cast<const float4*>(qrow + (4 * k + g) * (TYPE == ZQ_KV_F32 ? 4 : 8) + 4 * j);
-                if (uint32_t(i) >= R) y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                x0[k][j] = y;
-                most = fmaxf(most, fmaxf(fmaxf(fabsf(y.x), fabsf(y.y)), fmaxf(fabsf(y.z), fabsf(y.w))));
-            }
-        // (asked for behind the queries, which are waited for first; a wave without tiles reads rows of page 0)
-        load_k(0);
-        load_v(0);
-        float up = 1.0f;
-        if constexpr (TYPE == ZQ_KV_F16) {  // the row's largest element to 2^14 .. 2^15
-            most = max_groups(most);
-            if (most > 0.0f) {
-                const int e = min(max(15 - __builtin_amdgcn_frexp_expf(most), -113), 126);
-                up = pow2f(e);
-                c *= pow2f(-e);
-            }
-        }
-#pragma unroll
-        for (int k = 0; k < KC; ++k) {
-            v4u_t op[NP];
-            if constexpr (TYPE == ZQ_KV_F32) {
-                op[0] = v4u_t{f_bits(x0[k][0].x), f_bits(x0[k][0].y), f_bits(x0[k][0].z), f_bits(x0[k][0].w)};
-            } else {
-                Parts<TYPE> p;
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    p.set2(4 * j, x0[k][j].x * up, x0[k][j].y * up);
-                    p.set2(4 * j + 2, x0[k][j].z * up, x0[k][j].w * up);
-                }
-#pragma unroll
-                for (int n = 0; n < NP; ++n) op[n] = p.bits(n);
-            }
-            if (k % kWaves == wave)
-#pragma unroll
-                for (int n = 0; n < NP; ++n) held_q[(k * NP + n) * 64 + lane] = op[n];
-        }
-        __syncthreads();
-
-        v4f_t o[VC][VE];
-#pragma unroll
-        for (int n = 0; n < VC; ++n)
-#pragma unroll
-            for (int e = 0; e < VE; ++e) o[n][e] = v4f_t{0.0f, 0.0f, 0.0f, 0.0f};
-        float m = -INFINITY, l = 0.0f;
-        auto step = [&](uint32_t j, auto last) {
-            v4f_t s[H];
-#pragma unroll
-            for (int h = 0; h < H; ++h) s[h] = v4f_t{0.0f, 0.0f, 0.0f, 0.0f};
-            asm volatile("" ::: "memory");  // q is read again, not held
-#pragma unroll
-            for (int k = 0; k < KC; ++k) {
-                v4u_t op[NP];
-#pragma unroll
-                for (int n = 0; n < NP; ++n) op[n] = held_q[(k * NP + n) * 64 + lane];
-#pragma unroll
-                for (int h = 0; h < H; ++h) {
-                    if constexpr (TYPE == ZQ_KV_F32) {
-#pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            s[h] = __builtin_amdgcn_mfma_f32_16x16x4f32(bits_f(kt[h][k][e]), bits_f(op[0][e]), s[h], 0, 0, 0);
-                    } else {
-#pragma unroll
-                        for (int n = NP - 1; n >= 0; --n) s[h] = mma<TYPE>(kt[h][k], op[n], s[h]);
-                    }
-                }
-            }
-            uint32_t rows[H];
-            bool cut = false;
-#pragma unroll
-            for (int h = 0; h < H; ++h) {
-                rows[h] = rows_at(j * H + h);
-                cut |= rows[h] < 16;
-                if (GROUP) cut |= (((t0 + (b + j) * kWaves) * H + h) << 4) + 16 > x.least;
-            }
-            if constexpr (!decltype(last)::value) load_k(j + 1);
-#pragma unroll
-            for (int h = 0; h < H; ++h) s[h] *= c;
-            if (cut) {  // uniform
-#pragma unroll
-                for (int h = 0; h < H; ++h) {
-                    uint32_t n = rows[h];
-                    if (GROUP) n = min(n, uint32_t(max(int32_t(my_rows - (((t0 + (b + j) * kWaves) * H + h) << 4)), 0)));
-#pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                        if (uint32_t(4 * g + r) >= n) s[h][r] = -INFINITY;
-                }
-            }
-            float most = -INFINITY;
-#pragma unroll
-            for (int h = 0; h < H; ++h)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) most = fmaxf(most, s[h][r]);
-            if (__any(most > m + kSlack)) {
-                const float to = fmaxf(m, max_groups(most));
-                const float f = to == -INFINITY ? 1.0f : exp2_(m - to);
-                m = to;
-                l *= f;
-#pragma unroll
-                for (int n = 0; n < VC; ++n)
-#pragma unroll
-                    for (int e = 0; e < VE; ++e) o[n][e] *= f;
-            }
-            const float ms = (m == -INFINITY ? 0.0f : m) - kShift;
-            float p[VR];
-#pragma unroll
-            for (int h = 0; h < H; ++h)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    p[h * 4 + r] = exp2_(s[h][r] - ms);
-                    l += p[h * 4 + r];
-                }
-            if (cut) {
-#pragma unroll
-                for (int h = 0; h < H; ++h)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                        if (uint32_t(4 * g + r) >= rows[h])
-#pragma unroll
-                            for (int n = 0; n < VC; ++n)
-#pragma unroll
-                                for (int z = 0; z < VW; ++z) vt[h * 4 + r][n][z] = 0;
-            }
-            const Weights<TYPE, VR> pw(p);
-            if (GROUP && cut && x.least < x.most) {
-                // a value that is no number must not reach (0 times it) the queries that do not see its row
-                bool odd = false;
-#pragma unroll
-                for (int r = 0; r < VR; ++r)
-#pragma unroll
-                    for (int n = 0; n < VC; ++n)
-#pragma unroll
-                        for (int z = 0; z < VW; ++z) odd |= not_finite<TYPE>(vt[r][n][z]);
-                if (__any(odd)) {
-                    // per element: how many such values a query sees; more than none gives NaN
-                    float sees[VR];
-#pragma unroll
-                    for (int r = 0; r < VR; ++r)
-                        sees[r] = (((t0 + (b + j) * kWaves) * H + r / 4) << 4) + 4 * g + r % 4 < my_rows ? 1.0f : 0.0f;
-                    const Weights<TYPE, VR> ps(sees);
-#pragma unroll
-                    for (int n = 0; n < VC; ++n)
-#pragma unroll
-                        for (int z = 0; z < VW; ++z) {
-                            uint32_t w[VR][1][1];
-#pragma unroll
-                            for (int r = 0; r < VR; ++r) {
-                                w[r][0][0] = take_odd<TYPE>(vt[r][n][z]);
-                            }
-#pragma unroll
-                            for (int e = 0; e < VE / VW; ++e) {
-                                const v4f_t y = add_pv<TYPE, VR, 1, 1, 1>(w, ps, 0, e, v4f_t{0.0f, 0.0f, 0.0f, 0.0f});
-                                v4f_t& to = o[n][z * (VE / VW) + e];
-#pragma unroll
-                                for (int k = 0; k < 4; ++k) to[k] = y[k] > 0.0f ? NAN : to[k];
-                            }
-                        }
-                }
-            }
-#pragma unroll
-            for (int n = 0; n < VC; ++n)
-#pragma unroll
-                for (int e = 0; e < VE; ++e) o[n][e] = add_pv<TYPE, VR, VC, VW>(vt, pw, n, e, o[n][e]);
-            if constexpr (!decltype(last)::value) load_v(j + 1);
-        };
-        while (b < nt) {
-            const uint32_t count = min(nt - b, kBatch);
-            for (uint32_t j = 0; j + 1 < count; ++j) step(j, std::false_type{});
-            step(count - 1, std::true_type{});
-            b += kBatch;
-            if (b < nt) {
-                load_places();
-                load_k(0);
-                load_v(0);
-            }
-        }
-
-        // ---- the four waves' sums as one ----
-        uint32_t ln = threadIdx.x;
-        asm volatile("" : "+v"(ln));  // the addresses below are made here, not held through the tiles
-        const uint32_t mi = ln & 15, mg = (ln >> 4) & 3;
-        l = sum_groups(l);
-        if (mg == 0) {
-            sm[wave][mi] = m;
-            sl[wave][mi] = l;
-        }
-        if (mi < R) {
-            float* to = dyn + (size_t(wave) * a.RL + mi) * (D + 4);
-#pragma unroll
-            for (int n = 0; n < VC; ++n)
-#pragma unroll
-                for (int r = 0; r < 4; ++r)
-#pragma unroll
-                    for (int e = 0; e < VE; e += 4)
-                        *reinterpret_cast<float4*>(to + n * 16 * VE + VE * (4 * mg + r) + e) =
-                            make_float4(o[n][e][r], o[n][e + 1][r], o[n][e + 2][r], o[n][e + 3][r]);
-        }
-        __syncthreads();
         const bool whole = u0 == 0 && v1 == u;
-        const size_t at = size_t(blockIdx.x) * 2 + (pos != begin), slot = at * a.RS + row0;
+        const size_t at = size_t(blockIdx.x) * 2 + (pos != begin);
         if (u0 == 0 && v1 < u && threadIdx.x == 0 && blockIdx.y == 0) {
             // shares with a part of the pair: up to the last one that starts below its end
             const uint64_t last = ((pos - v0 + u) * sh.used + sh.all - 1) / sh.all - 1;
-            a.cut[blockIdx.x] = {qi, kh, GROUP ? R : a.G, uint32_t(last - blockIdx.x + 1), at};
+            a.cut[blockIdx.x] = {qi, kh, GROUP ? x.queries * a.G : a.G, uint32_t(last - blockIdx.x + 1), at};
         }
-        for (uint32_t z = threadIdx.x; z < R * (D / 4); z += kT) {
-            const uint32_t r = z / (D / 4), d = z % (D / 4) * 4;
-            float M = sm[0][r];
-#pragma unroll
-            for (int w = 1; w < kWaves; ++w) M = fmaxf(M, sm[w][r]);
-            const float Ms = M == -INFINITY ? 0.0f : M;
-            float L = 0.0f;
-            float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-            for (int w = 0; w < kWaves; ++w) {
-                const float f = exp2_(sm[w][r] - Ms);
-                const float4 t = *reinterpret_cast<const float4*>(dyn + (w * a.RL + r) * (D + 4) + d);
-                L += sl[w][r] * f;
-                y.x += t.x * f, y.y += t.y * f, y.z += t.z * f, y.w += t.w * f;
-            }
-            if (whole) {
-                const float inv = L > 0.0f ? 1.0f / L : (L == 0.0f ? 0.0f : L);  // no row: 0; NaN stays
-                y.x *= inv, y.y *= inv, y.z *= inv, y.w *= inv;
-            } else if (d == 0) {
-                a.part_ml[(slot + r) * 2] = M;
-                a.part_ml[(slot + r) * 2 + 1] = L;
-            }
-            float* to = whole ? out_row(a, qi, kh, row0 + r) * D + a.out : a.part + (slot + r) * D;
-            *reinterpret_cast<float4*>(to + d) = y;
-        }
-        __syncthreads();
+        attend<TYPE, D, GROUP>(a, dyn, sm, sl, qi, kh, x, row0, u0, u1, whole, at * a.RS + row0,
+                                       [&](uint32_t n) { return seen_held(a.see, scan, n).rows; });
         pos += v1 - v0;
     }
+}
+
+// A workgroup for every pair: nothing to share out and nothing to join.
+template <int TYPE, int D>
+__global__ __launch_bounds__(kT, D == 64 ? 4 : D == 128 ? 3 : 2) void attn_paged_pair_kernel(AttnPaged a) {
+    extern __shared__ float dyn[];
+    __shared__ float sm[kWaves][16], sl[kWaves][16];
+    const uint32_t qi = blockIdx.x / a.KH, kh = blockIdx.x % a.KH;
+    const Seen s = seen_by(a.see, qi);
+    if (s.seq < 0) return;
+    const Group x{s, 1, s.rows, s.rows};
+    const uint32_t rows = a.select ? entries_of(a, s.rows) << a.lp : s.rows, u = max((rows + Tile<TYPE>::kUnit - 1) / Tile<TYPE>::kUnit, 1u);
+    attend<TYPE, D, false>(a, dyn, sm, sl, qi, kh, x, blockIdx.y * 16, 0, u, true, 0, [](uint32_t) { return 0u; });
 }
 
 // ---- join ------------------------------------------------------------------------
@@ -625,6 +652,18 @@ __global__ __launch_bounds__(kT) void attn_paged_join_kernel(AttnPaged a) {
     for (uint32_t d = threadIdx.x; d < D; d += kT) out[d] = ((acc[0][d] + acc[1][d]) + (acc[2][d] + acc[3][d])) * inv;
 }
 
+// Whether every pair gets a workgroup of its own: where pairs are short (up to 320 KB of rows, as the tables' width, or the
+// pages selected, have it), or there are two for every CU of up to 1.1 MB, or they all have as many selected pages and fill
+// rounds of a workgroup a CU.  us, such workgroups and shares: one sequence of 600 rows, 8 kv heads, D = 128: 9.5, 10.4;
+// 512 sequences of up to 400 rows: 84, 110; 256 of up to 2000: 165, 189; 300 of up to 3000 rows of 1.5 MB, 2 kv heads: 90, 81;
+// 64 of up to 8190, 4 MB: 206, 176; 32 with 2048 selected rows: 61, 69; 40: 97, 88; 4 with 4096: 86, 48.
+bool by_pairs(const AttnPaged& a, size_t row_bytes) {
+    const uint64_t cap = a.see.cap, picked = a.select ? uint64_t(a.keep) << a.lp : cap;
+    const uint64_t bytes = (picked < cap ? picked : cap) * 2 * row_bytes, pairs = uint64_t(a.see.n) * a.KH;
+    const uint64_t rounds = (pairs + 255) / 256;
+    return bytes <= 320 * 1024 || (bytes <= 1100 * 1024 && (pairs >= 512 || (a.select && pairs * 10 >= rounds * 256 * 9)));
+}
+
 // Workgroups for a call, as many as there are units at most: two a CU, and a third (all that are resident) where there
 // are so many pairs that every one starts on several of them; with D = 256 one.  (512, 768, 1536 workgroups, us: 64
 // sequences of up to 8190 rows, 512 pairs: 175, 177, 182; 512 of up to 400, 4096 pairs: 114, 110, 104; 131,072 rows of
@@ -640,17 +679,27 @@ uint32_t shares_of(const zq_kv_paged& c, const zq_page_tables& t, size_t queries
 uint32_t group_most(size_t G) { return G <= 8 ? uint32_t(16 / G) : 1; }
 size_t part_rows(size_t G) { return G * group_most(G); }
 
+template <class K>
+hipError_t allow_lds(K kernel, size_t lds) {
+    if (lds <= 64 * 1024) return hipSuccess;
+    return hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, int(lds));
+}
+
 template <int TYPE, int D, bool GROUP>
 hipError_t run_attention(const AttnPaged& a, uint32_t W, hipStream_t stream) {
     using S = Shape<TYPE, D>;
     const size_t lds = size_t(kWaves) * a.RL * (D + 4) * 4 + size_t(S::KC) * S::NP * 64 * 16;
-    if (lds > 64 * 1024) {
-        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&attn_paged_kernel<TYPE, D, GROUP>),
-                                                 hipFuncAttributeMaxDynamicSharedMemorySize, int(lds));
+    const uint32_t tiles = GROUP ? 1 : (a.G + 15) / 16;
+    if (!GROUP && by_pairs(a, D * S::ES)) {
+        const hipError_t e = allow_lds(&attn_paged_pair_kernel<TYPE, D>, lds);
         if (e != hipSuccess) return e;
+        hipLaunchKernelGGL((attn_paged_pair_kernel<TYPE, D>), dim3(a.see.n * a.KH, tiles), dim3(kT), lds, stream, a);
+        return hipGetLastError();
     }
-    hipLaunchKernelGGL((attn_paged_kernel<TYPE, D, GROUP>), dim3(W, GROUP ? 1 : (a.G + 15) / 16), dim3(kT), lds, stream, a);
-    hipError_t e = hipGetLastError();
+    hipError_t e = allow_lds(&attn_paged_kernel<TYPE, D, GROUP>, lds);
+    if (e != hipSuccess) return e;
+    hipLaunchKernelGGL((attn_paged_kernel<TYPE, D, GROUP>), dim3(W, tiles), dim3(kT), lds, stream, a);
+    e = hipGetLastError();
     if (e != hipSuccess || W == 1) return e;
     hipLaunchKernelGGL(attn_paged_join_kernel<D>, dim3(W - 1, a.RS), dim3(kT), 0, stream, a);
     return hipGetLastError();

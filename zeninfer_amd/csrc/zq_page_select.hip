@@ -37,7 +37,8 @@ __device__ __forceinline__ uint32_t pages_seen(const SelectArgs& a, const Seen& 
 // A wave takes B tiles of 16 pages at once, all their bounds under way together; a
 // workgroup's four waves are a unit of 64 B pages of one (query, kv head), shared out
 // evenly.  v_mfma_i32_16x16x64_i8: lane (i, g) loads bytes 64 k + 16 g of page i's
-// bounds; it then holds the sums of head i and pages 4 g .. 4 g + 3.
+// bounds; it then holds the sums of head i and pages 4 g .. 4 g + 3.  The bounds are
+// asked for before the query's codes are made, of which each wave makes a quarter.
 template <int D>
 struct ScoreShape {
     static constexpr int B = D == 256 ? 2 : 4;
@@ -45,9 +46,11 @@ struct ScoreShape {
     static constexpr int KC = 2 * D / 64;
 };
 template <int D>
-__global__ __launch_bounds__(kShareT) void page_score_kernel(SelectArgs a) {
+__global__ __launch_bounds__(kShareT, 3) void page_score_kernel(SelectArgs a) {
     using S = ScoreShape<D>;
     __shared__ ShareScan scan;
+    __shared__ v4i_t held_q[S::KC][64];  // [min(c, 0) | max(c, 0)] as operands
+    __shared__ float largest[kShareWaves][16];
     hold_seen(a.see, scan);
     const auto units = [&](uint32_t i) {
         const Seen x = seen_held(a.see, scan, i);
@@ -55,7 +58,7 @@ __global__ __launch_bounds__(kShareT) void page_score_kernel(SelectArgs a) {
         return n > a.keep ? (n + S::kUnit - 1) / S::kUnit : 0u;
     };
     uint32_t mine, own;
-    const Shares sh = scan_units(a.see.n, a.KH, gridDim.x, units, scan, mine, own);
+    const Shares sh = scan_units(a.see.n, a.KH, gridDim.x, 1, units, scan, mine, own);
     if (blockIdx.x >= sh.used) return;
     uint64_t pos = share_start(sh, blockIdx.x);
     const uint64_t end = share_start(sh, blockIdx.x + 1);
@@ -77,69 +80,78 @@ __global__ __launch_bounds__(kShareT) void page_score_kernel(SelectArgs a) {
         const uint32_t n = uniform(pages_seen(a, x));
         const int32_t* table = a.table + size_t(x.seq) * a.width;
         float* score = a.score + (size_t(qi) * a.KH + kh) * a.pitch;
+        v4i_t b[S::B][S::KC];
+        float scale;
+        // pages of unit t: lane l < 16 B has the l-th (past the last one: the last one's place is read)
+        auto load_page = [&](uint32_t t) {
+            const uint32_t j = (t * kShareWaves + wave) * 16 * S::B + uint32_t(lane % (16 * S::B));
+            return uint32_t(table[min(j, n - 1)]);
+        };
+        auto load_bounds = [&](uint32_t page) {
+            const bool good = page < a.pages;
+            if (!good) page = 0;
+            const int e = a.bounds_exp[size_t(page) * a.KH + kh];
+#pragma unroll
+            for (int w = 0; w < S::B; ++w) {
+                const uint32_t pg = uint32_t(__shfl(int(page), w * 16 + i));
+                const int8_t* from = a.bounds + (size_t(pg) * a.KH + kh) * 2 * D + g * 16;
+#pragma unroll
+                for (int k = 0; k < S::KC; ++k) b[w][k] = *reinterpret_cast<const v4i_t*>(from + k * 64);
+            }
+            scale = good ? pow2f(e) : -1.0f;
+        };
         for (uint32_t h0 = 0; h0 < a.G; h0 += 16) {  // 16 heads at once
-            // codes of head h0 + i: elements 16 g .. of every 64
+            const uint32_t first_page = load_page(u0);
+            // codes of head h0 + i, elements 64 k + 16 g ..: this wave's are dword `wave` of every 16 bytes
             const uint32_t R = min(a.G - h0, 16u);
-            const float* q = a.q + qi * a.stride + (size_t(kh) * a.G + h0 + min(uint32_t(i), R - 1)) * D;
-            float4 y[D / 64][4];
+            const float* q = a.q + qi * a.stride + (size_t(kh) * a.G + h0 + min(uint32_t(i), R - 1)) * D + g * 16 + wave * 4;
+            float4 y[D / 64];
             float most = 0.0f;
 #pragma unroll
-            for (int k = 0; k < D / 64; ++k)
+            for (int k = 0; k < D / 64; ++k) y[k] = *reinterpret_cast<const float4*>(q + k * 64);
+            load_bounds(first_page);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    y[k][j] = *reinterpret_cast<const float4*>(q + k * 64 + g * 16 + j * 4);
-                    const float4 z = y[k][j];
-                    most = fmaxf(most, fmaxf(fmaxf(fabsf(z.x), fabsf(z.y)), fmaxf(fabsf(z.z), fabsf(z.w))));
-                }
+            for (int k = 0; k < D / 64; ++k)
+                most = fmaxf(most, fmaxf(fmaxf(fabsf(y[k].x), fabsf(y[k].y)), fmaxf(fabsf(y[k].z), fabsf(y[k].w))));
             most = fmaxf(most, __shfl_xor(most, 16));
             most = fmaxf(most, __shfl_xor(most, 32));
+            if (g == 0) largest[wave][i] = most;
+            __syncthreads();  // (and the operands before these have been read)
+            most = fmaxf(fmaxf(largest[0][i], largest[1][i]), fmaxf(largest[2][i], largest[3][i]));
             const int eq = bound_exp(most);
-            const float unit = pow2f(-eq);
-            v4i_t op[S::KC];  // [min(c, 0) | max(c, 0)]
+            const float unit = pow2f(-eq), up = pow2f(eq);
 #pragma unroll
-            for (int k = 0; k < D / 64; ++k)
+            for (int k = 0; k < D / 64; ++k) {
+                const float e[4] = {y[k].x, y[k].y, y[k].z, y[k].w};
+                uint32_t neg = 0, plus = 0;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const float4 z = y[k][j];
-                    const float e[4] = {z.x, z.y, z.z, z.w};
-                    uint32_t neg = 0, plus = 0;
-#pragma unroll
-                    for (int b = 0; b < 4; ++b) {
-                        const float f = rintf(e[b] * unit);
-                        const int c = f != f ? 0 : bound_code(f);
-                        neg |= (uint32_t(min(c, 0)) & 255u) << (8 * b);
-                        plus |= (uint32_t(max(c, 0)) & 255u) << (8 * b);
-                    }
-                    op[k][j] = int(neg);
-                    op[D / 64 + k][j] = int(plus);
+                for (int c4 = 0; c4 < 4; ++c4) {
+                    const float f = rintf(e[c4] * unit);
+                    const int c = f != f ? 0 : bound_code(f);
+                    neg |= (uint32_t(min(c, 0)) & 255u) << (8 * c4);
+                    plus |= uint32_t(max(c, 0)) << (8 * c4);
                 }
-            const float up = pow2f(eq);
+                reinterpret_cast<uint32_t*>(&held_q[k][lane])[wave] = neg;
+                reinterpret_cast<uint32_t*>(&held_q[D / 64 + k][lane])[wave] = plus;
+            }
+            __syncthreads();
             for (uint32_t t = u0; t < u1; ++t) {
-                const uint32_t p0 = (t * kShareWaves + wave) * 16 * S::B;
-                if (p0 >= n) break;
-                // lane: page p0 + lane (B tiles of 16)
-                const uint32_t j = p0 + uint32_t(lane);
-                uint32_t page = j < n && lane < 16 * S::B ? uint32_t(table[j]) : 0u;
-                const bool good = page < a.pages;
-                if (!good) page = 0;
-                const float scale = good ? pow2f(a.bounds_exp[size_t(page) * a.KH + kh]) : INFINITY;
-                v4i_t b[S::B][S::KC];
-#pragma unroll
-                for (int w = 0; w < S::B; ++w) {
-                    const uint32_t pg = uint32_t(__shfl(int(page), w * 16 + i));
-                    const int8_t* at = a.bounds + (size_t(pg) * a.KH + kh) * 2 * D + g * 16;
-#pragma unroll
-                    for (int k = 0; k < S::KC; ++k) b[w][k] = load_once<v4i_t>(at + k * 64);
-                }
+                if (t != u0) load_bounds(load_page(t));
                 float mine_s = 0.0f;
+                v4i_t s[S::B];
 #pragma unroll
-                for (int w = 0; w < S::B; ++w) {
-                    v4i_t s{0, 0, 0, 0};
+                for (int w = 0; w < S::B; ++w) s[w] = v4i_t{0, 0, 0, 0};
 #pragma unroll
-                    for (int k = 0; k < S::KC; ++k) s = __builtin_amdgcn_mfma_i32_16x16x64_i8(b[w][k], op[k], s, 0, 0, 0);
+                for (int k = 0; k < S::KC; ++k) {
+                    const v4i_t op = held_q[k][lane];
+#pragma unroll
+                    for (int w = 0; w < S::B; ++w) s[w] = __builtin_amdgcn_mfma_i32_16x16x64_i8(b[w][k], op, s[w], 0, 0, 0);
+                }
+#pragma unroll
+                for (int w = 0; w < S::B; ++w)
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
-                        float f = uint32_t(i) < R ? float(s[r]) * up : -INFINITY;
+                        float f = uint32_t(i) < R ? float(s[w][r]) * up : -INFINITY;
                         f = fmaxf(f, dpp_f<kDppXor1>(f));
                         f = fmaxf(f, dpp_f<kDppXor2>(f));
                         f = fmaxf(f, dpp_f<kDppHalfMirror>(f));
@@ -148,9 +160,9 @@ __global__ __launch_bounds__(kShareT) void page_score_kernel(SelectArgs a) {
                         const float of = __shfl(f, ((lane >> 2) & 3) * 16);
                         if ((lane >> 4) == w && (lane & 3) == r) mine_s = of;
                     }
-                }
+                const uint32_t j = (t * kShareWaves + wave) * 16 * S::B + uint32_t(lane);
                 if (j < n && lane < 16 * S::B) {
-                    float f = good ? mine_s * scale : -INFINITY;
+                    float f = scale > 0.0f ? mine_s * scale : -INFINITY;
                     if (h0) f = fmaxf(f, score[j]);
                     score[j] = f;
                 }
@@ -330,7 +342,7 @@ __global__ __launch_bounds__(kTopT) void page_top_kernel(SelectArgs a) {
 uint32_t score_shares(const zq_kv_paged& c, const zq_page_tables& t, size_t queries) {
     const size_t unit = c.head_dim == 256 ? 128 : 256;
     const size_t most = queries * c.kv_heads * ((t.width + unit - 1) / unit);
-    return uint32_t(most < 1024 ? most : 1024);
+    return uint32_t(most < 768 ? most : 768);
 }
 
 uint32_t pitch_of(const zq_page_tables& t) { return uint32_t(t.width + 3) / 4 * 4; }

@@ -306,106 +306,134 @@ __global__ __launch_bounds__(256) void paged_append_kernel(AppendArgs a) {
 }
 
 // The same with the bounds of the pages that get rows.  The rows of one page in a call
-// are neighbours: a wave takes such a run for one kv head, writes its rows, reads the
-// page's rows before them, and has the bounds without reading the new ones back.  A
-// workgroup looks for the runs that end in its B tokens and shares them out over its
-// waves: B is 4 where there are few tokens (a decode step: a wave a token) and 64 where
-// there are many.
-template <int TYPE, int D>
-__global__ __launch_bounds__(256) void paged_append_bounds_kernel(AppendArgs a, uint32_t tokens, uint32_t B) {
+// are neighbours: C waves share such a run for one kv head, write its rows, read the
+// page's rows before them, and have the bounds without reading the new rows back.  A
+// workgroup looks for the runs that end in its B tokens: one token where there are few
+// (a decode step), else about a page's, as a workgroup that finds none has cost a wait.
+template <int TYPE, int D, int C>
+__global__ __launch_bounds__(C < 4 ? 256 : C * 64) void paged_append_bounds_kernel(AppendArgs a, uint32_t tokens, uint32_t B) {
     typedef typename Held<TYPE>::type T;
     constexpr int E = 16 / sizeof(T), L = D / E, R = 64 / L;  // elements a lane, lanes a row, rows at once
+    constexpr int U = 4;
     typedef T vec __attribute__((ext_vector_type(E)));
+    __shared__ float ends_of[2][C][2][D];  // with C > 1: least and greatest of waves 1 ..
     const int lane = threadIdx.x & 63, l = lane % L, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const uint32_t h = blockIdx.y, t0 = blockIdx.x * B;
+    const int part = C > 1 ? wave : 0;
+    const uint32_t h = blockIdx.x % a.KH, block0 = blockIdx.x / a.KH * B;
     const int64_t ps = int64_t(1) << a.lp;
-    bool ends = false;
-    int64_t mine = -1;
-    if (uint32_t(lane) < B && t0 + lane < tokens) {
-        mine = a.slots[t0 + lane];
-        const int64_t next = t0 + lane + 1 < tokens ? a.slots[t0 + lane + 1] : -1;
-        ends = mine >= 0 && mine < a.all_slots && !(next == mine + 1 && (next & (ps - 1)) != 0);
-    }
-    uint64_t runs = __ballot(ends);
-    for (int z = 0; runs; ++z) {
-        const int at = __builtin_ctzll(runs);
-        runs &= runs - 1;
-        if (z % 4 != wave) continue;
-        const uint32_t t = t0 + uint32_t(at);  // the run's last token
-        const uint64_t slot = uint64_t(uint32_t(__builtin_amdgcn_readlane(int(mine), at))) |
-                              uint64_t(uint32_t(__builtin_amdgcn_readlane(int(mine >> 32), at))) << 32;
-        const int last = int(slot & uint64_t(ps - 1));
-        int n = 0;  // rows of the run
-        for (bool more = true; more; n += 64) {  // ends: at token 0, at the page's first row, or before
-            const int64_t back = int64_t(n) + lane;
-            const bool same = back <= last && back <= int64_t(t) && a.slots[int64_t(t) - back] == int64_t(slot) - back;
-            const uint64_t m = ~__ballot(same);
-            if (m) {
-                n += __builtin_ctzll(m) - 64;
-                more = false;
+    auto slot_at = [&](uint32_t t) { return t < tokens ? a.slots[t] : int64_t(-1); };
+    int z = 0;  // runs so far (the same in every wave)
+    for (uint32_t t0 = block0; t0 < block0 + B && t0 < tokens; t0 += 64) {
+        const int64_t mine = uint32_t(lane) < block0 + B - t0 ? slot_at(t0 + lane) : -1, next = slot_at(t0 + lane + 1);
+        uint64_t runs = __ballot(mine >= 0 && mine < a.all_slots && !(next == mine + 1 && (next & (ps - 1)) != 0));
+        for (; runs; ++z) {
+            const int at = __builtin_ctzll(runs);
+            runs &= runs - 1;
+            if (C == 1 && z % 4 != wave) continue;
+            const uint32_t t = t0 + uint32_t(at);  // the run's last token
+            const uint64_t slot = uint64_t(uint32_t(__builtin_amdgcn_readlane(int(mine), at))) |
+                                  uint64_t(uint32_t(__builtin_amdgcn_readlane(int(mine >> 32), at))) << 32;
+            const int last = int(slot & uint64_t(ps - 1));
+            int n = 0;  // rows of the run
+            for (bool more = true; more; n += 64) {  // ends: at token 0, at the page's first row, or before
+                const int64_t back = int64_t(n) + lane;
+                const bool same = back <= last && back <= int64_t(t) && a.slots[int64_t(t) - back] == int64_t(slot) - back;
+                const uint64_t m = ~__ballot(same);
+                if (m) {
+                    n += __builtin_ctzll(m) - 64;
+                    more = false;
+                }
             }
-        }
-        const size_t head = size_t(slot >> a.lp) * a.KH + h;
-        const size_t base = (head << a.lp) * D + l * E;
-        T* pk = reinterpret_cast<T*>(a.k) + base;
-        T* pv = reinterpret_cast<T*>(a.v) + base;
-        float lo[E], hi[E];
+            const size_t head = size_t(slot >> a.lp) * a.KH + h;
+            const size_t base = (head << a.lp) * D + l * E;
+            T* pk = reinterpret_cast<T*>(a.k) + base;
+            T* pv = reinterpret_cast<T*>(a.v) + base;
+            float lo[E], hi[E];
 #pragma unroll
-        for (int i = 0; i < E; ++i) lo[i] = INFINITY, hi[i] = -INFINITY;
-        auto take = [&](const vec& x) {
+            for (int i = 0; i < E; ++i) lo[i] = INFINITY, hi[i] = -INFINITY;
+            auto take = [&](const vec& x) {
+#pragma unroll
+                for (int i = 0; i < E; ++i) {
+                    lo[i] = fminf(lo[i], float(x[i]));
+                    hi[i] = fmaxf(hi[i], float(x[i]));
+                }
+            };
+            const int first = last + 1 - n;
+#pragma unroll 4
+            for (int r = part * R + lane / L; r < first; r += C * R) take(*reinterpret_cast<const vec*>(pk + size_t(r) * D));
+            const size_t src = size_t(t - uint32_t(n - 1)) * a.stride + h * D + l * E;
+            // U rows' loads before their stores: a load behind a store waits until that is done
+            for (int r0 = part * R + lane / L; r0 < n; r0 += U * C * R) {
+                float4 x[U][E / 4], y[U][E / 4];
+#pragma unroll
+                for (int j = 0; j < U; ++j)
+#pragma unroll
+                    for (int i = 0; i < E / 4; ++i) {
+                        const size_t from = src + min(r0 + j * C * R, n - 1) * a.stride + 4 * i;
+                        x[j][i] = *reinterpret_cast<const float4*>(a.src_k + from);
+                        y[j][i] = *reinterpret_cast<const float4*>(a.src_v + from);
+                    }
+#pragma unroll
+                for (int j = 0; j < U; ++j) {
+                    const int r = r0 + j * C * R;
+                    if (r >= n) break;
+                    vec k, v;
+#pragma unroll
+                    for (int i = 0; i < E / 4; ++i) {
+                        const float4 p = x[j][i], q = y[j][i];
+                        k[4 * i] = T(p.x), k[4 * i + 1] = T(p.y), k[4 * i + 2] = T(p.z), k[4 * i + 3] = T(p.w);
+                        v[4 * i] = T(q.x), v[4 * i + 1] = T(q.y), v[4 * i + 2] = T(q.z), v[4 * i + 3] = T(q.w);
+                    }
+                    *reinterpret_cast<vec*>(pk + size_t(first + r) * D) = k;
+                    *reinterpret_cast<vec*>(pv + size_t(first + r) * D) = v;
+                    take(k);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < E; ++i)
+#pragma unroll
+                for (int m = L; m < 64; m *= 2) {
+                    lo[i] = fminf(lo[i], __shfl_xor(lo[i], m));
+                    hi[i] = fmaxf(hi[i], __shfl_xor(hi[i], m));
+                }
+            // (two buffers: a wave that is a run ahead has passed the barrier that the first one came to after reading)
+            if constexpr (C > 1) {
+                if (wave && lane < L)
+#pragma unroll
+                    for (int i = 0; i < E; ++i) ends_of[z & 1][wave][0][l * E + i] = lo[i], ends_of[z & 1][wave][1][l * E + i] = hi[i];
+                __syncthreads();
+                if (wave) continue;
+            }
+            float most = 0.0f;
 #pragma unroll
             for (int i = 0; i < E; ++i) {
-                lo[i] = fminf(lo[i], float(x[i]));
-                hi[i] = fmaxf(hi[i], float(x[i]));
+#pragma unroll
+                for (int w = 1; w < C; ++w) {
+                    lo[i] = fminf(lo[i], ends_of[z & 1][w][0][l * E + i]);
+                    hi[i] = fmaxf(hi[i], ends_of[z & 1][w][1][l * E + i]);
+                }
+                if (lo[i] > hi[i]) lo[i] = hi[i] = 0.0f;  // NaN only
+                most = fmaxf(most, fmaxf(fabsf(lo[i]), fabsf(hi[i])));
             }
-        };
-        const int first = last + 1 - n;
-#pragma unroll 2
-        for (int r = lane / L; r < first; r += R) take(*reinterpret_cast<const vec*>(pk + size_t(r) * D));
-        const size_t src = size_t(t - uint32_t(n - 1)) * a.stride + h * D + l * E;
-#pragma unroll 2
-        for (int r = lane / L; r < n; r += R) {
-            vec k, v;
 #pragma unroll
-            for (int i = 0; i < E; i += 4) {
-                const float4 x = *reinterpret_cast<const float4*>(a.src_k + src + r * a.stride + i);
-                const float4 y = *reinterpret_cast<const float4*>(a.src_v + src + r * a.stride + i);
-                k[i] = T(x.x), k[i + 1] = T(x.y), k[i + 2] = T(x.z), k[i + 3] = T(x.w);
-                v[i] = T(y.x), v[i + 1] = T(y.y), v[i + 2] = T(y.z), v[i + 3] = T(y.w);
+            for (int m = 1; m < L; m *= 2) most = fmaxf(most, __shfl_xor(most, m));
+            const int e = bound_exp(most);
+            uint32_t w[2][E / 4] = {};
+#pragma unroll
+            for (int i = 0; i < E; ++i) {
+                const int c0 = bound_code(floorf(ldexpf(lo[i], -e))), c1 = bound_code(ceilf(ldexpf(hi[i], -e)));
+                w[0][i / 4] |= uint32_t(c0 & 255) << (8 * (i % 4));
+                w[1][i / 4] |= uint32_t(c1 & 255) << (8 * (i % 4));
             }
-            *reinterpret_cast<vec*>(pk + size_t(first + r) * D) = k;
-            *reinterpret_cast<vec*>(pv + size_t(first + r) * D) = v;
-            take(k);
-        }
-        float most = 0.0f;
+            if (lane < L) {
+                int8_t* b = a.bounds + head * 2 * D + l * E;
 #pragma unroll
-        for (int i = 0; i < E; ++i) {
-#pragma unroll
-            for (int m = L; m < 64; m *= 2) {
-                lo[i] = fminf(lo[i], __shfl_xor(lo[i], m));
-                hi[i] = fmaxf(hi[i], __shfl_xor(hi[i], m));
+                for (int i = 0; i < E / 4; ++i) {
+                    reinterpret_cast<uint32_t*>(b)[i] = w[0][i];
+                    reinterpret_cast<uint32_t*>(b + D)[i] = w[1][i];
+                }
+                if (lane == 0) a.bounds_exp[head] = int8_t(e);
             }
-            if (lo[i] > hi[i]) lo[i] = hi[i] = 0.0f;  // NaN only
-            most = fmaxf(most, fmaxf(fabsf(lo[i]), fabsf(hi[i])));
-        }
-#pragma unroll
-        for (int m = 1; m < L; m *= 2) most = fmaxf(most, __shfl_xor(most, m));
-        const int e = bound_exp(most);
-        uint32_t w[2][E / 4] = {};
-#pragma unroll
-        for (int i = 0; i < E; ++i) {
-            const int c0 = bound_code(floorf(ldexpf(lo[i], -e))), c1 = bound_code(ceilf(ldexpf(hi[i], -e)));
-            w[0][i / 4] |= uint32_t(c0 & 255) << (8 * (i % 4));
-            w[1][i / 4] |= uint32_t(c1 & 255) << (8 * (i % 4));
-        }
-        if (lane < L) {
-            int8_t* b = a.bounds + head * 2 * D + l * E;
-#pragma unroll
-            for (int i = 0; i < E / 4; ++i) {
-                reinterpret_cast<uint32_t*>(b)[i] = w[0][i];
-                reinterpret_cast<uint32_t*>(b + D)[i] = w[1][i];
-            }
-            if (lane == 0) a.bounds_exp[head] = int8_t(e);
         }
     }
 }
@@ -414,9 +442,16 @@ constexpr uint32_t kManyTokens = 1024;
 template <int TYPE, int D>
 void run_append(const AppendArgs& a, hipStream_t stream) {
     if (a.bounds) {
-        const uint32_t tokens = a.rows / a.KH, B = tokens < kManyTokens ? 4 : 64;
-        hipLaunchKernelGGL((paged_append_bounds_kernel<TYPE, D>), dim3((tokens + B - 1) / B, a.KH), dim3(256), 0, stream, a,
-                           tokens, B);
+        // us, C = 1 / 4 or 8 waves a run, bf16, 8 kv heads, D = 128 (fp32, 2 kv heads, D = 256 for the last): 8200 tokens
+        // and pages of 32: 22 / 44, of 256: 52 / 58; 1402 tokens, pages of 64: 12 / 6.  Blocks of 16, 32, 64 tokens at
+        // pages of 32: 26, 22, 25; of 16: 22, 23, 25.
+        const uint32_t tokens = a.rows / a.KH, ps = 1u << a.lp;
+        auto run = [&](auto kernel, uint32_t threads, uint32_t B) {
+            hipLaunchKernelGGL(kernel, dim3((tokens + B - 1) / B * a.KH), dim3(threads), 0, stream, a, tokens, B);
+        };
+        if (tokens < kManyTokens) run(paged_append_bounds_kernel<TYPE, D, 4>, 256, 1);
+        else if (a.rows / ps < 256) run(paged_append_bounds_kernel<TYPE, D, 8>, 512, ps);  // fewer runs than CUs
+        else run(paged_append_bounds_kernel<TYPE, D, 1>, 256, ps < 32 ? 16 : 32);
         return;
     }
     constexpr uint32_t per = 256 / (D * sizeof(typename Held<TYPE>::type) / 16);

@@ -103,9 +103,10 @@ __device__ __forceinline__ Seen seen_held(const Queries& a, const ShareScan& sh,
     if (a.n > kSeenHeld) return seen_by(a, i);
     return {sh.seq[i], sh.rows[i]};
 }
-// The sums; mine: before this thread's queries (t * each ...), own: of them.
+// The sums; mine: before this thread's queries (t * each ...), own: of them.  W: workgroups; with more than one a CU
+// each gets `few` units at least.
 template <class F>
-__device__ __forceinline__ Shares scan_units(uint32_t n, uint32_t mult, uint32_t W, F units, ShareScan& sh, uint32_t& mine,
+__device__ __forceinline__ Shares scan_units(uint32_t n, uint32_t mult, uint32_t W, uint32_t few, F units, ShareScan& sh, uint32_t& mine,
                                              uint32_t& own) {
     const uint32_t tid = threadIdx.x, each = (n + kShareT - 1) / kShareT, i0 = tid * each, i1 = min(i0 + each, n);
     own = 0;
@@ -122,10 +123,8 @@ __device__ __forceinline__ Shares scan_units(uint32_t n, uint32_t mult, uint32_t
     }
     s.units = uint32_t(__builtin_amdgcn_readfirstlane(int(s.units)));  // one for the workgroup
     s.all = uint64_t(s.units) * mult;
-    // few units: a workgroup a CU, and more of them only where each has kFew units to itself (a share's start and what
-    // it leaves to be joined cost as much as several units; 100,000 rows of one kv head: 23 us so, 37 with a unit each)
-    constexpr uint32_t kFew = 6, kCUs = 256;
-    s.used = uint32_t(min(min(uint64_t(W), s.all), max(uint64_t(kCUs), s.all / kFew)));
+    constexpr uint32_t kCUs = 256;
+    s.used = uint32_t(min(min(uint64_t(W), s.all), max(uint64_t(kCUs), s.all / few)));
     return s;
 }
 // The query that has unit x (< all) of all kv heads, and the units of one kv head before it.

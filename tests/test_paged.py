@@ -448,13 +448,20 @@ def queries(rng, n, H, D, size=1.0):
 KINDS = ("f16", "bf16", "f32")
 
 
+@pytest.fixture(params=[2, 3000], ids=["pairs", "shares"])
+def spare(request):
+    """Entries of the tables that no sequence uses.  With few, a (query, kv head) pair has a workgroup of its own; with
+    many, pairs are cut into shares and joined."""
+    return request.param
+
+
 @gpu
 @pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("D", [64, 128, 256])
 @pytest.mark.parametrize("ps, KH, G, lens", [
     (16, 2, 4, [1, 16, 17, 300]), (64, 1, 1, [63, 64, 65, 129]), (256, 3, 7, [500, 2]), (32, 2, 16, [33, 700, 31])])
-def test_attention(zq, kind, D, ps, KH, G, lens):
-    pool = Pool(zq, kind, lens, KH, D, ps, seed=D + ps)
+def test_attention(zq, kind, D, ps, KH, G, lens, spare):
+    pool = Pool(zq, kind, lens, KH, D, ps, seed=D + ps, spare_width=spare)
     held = [n - 1 for n in lens]
     check_attention(zq, pool, queries(pool.rng, len(lens), KH * G, D), held, 1 / math.sqrt(D))
 
@@ -490,9 +497,20 @@ def test_attention_lengths_counts_and_idle_queries(zq, kind):
 
 
 @gpu
+@pytest.mark.parametrize("kind, G, n", [("f16", 4, 1500), ("bf16", 9, 1025), ("f32", 1, 3001), ("f16", 8, 8192)])
+def test_attention_of_more_queries_than_a_workgroup_holds(zq, kind, G, n):
+    pool = Pool(zq, kind, [90, 17, 200], 1, 64, 16, seed=n, spare_width=3000)
+    seq_of = pool.rng.integers(-1, 3, n)
+    if n != 1025:
+        seq_of = np.sort(seq_of)
+    lens = [int(pool.rng.integers(0, pool.lens[max(s, 0)])) for s in seq_of]
+    check_attention(zq, pool, queries(pool.rng, n, G, 64), lens, 0.125, seq_of=seq_of)
+
+
+@gpu
 @pytest.mark.parametrize("kind", KINDS)
-def test_attention_of_queries_that_share_a_sequence(zq, kind):
-    pool = Pool(zq, kind, [700, 33], 2, 128, 32, seed=4)
+def test_attention_of_queries_that_share_a_sequence(zq, kind, spare):
+    pool = Pool(zq, kind, [700, 33], 2, 128, 32, seed=4, spare_width=spare)
     seq_of = [0] * 37 + [1] * 33 + [-1] * 3
     lens = list(range(663, 700)) + list(range(33)) + [0] * 3
     check_attention(zq, pool, queries(pool.rng, len(lens), 8, 128), lens, 0.09, seq_of=seq_of)
@@ -500,9 +518,9 @@ def test_attention_of_queries_that_share_a_sequence(zq, kind):
 
 @gpu
 @pytest.mark.parametrize("kind", KINDS)
-def test_attention_over_selected_pages(zq, kind):
+def test_attention_over_selected_pages(zq, kind, spare):
     """Any order, places twice, past the rows seen, none; fewer pages than keep."""
-    pool = Pool(zq, kind, [333, 40, 500], 2, 64, 16, seed=6)
+    pool = Pool(zq, kind, [333, 40, 500], 2, 64, 16, seed=6, spare_width=spare)
     K = 9
     select = np.full((3, 2, K), -1)
     select[0, 0] = [20, 3, 3, 0, 19, -1, 7, 1000, 5]
@@ -517,8 +535,8 @@ def test_attention_over_selected_pages(zq, kind):
 
 
 @gpu
-def test_attention_pages_that_were_given_up(zq):
-    pool = Pool(zq, "f16", [300, 64], 2, 128, 16, seed=8)
+def test_attention_pages_that_were_given_up(zq, spare):
+    pool = Pool(zq, "f16", [300, 64], 2, 128, 16, seed=8, spare_width=spare)
     pool.table[0, [0, 1, 2, 7]] = [-1, pool.pages, 2 ** 31 - 1, -2 ** 31]
     pool.table[1, :4] = -1
     pool.upload(zq)
@@ -528,9 +546,9 @@ def test_attention_pages_that_were_given_up(zq):
 
 @gpu
 @pytest.mark.parametrize("kind", KINDS)
-def test_attention_strides_scales_and_peaks(zq, kind):
+def test_attention_strides_scales_and_peaks(zq, kind, spare):
     """Columns of a packed row; a negative scale, zero and one so large that one row takes all; rows far apart in size."""
-    pool = Pool(zq, kind, [200, 77], 2, 64, 32, seed=9)
+    pool = Pool(zq, kind, [200, 77], 2, 64, 32, seed=9, spare_width=spare)
     q = queries(pool.rng, 2, 6, 64)
     for scale in (0.125, -0.3, 0.0, 30.0):
         check_attention(zq, pool, q, [199, 76], scale, stride=6 * 64 + 128)
@@ -543,8 +561,8 @@ def test_attention_strides_scales_and_peaks(zq, kind):
 
 @gpu
 @pytest.mark.parametrize("kind", KINDS)
-def test_attention_nan_and_infinity_reach_only_those_who_see_them(zq, kind):
-    pool = Pool(zq, kind, [100, 100], 2, 64, 16, seed=10)
+def test_attention_nan_and_infinity_reach_only_those_who_see_them(zq, kind, spare):
+    pool = Pool(zq, kind, [100, 100], 2, 64, 16, seed=10, spare_width=spare)
     pool.k[pool.table[0, 3], 1, 5, 7] = math.nan      # row 53 of kv head 1
     pool.v[pool.table[1, 2], 0, 0, 9] = math.inf      # row 32 of kv head 0
     pool.upload(zq)
@@ -561,9 +579,9 @@ def test_attention_nan_and_infinity_reach_only_those_who_see_them(zq, kind):
 @gpu
 @pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("value", [math.nan, math.inf])
-def test_a_value_that_is_no_number_reaches_only_the_drafted_tokens_that_see_it(zq, kind, value):
+def test_a_value_that_is_no_number_reaches_only_the_drafted_tokens_that_see_it(zq, kind, value, spare):
     """Queries of one sequence share products; each of them sees one row more."""
-    pool = Pool(zq, kind, [70], 2, 64, 16, seed=13)
+    pool = Pool(zq, kind, [70], 2, 64, 16, seed=13, spare_width=spare)
     pool.v[pool.table[0, 4], 1, 1, 9] = value      # row 65 of kv head 1
     pool.v[pool.table[0, 3], 0, 15, 63] = -value   # row 63 of kv head 0
     pool.upload(zq)
@@ -579,9 +597,9 @@ def test_a_value_that_is_no_number_reaches_only_the_drafted_tokens_that_see_it(z
 @gpu
 @pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("G", [1, 2, 3, 5, 8, 9])
-def test_attention_of_drafted_tokens(zq, kind, G):
+def test_attention_of_drafted_tokens(zq, kind, G, spare):
     """Runs of queries of one sequence, of all lengths, in any order of lengths, idle ones among them."""
-    pool = Pool(zq, kind, [400, 40, 17, 1], 2, 64, 16, seed=G)
+    pool = Pool(zq, kind, [400, 40, 17, 1], 2, 64, 16, seed=G, spare_width=spare)
     seq_of = [0] * 21 + [1] * 3 + [2] + [0] + [3] + [1] * 9 + [-1] + [1] * 2
     lens = [int(pool.rng.integers(0, pool.lens[max(s, 0)])) for s in seq_of]
     counts = [int(pool.rng.integers(0, 3)) for _ in seq_of]
@@ -592,9 +610,9 @@ def test_attention_of_drafted_tokens(zq, kind, G):
 
 
 @gpu
-def test_attention_of_infinite_scores_and_a_spread_of_sizes(zq):
+def test_attention_of_infinite_scores_and_a_spread_of_sizes(zq, spare):
     """Keys so large that the scores of the reference are past fp32's range in exp only: the largest takes all."""
-    pool = Pool(zq, "bf16", [90], 1, 64, 16, seed=11, fill=1e4)
+    pool = Pool(zq, "bf16", [90], 1, 64, 16, seed=11, fill=1e4, spare_width=spare)
     check_attention(zq, pool, queries(pool.rng, 1, 3, 64, 100.0), [89], 1.0)
 
 
@@ -778,6 +796,14 @@ def test_select_of_many_pages(zq, pages, keep):
 
 
 @gpu
+def test_select_for_more_queries_than_a_workgroup_holds(zq):
+    pool = scored(zq, [100, 40, 3], 2, 64, 16, seed=14)
+    n = 1700
+    seq_of = pool.rng.integers(-1, 4, n)
+    check_select(zq, pool, queries(pool.rng, n, 2, 64), pool.rng.integers(-2, 1700, n), 9, 2, 1, seq_of=seq_of)
+
+
+@gpu
 def test_select_ties_go_to_the_lowest(zq):
     """All pages alike; a query of zeros; two values only."""
     pool = scored(zq, [500, 3000], 2, 64, 16, 1, like=np.stack([np.full(64, -3), np.full(64, 5)]))
@@ -838,8 +864,8 @@ def test_bound_is_above_every_score(zq):
 # ---- as they are used ---------------------------------------------------------------
 @gpu
 @pytest.mark.parametrize("kind", KINDS)
-def test_equal_calls_give_equal_bits(zq, kind):
-    pool = Pool(zq, kind, [3000, 100, 1], 2, 128, 16, seed=20)
+def test_equal_calls_give_equal_bits(zq, kind, spare):
+    pool = Pool(zq, kind, [3000, 100, 1], 2, 128, 16, seed=20, spare_width=spare)
     q = queries(pool.rng, 3, 8, 128)
     a = [run_attention(zq, pool, q, [2999, 99, 0], 0.1) for _ in range(4)]
     assert all(np.array_equal(a[0], x) for x in a[1:])

@@ -38,16 +38,16 @@ struct AttnPaged {
     size_t stride;   // floats between queries
     float scale2;    // scale * log2(e): scores are in log2 units
     uint32_t width, pages, KH, G, keep, lp;
+    uint32_t start;  // units that a pair's start counts as
     uint32_t P, RS, RL;  // queries of a group at most, rows of a partial and of a workgroup
 };
 
 // ---- work of a workgroup ---------------------------------------------------------
 // The rows of a (query, kv head) pair are cut into units of kUnit keys, and these are
 // shared out evenly (zq_paged.hpp).  A pair that a share's end cuts is put together by
-// the join kernel.  Starting on a pair and writing its outputs takes as long as kStart
+// the join kernel.  Starting on a pair and writing its outputs takes as long as `start`
 // units more, which count as units without keys at its start.
 constexpr int kT = kShareT, kWaves = kShareWaves;
-constexpr uint32_t kStart = 2;
 // More workgroups than CUs only where each has this many units: 100,000 rows of one kv head take 23 us so, 37 with a unit
 // each (768 partials to join).
 constexpr uint32_t kFew = 6;
@@ -90,7 +90,7 @@ __device__ __forceinline__ uint32_t units_of(const AttnPaged& a, const ShareScan
     if (x.first.seq < 0) return 0;
     if (GROUP && i % a.P && seen_held(a.see, sh, i - 1).seq == x.first.seq) return 0;
     const uint32_t rows = a.select ? entries_of(a, x.most) << a.lp : x.most;
-    return kStart + max((rows + Tile<TYPE>::kUnit - 1) / Tile<TYPE>::kUnit, 1u);  // no rows: a unit that writes zeros
+    return a.start + max((rows + Tile<TYPE>::kUnit - 1) / Tile<TYPE>::kUnit, 1u);  // no rows: a unit that writes zeros
 }
 
 // Where row r (query, head) of a group goes; without groups r is a head, G of them and no more.
@@ -554,9 +554,9 @@ __device__ __forceinline__ void attend(const AttnPaged& a, float* dyn, float (&s
     __syncthreads();
 }
 
-// Shares of all pairs' units, as they come.
+// Shares of all pairs' units, as they come.  (With D = 256 there is a workgroup a CU: a wave may have all registers.)
 template <int TYPE, int D, bool GROUP>
-__global__ __launch_bounds__(kT, D == 64 ? 4 : D == 128 ? 3 : 2) void attn_paged_kernel(AttnPaged a) {
+__global__ __launch_bounds__(kT, D == 64 ? 4 : D == 128 ? 3 : 1) void attn_paged_kernel(AttnPaged a) {
     extern __shared__ float dyn[];  // [waves][rows][D + 4], then q's operands
     __shared__ ShareScan scan;
     __shared__ float sm[kWaves][16], sl[kWaves][16];
@@ -580,7 +580,7 @@ __global__ __launch_bounds__(kT, D == 64 ? 4 : D == 128 ? 3 : 2) void attn_paged
         }
         const uint32_t rel = uint32_t(pos - uint64_t(before) * a.KH), kh = rel / u, v0 = rel % u;
         const uint32_t v1 = uint32_t(min(uint64_t(u), v0 + (end - pos)));
-        const uint32_t u0 = v0 > kStart ? v0 - kStart : 0u, u1 = v1 > kStart ? v1 - kStart : 0u;  // with keys
+        const uint32_t u0 = v0 > a.start ? v0 - a.start : 0u, u1 = v1 > a.start ? v1 - a.start : 0u;  // with keys
         if (u1 == 0) {
             pos += v1 - v0;
             continue;
@@ -664,13 +664,17 @@ bool by_pairs(const AttnPaged& a, size_t row_bytes) {
     return bytes <= 320 * 1024 || (bytes <= 1100 * 1024 && (pairs >= 512 || (a.select && pairs * 10 >= rounds * 256 * 9)));
 }
 
+// What a pair's start counts as, in units (us with 2 and as here: drafted tokens at D = 64: 26, 24; a prompt of 500 tokens
+// of each of two sequences: 64, 62; without groups 1, 2 and 3: 198, 187, 187 for 128 sequences of up to 2000 rows, D = 256).
+constexpr uint32_t kMostStart = 4;
+uint32_t start_units(bool group, size_t head_dim) { return !group ? 2 : head_dim == 64 ? kMostStart : 3; }
 // Workgroups for a call, as many as there are units at most: two a CU, and a third (all that are resident) where there
 // are so many pairs that every one starts on several of them; with D = 256 one.  (512, 768, 1536 workgroups, us: 64
 // sequences of up to 8190 rows, 512 pairs: 175, 177, 182; 512 of up to 400, 4096 pairs: 114, 110, 104; 131,072 rows of
 // one: 89, 91, 100; 32 of up to 8000, bf16, D = 256, with 256, 512 and 1024: 97, 110, 131.)
 uint32_t shares_of(const zq_kv_paged& c, const zq_page_tables& t, size_t queries) {
     const size_t unit = c.type == ZQ_KV_F32 ? 64 : 128, pairs = queries * c.kv_heads;
-    const size_t most = pairs * ((t.width * t.page_size + unit - 1) / unit + kStart);
+    const size_t most = pairs * ((t.width * t.page_size + unit - 1) / unit + kMostStart);
     const size_t want = 256 * (c.head_dim == 256 ? 1 : pairs < 2048 ? 2 : 3);
     return uint32_t(most < want ? most : want);
 }
@@ -758,6 +762,7 @@ int zq_hip_attention_paged_dev(const zq_kv_paged* cache, const zq_page_tables* t
     a.out = out;
     const bool group = seq_of && !select && zq::group_most(G) > 1;
     a.P = group ? zq::group_most(G) : 1;
+    a.start = zq::start_units(group, cache->head_dim);
     a.RS = a.P * G;
     a.RL = a.RS < 16 ? a.RS : 16;
     a.part = static_cast<float*>(workspace);

@@ -245,7 +245,7 @@ __device__ __forceinline__ V load_held(const uint8_t* p) {
 template <int TYPE, int D, bool GROUP, class F>
 __device__ __forceinline__ void attend(const AttnPaged& a, float* dyn, float (&sm)[kWaves][16], float (&sl)[kWaves][16], uint32_t qi,
                                        uint32_t kh, const Group& x, uint32_t row0, uint32_t u0, uint32_t u1, bool whole,
-                                       size_t slot, F rows_of) {
+                                       size_t slot, F rows_of, bool has_ahead = false, uint32_t ahead = 0) {
     using S = Shape<TYPE, D>;
     constexpr int H = S::H, KC = S::KC, VE = S::VE, VC = S::VC, VW = S::VW, VR = S::VR, NP = S::NP;
     const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
@@ -280,7 +280,7 @@ __device__ __forceinline__ void attend(const AttnPaged& a, float* dyn, float (&s
         if (j < nt && e < entries) {
             const uint32_t y = select ? uint32_t(select[e]) : e;  // place in the sequence
             if (y < a.width && (y << a.lp) < x.most) {
-                const uint32_t page = uint32_t(table[y]);
+                const uint32_t page = has_ahead && b == 0 ? ahead : uint32_t(table[y]);
                 const uint32_t first = (y << a.lp) + ((part << 4) & (uint32_t(head_rows) - 1));
                 if (page < a.pages && first < x.most) place = page | min(x.most - first, 16u) << 24;
             }
@@ -607,11 +607,17 @@ __global__ __launch_bounds__(kT, D == 64 ? 4 : D == 128 ? 3 : 2) void attn_paged
     extern __shared__ float dyn[];
     __shared__ float sm[kWaves][16], sl[kWaves][16];
     const uint32_t qi = blockIdx.x / a.KH, kh = blockIdx.x % a.KH;
+    // the table entries of a wave's first parts, asked for before it is known how many there are
+    constexpr uint32_t H = Tile<TYPE>::H;
+    const uint32_t lane = threadIdx.x & 63, e = ((lane / H * kWaves + threadIdx.x / 64) * H + lane % H) >> (a.lp - 4);
+    const bool has_ahead = !a.see.seq_of && !a.select;
+    uint32_t ahead = 0;
+    if (has_ahead && e < a.width) ahead = uint32_t(a.table[size_t(qi) * a.width + e]);
     const Seen s = seen_by(a.see, qi);
     if (s.seq < 0) return;
     const Group x{s, 1, s.rows, s.rows};
     const uint32_t rows = a.select ? entries_of(a, s.rows) << a.lp : s.rows, u = max((rows + Tile<TYPE>::kUnit - 1) / Tile<TYPE>::kUnit, 1u);
-    attend<TYPE, D, false>(a, dyn, sm, sl, qi, kh, x, blockIdx.y * 16, 0, u, true, 0, [](uint32_t) { return 0u; });
+    attend<TYPE, D, false>(a, dyn, sm, sl, qi, kh, x, blockIdx.y * 16, 0, u, true, 0, [](uint32_t) { return 0u; }, has_ahead, ahead);
 }
 
 // ---- join ------------------------------------------------------------------------

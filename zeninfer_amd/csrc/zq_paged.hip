@@ -69,8 +69,10 @@ template <int T, int N>
 __global__ __launch_bounds__(T) void page_step_kernel(StepArgs a, uint32_t role) {
     __shared__ uint32_t end[T * N];    // granted tokens up to and with a sequence
     __shared__ uint32_t taken[T * N];  // pages taken before it
+    __shared__ uint32_t held[T * N];   // tokens it holds
     __shared__ uint32_t part[2][T / 64];
     __shared__ uint32_t total[3];
+    __shared__ int32_t top[N == 1 ? T : 1];
     const uint32_t tid = threadIdx.x, cap = a.width << a.lp;
     const uint32_t fc = uint32_t(min(max(a.free_count[0], 0), int32_t(a.pages)));
     auto len_of = [&](uint32_t s) { return uint32_t(min(max(a.lens[s], 0), int32_t(cap))); };
@@ -94,14 +96,17 @@ __global__ __launch_bounds__(T) void page_step_kernel(StepArgs a, uint32_t role)
     }
     // (the page that the first new token of this thread's sequence continues, if it does: asked for before the sums)
     const uint32_t row_n = n[0] & ((1u << a.lp) - 1);
-    int32_t last_page = -1;
+    // and the stack's top, one page a sequence
+    int32_t last_page = -1, top_page = -1;
     if (N == 1 && tid < a.seqs && c[0] && row_n) last_page = a.table[size_t(tid) * a.width + (n[0] >> a.lp)];
+    if (N == 1 && tid < fc) top_page = a.free_pages[fc - 1 - tid];
     Sums2 at = block_before2<T / 64>(own, part, all);
     uint32_t tok = 0, pg = 0;  // the sums of the last one served
     const Sums2 first = at;
 #pragma unroll
     for (int j = 0; j < N; ++j) {
         taken[tid * N + j] = at.b;
+        held[tid * N + j] = n[j];
         at.a = add_sat31(at.a, c[j]);
         at.b = add_sat31(at.b, need[j]);
         end[tid * N + j] = at.a;
@@ -110,6 +115,7 @@ __global__ __launch_bounds__(T) void page_step_kernel(StepArgs a, uint32_t role)
     if (tok) atomicMax(&total[0], tok);
     if (pg) atomicMax(&total[1], pg);
     if (N == 1 && c[0] > 1) total[2] = 1;
+    if (N == 1) top[tid] = top_page;
     __syncthreads();
     const uint32_t served = total[0], taken_all = total[1];
     if (role & kExpand) {
@@ -122,7 +128,7 @@ __global__ __launch_bounds__(T) void page_step_kernel(StepArgs a, uint32_t role)
             if (blockIdx.x == 0 && c[0] && at.a <= served) {
                 uint32_t page = uint32_t(last_page);
                 if (!row_n) {
-                    page = uint32_t(a.free_pages[fc - 1 - first.b]);
+                    page = uint32_t(top[first.b]);  // (a page each: below T)
                     a.table[size_t(tid) * a.width + (n[0] >> a.lp)] = int32_t(page);
                 }
                 put(first.a, page < a.pages ? (int64_t(page) << a.lp) + row_n : -1, int32_t(n[0]), int32_t(tid));
@@ -139,7 +145,7 @@ __global__ __launch_bounds__(T) void page_step_kernel(StepArgs a, uint32_t role)
                         if (end[mid] > r) hi = mid;
                         else lo = mid + 1;
                     }
-                    const uint32_t len = len_of(lo), p = len + r - (lo ? end[lo - 1] : 0u), j = p >> a.lp;
+                    const uint32_t len = held[lo], p = len + r - (lo ? end[lo - 1] : 0u), j = p >> a.lp;
                     const uint32_t old = pages_of(len, a.lp), row = p & ((1u << a.lp) - 1);
                     const uint32_t page = uint32_t(j < old ? a.table[size_t(lo) * a.width + j]
                                                            : a.free_pages[fc - 1 - (taken[lo] + j - old)]);

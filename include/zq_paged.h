@@ -98,8 +98,8 @@ typedef struct zq_kv_paged {
 
 /* Keys and values of `tokens` rows [tokens][stride] fp32 (kv_heads * head_dim
  * used; stride in floats, 0 = kv_heads * head_dim; a multiple of 4, 16-byte
- * aligned) into slots[r], rounded to the cache's type (to nearest, ties to even).
- * Rows whose slot is outside 0 .. pages * page_size - 1 are not written.  Slots
+ * aligned) into slots[r], rounded to the cache's type (to nearest, ties to even;
+ * past its range to infinity).  Rows whose slot is outside 0 .. pages * page_size - 1 are not written.  Slots
  * of a call differ.
  * With bounds, those of every page that gets a row are made anew of the page's
  * rows up to the last one written.  A page's rows of one call have to be
@@ -125,7 +125,9 @@ int zq_hip_kv_paged_append_dev(const zq_kv_paged* cache, const float* k, const f
  * pages seen hold nothing.
  * Scores, exponentials and sums are fp32; q and the softmax weights have 24
  * bits with an fp32 or bf16 cache and 22 with an fp16 one, and the held rows are
- * exact.  NaN and infinities of rows that are not seen do not matter.
+ * exact.  NaN and infinities of rows that are not seen do not matter; a seen one
+ * gives NaN or an infinity: in the keys in all of the heads' outputs, in the values
+ * in that element.
  * At most 8192 queries a call and 1024 heads; workspace: zq_hip_attention_paged_workspace_bytes(),
  * 16-byte aligned, of any contents (calls that may run at the same time need
  * one each); with less, the call fails with ZQ_ERR_ARG. */

@@ -578,35 +578,37 @@ def test_attention_nan_and_infinity_reach_only_those_who_see_them(zq, kind, spar
 
 @gpu
 @pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("D", [64, 128, 256])
 @pytest.mark.parametrize("value", [math.nan, math.inf])
-def test_a_value_that_is_no_number_reaches_only_the_drafted_tokens_that_see_it(zq, kind, value, spare):
+def test_a_value_that_is_no_number_reaches_only_the_drafted_tokens_that_see_it(zq, kind, D, value, spare):
     """Queries of one sequence share products; each of them sees one row more."""
-    pool = Pool(zq, kind, [70], 2, 64, 16, seed=13, spare_width=spare)
+    pool = Pool(zq, kind, [70], 2, D, 16, seed=13, spare_width=spare)
     pool.v[pool.table[0, 4], 1, 1, 9] = value      # row 65 of kv head 1
-    pool.v[pool.table[0, 3], 0, 15, 63] = -value   # row 63 of kv head 0
+    pool.v[pool.table[0, 3], 0, 15, D - 1] = -value   # row 63 of kv head 0
     pool.upload(zq)
     lens = list(range(58, 70))
-    got = run_attention(zq, pool, queries(pool.rng, 12, 6, 64), lens, 0.125, seq_of=[0] * 12)
-    bad = np.zeros((12, 6, 64), bool)
+    got = run_attention(zq, pool, queries(pool.rng, 12, 6, D), lens, 0.125, seq_of=[0] * 12)
+    bad = np.zeros((12, 6, D), bool)
     for i, n in enumerate(lens):
         bad[i, 3:, 9] = n >= 65
-        bad[i, :3, 63] = n >= 63
+        bad[i, :3, D - 1] = n >= 63
     assert (np.isfinite(got) == ~bad).all()
 
 
 @gpu
 @pytest.mark.parametrize("kind", KINDS)
-@pytest.mark.parametrize("G", [1, 2, 3, 5, 8, 9])
-def test_attention_of_drafted_tokens(zq, kind, G, spare):
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("G", [1, 2, 3, 5, 8, 9, 16, 17])
+def test_attention_of_drafted_tokens(zq, kind, D, G, spare):
     """Runs of queries of one sequence, of all lengths, in any order of lengths, idle ones among them."""
-    pool = Pool(zq, kind, [400, 40, 17, 1], 2, 64, 16, seed=G, spare_width=spare)
+    pool = Pool(zq, kind, [400, 40, 17, 1], 2, D, 16, seed=G, spare_width=spare)
     seq_of = [0] * 21 + [1] * 3 + [2] + [0] + [3] + [1] * 9 + [-1] + [1] * 2
     lens = [int(pool.rng.integers(0, pool.lens[max(s, 0)])) for s in seq_of]
     counts = [int(pool.rng.integers(0, 3)) for _ in seq_of]
     for c in (None, counts):
         if c is not None:
             lens = [min(n, pool.lens[max(s, 0)] - x) for n, s, x in zip(lens, seq_of, c)]
-        check_attention(zq, pool, queries(pool.rng, len(lens), 2 * G, 64), lens, 0.125, seq_of=seq_of, counts=c)
+        check_attention(zq, pool, queries(pool.rng, len(lens), 2 * G, D), lens, 0.125, seq_of=seq_of, counts=c)
 
 
 @gpu
@@ -983,6 +985,71 @@ def test_a_captured_step_replays_while_sequences_grow(zq):
         torch.cuda.synchronize()
         graph.replay()
         s.check()
+
+
+@gpu
+@pytest.mark.parametrize("kind", KINDS)
+def test_captured_calls_of_wide_heads_replay(zq, kind):
+    """Workgroups of more than 64 KB of LDS; a replay after other work, with other queries and lengths."""
+    pool = Pool(zq, kind, [700, 90, 5], 1, 256, 32, seed=21, spare_width=3000)
+    n, H = 3, 16
+    need = max(zq.attention_paged_workspace_bytes(pool.cache, pool.tables, n, H),
+               zq.page_select_workspace_bytes(pool.cache, pool.tables, n, H, 4))
+    ws = torch.zeros(need, dtype=torch.uint8, device=DEV)
+    q, out, lens = torch.zeros(n, H, 256, device=DEV), torch.zeros(n, H, 256, device=DEV), dev([0] * n)
+    select, sparse = dev(np.zeros((n, 1, 4))), torch.zeros(n, H, 256, device=DEV)
+    w = dict(workspace=ws, workspace_bytes=need)
+
+    def enqueue(stream):
+        zq.attention_paged_dev(pool.cache, pool.tables, q, out, n, H, lens, 0.06, stream=stream, **w)
+        zq.page_select_dev(pool.cache, pool.tables, q, select, n, H, lens, 4, recent=1, first=1, stream=stream, **w)
+        zq.attention_paged_dev(pool.cache, pool.tables, q, sparse, n, H, lens, 0.06, select=select, keep=4, stream=stream, **w)
+
+    stream = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        enqueue(stream)
+    for ls in ([699, 89, 4], [3, 60, 0], [512, 33, 2]):
+        x = queries(pool.rng, n, H, 256)
+        q.copy_(torch.from_numpy(x))
+        lens.copy_(dev(ls))
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        picked = pool.choose(x, ls, 4, 1, 1)
+        assert np.array_equal(select.cpu().numpy(), picked)
+        for got, sel in ((out, None), (sparse, picked)):
+            want, tol = pool.attend(x, ls, 0.06, select=sel)
+            assert (np.abs(got.cpu().numpy() - want) <= tol).all()
+        eager = [t.clone() for t in (out, sparse)]
+        enqueue(None)
+        torch.cuda.synchronize()
+        assert torch.equal(eager[0], out) and torch.equal(eager[1], sparse)
+
+
+@gpu
+def test_two_calls_at_once(zq):
+    """Two streams read one cache, with a workspace each."""
+    pool = Pool(zq, "bf16", [4000, 300, 2500], 2, 128, 16, seed=22)
+    x = [queries(pool.rng, 3, 8, 128) for _ in range(2)]
+    lens = [[3999, 299, 2499], [3000, 10, 2400]]
+    alone = [run_attention(zq, pool, q, n, 0.1) for q, n in zip(x, lens)]
+    need = zq.attention_paged_workspace_bytes(pool.cache, pool.tables, 3, 8)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    ws = [torch.zeros(need, dtype=torch.uint8, device=DEV) for _ in range(2)]
+    q = [torch.from_numpy(a).to(DEV) for a in x]
+    gl = [dev(n) for n in lens]
+    out = [[torch.zeros(3, 8, 128, device=DEV) for _ in range(2)] for _ in range(10)]
+    torch.cuda.synchronize()
+    for o in out:
+        for i in range(2):
+            zq.attention_paged_dev(pool.cache, pool.tables, q[i], o[i], 3, 8, gl[i], 0.1, workspace=ws[i], workspace_bytes=need,
+                                   stream=streams[i])
+    torch.cuda.synchronize()
+    for o in out:
+        for i in range(2):
+            assert np.array_equal(o[i].cpu().numpy(), alone[i])
 
 
 @gpu

@@ -18,7 +18,6 @@ namespace {
 typedef float v4f_t __attribute__((ext_vector_type(4)));
 typedef __bf16 b8_t __attribute__((ext_vector_type(8)));
 typedef uint32_t v4u_t __attribute__((ext_vector_type(4)));
-typedef uint32_t v2u_t __attribute__((ext_vector_type(2)));
 
 struct Cut {
     uint32_t query, kh, rows, parts;  // parts 0: none
@@ -181,16 +180,17 @@ struct Weights<ZQ_KV_F32, VR> {
         for (int r = 0; r < VR; ++r) x[r] = p[r];
     }
 };
-template <int TYPE, int VR, int VC, int VW, int PARTS = Shape<TYPE, 128>::NP>
-__device__ __forceinline__ v4f_t add_pv(const uint32_t (&v)[VR][VC][VW], const Weights<TYPE, VR>& p, int n, int e, v4f_t o) {
+// (word(r): the dword of row r that has the tile's element e of every V load)
+template <int TYPE, int VR, int PARTS = Shape<TYPE, 128>::NP, class F>
+__device__ __forceinline__ v4f_t add_pv(F word, const Weights<TYPE, VR>& p, int e, v4f_t o) {
     if constexpr (TYPE == ZQ_KV_F32) {
 #pragma unroll
-        for (int r = 0; r < VR; ++r) o = __builtin_amdgcn_mfma_f32_16x16x4f32(bits_f(v[r][n][e]), p.x[r], o, 0, 0, 0);
+        for (int r = 0; r < VR; ++r) o = __builtin_amdgcn_mfma_f32_16x16x4f32(bits_f(word(r)), p.x[r], o, 0, 0, 0);
     } else {
         v4u_t w;
 #pragma unroll
         for (int z = 0; z < 4; ++z)
-            w[z] = __builtin_amdgcn_perm(v[2 * z + 1][n][e / 2], v[2 * z][n][e / 2], e & 1 ? 0x07060302u : 0x05040100u);
+            w[z] = __builtin_amdgcn_perm(word(2 * z + 1), word(2 * z), e & 1 ? 0x07060302u : 0x05040100u);
 #pragma unroll
         for (int y = PARTS - 1; y >= 0; --y) o = mma<TYPE>(w, p.x.bits(y), o);
     }
@@ -263,7 +263,9 @@ __device__ __forceinline__ void attend(const AttnPaged& a, float* dyn, float (&s
 
     // ---- the wave's tiles ----
     v4u_t kt[H][KC];
-    uint32_t vt[VR][VC][VW];
+    // (vectors: as dwords of their own they have met a register allocation that overwrote two of four)
+    typedef uint32_t vw_t __attribute__((ext_vector_type(VW)));
+    vw_t vt[VR][VC];
     uint32_t place = 0;  // lane p: page | rows there << 24 of the p-th part that the wave has ahead
     // byte offset of the wave's part p (of 64) from the cache's start
     auto part_at = [&](uint32_t p, uint32_t part) {
@@ -304,15 +306,7 @@ __device__ __forceinline__ void attend(const AttnPaged& a, float* dyn, float (&s
 #pragma unroll
                 for (int n = 0; n < VC; ++n) {
                     const uint8_t* at = p + uint32_t((4 * g + r) * D * S::ES + (n * 16 + i) * VE * S::ES);
-                    if constexpr (VW == 4) {
-                        const v4u_t w = load_held<GROUP, v4u_t>(at);
-#pragma unroll
-                        for (int z = 0; z < 4; ++z) vt[h * 4 + r][n][z] = w[z];
-                    } else {
-                        const v2u_t w = load_held<GROUP, v2u_t>(at);
-                        vt[h * 4 + r][n][0] = w[0];
-                        vt[h * 4 + r][n][1] = w[1];
-                    }
+                    vt[h * 4 + r][n] = load_held<GROUP, vw_t>(at);
                 }
         }
     };
@@ -442,14 +436,11 @@ __device__ __forceinline__ void attend(const AttnPaged& a, float* dyn, float (&s
             }
         if (cut) {
 #pragma unroll
-            for (int h = 0; h < H; ++h)
+            for (int r = 0; r < VR; ++r) {
+                const uint32_t keep = uint32_t(4 * g + r % 4) < rows[r / 4] ? 0xffffffffu : 0u;
 #pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    if (uint32_t(4 * g + r) >= rows[h])
-#pragma unroll
-                        for (int n = 0; n < VC; ++n)
-#pragma unroll
-                            for (int z = 0; z < VW; ++z) vt[h * 4 + r][n][z] = 0;
+                for (int n = 0; n < VC; ++n) vt[r][n] &= keep;
+            }
         }
         const Weights<TYPE, VR> pw(p);
         if (GROUP && cut && x.least < x.most) {
@@ -472,14 +463,16 @@ __device__ __forceinline__ void attend(const AttnPaged& a, float* dyn, float (&s
                 for (int n = 0; n < VC; ++n)
 #pragma unroll
                     for (int z = 0; z < VW; ++z) {
-                        uint32_t w[VR][1][1];
+                        uint32_t ones[VR];
 #pragma unroll
                         for (int r = 0; r < VR; ++r) {
-                            w[r][0][0] = take_odd<TYPE>(vt[r][n][z]);
+                            uint32_t w = vt[r][n][z];
+                            ones[r] = take_odd<TYPE>(w);
+                            vt[r][n][z] = w;
                         }
 #pragma unroll
                         for (int e = 0; e < VE / VW; ++e) {
-                            const v4f_t y = add_pv<TYPE, VR, 1, 1, 1>(w, ps, 0, e, v4f_t{0.0f, 0.0f, 0.0f, 0.0f});
+                            const v4f_t y = add_pv<TYPE, VR, 1>([&](int r) { return ones[r]; }, ps, e, v4f_t{0.0f, 0.0f, 0.0f, 0.0f});
                             v4f_t& to = o[n][z * (VE / VW) + e];
 #pragma unroll
                             for (int k = 0; k < 4; ++k) to[k] = y[k] > 0.0f ? NAN : to[k];
@@ -490,7 +483,8 @@ __device__ __forceinline__ void attend(const AttnPaged& a, float* dyn, float (&s
 #pragma unroll
         for (int n = 0; n < VC; ++n)
 #pragma unroll
-            for (int e = 0; e < VE; ++e) o[n][e] = add_pv<TYPE, VR, VC, VW>(vt, pw, n, e, o[n][e]);
+            for (int e = 0; e < VE; ++e)
+                o[n][e] = add_pv<TYPE, VR>([&](int r) { return uint32_t(vt[r][n][e * VW / VE]); }, pw, e, o[n][e]);
         if constexpr (!decltype(last)::value) load_v(j + 1);
     };
     while (b < nt) {

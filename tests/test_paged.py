@@ -579,6 +579,18 @@ def test_attention_nan_and_infinity_reach_only_those_who_see_them(zq, kind, spar
 @gpu
 @pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("G, each", [(8, 8), (3, 23), (16, 5), (1, 50), (7, 9)])
+def test_attention_of_many_drafted_tokens(zq, kind, D, G, each):
+    """More queries a sequence than one tile of rows takes, and long tables: two tiles."""
+    pool = Pool(zq, kind, [1500, 200, 77], 1, D, 16, seed=G, spare_width=3000)
+    seq_of = np.repeat([0, 1, 2], each)
+    lens = np.concatenate([np.arange(n - each, n) for n in pool.lens])
+    check_attention(zq, pool, queries(pool.rng, 3 * each, G, D), lens, 0.1, seq_of=seq_of)
+
+
+@gpu
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("D", [64, 128, 256])
 @pytest.mark.parametrize("value", [math.nan, math.inf])
 def test_a_value_that_is_no_number_reaches_only_the_drafted_tokens_that_see_it(zq, kind, D, value, spare):
     """Queries of one sequence share products; each of them sees one row more."""

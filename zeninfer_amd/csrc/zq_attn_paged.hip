@@ -68,11 +68,11 @@ struct Group {
     Seen first;
     uint32_t queries, most, least;  // rows that they see
 };
-template <bool GROUP>
+template <int GROUP>
 __device__ __forceinline__ Group group_of(const AttnPaged& a, const ShareScan& sh, uint32_t i) {
     Group x{seen_held(a.see, sh, i), 1, 0, 0};
     x.most = x.least = x.first.rows;
-    if constexpr (GROUP) {
+    if constexpr (GROUP != 0) {
         for (uint32_t j = i + 1; x.first.seq >= 0 && j < a.see.n && j % a.P; ++j) {
             const Seen y = seen_held(a.see, sh, j);
             if (y.seq != x.first.seq) break;
@@ -83,7 +83,7 @@ __device__ __forceinline__ Group group_of(const AttnPaged& a, const ShareScan& s
     }
     return x;
 }
-template <int TYPE, bool GROUP>
+template <int TYPE, int GROUP>
 __device__ __forceinline__ uint32_t units_of(const AttnPaged& a, const ShareScan& sh, uint32_t i) {
     const Group x = group_of<GROUP>(a, sh, i);
     if (x.first.seq < 0) return 0;
@@ -161,6 +161,7 @@ struct Shape {
     static constexpr int VW = VE * ES / 4;                          // dwords of one
     static constexpr int VR = 4 * H;                                // rows whose V a lane loads
     static constexpr int NP = TYPE == ZQ_KV_F32 ? 1 : TYPE == ZQ_KV_F16 ? 2 : 3;
+    static constexpr int QL = TYPE == ZQ_KV_F32 ? 1 : 2;            // 16-byte loads of q for 16 bytes of a key
 };
 
 // The softmax weights of a lane's rows as operands, and what they add to one tile of O^T.
@@ -242,17 +243,19 @@ __device__ __forceinline__ V load_held(const uint8_t* p) {
 // next V when this one is used.
 // One (query or group, kv head) pair, or the units u0 .. u1 of it, by a workgroup.
 // whole: straight into the output; else into partial `slot`.
-template <int TYPE, int D, bool GROUP, class F>
+template <int TYPE, int D, int GROUP, class F>
 __device__ __forceinline__ void attend(const AttnPaged& a, float* dyn, float (&sm)[kWaves][16], float (&sl)[kWaves][16], uint32_t qi,
                                        uint32_t kh, const Group& x, uint32_t row0, uint32_t u0, uint32_t u1, bool whole,
                                        size_t slot, F rows_of, bool has_ahead = false, uint32_t ahead = 0) {
     using S = Shape<TYPE, D>;
     constexpr int H = S::H, KC = S::KC, VE = S::VE, VC = S::VC, VW = S::VW, VR = S::VR, NP = S::NP;
+    constexpr int RT = GROUP ? GROUP : 1;  // tiles of 16 rows
     const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const size_t head_rows = size_t(1) << a.lp;
-    v4u_t* held_q = reinterpret_cast<v4u_t*>(dyn + kWaves * a.RL * (D + 4));  // q's operands [KC][NP][64]
+    v4u_t* held_q = reinterpret_cast<v4u_t*>(dyn + kWaves * a.RL * (D + 4));  // q's operands [RT][KC][NP][64]
     const uint32_t R = GROUP ? x.queries * a.G : min(a.G - row0, 16u);  // rows: query, head
+    const bool two = RT > 1 && R > 16;
     const uint32_t entries = entries_of(a, x.most);
     const uint32_t parts = a.select ? entries << (a.lp - 4) : (x.most + 15) >> 4;  // 16-key parts of the pair
     const uint32_t tiles = (parts + H - 1) / H;
@@ -294,10 +297,11 @@ __device__ __forceinline__ void attend(const AttnPaged& a, float* dyn, float (&s
             const uint8_t* p = a.k + part_at(j * H + h, (t0 + (b + j) * kWaves) * H + h);
 #pragma unroll
             for (int k = 0; k < KC; ++k)
-                kt[h][k] = load_held<GROUP, v4u_t>(p + uint32_t(i * D * S::ES + k * 64 + g * 16));
+                kt[h][k] = load_held<GROUP != 0, v4u_t>(p + uint32_t(i * D * S::ES + k * 64 + g * 16));
         }
     };
     auto load_v = [&](uint32_t j) {
+        asm volatile("" ::: "memory");  // behind K: a wait for K is none for V
 #pragma unroll
         for (int h = 0; h < H; ++h) {
             const uint8_t* p = a.v + part_at(j * H + h, (t0 + (b + j) * kWaves) * H + h);
@@ -306,185 +310,224 @@ __device__ __forceinline__ void attend(const AttnPaged& a, float* dyn, float (&s
 #pragma unroll
                 for (int n = 0; n < VC; ++n) {
                     const uint8_t* at = p + uint32_t((4 * g + r) * D * S::ES + (n * 16 + i) * VE * S::ES);
-                    vt[h * 4 + r][n] = load_held<GROUP, vw_t>(at);
+                    vt[h * 4 + r][n] = load_held<GROUP != 0, vw_t>(at);
                 }
         }
     };
     load_places();
 
     // ---- the queries as operands ----
-    const uint32_t row = min(uint32_t(i), R - 1), member = GROUP ? row / a.G : 0u;
-    const float* qrow = a.q + (qi + member) * a.stride + (size_t(kh) * a.G + row0 + row - member * a.G) * D;
-    const uint32_t my_rows = GROUP ? rows_of(qi + member) : 0u;  // that this lane's query sees
-    float c = a.scale2;  // takes a score into log2 units
-    float4 x0[KC][TYPE == ZQ_KV_F32 ? 1 : 2];
-    float most = 0.0f;
+    uint32_t my_rows[RT];  // that this lane's query sees
+    float c[RT];           // takes a score into log2 units
+    auto load_q = [&](int t, float4 (&x0)[KC][S::QL]) {
+        const uint32_t at = uint32_t(t * 16 + i), row = min(at, R - 1), member = GROUP ? row / a.G : 0u;
+        const float* qrow = a.q + (qi + member) * a.stride + (size_t(kh) * a.G + row0 + row - member * a.G) * D;
+        my_rows[t] = GROUP ? rows_of(qi + member) : 0u;
 #pragma unroll
-    for (int k = 0; k < KC; ++k)
+        for (int k = 0; k < KC; ++k)
 #pragma unroll
-        for (int j = 0; j < (TYPE == ZQ_KV_F32 ? 1 : 2); ++j) {
-            float4 y = *reinterpret_cast<const float4*>(qrow + (4 * k + g) * (TYPE == ZQ_KV_F32 ? 4 : 8) + 4 * j);
-            if (uint32_t(i) >= R) y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            x0[k][j] = y;
-            most = fmaxf(most, fmaxf(fmaxf(fabsf(y.x), fabsf(y.y)), fmaxf(fabsf(y.z), fabsf(y.w))));
-        }
-    // (asked for behind the queries, which are waited for first; a wave without tiles reads rows of page 0)
-    load_k(0);
-    load_v(0);
-    float up = 1.0f;
-    if constexpr (TYPE == ZQ_KV_F16) {  // the row's largest element to 2^14 .. 2^15
-        most = max_groups(most);
-        if (most > 0.0f) {
-            const int e = min(max(15 - __builtin_amdgcn_frexp_expf(most), -113), 126);
-            up = pow2f(e);
-            c *= pow2f(-e);
-        }
-    }
-#pragma unroll
-    for (int k = 0; k < KC; ++k) {
-        v4u_t op[NP];
-        if constexpr (TYPE == ZQ_KV_F32) {
-            op[0] = v4u_t{f_bits(x0[k][0].x), f_bits(x0[k][0].y), f_bits(x0[k][0].z), f_bits(x0[k][0].w)};
-        } else {
-            Parts<TYPE> p;
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                p.set2(4 * j, x0[k][j].x * up, x0[k][j].y * up);
-                p.set2(4 * j + 2, x0[k][j].z * up, x0[k][j].w * up);
+            for (int j = 0; j < S::QL; ++j) {
+                x0[k][j] = *reinterpret_cast<const float4*>(qrow + ((4 * k + g) * S::QL + j) * 4);
+                if (at >= R) x0[k][j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
             }
+    };
+    auto make_q = [&](int t, const float4 (&x0)[KC][S::QL]) {
+        c[t] = a.scale2;
+        float up = 1.0f;
+        if constexpr (TYPE == ZQ_KV_F16) {  // the row's largest element to 2^14 .. 2^15
+            float most = 0.0f;
 #pragma unroll
-            for (int n = 0; n < NP; ++n) op[n] = p.bits(n);
+            for (int k = 0; k < KC; ++k)
+#pragma unroll
+                for (int j = 0; j < S::QL; ++j)
+                    most = fmaxf(most, fmaxf(fmaxf(fabsf(x0[k][j].x), fabsf(x0[k][j].y)), fmaxf(fabsf(x0[k][j].z), fabsf(x0[k][j].w))));
+            most = max_groups(most);
+            if (most > 0.0f) {
+                const int e = min(max(15 - __builtin_amdgcn_frexp_expf(most), -113), 126);
+                up = pow2f(e);
+                c[t] *= pow2f(-e);
+            }
         }
-        if (k % kWaves == wave)
-#pragma unroll
-            for (int n = 0; n < NP; ++n) held_q[(k * NP + n) * 64 + lane] = op[n];
-    }
-    __syncthreads();
-
-    v4f_t o[VC][VE];
-#pragma unroll
-    for (int n = 0; n < VC; ++n)
-#pragma unroll
-        for (int e = 0; e < VE; ++e) o[n][e] = v4f_t{0.0f, 0.0f, 0.0f, 0.0f};
-    float m = -INFINITY, l = 0.0f;
-    auto step = [&](uint32_t j, auto last) {
-        v4f_t s[H];
-#pragma unroll
-        for (int h = 0; h < H; ++h) s[h] = v4f_t{0.0f, 0.0f, 0.0f, 0.0f};
-        asm volatile("" ::: "memory");  // q is read again, not held
 #pragma unroll
         for (int k = 0; k < KC; ++k) {
             v4u_t op[NP];
+            if constexpr (TYPE == ZQ_KV_F32) {
+                op[0] = v4u_t{f_bits(x0[k][0].x), f_bits(x0[k][0].y), f_bits(x0[k][0].z), f_bits(x0[k][0].w)};
+            } else {
+                Parts<TYPE> p;
 #pragma unroll
-            for (int n = 0; n < NP; ++n) op[n] = held_q[(k * NP + n) * 64 + lane];
+                for (int j = 0; j < 2; ++j) {
+                    p.set2(4 * j, x0[k][j].x * up, x0[k][j].y * up);
+                    p.set2(4 * j + 2, x0[k][j].z * up, x0[k][j].w * up);
+                }
 #pragma unroll
-            for (int h = 0; h < H; ++h) {
-                if constexpr (TYPE == ZQ_KV_F32) {
+                for (int n = 0; n < NP; ++n) op[n] = p.bits(n);
+            }
+            if (k % kWaves == wave)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        s[h] = __builtin_amdgcn_mfma_f32_16x16x4f32(bits_f(kt[h][k][e]), bits_f(op[0][e]), s[h], 0, 0, 0);
-                } else {
+                for (int n = 0; n < NP; ++n) held_q[((t * KC + k) * NP + n) * 64 + lane] = op[n];
+        }
+    };
+    {
+        float4 x0[KC][S::QL];
+        if (RT > 1) my_rows[RT - 1] = 0, c[RT - 1] = 0.0f;
+        if (two) {
+            load_q(RT - 1, x0);
+            make_q(RT - 1, x0);
+        }
+        load_q(0, x0);
+        // (asked for behind the queries, which are waited for first; a wave without tiles reads rows of page 0)
+        load_k(0);
+        load_v(0);
+        make_q(0, x0);
+    }
+    __syncthreads();
+
+    v4f_t o[RT][VC][VE];
+    float m[RT], l[RT];
 #pragma unroll
-                    for (int n = NP - 1; n >= 0; --n) s[h] = mma<TYPE>(kt[h][k], op[n], s[h]);
+    for (int t = 0; t < RT; ++t) {
+        m[t] = -INFINITY;
+        l[t] = 0.0f;
+#pragma unroll
+        for (int n = 0; n < VC; ++n)
+#pragma unroll
+            for (int e = 0; e < VE; ++e) o[t][n][e] = v4f_t{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    auto step = [&](uint32_t j, auto last) {
+        v4f_t s[RT][H];
+        asm volatile("" ::: "memory");  // q is read again, not held
+#pragma unroll
+        for (int t = 0; t < RT; ++t) {
+#pragma unroll
+            for (int h = 0; h < H; ++h) s[t][h] = v4f_t{0.0f, 0.0f, 0.0f, 0.0f};
+            if (t && !two) break;  // uniform
+#pragma unroll
+            for (int k = 0; k < KC; ++k) {
+                v4u_t op[NP];
+#pragma unroll
+                for (int n = 0; n < NP; ++n) op[n] = held_q[((t * KC + k) * NP + n) * 64 + lane];
+#pragma unroll
+                for (int h = 0; h < H; ++h) {
+                    if constexpr (TYPE == ZQ_KV_F32) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            s[t][h] = __builtin_amdgcn_mfma_f32_16x16x4f32(bits_f(kt[h][k][e]), bits_f(op[0][e]), s[t][h], 0, 0, 0);
+                    } else {
+#pragma unroll
+                        for (int n = NP - 1; n >= 0; --n) s[t][h] = mma<TYPE>(kt[h][k], op[n], s[t][h]);
+                    }
                 }
             }
         }
+        const uint32_t key0 = (t0 + (b + j) * kWaves) * H * 16;  // (without selected pages) the tile's first key
         uint32_t rows[H];
         bool cut = false;
 #pragma unroll
         for (int h = 0; h < H; ++h) {
             rows[h] = rows_at(j * H + h);
             cut |= rows[h] < 16;
-            if (GROUP) cut |= (((t0 + (b + j) * kWaves) * H + h) << 4) + 16 > x.least;
+            if (GROUP) cut |= key0 + h * 16 + 16 > x.least;
         }
         if constexpr (!decltype(last)::value) load_k(j + 1);
-#pragma unroll
-        for (int h = 0; h < H; ++h) s[h] *= c;
-        if (cut) {  // uniform
-#pragma unroll
-            for (int h = 0; h < H; ++h) {
-                uint32_t n = rows[h];
-                if (GROUP) n = min(n, uint32_t(max(int32_t(my_rows - (((t0 + (b + j) * kWaves) * H + h) << 4)), 0)));
-#pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    if (uint32_t(4 * g + r) >= n) s[h][r] = -INFINITY;
-            }
-        }
-        float most = -INFINITY;
-#pragma unroll
-        for (int h = 0; h < H; ++h)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) most = fmaxf(most, s[h][r]);
-        if (__any(most > m + kSlack)) {
-            const float to = fmaxf(m, max_groups(most));
-            const float f = to == -INFINITY ? 1.0f : exp2_(m - to);
-            m = to;
-            l *= f;
-#pragma unroll
-            for (int n = 0; n < VC; ++n)
-#pragma unroll
-                for (int e = 0; e < VE; ++e) o[n][e] *= f;
-        }
-        const float ms = (m == -INFINITY ? 0.0f : m) - kShift;
-        float p[VR];
-#pragma unroll
-        for (int h = 0; h < H; ++h)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                p[h * 4 + r] = exp2_(s[h][r] - ms);
-                l += p[h * 4 + r];
-            }
-        if (cut) {
+        auto cut_v = [&] {  // rows behind the last one
+            if (!cut) return;  // uniform
 #pragma unroll
             for (int r = 0; r < VR; ++r) {
                 const uint32_t keep = uint32_t(4 * g + r % 4) < rows[r / 4] ? 0xffffffffu : 0u;
 #pragma unroll
                 for (int n = 0; n < VC; ++n) vt[r][n] &= keep;
             }
-        }
-        const Weights<TYPE, VR> pw(p);
+        };
+        if (GROUP) cut_v();
+        // a value that is no number must not reach (0 times it) the queries that do not see its row
+        bool odd = false;
         if (GROUP && cut && x.least < x.most) {
-            // a value that is no number must not reach (0 times it) the queries that do not see its row
-            bool odd = false;
 #pragma unroll
             for (int r = 0; r < VR; ++r)
 #pragma unroll
                 for (int n = 0; n < VC; ++n)
 #pragma unroll
                     for (int z = 0; z < VW; ++z) odd |= not_finite<TYPE>(vt[r][n][z]);
-            if (__any(odd)) {
-                // per element: how many such values a query sees; more than none gives NaN
-                float sees[VR];
+            odd = __any(odd);
+        }
+        if (odd) {  // per element: how many such values a query sees; more than none gives NaN
+            uint32_t ln = threadIdx.x;
+            asm volatile("" : "+v"(ln));  // made here, not held through the tiles
+            const uint32_t og = (ln >> 4) & 3;
 #pragma unroll
-                for (int r = 0; r < VR; ++r)
-                    sees[r] = (((t0 + (b + j) * kWaves) * H + r / 4) << 4) + 4 * g + r % 4 < my_rows ? 1.0f : 0.0f;
-                const Weights<TYPE, VR> ps(sees);
+            for (int n = 0; n < VC; ++n)
 #pragma unroll
-                for (int n = 0; n < VC; ++n)
+                for (int z = 0; z < VW; ++z) {
+                    uint32_t ones[VR];
 #pragma unroll
-                    for (int z = 0; z < VW; ++z) {
-                        uint32_t ones[VR];
+                    for (int r = 0; r < VR; ++r) {
+                        uint32_t w = vt[r][n][z];
+                        ones[r] = take_odd<TYPE>(w);
+                        vt[r][n][z] = w;
+                    }
 #pragma unroll
-                        for (int r = 0; r < VR; ++r) {
-                            uint32_t w = vt[r][n][z];
-                            ones[r] = take_odd<TYPE>(w);
-                            vt[r][n][z] = w;
-                        }
+                    for (int t = 0; t < RT; ++t) {
+                        float sees[VR];
+#pragma unroll
+                        for (int r = 0; r < VR; ++r) sees[r] = key0 + r / 4 * 16 + 4 * og + r % 4 < my_rows[t] ? 1.0f : 0.0f;
+                        const Weights<TYPE, VR> ps(sees);
 #pragma unroll
                         for (int e = 0; e < VE / VW; ++e) {
                             const v4f_t y = add_pv<TYPE, VR, 1>([&](int r) { return ones[r]; }, ps, e, v4f_t{0.0f, 0.0f, 0.0f, 0.0f});
-                            v4f_t& to = o[n][z * (VE / VW) + e];
+                            v4f_t& to = o[t][n][z * (VE / VW) + e];
 #pragma unroll
                             for (int k = 0; k < 4; ++k) to[k] = y[k] > 0.0f ? NAN : to[k];
                         }
                     }
-            }
+                    __builtin_amdgcn_sched_barrier(0);  // one after the other: in few registers
+                }
         }
 #pragma unroll
-        for (int n = 0; n < VC; ++n)
+        for (int t = 0; t < RT; ++t) {
+            if (t && !two) break;
 #pragma unroll
-            for (int e = 0; e < VE; ++e)
-                o[n][e] = add_pv<TYPE, VR>([&](int r) { return uint32_t(vt[r][n][e * VW / VE]); }, pw, e, o[n][e]);
+            for (int h = 0; h < H; ++h) s[t][h] *= c[t];
+            if (cut) {
+#pragma unroll
+                for (int h = 0; h < H; ++h) {
+                    uint32_t n = rows[h];
+                    if (GROUP) n = min(n, uint32_t(max(int32_t(my_rows[t] - (key0 + h * 16)), 0)));
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (uint32_t(4 * g + r) >= n) s[t][h][r] = -INFINITY;
+                }
+            }
+            float most = -INFINITY;
+#pragma unroll
+            for (int h = 0; h < H; ++h)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) most = fmaxf(most, s[t][h][r]);
+            if (__any(most > m[t] + kSlack)) {
+                const float to = fmaxf(m[t], max_groups(most));
+                const float f = to == -INFINITY ? 1.0f : exp2_(m[t] - to);
+                m[t] = to;
+                l[t] *= f;
+#pragma unroll
+                for (int n = 0; n < VC; ++n)
+#pragma unroll
+                    for (int e = 0; e < VE; ++e) o[t][n][e] *= f;
+            }
+            const float ms = (m[t] == -INFINITY ? 0.0f : m[t]) - kShift;
+            float p[VR];
+#pragma unroll
+            for (int r = 0; r < VR; ++r) {
+                p[r] = exp2_(s[t][r / 4][r % 4] - ms);
+                l[t] += p[r];
+            }
+            if (!GROUP) cut_v();  // (as late as it can be: it waits for V)
+            const Weights<TYPE, VR> pw(p);
+#pragma unroll
+            for (int n = 0; n < VC; ++n)
+#pragma unroll
+                for (int e = 0; e < VE; ++e)
+                    o[t][n][e] = add_pv<TYPE, VR>([&](int r) { return uint32_t(vt[r][n][e * VW / VE]); }, pw, e, o[t][n][e]);
+        }
         if constexpr (!decltype(last)::value) load_v(j + 1);
     };
     while (b < nt) {
@@ -503,54 +546,59 @@ __device__ __forceinline__ void attend(const AttnPaged& a, float* dyn, float (&s
     uint32_t ln = threadIdx.x;
     asm volatile("" : "+v"(ln));  // the addresses below are made here, not held through the tiles
     const uint32_t mi = ln & 15, mg = (ln >> 4) & 3;
-    l = sum_groups(l);
-    if (mg == 0) {
-        sm[wave][mi] = m;
-        sl[wave][mi] = l;
-    }
-    if (mi < R) {
-        float* to = dyn + (size_t(wave) * a.RL + mi) * (D + 4);
 #pragma unroll
-        for (int n = 0; n < VC; ++n)
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-#pragma unroll
-                for (int e = 0; e < VE; e += 4)
-                    *reinterpret_cast<float4*>(to + n * 16 * VE + VE * (4 * mg + r) + e) =
-                        make_float4(o[n][e][r], o[n][e + 1][r], o[n][e + 2][r], o[n][e + 3][r]);
-    }
-    __syncthreads();
-    for (uint32_t z = threadIdx.x; z < R * (D / 4); z += kT) {
-        const uint32_t r = z / (D / 4), d = z % (D / 4) * 4;
-        float M = sm[0][r];
-#pragma unroll
-        for (int w = 1; w < kWaves; ++w) M = fmaxf(M, sm[w][r]);
-        const float Ms = M == -INFINITY ? 0.0f : M;
-        float L = 0.0f;
-        float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-        for (int w = 0; w < kWaves; ++w) {
-            const float f = exp2_(sm[w][r] - Ms);
-            const float4 t = *reinterpret_cast<const float4*>(dyn + (w * a.RL + r) * (D + 4) + d);
-            L += sl[w][r] * f;
-            y.x += t.x * f, y.y += t.y * f, y.z += t.z * f, y.w += t.w * f;
+    for (int t = 0; t < RT; ++t) {
+        if (t && !two) break;
+        const uint32_t rows = min(R - t * 16, 16u);
+        l[t] = sum_groups(l[t]);
+        if (mg == 0) {
+            sm[wave][mi] = m[t];
+            sl[wave][mi] = l[t];
         }
-        if (whole) {
-            const float inv = L > 0.0f ? 1.0f / L : (L == 0.0f ? 0.0f : L);  // no row: 0; NaN stays
-            y.x *= inv, y.y *= inv, y.z *= inv, y.w *= inv;
-        } else if (d == 0) {
-            a.part_ml[(slot + r) * 2] = M;
-            a.part_ml[(slot + r) * 2 + 1] = L;
+        if (mi < rows) {
+            float* to = dyn + (size_t(wave) * a.RL + mi) * (D + 4);
+#pragma unroll
+            for (int n = 0; n < VC; ++n)
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+#pragma unroll
+                    for (int e = 0; e < VE; e += 4)
+                        *reinterpret_cast<float4*>(to + n * 16 * VE + VE * (4 * mg + r) + e) =
+                            make_float4(o[t][n][e][r], o[t][n][e + 1][r], o[t][n][e + 2][r], o[t][n][e + 3][r]);
         }
-        float* to = whole ? out_row(a, qi, kh, row0 + r) * D + a.out : a.part + (slot + r) * D;
-        *reinterpret_cast<float4*>(to + d) = y;
+        __syncthreads();
+        for (uint32_t z = ln; z < rows * (D / 4); z += kT) {
+            const uint32_t r = z / (D / 4), d = z % (D / 4) * 4, at = t * 16 + r;
+            float M = sm[0][r];
+#pragma unroll
+            for (int w = 1; w < kWaves; ++w) M = fmaxf(M, sm[w][r]);
+            const float Ms = M == -INFINITY ? 0.0f : M;
+            float L = 0.0f;
+            float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+            for (int w = 0; w < kWaves; ++w) {
+                const float f = exp2_(sm[w][r] - Ms);
+                const float4 q = *reinterpret_cast<const float4*>(dyn + (w * a.RL + r) * (D + 4) + d);
+                L += sl[w][r] * f;
+                y.x += q.x * f, y.y += q.y * f, y.z += q.z * f, y.w += q.w * f;
+            }
+            if (whole) {
+                const float inv = L > 0.0f ? 1.0f / L : (L == 0.0f ? 0.0f : L);  // no row: 0; NaN stays
+                y.x *= inv, y.y *= inv, y.z *= inv, y.w *= inv;
+            } else if (d == 0) {
+                a.part_ml[(slot + at) * 2] = M;
+                a.part_ml[(slot + at) * 2 + 1] = L;
+            }
+            float* to = whole ? out_row(a, qi, kh, row0 + at) * D + a.out : a.part + (slot + at) * D;
+            *reinterpret_cast<float4*>(to + d) = y;
+        }
+        __syncthreads();
     }
-    __syncthreads();
 }
 
 // Shares of all pairs' units, as they come.  (With D = 256 there is a workgroup a CU: a wave may have all registers.)
-template <int TYPE, int D, bool GROUP>
-__global__ __launch_bounds__(kT, D == 64 ? 4 : D == 128 ? 3 : 1) void attn_paged_kernel(AttnPaged a) {
+template <int TYPE, int D, int GROUP>
+__global__ __launch_bounds__(kT, D == 256 ? 1 : GROUP > 1 ? 2 : (D == 64 ? 4 : 3) - GROUP) void attn_paged_kernel(AttnPaged a) {
     extern __shared__ float dyn[];  // [waves][rows][D + 4], then q's operands
     __shared__ ShareScan scan;
     __shared__ float sm[kWaves][16], sl[kWaves][16];
@@ -586,7 +634,9 @@ __global__ __launch_bounds__(kT, D == 64 ? 4 : D == 128 ? 3 : 1) void attn_paged
         const size_t at = size_t(blockIdx.x) * 2 + (pos != begin);
         if (u0 == 0 && v1 < u && threadIdx.x == 0 && blockIdx.y == 0) {
             // shares with a part of the pair: up to the last one that starts below its end
-            const uint64_t last = ((pos - v0 + u) * sh.used + sh.all - 1) / sh.all - 1;
+            uint64_t all = sh.all;
+            asm volatile("" : "+s"(all));  // its reciprocal is made here, not held through the pairs
+            const uint64_t last = ((pos - v0 + u) * sh.used + all - 1) / all - 1;
             a.cut[blockIdx.x] = {qi, kh, GROUP ? x.queries * a.G : a.G, uint32_t(last - blockIdx.x + 1), at};
         }
         attend<TYPE, D, GROUP>(a, dyn, sm, sl, qi, kh, x, row0, u0, u1, whole, at * a.RS + row0,
@@ -595,23 +645,60 @@ __global__ __launch_bounds__(kT, D == 64 ? 4 : D == 128 ? 3 : 1) void attn_paged
     }
 }
 
+// The group that query i leads, by a wave whose lanes each look at one query of those that
+// might be in it; queries 0 where it leads none.  rows: what query base + lane sees.
+struct GroupLanes {
+    Group x;
+    uint32_t base, rows;
+};
+__device__ __forceinline__ GroupLanes group_by_lanes(const AttnPaged& a, uint32_t i) {
+    const uint32_t lane = threadIdx.x & 63, base = i / a.P * a.P, o = i - base;  // P <= 16
+    Seen s{-1, 0};
+    if (lane < a.P && base + lane < a.see.n) s = seen_by(a.see, base + lane);
+    const int32_t seq = __builtin_amdgcn_readlane(s.seq, int(o));
+    const uint64_t same = __ballot(s.seq == seq) >> o;
+    GroupLanes g{{{seq, 0}, 0, 0, 0}, base, s.rows};
+    if (seq < 0 || (o && __builtin_amdgcn_readlane(s.seq, int(o) - 1) == seq)) return g;
+    const uint32_t n = min(uint32_t(__builtin_ctzll(~same)), a.P - o);
+    g.x.queries = n;
+    uint32_t most = 0, least = 0xffffffffu;
+    if (lane >= o && lane < o + n) most = least = s.rows;
+#pragma unroll
+    for (int m = 1; m < 16; m *= 2) {
+        most = max(most, uint32_t(__shfl_xor(int(most), m)));
+        least = min(least, uint32_t(__shfl_xor(int(least), m)));
+    }
+    g.x.most = uniform(most), g.x.least = uniform(least);
+    return g;
+}
+
 // A workgroup for every pair: nothing to share out and nothing to join.
-template <int TYPE, int D>
-__global__ __launch_bounds__(kT, D == 64 ? 4 : D == 128 ? 3 : 2) void attn_paged_pair_kernel(AttnPaged a) {
+template <int TYPE, int D, bool GROUP>
+__global__ __launch_bounds__(kT, D == 64 ? 4 : GROUP ? 256 / D : D == 128 ? 3 : 2) void attn_paged_pair_kernel(AttnPaged a) {
     extern __shared__ float dyn[];
     __shared__ float sm[kWaves][16], sl[kWaves][16];
     const uint32_t qi = blockIdx.x / a.KH, kh = blockIdx.x % a.KH;
-    // the table entries of a wave's first parts, asked for before it is known how many there are
-    constexpr uint32_t H = Tile<TYPE>::H;
-    const uint32_t lane = threadIdx.x & 63, e = ((lane / H * kWaves + threadIdx.x / 64) * H + lane % H) >> (a.lp - 4);
-    const bool has_ahead = !a.see.seq_of && !a.select;
-    uint32_t ahead = 0;
-    if (has_ahead && e < a.width) ahead = uint32_t(a.table[size_t(qi) * a.width + e]);
-    const Seen s = seen_by(a.see, qi);
-    if (s.seq < 0) return;
-    const Group x{s, 1, s.rows, s.rows};
-    const uint32_t rows = a.select ? entries_of(a, s.rows) << a.lp : s.rows, u = max((rows + Tile<TYPE>::kUnit - 1) / Tile<TYPE>::kUnit, 1u);
-    attend<TYPE, D, false>(a, dyn, sm, sl, qi, kh, x, blockIdx.y * 16, 0, u, true, 0, [](uint32_t) { return 0u; }, has_ahead, ahead);
+    const auto units = [&](uint32_t most) {
+        const uint32_t rows = a.select ? entries_of(a, most) << a.lp : most;
+        return max((rows + Tile<TYPE>::kUnit - 1) / Tile<TYPE>::kUnit, 1u);
+    };
+    if constexpr (GROUP) {
+        const GroupLanes g = group_by_lanes(a, qi);
+        if (g.x.queries == 0) return;
+        attend<TYPE, D, 1>(a, dyn, sm, sl, qi, kh, g.x, 0, 0, units(g.x.most), true, 0,
+                              [&](uint32_t q) { return uint32_t(__shfl(int(g.rows), int(q - g.base))); });
+    } else {
+        // the table entries of a wave's first parts, asked for before it is known how many there are
+        constexpr uint32_t H = Tile<TYPE>::H;
+        const uint32_t lane = threadIdx.x & 63, e = ((lane / H * kWaves + threadIdx.x / 64) * H + lane % H) >> (a.lp - 4);
+        const bool has_ahead = !a.see.seq_of && !a.select;
+        uint32_t ahead = 0;
+        if (has_ahead && e < a.width) ahead = uint32_t(a.table[size_t(qi) * a.width + e]);
+        const Seen s = seen_by(a.see, qi);
+        if (s.seq < 0) return;
+        attend<TYPE, D, 0>(a, dyn, sm, sl, qi, kh, Group{s, 1, s.rows, s.rows}, blockIdx.y * 16, 0, units(s.rows), true, 0,
+                               [](uint32_t) { return 0u; }, has_ahead, ahead);
+    }
 }
 
 // ---- join ------------------------------------------------------------------------
@@ -657,31 +744,34 @@ __global__ __launch_bounds__(kT) void attn_paged_join_kernel(AttnPaged a) {
 // rounds of a workgroup a CU.  us, such workgroups and shares: one sequence of 600 rows, 8 kv heads, D = 128: 9.5, 10.4;
 // 512 sequences of up to 400 rows: 84, 110; 256 of up to 2000: 165, 189; 300 of up to 3000 rows of 1.5 MB, 2 kv heads: 90, 81;
 // 64 of up to 8190, 4 MB: 206, 176; 32 with 2048 selected rows: 61, 69; 40: 97, 88; 4 with 4096: 86, 48.
+// Of groups, all but the first query's workgroups have nothing to do: only where that is a few waves (62 sequences of 6 rows
+// with 8 drafted tokens, 2 kv heads: 18, 25; 74 of 107 with 3, 8 kv heads: 25, 29; two prompts of 500 tokens, 8: 130, 62).
 bool by_pairs(const AttnPaged& a, size_t row_bytes) {
+    if (a.P > 1 && uint64_t(a.see.n) * a.KH > 2048) return false;
     const uint64_t cap = a.see.cap, picked = a.select ? uint64_t(a.keep) << a.lp : cap;
-    const uint64_t bytes = (picked < cap ? picked : cap) * 2 * row_bytes, pairs = uint64_t(a.see.n) * a.KH;
+    const uint64_t bytes = (picked < cap ? picked : cap) * 2 * row_bytes, pairs = uint64_t(a.see.n) * a.KH / a.P;
     const uint64_t rounds = (pairs + 255) / 256;
     return bytes <= 320 * 1024 || (bytes <= 1100 * 1024 && (pairs >= 512 || (a.select && pairs * 10 >= rounds * 256 * 9)));
 }
 
-// What a pair's start counts as, in units (us with 2 and as here: drafted tokens at D = 64: 26, 24; a prompt of 500 tokens
-// of each of two sequences: 64, 62; without groups 1, 2 and 3: 198, 187, 187 for 128 sequences of up to 2000 rows, D = 256).
+// What a pair's start counts as, in units.  us with 2, 3 and 4: drafted tokens of 16 sequences at D = 64: 26, 25, 25; of 8 at
+// D = 128 in two tiles: 50, 47, 41; without groups 1, 2 and 3: 128 sequences of up to 2000 rows, D = 256: 198, 187, 187.
 constexpr uint32_t kMostStart = 4;
-uint32_t start_units(bool group, size_t head_dim) { return !group ? 2 : head_dim == 64 ? kMostStart : 3; }
+uint32_t start_units(bool group) { return group ? kMostStart : 2; }
 // Workgroups for a call, as many as there are units at most: two a CU, and a third (all that are resident) where there
-// are so many pairs that every one starts on several of them; with D = 256 one.  (512, 768, 1536 workgroups, us: 64
+// are so many pairs that every one starts on several of them; with D = 256 one, with groups two.  (512, 768, 1536 workgroups, us: 64
 // sequences of up to 8190 rows, 512 pairs: 175, 177, 182; 512 of up to 400, 4096 pairs: 114, 110, 104; 131,072 rows of
 // one: 89, 91, 100; 32 of up to 8000, bf16, D = 256, with 256, 512 and 1024: 97, 110, 131.)
-uint32_t shares_of(const zq_kv_paged& c, const zq_page_tables& t, size_t queries) {
+uint32_t shares_of(const zq_kv_paged& c, const zq_page_tables& t, size_t queries, bool group) {
     const size_t unit = c.type == ZQ_KV_F32 ? 64 : 128, pairs = queries * c.kv_heads;
     const size_t most = pairs * ((t.width * t.page_size + unit - 1) / unit + kMostStart);
-    const size_t want = 256 * (c.head_dim == 256 ? 1 : pairs < 2048 ? 2 : 3);
+    const size_t want = 256 * (c.head_dim == 256 ? 1 : group || pairs < 2048 ? 2 : 3);
     return uint32_t(most < want ? most : want);
 }
 
 // Queries of a group at most, and rows of a partial, for G heads of a kv head.
-uint32_t group_most(size_t G) { return G <= 8 ? uint32_t(16 / G) : 1; }
-size_t part_rows(size_t G) { return G * group_most(G); }
+uint32_t group_most(size_t G, int tiles) { return G * 2 <= size_t(16 * tiles) ? uint32_t(16 * tiles / G) : 1; }
+size_t part_rows(size_t G) { return G * group_most(G, 2); }
 
 template <class K>
 hipError_t allow_lds(K kernel, size_t lds) {
@@ -689,17 +779,18 @@ hipError_t allow_lds(K kernel, size_t lds) {
     return hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, int(lds));
 }
 
-template <int TYPE, int D, bool GROUP>
+template <int TYPE, int D, int GROUP>
 hipError_t run_attention(const AttnPaged& a, uint32_t W, hipStream_t stream) {
     using S = Shape<TYPE, D>;
-    const size_t lds = size_t(kWaves) * a.RL * (D + 4) * 4 + size_t(S::KC) * S::NP * 64 * 16;
+    const size_t lds = size_t(kWaves) * a.RL * (D + 4) * 4 + size_t(GROUP ? GROUP : 1) * S::KC * S::NP * 64 * 16;
     const uint32_t tiles = GROUP ? 1 : (a.G + 15) / 16;
-    if (!GROUP && by_pairs(a, D * S::ES)) {
-        const hipError_t e = allow_lds(&attn_paged_pair_kernel<TYPE, D>, lds);
-        if (e != hipSuccess) return e;
-        hipLaunchKernelGGL((attn_paged_pair_kernel<TYPE, D>), dim3(a.see.n * a.KH, tiles), dim3(kT), lds, stream, a);
-        return hipGetLastError();
-    }
+    if constexpr (GROUP < 2)
+        if (by_pairs(a, D * S::ES)) {
+            const hipError_t e = allow_lds(&attn_paged_pair_kernel<TYPE, D, GROUP != 0>, lds);
+            if (e != hipSuccess) return e;
+            hipLaunchKernelGGL((attn_paged_pair_kernel<TYPE, D, GROUP != 0>), dim3(a.see.n * a.KH, tiles), dim3(kT), lds, stream, a);
+            return hipGetLastError();
+        }
     hipError_t e = allow_lds(&attn_paged_kernel<TYPE, D, GROUP>, lds);
     if (e != hipSuccess) return e;
     hipLaunchKernelGGL((attn_paged_kernel<TYPE, D, GROUP>), dim3(W, tiles), dim3(kT), lds, stream, a);
@@ -708,18 +799,29 @@ hipError_t run_attention(const AttnPaged& a, uint32_t W, hipStream_t stream) {
     hipLaunchKernelGGL(attn_paged_join_kernel<D>, dim3(W - 1, a.RS), dim3(kT), 0, stream, a);
     return hipGetLastError();
 }
-template <int TYPE, bool GROUP>
+template <int TYPE, int GROUP>
 hipError_t run_attention(const AttnPaged& a, uint32_t W, size_t D, hipStream_t stream) {
     return D == 64 ? run_attention<TYPE, 64, GROUP>(a, W, stream)
                    : D == 128 ? run_attention<TYPE, 128, GROUP>(a, W, stream) : run_attention<TYPE, 256, GROUP>(a, W, stream);
 }
 template <int TYPE>
-hipError_t run_attention(const AttnPaged& a, uint32_t W, size_t D, bool group, hipStream_t stream) {
-    return group ? run_attention<TYPE, true>(a, W, D, stream) : run_attention<TYPE, false>(a, W, D, stream);
+hipError_t run_attention(const AttnPaged& a, uint32_t W, size_t D, int group, hipStream_t stream) {
+    return group == 2   ? run_attention<TYPE, 2>(a, W, D, stream)
+           : group == 1 ? run_attention<TYPE, 1>(a, W, D, stream) : run_attention<TYPE, 0>(a, W, D, stream);
+}
+
+// Tiles of 16 rows for groups of queries of one sequence: 0: no groups; 2, which halve the times that keys are read, where
+// sequences have more queries on average than one tile takes and keys are many.  us, 1 and 2 tiles: 8 sequences of up to 4000
+// rows with 8 queries of 8 heads: 53, 46; 16 of up to 3001 with 5 of 7, D = 64: 25, 30.
+int group_tiles(const zq_kv_paged& c, const zq_page_tables& t, size_t queries, size_t G, bool may) {
+    const size_t bytes = t.width * t.page_size * 2 * c.head_dim * (c.type == ZQ_KV_F32 ? 4 : 2);
+    if (!may || group_most(G, 2) == 1) return 0;
+    if (queries > t.seqs * group_most(G, 1) && bytes >= 1024 * 1024) return 2;
+    return group_most(G, 1) > 1 ? 1 : 0;
 }
 
 size_t workspace(const zq_kv_paged& c, const zq_page_tables& t, size_t queries, size_t heads) {
-    const size_t W = shares_of(c, t, queries), rows = W * 2 * part_rows(heads / c.kv_heads);
+    const size_t W = shares_of(c, t, queries, false), rows = W * 2 * part_rows(heads / c.kv_heads);
     return (W * sizeof(Cut) + rows * (c.head_dim + 2) * 4 + 255) / 256 * 256;
 }
 
@@ -752,7 +854,7 @@ int zq_hip_attention_paged_dev(const zq_kv_paged* cache, const zq_page_tables* t
     if (!workspace || !a16(workspace) || workspace_bytes < zq::workspace(*cache, *tables, queries, heads)) return ZQ_ERR_ARG;
     const zq::OnDeviceOf dev(cache->k);
     if (dev.status() != ZQ_OK) return dev.status();
-    const uint32_t W = zq::shares_of(*cache, *tables, queries), G = uint32_t(heads / cache->kv_heads);
+    const uint32_t G = uint32_t(heads / cache->kv_heads);
     zq::AttnPaged a{};
     a.k = static_cast<const uint8_t*>(cache->k);
     a.v = static_cast<const uint8_t*>(cache->v);
@@ -760,9 +862,10 @@ int zq_hip_attention_paged_dev(const zq_kv_paged* cache, const zq_page_tables* t
     a.select = select;
     a.q = q;
     a.out = out;
-    const bool group = seq_of && !select && zq::group_most(G) > 1;
-    a.P = group ? zq::group_most(G) : 1;
-    a.start = zq::start_units(group, cache->head_dim);
+    const int group = zq::group_tiles(*cache, *tables, queries, G, seq_of && !select);
+    const uint32_t W = zq::shares_of(*cache, *tables, queries, group != 0);
+    a.P = group ? zq::group_most(G, group) : 1;
+    a.start = zq::start_units(group != 0);
     a.RS = a.P * G;
     a.RL = a.RS < 16 ? a.RS : 16;
     a.part = static_cast<float*>(workspace);

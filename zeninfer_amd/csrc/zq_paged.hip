@@ -317,7 +317,7 @@ __global__ __launch_bounds__(256) void paged_append_kernel(AppendArgs a) {
 // workgroup looks for the runs that end in its B tokens: one token where there are few
 // (a decode step), else about a page's, as a workgroup that finds none has cost a wait.
 template <int TYPE, int D, int C>
-__global__ __launch_bounds__(C < 4 ? 256 : C * 64) void paged_append_bounds_kernel(AppendArgs a, uint32_t tokens, uint32_t B) {
+__global__ __launch_bounds__(256) void paged_append_bounds_kernel(AppendArgs a, uint32_t tokens, uint32_t B) {
     typedef typename Held<TYPE>::type T;
     constexpr int E = 16 / sizeof(T), L = D / E, R = 64 / L;  // elements a lane, lanes a row, rows at once
     constexpr int U = 4;
@@ -443,21 +443,20 @@ __global__ __launch_bounds__(C < 4 ? 256 : C * 64) void paged_append_bounds_kern
         }
     }
 }
-constexpr uint32_t kManyTokens = 1024;
+constexpr uint32_t kFewRows = 8192;
 
 template <int TYPE, int D>
 void run_append(const AppendArgs& a, hipStream_t stream) {
     if (a.bounds) {
-        // us, C = 1 / 4 or 8 waves a run, bf16, 8 kv heads, D = 128 (fp32, 2 kv heads, D = 256 for the last): 8200 tokens
-        // and pages of 32: 22 / 44, of 256: 52 / 58; 1402 tokens, pages of 64: 12 / 6.  Blocks of 16, 32, 64 tokens at
-        // pages of 32: 26, 22, 25; of 16: 22, 23, 25.
+        // us with C = 4 and a workgroup a (token, head), and with C = 1 in blocks: 300 decoding sequences of 8 kv heads, pages of
+        // 256, fp32: 37, 124; 1000 tokens of two prompts, pages of 16: 16, 10; 2000: 30, 11.  Blocks of 16 and 32: 8200 tokens,
+        // pages of 16: 22, 23; of 32: 26, 22.
         const uint32_t tokens = a.rows / a.KH, ps = 1u << a.lp;
         auto run = [&](auto kernel, uint32_t threads, uint32_t B) {
             hipLaunchKernelGGL(kernel, dim3((tokens + B - 1) / B * a.KH), dim3(threads), 0, stream, a, tokens, B);
         };
-        if (tokens < kManyTokens) run(paged_append_bounds_kernel<TYPE, D, 4>, 256, 1);
-        else if (a.rows / ps < 256) run(paged_append_bounds_kernel<TYPE, D, 8>, 512, ps);  // fewer runs than CUs
-        else run(paged_append_bounds_kernel<TYPE, D, 1>, 256, ps < 32 ? 16 : 32);
+        if (a.rows <= kFewRows) run(paged_append_bounds_kernel<TYPE, D, 4>, 256, 1);
+        else run(paged_append_bounds_kernel<TYPE, D, 1>, 256, ps < 32 || a.rows <= 4 * kFewRows ? 16 : 32);
         return;
     }
     constexpr uint32_t per = 256 / (D * sizeof(typename Held<TYPE>::type) / 16);

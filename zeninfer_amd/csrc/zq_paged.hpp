@@ -89,7 +89,11 @@ struct Shares {
     uint64_t all;    // of all kv heads
     uint32_t used;   // workgroups that have a share
 };
-__device__ __forceinline__ uint64_t share_start(const Shares& s, uint32_t w) { return uint64_t(w) * s.all / s.used; }
+__device__ __forceinline__ uint32_t uniform(uint32_t x) { return uint32_t(__builtin_amdgcn_readfirstlane(int(x))); }
+__device__ __forceinline__ uint64_t share_start(const Shares& s, uint32_t w) {
+    const uint64_t x = uint64_t(w) * s.all / s.used;
+    return uint64_t(uniform(uint32_t(x))) | uint64_t(uniform(uint32_t(x >> 32))) << 32;
+}
 __device__ __forceinline__ void hold_seen(const Queries& a, ShareScan& sh) {
     if (a.n > kSeenHeld) return;
     for (uint32_t i = threadIdx.x; i < a.n; i += kShareT) {
@@ -153,7 +157,6 @@ template <class V>
 __device__ __forceinline__ V load_once(const void* p) {
     return __builtin_nontemporal_load(reinterpret_cast<const V*>(p));
 }
-__device__ __forceinline__ uint32_t uniform(uint32_t x) { return uint32_t(__builtin_amdgcn_readfirstlane(int(x))); }
 #endif
 
 }  // namespace zq

@@ -818,6 +818,22 @@ def test_select_for_more_queries_than_a_workgroup_holds(zq):
 
 
 @gpu
+def test_select_for_more_heads_and_queries_than_one_grid_dimension_takes(zq):
+    """4200 * 1024 workgroups of 1024 threads are more than 2^32 threads."""
+    n, KH = 4200, 1024
+    pool = scored(zq, [2], KH, 64, 16, seed=3)
+    lens = np.full(n, 15, np.int32)
+    lens[7] = lens[-1] = 16  # these see the second page, which is the recent one
+    q = torch.zeros(n, KH * 64, device=DEV)
+    got = torch.full((n, KH, 1), 55, dtype=torch.int32, device=DEV)
+    need = zq.page_select_workspace_bytes(pool.cache, pool.tables, n, KH, 1)
+    ws = torch.empty(need, dtype=torch.uint8, device=DEV)
+    zq.page_select_dev(pool.cache, pool.tables, q, got, n, KH, dev(lens), 1, recent=1,
+                       seq_of=dev(np.zeros(n, np.int32)), workspace=ws, workspace_bytes=need)
+    assert torch.equal(got[:, :, 0], dev(lens - 15)[:, None].expand(n, KH))
+
+
+@gpu
 def test_select_ties_go_to_the_lowest(zq):
     """All pages alike; a query of zeros; two values only."""
     pool = scored(zq, [500, 3000], 2, 64, 16, 1, like=np.stack([np.full(64, -3), np.full(64, 5)]))

@@ -598,7 +598,7 @@ __device__ __forceinline__ void attend(const AttnPaged& a, float* dyn, float (&s
 
 // Shares of all pairs' units, as they come.  (With D = 256 there is a workgroup a CU: a wave may have all registers.)
 template <int TYPE, int D, int GROUP>
-__global__ __launch_bounds__(kT, D == 256 ? 1 : GROUP > 1 ? 2 : (D == 64 ? 4 : 3) - GROUP) void attn_paged_kernel(AttnPaged a) {
+__global__ __launch_bounds__(kT, D == 256 ? 1 : GROUP > 1 ? 2 : D == 64 ? 4 : 3) void attn_paged_kernel(AttnPaged a) {
     extern __shared__ float dyn[];  // [waves][rows][D + 4], then q's operands
     __shared__ ShareScan scan;
     __shared__ float sm[kWaves][16], sl[kWaves][16];
@@ -754,18 +754,19 @@ bool by_pairs(const AttnPaged& a, size_t row_bytes) {
     return bytes <= 320 * 1024 || (bytes <= 1100 * 1024 && (pairs >= 512 || (a.select && pairs * 10 >= rounds * 256 * 9)));
 }
 
-// What a pair's start counts as, in units.  us with 2, 3 and 4: drafted tokens of 16 sequences at D = 64: 26, 25, 25; of 8 at
-// D = 128 in two tiles: 50, 47, 41; without groups 1, 2 and 3: 128 sequences of up to 2000 rows, D = 256: 198, 187, 187.
+// What a pair's start counts as, in units, with groups in that many tiles (0: none).  us with 2, 3 and 4 in two: 8 drafted
+// tokens of 8 sequences at D = 128: 50, 47, 41; in one, of 32 sequences, 3 and 4: 68, 70; without groups 1, 2 and 3: 128
+// sequences of up to 2000 rows, D = 256: 198, 187, 187.
 constexpr uint32_t kMostStart = 4;
-uint32_t start_units(bool group) { return group ? kMostStart : 2; }
+uint32_t start_units(int tiles) { return uint32_t(2 + tiles); }
 // Workgroups for a call, as many as there are units at most: two a CU, and a third (all that are resident) where there
-// are so many pairs that every one starts on several of them; with D = 256 one, with groups two.  (512, 768, 1536 workgroups, us: 64
+// are so many pairs that every one starts on several of them; with D = 256 one, with two tiles two.  (512, 768, 1536 workgroups, us: 64
 // sequences of up to 8190 rows, 512 pairs: 175, 177, 182; 512 of up to 400, 4096 pairs: 114, 110, 104; 131,072 rows of
 // one: 89, 91, 100; 32 of up to 8000, bf16, D = 256, with 256, 512 and 1024: 97, 110, 131.)
-uint32_t shares_of(const zq_kv_paged& c, const zq_page_tables& t, size_t queries, bool group) {
+uint32_t shares_of(const zq_kv_paged& c, const zq_page_tables& t, size_t queries, int tiles) {
     const size_t unit = c.type == ZQ_KV_F32 ? 64 : 128, pairs = queries * c.kv_heads;
     const size_t most = pairs * ((t.width * t.page_size + unit - 1) / unit + kMostStart);
-    const size_t want = 256 * (c.head_dim == 256 ? 1 : group || pairs < 2048 ? 2 : 3);
+    const size_t want = 256 * (c.head_dim == 256 ? 1 : tiles > 1 || pairs < 2048 ? 2 : 3);
     return uint32_t(most < want ? most : want);
 }
 
@@ -811,17 +812,18 @@ hipError_t run_attention(const AttnPaged& a, uint32_t W, size_t D, int group, hi
 }
 
 // Tiles of 16 rows for groups of queries of one sequence: 0: no groups; 2, which halve the times that keys are read, where
-// sequences have more queries on average than one tile takes and keys are many.  us, 1 and 2 tiles: 8 sequences of up to 4000
-// rows with 8 queries of 8 heads: 53, 46; 16 of up to 3001 with 5 of 7, D = 64: 25, 30.
+// sequences have more queries on average than one tile takes and keys are many; not at D = 256, where the registers for two
+// leave few for loads.  us, 1 and 2 tiles: 8 sequences of up to 4000 rows with 8 queries of 8 heads: 53, 41; 30 of up to 9000
+// with 2 of 16, D = 64: 187, 125; 16 of up to 3001 with 5 of 7, D = 64: 25, 30; 40 of up to 1379 with 8 of 4, D = 256: 38, 46.
 int group_tiles(const zq_kv_paged& c, const zq_page_tables& t, size_t queries, size_t G, bool may) {
     const size_t bytes = t.width * t.page_size * 2 * c.head_dim * (c.type == ZQ_KV_F32 ? 4 : 2);
     if (!may || group_most(G, 2) == 1) return 0;
-    if (queries > t.seqs * group_most(G, 1) && bytes >= 1024 * 1024) return 2;
+    if (c.head_dim < 256 && queries > t.seqs * group_most(G, 1) && bytes >= 1024 * 1024) return 2;
     return group_most(G, 1) > 1 ? 1 : 0;
 }
 
 size_t workspace(const zq_kv_paged& c, const zq_page_tables& t, size_t queries, size_t heads) {
-    const size_t W = shares_of(c, t, queries, false), rows = W * 2 * part_rows(heads / c.kv_heads);
+    const size_t W = shares_of(c, t, queries, 0), rows = W * 2 * part_rows(heads / c.kv_heads);
     return (W * sizeof(Cut) + rows * (c.head_dim + 2) * 4 + 255) / 256 * 256;
 }
 
@@ -863,9 +865,9 @@ int zq_hip_attention_paged_dev(const zq_kv_paged* cache, const zq_page_tables* t
     a.q = q;
     a.out = out;
     const int group = zq::group_tiles(*cache, *tables, queries, G, seq_of && !select);
-    const uint32_t W = zq::shares_of(*cache, *tables, queries, group != 0);
+    const uint32_t W = zq::shares_of(*cache, *tables, queries, group);
     a.P = group ? zq::group_most(G, group) : 1;
-    a.start = zq::start_units(group != 0);
+    a.start = zq::start_units(group);
     a.RS = a.P * G;
     a.RL = a.RS < 16 ? a.RS : 16;
     a.part = static_cast<float*>(workspace);

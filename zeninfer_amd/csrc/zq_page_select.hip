@@ -321,7 +321,7 @@ __device__ __forceinline__ void top_pages(const SelectArgs& a, const float* scor
 }
 
 __global__ __launch_bounds__(kTopT) void page_top_kernel(SelectArgs a) {
-    const uint32_t pair = blockIdx.x, qi = pair / a.KH;
+    const uint32_t qi = blockIdx.y, pair = qi * a.KH + blockIdx.x;
     const Seen x = seen_by(a.see, qi);
     if (x.seq < 0) return;
     const uint32_t n = pages_seen(a, x);
@@ -413,7 +413,8 @@ int zq_hip_page_select_dev(const zq_kv_paged* cache, const zq_page_tables* table
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return zq::status(e);
     }
-    hipLaunchKernelGGL(zq::page_top_kernel, dim3(uint32_t(queries) * a.KH), dim3(zq::kTopT), 0, st, a);
+    // (in two dimensions: 2^23 workgroups of 1024 are more than one dimension takes)
+    hipLaunchKernelGGL(zq::page_top_kernel, dim3(a.KH, uint32_t(queries)), dim3(zq::kTopT), 0, st, a);
     return zq::status(hipGetLastError());
 }
 

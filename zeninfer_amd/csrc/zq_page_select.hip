@@ -39,6 +39,9 @@ __device__ __forceinline__ uint32_t pages_seen(const SelectArgs& a, const Seen& 
 // evenly.  v_mfma_i32_16x16x64_i8: lane (i, g) loads bytes 64 k + 16 g of page i's
 // bounds; it then holds the sums of head i and pages 4 g .. 4 g + 3.  The bounds are
 // asked for before the query's codes are made, of which each wave makes a quarter.
+// Bound by HBM latency: a kv head's bounds are 2 D bytes a page, in a place of their own, and
+// a workgroup has a few units.  4 sequences of 8192 pages, 8 kv heads of 128, 67 MB: 16 us,
+// 4.1 TB/s; 32 of up to 938 pages, 32 MB: 11.6 us.
 template <int D>
 struct ScoreShape {
     static constexpr int B = D == 256 ? 2 : 4;
@@ -177,7 +180,9 @@ __global__ __launch_bounds__(kShareT, 3) void page_score_kernel(SelectArgs a) {
 // every N * 1024), as whole numbers in the order of the scores, from the least one on.
 // The score of rank `want` is found by digits of 11 bits from the highest bit there is,
 // counted in LDS, until all that share its digits stay; one scan of (pages above it,
-// pages at it) then gives every page that stays its place.
+// pages at it) then gives every page that stays its place: what stays, and where, does not
+// depend on the order of the counts.  Bound by a digit's chain (LDS atomics, a scan over the
+// bins, four barriers): 8192 pages 9.8 us, 938 5.9.
 constexpr int kTopT = 1024, kTopWaves = kTopT / 64, kBins = 2048;
 
 __device__ __forceinline__ uint32_t score_key(float f) {

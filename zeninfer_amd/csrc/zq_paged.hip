@@ -19,6 +19,10 @@ namespace {
 // P says.  Every workgroup of a grid repeats the sums, so that one launch will do; where
 // an output is an input too (the granted ones' array the counts', the number of free
 // pages its own successor) and one workgroup is too few, a second launch writes them.
+// Bound by dependent round trips, not by bytes: lens, counts and the number of free pages; an
+// old page's entry or a new page's; the stores; and two barriers.  With a sequence a thread
+// (N = 1) the entries and the stack's top are asked for before the sums.  256 decoding
+// sequences: 6.2 us; 600 with 198,280 new tokens, 3.3 MB (0.6 us of a copy): 9.2.
 constexpr uint32_t kExpand = 1, kCommit = 2;
 constexpr size_t kOneTable = 4096;  // rows up to which one workgroup does it all then
 
@@ -177,7 +181,8 @@ __global__ __launch_bounds__(T) void page_step_kernel(StepArgs a, uint32_t role)
 }
 
 // The pages that the sequences do not need, by the same sums: page x of all that go
-// back, in order of sequence and place, is x below the new top.
+// back, in order of sequence and place, is x below the new top.  Bound like the step: 512
+// sequences that give back 32,896 pages: 3.5 us.
 struct ReleaseArgs {
     const int32_t* table;
     int32_t* free_pages;
@@ -285,7 +290,8 @@ struct AppendArgs {
 };
 
 // A lane takes 16 bytes of a held row, so a row (one token of one kv head) is
-// head_dim * size / 16 lanes.
+// head_dim * size / 16 lanes.  Each byte moves once: bound by HBM, and for a step's few
+// rows by a launch and two round trips (the slot, then the row).
 template <int TYPE, int D>
 __global__ __launch_bounds__(256) void paged_append_kernel(AppendArgs a) {
     typedef typename Held<TYPE>::type T;
@@ -316,6 +322,10 @@ __global__ __launch_bounds__(256) void paged_append_kernel(AppendArgs a) {
 // page's rows before them, and have the bounds without reading the new rows back.  A
 // workgroup looks for the runs that end in its B tokens: one token where there are few
 // (a decode step), else about a page's, as a workgroup that finds none has cost a wait.
+// Bound by HBM where rows are many (8218 tokens of 24 sequences, 8 kv heads of 128, bf16,
+// 102 MB: 23 us, 4.4 TB/s; a copy of as many bytes takes 20), else by the chain of slots,
+// held rows and bounds: 64 decoding sequences: 5.0 us.  With the bounds in a launch of their
+// own, which reads the new rows back, these took 41 and 6.7.
 template <int TYPE, int D, int C>
 __global__ __launch_bounds__(256) void paged_append_bounds_kernel(AppendArgs a, uint32_t tokens, uint32_t B) {
     typedef typename Held<TYPE>::type T;

@@ -604,6 +604,14 @@ __device__ __forceinline__ void attend(const AttnPaged& a, float* dyn, float (&s
     }
 }
 
+// The share of workgroup b of `used`: those of an XCD, which b % 8 says, are neighbours, so that the groups of a sequence
+// that are at the same rows find them in one L2 (drafted tokens of 16 sequences at D = 64: 24.9, 23.7 us).
+__device__ __forceinline__ uint32_t share_by_xcd(uint32_t b, uint32_t used) {
+    if (b >= used) return b;
+    const uint32_t x = b % 8;
+    return x * (used / 8) + min(x, used % 8) + b / 8;
+}
+
 // Shares of all pairs' units, as they come.  (With D = 256 there is a workgroup a CU: a wave may have all registers.)
 template <int TYPE, int D, int GROUP>
 __global__ __launch_bounds__(kT, D == 256 ? 1 : GROUP > 1 ? 2 : D == 64 ? 4 : 3) void attn_paged_kernel(AttnPaged a) {
@@ -615,9 +623,10 @@ __global__ __launch_bounds__(kT, D == 256 ? 1 : GROUP > 1 ? 2 : D == 64 ? 4 : 3)
     hold_seen(a.see, scan);
     uint32_t mine, own;
     const Shares sh = scan_units(a.see.n, a.KH, gridDim.x, kFew, units, scan, mine, own);
-    if (threadIdx.x == 0 && blockIdx.y == 0) a.cut[blockIdx.x].parts = 0;
-    if (blockIdx.x >= sh.used) return;
-    const uint64_t begin = share_start(sh, blockIdx.x), end = share_start(sh, blockIdx.x + 1);
+    const uint32_t share = GROUP ? share_by_xcd(blockIdx.x, sh.used) : blockIdx.x;
+    if (threadIdx.x == 0 && blockIdx.y == 0) a.cut[share].parts = 0;
+    if (share >= sh.used) return;
+    const uint64_t begin = share_start(sh, share), end = share_start(sh, share + 1);
     const Found at_begin = find_query(a.see.n, a.KH, units, scan, begin, mine, own);
     uint32_t qi = at_begin.query, before = at_begin.before;
     uint64_t pos = begin;
@@ -639,13 +648,13 @@ __global__ __launch_bounds__(kT, D == 256 ? 1 : GROUP > 1 ? 2 : D == 64 ? 4 : 3)
         x.first.seq = int32_t(uniform(uint32_t(x.first.seq)));
         x.queries = uniform(x.queries), x.most = uniform(x.most), x.least = uniform(x.least);
         const bool whole = u0 == 0 && v1 == u;
-        const size_t at = size_t(blockIdx.x) * 2 + (pos != begin);
+        const size_t at = size_t(share) * 2 + (pos != begin);
         if (u0 == 0 && v1 < u && threadIdx.x == 0 && blockIdx.y == 0) {
             // shares with a part of the pair: up to the last one that starts below its end
             uint64_t all = sh.all;
             asm volatile("" : "+s"(all));  // its reciprocal is made here, not held through the pairs
             const uint64_t last = ((pos - v0 + u) * sh.used + all - 1) / all - 1;
-            a.cut[blockIdx.x] = {qi, kh, GROUP ? x.queries * a.G : a.G, uint32_t(last - blockIdx.x + 1), at};
+            a.cut[share] = {qi, kh, GROUP ? x.queries * a.G : a.G, uint32_t(last - share + 1), at};
         }
         attend<TYPE, D, GROUP>(a, dyn, sm, sl, qi, kh, x, row0, u0, u1, whole, at * a.RS + row0,
                                        [&](uint32_t n) { return seen_held(a.see, scan, n).rows; });
@@ -755,12 +764,13 @@ __global__ __launch_bounds__(kT) void attn_paged_join_kernel(AttnPaged a) {
 // rounds of a workgroup a CU.  us, such workgroups and shares: one sequence of 600 rows, 8 kv heads, D = 128: 9.5, 10.4;
 // 512 sequences of up to 400 rows: 84, 110; 256 of up to 2000: 165, 189; 300 of up to 3000 rows of 1.5 MB, 2 kv heads: 90, 81;
 // 64 of up to 8190, 4 MB: 206, 176; 32 with 2048 selected rows: 61, 69; 40: 97, 88; 4 with 4096: 86, 48.
-// Of groups, all but the first query's workgroups have nothing to do: only where that is a few waves (62 sequences of 6 rows
-// with 8 drafted tokens, 2 kv heads: 18, 25; 74 of 107 with 3, 8 kv heads: 25, 29; two prompts of 500 tokens, 8: 130, 62).
+// Of groups, all but the first query's workgroups have nothing to do: only where these are few, or all of them (62 sequences
+// of 6 rows with 8 drafted tokens, 2 kv heads: 18, 25; 100 of up to 200 with 2 of 8 heads, 8 kv heads: 26, 28; 128 of up to
+// 300 with 8 of one head, 8: 37, 40; 100 of up to 300 with 4 of 4, 8: 47, 36; two prompts of 500 tokens, 8: 130, 62).
 bool by_pairs(const AttnPaged& a, size_t row_bytes) {
-    if (a.P > 1 && uint64_t(a.see.n) * a.KH > 2048) return false;
     const uint64_t cap = a.see.cap, picked = a.select ? uint64_t(a.keep) << a.lp : cap;
-    const uint64_t bytes = (picked < cap ? picked : cap) * 2 * row_bytes, pairs = uint64_t(a.see.n) * a.KH / a.P;
+    const uint64_t bytes = (picked < cap ? picked : cap) * 2 * row_bytes, all = uint64_t(a.see.n) * a.KH, pairs = all / a.P;
+    if (a.P > 1 && all > 2048 && pairs > 512) return false;
     const uint64_t rounds = (pairs + 255) / 256;
     return bytes <= 320 * 1024 || (bytes <= 1100 * 1024 && (pairs >= 512 || (a.select && pairs * 10 >= rounds * 256 * 9)));
 }

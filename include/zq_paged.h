@@ -103,7 +103,8 @@ typedef struct zq_kv_paged {
  * of a call differ.
  * With bounds, those of every page that gets a row are made anew of the page's
  * rows up to the last one written.  A page's rows of one call have to be
- * neighbours in it and ascend, as a step's do. */
+ * neighbours in it and ascend, as a step's do: consecutive slots in consecutive
+ * rows (of other orders the rows are right and the bounds need not be). */
 int zq_hip_kv_paged_append_dev(const zq_kv_paged* cache, const float* k, const float* v, size_t tokens, size_t stride,
                                const int64_t* slots, void* stream);
 

@@ -31,7 +31,7 @@ FLAGS = [
 def build(verbose=False):
     os.makedirs(LIB_DIR, exist_ok=True)
     tmp = LIB + ".tmp"
-    cmd = [HIPCC, *FLAGS, "-o", tmp, *[os.path.join(SRC, s) for s in SOURCES]]
+    cmd = [HIPCC, *FLAGS, "-parallel-jobs=8", "-o", tmp, *[os.path.join(SRC, s) for s in SOURCES]]
     res = subprocess.run(cmd, capture_output=True, text=True)
     noise = "is not a recognized feature for this target"
     err = "\n".join(l for l in (res.stdout + res.stderr).splitlines() if noise not in l)

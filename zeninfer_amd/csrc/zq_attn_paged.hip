@@ -781,9 +781,9 @@ bool by_pairs(const AttnPaged& a, size_t row_bytes) {
 constexpr uint32_t kMostStart = 4;
 uint32_t start_units(int tiles) { return uint32_t(2 + tiles); }
 // Workgroups for a call, as many as there are units at most: two a CU, and a third (all that are resident) where there
-// are so many pairs that every one starts on several of them; with D = 256 one, with two tiles two.  (512, 768, 1536 workgroups, us: 64
-// sequences of up to 8190 rows, 512 pairs: 175, 177, 182; 512 of up to 400, 4096 pairs: 114, 110, 104; 131,072 rows of
-// one: 89, 91, 100; 32 of up to 8000, bf16, D = 256, with 256, 512 and 1024: 97, 110, 131.)
+// are so many pairs that every one starts on several of them; with D = 256 one, with two tiles two.  (512, 768, 1536
+// workgroups, us: 64 sequences of up to 8190 rows, 512 pairs: 175, 177, 182; 512 of up to 400, 4096 pairs: 114, 110, 104;
+// 131,072 rows of one: 89, 91, 100; 32 of up to 8000, bf16, D = 256, with 256, 512 and 1024: 97, 110, 131.)
 uint32_t shares_of(const zq_kv_paged& c, const zq_page_tables& t, size_t queries, int tiles) {
     const size_t unit = c.type == ZQ_KV_F32 ? 64 : 128, pairs = queries * c.kv_heads;
     const size_t most = pairs * ((t.width * t.page_size + unit - 1) / unit + kMostStart);

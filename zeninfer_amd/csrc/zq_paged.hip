@@ -323,9 +323,9 @@ __global__ __launch_bounds__(256) void paged_append_kernel(AppendArgs a) {
 // workgroup looks for the runs that end in its B tokens: one token where there are few
 // (a decode step), else about a page's, as a workgroup that finds none has cost a wait.
 // Bound by HBM where rows are many (8218 tokens of 24 sequences, 8 kv heads of 128, bf16,
-// 102 MB: 22 to 27 us, 3.8 to 4.4 TB/s; a copy of as many bytes takes 20), else by the chain of slots,
-// held rows and bounds: 64 decoding sequences: 5.0 us.  With the bounds in a launch of their
-// own, which reads the new rows back, these took 41 and 6.7.
+// 102 MB: 22 to 27 us, 3.8 to 4.4 TB/s; a copy of as many bytes takes 20), else by the chain
+// of slots, held rows and bounds: 64 decoding sequences: 5.0 us.  With the bounds in a launch
+// of their own, which reads the new rows back, these took 41 and 6.7.
 template <int TYPE, int D, int C>
 __global__ __launch_bounds__(256) void paged_append_bounds_kernel(AppendArgs a, uint32_t tokens, uint32_t B) {
     typedef typename Held<TYPE>::type T;

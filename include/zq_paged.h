@@ -125,8 +125,8 @@ int zq_hip_kv_paged_append_dev(const zq_kv_paged* cache, const float* k, const f
  * first min(keep, pages of the rows seen) entries count, and those outside the
  * pages seen hold nothing.
  * Scores, exponentials and sums are fp32; q and the softmax weights have 24
- * bits with an fp32 or bf16 cache and 22 with an fp16 one, and the held rows are
- * exact.  NaN and infinities of rows that are not seen do not matter; a seen one
+ * bits with an fp32 or bf16 cache and 22 with an fp16 one (weights below 2^-17 of
+ * the largest are off by 2^-39 of that at most), and the held rows are exact.  NaN and infinities of rows that are not seen do not matter; a seen one
  * gives NaN or an infinity: in the keys in all of the heads' outputs, in the values
  * in that element.
  * At most 8192 queries a call and 1024 heads; workspace: zq_hip_attention_paged_workspace_bytes(),

@@ -106,8 +106,15 @@ __device__ __forceinline__ float sum_groups(float v) {
     return v + __shfl_xor(v, 32);
 }
 
-constexpr float kShift = 6.0f;  // weights are 2^(s - max + kShift)
-constexpr float kSlack = 8.0f;  // how far a score may pass the running maximum
+// Weights are 2^(s - m + kShift) with m the running maximum, which a score may pass by kSlack before the sums are scaled
+// anew.  An fp16 cache's weights are two fp16 parts, multiples of 2^-24 at most 2^15: as far up as they go, a weight has 22
+// bits down to 2^-17 of the largest and is off by 2^-39 of that below; with 6 and 8 as elsewhere it was 2^-31, which 1200
+// rows 2^-20 below a first one showed as 1.3e-4 of their share.  (Sums are scaled more often so, which costs no time:
+// 64 sequences of up to 8190 rows: 176 us either way.)
+template <int TYPE>
+constexpr float kShift = TYPE == ZQ_KV_F16 ? 14.0f : 6.0f;
+template <int TYPE>
+constexpr float kSlack = TYPE == ZQ_KV_F16 ? 1.0f : 8.0f;
 
 // An fp32 factor as operands of the cache's type: fp16 in two parts (22 bits; the
 // factors are scaled so that the second one stays normal), bf16 in three (exact: 8
@@ -511,7 +518,7 @@ __device__ __forceinline__ void attend(const AttnPaged& a, float* dyn, float (&s
             for (int h = 0; h < H; ++h)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) most = fmaxf(most, s[t][h][r]);
-            if (__any(most > m[t] + kSlack)) {
+            if (__any(most > m[t] + kSlack<TYPE>)) {
                 const float to = fmaxf(m[t], max_groups(most));
                 const float f = to == -INFINITY ? 1.0f : exp2_(m[t] - to);
                 m[t] = to;
@@ -521,7 +528,7 @@ __device__ __forceinline__ void attend(const AttnPaged& a, float* dyn, float (&s
 #pragma unroll
                     for (int e = 0; e < VE; ++e) o[t][n][e] *= f;
             }
-            const float ms = (m[t] == -INFINITY ? 0.0f : m[t]) - kShift;
+            const float ms = (m[t] == -INFINITY ? 0.0f : m[t]) - kShift<TYPE>;
             float p[VR];
 #pragma unroll
             for (int r = 0; r < VR; ++r) {

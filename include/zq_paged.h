@@ -69,7 +69,8 @@ int zq_hip_page_tables_step_dev(const zq_page_tables* tables, const int32_t* len
  * the release of what the last step took its inverse.  table is not changed (its
  * entries past the kept pages are no longer the sequence's); *free_left =
  * *free_count plus the pages given back, at most `pages` (may be the same
- * address).  Entries go onto the stack as they are. */
+ * address).  Entries outside 0 .. pages - 1 (given up before) are left out; a page
+ * that stands in several entries comes back as often. */
 int zq_hip_page_tables_release_dev(const zq_page_tables* tables, const int32_t* lens, const int32_t* keep,
                                    const int32_t* free_count, int32_t* free_left, void* stream);
 

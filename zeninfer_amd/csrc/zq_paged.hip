@@ -180,9 +180,13 @@ __global__ __launch_bounds__(T) void page_step_kernel(StepArgs a, uint32_t role)
     }
 }
 
-// The pages that the sequences do not need, by the same sums: page x of all that go
-// back, in order of sequence and place, is x below the new top.  Bound like the step: 512
-// sequences that give back 32,896 pages: 3.5 us.
+// The pages that the sequences do not need go back: of all entries of theirs, in order of sequence and place, those that
+// are pages; a page lies as far above the old top as there are pages behind it.  Entries that are none (pages given up)
+// must not be handed out again, so a workgroup has to know how many of the entries behind its own 1024 are pages, and
+// reads all of these: a wave its part of them, four sequences and up to 256 neighbours of each at once (8 and 256: the
+// same; 8 and 128 or 4 and 512: 10 and 14 % slower); the sequence comes from a ballot over the ends that its lanes hold.
+// 1024 entries and fewer are one workgroup's and no more than a launch, 3.3 us; 512 sequences that give back 32,896 pages:
+// 9.2 us, of which the reads and what finds their addresses are 6.
 struct ReleaseArgs {
     const int32_t* table;
     int32_t* free_pages;
@@ -192,12 +196,15 @@ struct ReleaseArgs {
     int32_t* free_left;
     uint32_t seqs, width, pages, lp;
 };
-template <int T, int N>
-__global__ __launch_bounds__(T) void page_release_kernel(ReleaseArgs a, uint32_t role) {
+constexpr int kReleaseT = 1024, kReleaseWaves = kReleaseT / 64;
+template <int N>
+__global__ __launch_bounds__(kReleaseT) void page_release_kernel(ReleaseArgs a, uint32_t role) {
+    constexpr int T = kReleaseT, W = kReleaseWaves;
     __shared__ uint32_t end[T * N];
-    __shared__ uint32_t from[T * N];  // the first page of a sequence that goes back
-    __shared__ uint32_t part[2][T / 64];
-    const uint32_t tid = threadIdx.x, cap = a.width << a.lp;
+    __shared__ uint32_t from[T * N];  // the first entry of a sequence that goes back
+    __shared__ uint32_t part[2][W];
+    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = uint32_t(__builtin_amdgcn_readfirstlane(int(tid >> 6)));
+    const uint32_t cap = a.width << a.lp;
     const uint32_t fc = uint32_t(min(max(a.free_count[0], 0), int32_t(a.pages)));
     uint32_t back[N];
     Sums2 own{0, 0}, all;
@@ -209,24 +216,98 @@ __global__ __launch_bounds__(T) void page_release_kernel(ReleaseArgs a, uint32_t
         back[j] = tid * N + j < a.seqs ? pages_of(n, a.lp) - k : 0u;
         own.a = add_sat31(own.a, back[j]);
     }
-    Sums2 at = block_before2<T / 64>(own, part, all);
+    Sums2 at = block_before2<W>(own, part, all);
 #pragma unroll
     for (int j = 0; j < N; ++j) end[tid * N + j] = at.a = add_sat31(at.a, back[j]);
     __syncthreads();
-    const uint32_t n = all.a;
-    if (role & kExpand) {
-        for (uint32_t x = blockIdx.x * T + tid; x < n; x += gridDim.x * T) {
-            uint32_t lo = 0, hi = a.seqs - 1;
-            while (lo < hi) {
-                const uint32_t mid = (lo + hi) >> 1;
-                if (end[mid] > x) hi = mid;
-                else lo = mid + 1;
+    const uint32_t n = uniform(all.a);
+    auto sequence_of = [&](uint32_t x) {  // the first one whose end is past x (< n)
+        uint32_t lo = 0, hi = a.seqs - 1;
+        while (lo < hi) {
+            const uint32_t mid = (lo + hi) >> 1;
+            if (end[mid] > x) hi = mid;
+            else lo = mid + 1;
+        }
+        return lo;
+    };
+    // entry x of sequence s is at this plus x (modulo 2^32) in its row
+    auto row_off = [&](uint32_t s) { return from[s] - (s ? end[s - 1] : 0u); };
+    // this workgroup's entries: c0 .. c1 - 1
+    const uint32_t groups = role & kExpand ? gridDim.x : 1u;
+    const uint32_t chunk = max((n + groups - 1) / groups, uint32_t(T));
+    const uint32_t c0 = uint32_t(min(uint64_t(blockIdx.x) * chunk, uint64_t(n))), c1 = role & kExpand ? min(c0 + chunk, n) : 0u;
+    if (blockIdx.x && c0 >= n) return;
+    // how many of those behind them are no pages, a part of these a wave
+    const uint32_t each = (n - c1 + W - 1) / W, x0 = min(c1 + wave * each, n), x1 = min(x0 + each, n);
+    uint32_t none = 0;
+    if (x0 < x1) {
+        uint32_t s0 = uniform(sequence_of(x0)), my_end, my_off;  // of sequence s0 + lane
+        auto hold = [&] {
+            const uint32_t s = min(s0 + lane, a.seqs - 1);
+            my_end = s0 + lane < a.seqs ? end[s] : 0u;
+            my_off = row_off(s);
+        };
+        hold();
+        for (uint32_t x = x0; x < x1;) {
+            constexpr int U = 4, Q = 4;  // sequences at once, and reads of each
+            int32_t v[U][Q];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                uint32_t i = 0, count = 0;
+                if (x < x1) {
+                    uint64_t past = __ballot(my_end > x);
+                    while (!past) {  // ends: x is below the last sequence's end
+                        s0 += 64;
+                        hold();
+                        past = __ballot(my_end > x);
+                    }
+                    i = uint32_t(__builtin_ctzll(past));
+                    count = min(min(uint32_t(__builtin_amdgcn_readlane(int(my_end), int(i))), x1) - x, 64u * Q);
+                }
+                const uint32_t j = count ? uint32_t(__builtin_amdgcn_readlane(int(my_off), int(i))) + x : 0u;
+                const int32_t* at = a.table + (count ? size_t(s0 + i) * a.width + j : 0);
+                // (lanes past the entries read nothing, and get 0, which is a page)
+                const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<int32_t*>(at), 0, int(count * 4), 0x00020000);
+#pragma unroll
+                for (int k = 0; k < Q; ++k) v[u][k] = int32_t(__builtin_amdgcn_raw_buffer_load_b32(r, lane * 4 + 256 * k, 0, 0));
+                x += count;
             }
-            const uint32_t j = from[lo] + x - (lo ? end[lo - 1] : 0u), to = fc + (n - 1 - x);
-            if (to < a.pages) a.free_pages[to] = a.table[size_t(lo) * a.width + j];
+            asm volatile("" ::: "memory");  // all of them are asked for before the first is looked at
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int k = 0; k < Q; ++k) none += uint32_t(v[u][k]) >= a.pages;
         }
     }
-    if ((role & kCommit) && blockIdx.x == 0 && tid == 0) a.free_left[0] = int32_t(min(fc + n, a.pages));
+    uint32_t in_wave;
+    wave_before_sat(none, in_wave);
+    if (lane == 0) part[1][wave] = in_wave;
+    __syncthreads();
+    uint32_t sum = n - c1;  // pages behind
+#pragma unroll
+    for (int w = 0; w < W; ++w) sum -= part[1][w];
+    for (uint32_t b = c1; b > c0;) {  // from the last entry on: a page's place is behind those of the pages behind it
+        const uint32_t x = b - 1 - tid;
+        int32_t v = -1;
+        if (tid < b - c0) {
+            const uint32_t s = sequence_of(x);
+            v = a.table[size_t(s) * a.width + (row_off(s) + x)];
+        }
+        const bool is = uint32_t(v) < a.pages;
+        const uint64_t m = __ballot(is);
+        __syncthreads();
+        if (lane == 0) part[0][wave] = uint32_t(__popcll(m));
+        __syncthreads();
+        uint32_t place = fc + sum + uint32_t(__popcll(m & ((uint64_t(1) << lane) - 1)));
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+            if (uint32_t(w) < wave) place += part[0][w];
+            sum += part[0][w];
+        }
+        if (is && place < a.pages) a.free_pages[place] = v;
+        b -= min(b - c0, uint32_t(T));
+    }
+    if ((role & kCommit) && blockIdx.x == 0 && tid == 0) a.free_left[0] = int32_t(min(fc + sum, a.pages));
 }
 
 // Workgroups of T threads for `rows` rows; where what one writes is what others read, one workgroup or two launches.
@@ -251,15 +332,14 @@ void run_step(const StepArgs& a, hipStream_t stream) {
     else run(page_step_kernel<1024, 8>, 1024);
 }
 void run_release(const ReleaseArgs& a, hipStream_t stream) {
-    const size_t all = size_t(a.seqs) * a.width;
-    auto run = [&](auto kernel, int T) {
-        expand_and_commit(all < a.pages ? all : a.pages, T, a.free_left == a.free_count, [&](uint32_t g, uint32_t role) {
-            hipLaunchKernelGGL(kernel, dim3(g), dim3(T), 0, stream, a, role);
+    const size_t all = size_t(a.seqs) * a.width, entries = all < a.pages ? all : a.pages, most = size_t(256) * kReleaseT;
+    auto run = [&](auto kernel) {  // (at most a workgroup a CU)
+        expand_and_commit(entries < most ? entries : most, kReleaseT, a.free_left == a.free_count, [&](uint32_t g, uint32_t role) {
+            hipLaunchKernelGGL(kernel, dim3(g), dim3(kReleaseT), 0, stream, a, role);
         });
     };
-    if (a.seqs <= 256) run(page_release_kernel<256, 1>, 256);
-    else if (a.seqs <= 1024) run(page_release_kernel<256, 4>, 256);
-    else run(page_release_kernel<1024, 8>, 1024);
+    if (a.seqs <= kReleaseT) run(page_release_kernel<1>);
+    else run(page_release_kernel<8>);
 }
 
 // ---- append ----------------------------------------------------------------------

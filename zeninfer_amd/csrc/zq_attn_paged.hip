@@ -281,7 +281,8 @@ __device__ __forceinline__ void attend(const AttnPaged& a, float* dyn, float (&s
 
     // ---- the wave's tiles ----
     v4u_t kt[H][KC];
-    // (vectors: as dwords of their own they have met a register allocation that overwrote two of four)
+    // (vectors: with dwords of their own a build, not kept, had two of four loaded over before their use; in today's code neither
+    // form has, and a test of the generated code looks for it)
     typedef uint32_t vw_t __attribute__((ext_vector_type(VW)));
     vw_t vt[VR][VC];
     uint32_t place = 0;  // lane p: page | rows there << 24 of the p-th part that the wave has ahead

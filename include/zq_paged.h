@@ -98,14 +98,15 @@ typedef struct zq_kv_paged {
 } zq_kv_paged;
 
 /* Keys and values of `tokens` rows [tokens][stride] fp32 (kv_heads * head_dim
- * used; stride in floats, 0 = kv_heads * head_dim; a multiple of 4, 16-byte
- * aligned) into slots[r], rounded to the cache's type (to nearest, ties to even;
- * past its range to infinity).  Rows whose slot is outside 0 .. pages * page_size - 1 are not written.  Slots
- * of a call differ.
+ * used; stride in floats, 0 = kv_heads * head_dim; a multiple of 4, at most 2^31;
+ * 16-byte aligned) into slots[r], rounded to the cache's type (to nearest, ties to
+ * even; past its range to infinity).  Rows whose slot is outside 0 .. pages *
+ * page_size - 1 are not written.  Slots of a call differ.
  * With bounds, those of every page that gets a row are made anew of the page's
  * rows up to the last one written.  A page's rows of one call have to be
  * neighbours in it and ascend, as a step's do: consecutive slots in consecutive
- * rows (of other orders the rows are right and the bounds need not be). */
+ * rows (of other orders the rows are right and the bounds need not be).
+ * At most 2^24 tokens a call, and tokens * kv_heads 2^25. */
 int zq_hip_kv_paged_append_dev(const zq_kv_paged* cache, const float* k, const float* v, size_t tokens, size_t stride,
                                const int64_t* slots, void* stream);
 
@@ -120,19 +121,24 @@ int zq_hip_kv_paged_append_dev(const zq_kv_paged* cache, const float* k, const f
  * decode step passes the lens and granted counts of its sequences; prompts and
  * drafted tokens the positions and seq_of of a step, with counts NULL.  A query
  * with counts[i] <= 0 or a seq_of outside 0 .. seqs - 1 is idle: its output is
- * left as it was.  One that sees no rows gets 0.
+ * left as it was.  Lengths below 0 count as 0.  One that sees no rows gets 0.
  * select [queries][kv_heads][keep] (NULL: all pages): of every kv head, the
  * pages that the query attends to, by their place in the sequence; of these the
  * first min(keep, pages of the rows seen) entries count, and those outside the
- * pages seen hold nothing.
+ * pages seen hold nothing.  A page named twice counts twice.  keep is at most 2^20.
  * Scores, exponentials and sums are fp32; q and the softmax weights have 24
  * bits with an fp32 or bf16 cache and 22 with an fp16 one (weights below 2^-17 of
- * the largest are off by 2^-39 of that at most), and the held rows are exact.  NaN and infinities of rows that are not seen do not matter; a seen one
- * gives NaN or an infinity: in the keys in all of the heads' outputs, in the values
- * in that element.
- * At most 8192 queries a call and 1024 heads; workspace: zq_hip_attention_paged_workspace_bytes(),
- * 16-byte aligned, of any contents (calls that may run at the same time need
- * one each); with less, the call fails with ZQ_ERR_ARG. */
+ * the largest are off by 2^-39 of that at most), and the held rows are exact.
+ * Before the division by their sum weights go up to 2^14 (fp32 and bf16 caches):
+ * values of 2^-14 of fp32's range, all rows of a sequence together, may overflow.
+ * NaN and infinities of rows that are not seen do not matter.  A seen key that
+ * makes a score of NaN or +infinity gives no numbers in that head's output; one
+ * that makes -infinity does too, or the row has no weight.  A seen NaN or infinity
+ * of the values gives a NaN or an infinity in its element of the outputs.
+ * At most 8192 queries a call and 1024 heads; workspace:
+ * zq_hip_attention_paged_workspace_bytes(), 16-byte aligned, of any contents (calls
+ * that may run at the same time need one each); with less, the call fails with
+ * ZQ_ERR_ARG. */
 #define ZQ_ATTN_PAGED_FULL 1
 size_t zq_hip_attention_paged_workspace_bytes(const zq_kv_paged* cache, const zq_page_tables* tables, size_t queries,
                                               size_t heads);

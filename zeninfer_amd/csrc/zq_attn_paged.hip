@@ -767,11 +767,18 @@ __global__ __launch_bounds__(kT) void attn_paged_join_kernel(AttnPaged a) {
     for (uint32_t d = threadIdx.x; d < D; d += kT) out[d] = ((acc[0][d] + acc[1][d]) + (acc[2][d] + acc[3][d])) * inv;
 }
 
-// Whether every pair gets a workgroup of its own: where pairs are short (up to 320 KB of rows, as the tables' width, or the
-// pages selected, have it), or there are two for every CU of up to 1.1 MB, or they all have as many selected pages and fill
-// rounds of a workgroup a CU.  us, such workgroups and shares: one sequence of 600 rows, 8 kv heads, D = 128: 9.5, 10.4;
-// 512 sequences of up to 400 rows: 84, 110; 256 of up to 2000: 165, 189; 300 of up to 3000 rows of 1.5 MB, 2 kv heads: 90, 81;
-// 64 of up to 8190, 4 MB: 206, 176; 32 with 2048 selected rows: 61, 69; 40: 97, 88; 4 with 4096: 86, 48.
+// Whether every pair gets a workgroup of its own.  The host knows how long a pair may be (the tables' width, or the pages
+// selected), not how long it is.  us, such workgroups and shares, of 8 kv heads of 128 and fp16 if not said otherwise:
+//  - pairs of up to 320 KB of rows: few pairs cross between 280 and 350 KB, more later (pages all over 4 GB: a sequence of
+//    272 KB 8.6, 9.9; 320 KB 9.8, 10.4; 368 KB 11.7, 10.5; bf16, D = 64, 284 KB 9.7, 9.7; 336 KB 11.3, 10.0; fp32, 4 kv heads
+//    of 256, 288 KB 11.0, 13.3; 352 KB 13.7, 13.3; 4 sequences of 272 KB 10.5, 10.9; 320 KB 11.9, 11.4; 16 of 320 KB 14.7,
+//    18.3; of up to 520 KB 18.5, 18.0);
+//  - two pairs for every CU of up to 1.1 MB (64 sequences of up to 1 MB 54, 55; 1.1 MB 56, 56; 1.5 MB 78, 74; 2 MB 103, 95;
+//    512 of up to 200 KB 84, 110);
+//  - as many selected pages each of up to 1.1 MB where the pairs fill rounds of a workgroup a CU (1 MB of longer sequences: 24
+//    sequences 66, 70; 29: 73, 80; 32: 71, 79; 33: 107, 91; 40: 104, 97; 48: 122, 115; 60: 136, 143).  Such pairs gain at 2 MB
+//    too (32: 123, 131), but where lengths are below what may be selected they are of all sizes: 32 sequences of up to 0.5 MB
+//    23, 32; 1 MB 39, 38; 2 MB 70, 58.
 // Of groups, all but the first query's workgroups have nothing to do: only where these are few, or all of them (62 sequences
 // of 6 rows with 8 drafted tokens, 2 kv heads: 18, 25; 100 of up to 200 with 2 of 8 heads, 8 kv heads: 26, 28; 128 of up to
 // 300 with 8 of one head, 8: 37, 40; 100 of up to 300 with 4 of 4, 8: 47, 36; two prompts of 500 tokens, 8: 130, 62).

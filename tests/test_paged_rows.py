@@ -1,6 +1,7 @@
-"""Attention over the paged KV cache (include/zq_paged.h) uses every row that a query sees once: queries of zeros give all
-rows one weight, values are small whole numbers, so an output times the number of rows is a whole number that a row
-too few, too many or of another page changes.  Sequences share their pages, which keeps the caches small where a
+"""Attention over the paged KV cache (include/zq_paged.h) uses every row that a query sees once, with its own key and value.
+Values are small whole numbers, and scores are all equal (queries of zeros) or one of two, so far apart that only the rows
+whose key has a one in a head's place count: an output times the number of rows that count is then a whole number that a
+row too few, too many or of another page changes.  Sequences share their pages, which keeps the caches small where a
 workgroup has more than 4096 keys of a pair in a row."""
 import math
 
@@ -24,23 +25,26 @@ class Whole:
         self.pages = n + extra
         self.order = rng.permutation(self.pages)[:n]
         self.v = rng.integers(-8, 9, (rows, KH, D))
-        self.before = np.concatenate([np.zeros((1, KH, D), np.int64), self.v.cumsum(0)])
+        self.k = rng.integers(0, 2, (rows, KH, D))
 
-    def sum(self, n):
-        """Of the first n rows' values [KH][D]."""
-        return self.before[n]
+    def before(self, h, place):
+        """(numbers of rows, sums of values [D]) of the first 0, 1, .. rows of kv head h whose keys have a one at `place`
+        (None: of all rows)."""
+        one = np.ones(self.rows, np.int64) if place is None else self.k[:, h, place]
+        add = lambda x: np.concatenate([np.zeros_like(x[:1]), x.cumsum(0)])
+        return add(one), add(one[:, None] * self.v[:, h])
 
     def upload(self, zq, seqs, width):
         KH, D, ps, n = self.KH, self.D, self.ps, len(self.order)
-        v = np.full((n * ps, KH, D), math.nan)
-        v[:self.rows] = self.v
-        v = torch.from_numpy(v.reshape(n, ps, KH, D).transpose(0, 2, 1, 3).copy()).to(P.TYPES[self.kind])
-        k = torch.from_numpy(self.rng.standard_normal(v.shape).astype(np.float32)).to(v.dtype)
-        k = torch.where(torch.isnan(v), v, k)
         at = torch.from_numpy(self.order).to(DEV)
-        self.gk = torch.full((self.pages, KH, ps, D), math.nan, dtype=v.dtype, device=DEV)
-        self.gv = self.gk.clone()
-        self.gk[at], self.gv[at] = k.to(DEV), v.to(DEV)
+        to = []
+        for x in (self.k, self.v):  # what no sequence has is NaN
+            rows = np.full((n * ps, KH, D), math.nan, np.float32)
+            rows[:self.rows] = x
+            pool = torch.full((self.pages, KH, ps, D), math.nan, dtype=P.TYPES[self.kind], device=DEV)
+            pool[at] = torch.from_numpy(rows.reshape(n, ps, KH, D).transpose(0, 2, 1, 3).copy()).to(pool.dtype).to(DEV)
+            to.append(pool)
+        self.gk, self.gv = to
         self.gt = torch.full((seqs, width), -1, dtype=torch.int32, device=DEV)
         self.gt[:, :n] = at.int()
         self.cache = zq.KVPaged(self.gk, self.gv, self.pages, KH, D, ps)
@@ -48,49 +52,58 @@ class Whole:
 
 
 def wrong(got, sums, rows):
-    """Outputs [n][G] [D] of one kv head that are not sums [n][D] / rows [n].
+    """Outputs [n][D] that are not sums [n][D] / rows [n].
 
-    All weights are equal, and so their products with whole numbers below 2^4, and the sums of fewer than 2^20 of them, are
-    exact in fp32 in any order; the quotient and the product with it are off by 2^-23 of at most 8 rows: below 1/4."""
-    off = np.abs(got.astype(np.float64) * rows[:, None, None] - sums[:, None, :])
-    return ~(off < 0.25)
+    The rows that count have one weight; its products with whole numbers below 2^4, and the sums of fewer than 2^20 of
+    them, are exact in fp32 in any order.  Others weigh e^-40 of that, 2^20 * 8 * e^-40 < 2^-34 in all.  The quotient and the
+    product with it are off by 2^-23 of at most 8 rows: below 1/4 in all."""
+    return ~(np.abs(got.astype(np.float64) * rows[:, None] - sums) < 0.25)
 
 
 def test_a_lost_row_shows():
     """The check refuses outputs without one row, a page, a unit of keys, and with these rows twice."""
     x = Whole("f16", 1, 64, 16, 20011, seed=1)
-    for n in (300, 4097, 9000, 20011):
-        sums = x.sum(n)
-        fine = (sums / n).astype(np.float32)[:, None]
-        assert not wrong(fine, sums, np.array([n])).any()
-        for a, b in ((n - 1, n), (0, 16), (max(0, n - 128), n), (0, 1), (n // 2, n // 2 + 32)):
-            lost = x.before[min(b, n)] - x.before[a]
-            for y in ((sums - lost) / max(n - (min(b, n) - a), 1), (sums + lost) / (n + min(b, n) - a)):
-                assert wrong(y.astype(np.float32)[:, None], sums, np.array([n])).any() or not lost.any()
+    for place in (None, 3):
+        rows, sums = x.before(0, place)
+        for n in (300, 4097, 9000, 20011):
+            assert not wrong((sums[n] / rows[n]).astype(np.float32)[None], sums[n], rows[n:n + 1]).any()
+            for a, b in ((n - 1, n), (0, 16), (n - 128, n), (0, 1), (n // 2, n // 2 + 32)):
+                count, lost = rows[b] - rows[a], sums[b] - sums[a]
+                for y in ((sums[n] - lost) / (rows[n] - count), (sums[n] + lost) / (rows[n] + count)):
+                    assert wrong(y.astype(np.float32)[None], sums[n], rows[n:n + 1]).any() or not count
 
 
-def check(zq, x, G, lens, seq_of, width, seqs, select=None, select_rows=None):
-    """Queries with lens[i] rows before them, of sequences seq_of (None: one each); select [pages] for all of them."""
+def check(zq, x, G, lens, seq_of, width, seqs, select=None, runs=lambda n: [(0, n)]):
+    """Queries with lens[i] rows before them, of sequences seq_of (None: one each); select [pages] for all of them, and the
+    runs of rows (a, b) that a query with n rows sees then."""
     n, H = len(lens), x.KH * G
     x.upload(zq, seqs, width)
-    q, out = torch.zeros(n, H, x.D, device=DEV), torch.full((n, H, x.D), math.nan, device=DEV)
     need = zq.attention_paged_workspace_bytes(x.cache, x.tables, n, H)
     ws = torch.full((max(need, 16),), 255, dtype=torch.uint8, device=DEV)
     more = {}
     if select is not None:
         more = dict(select=dev(np.broadcast_to(select, (n, x.KH, len(select))).copy()), keep=len(select))
-    zq.attention_paged_dev(x.cache, x.tables, q, out, n, H, dev(lens), 0.1, seq_of=None if seq_of is None else dev(seq_of),
-                           workspace=ws, workspace_bytes=need, **more)
-    got = out.cpu().numpy().reshape(n, x.KH, G, x.D)
-    if select is None:
-        rows = np.asarray(lens) + 1
-        sums = np.stack([x.sum(r) for r in rows])
-    else:
-        picked = [select_rows(r + 1) for r in lens]
-        rows, sums = np.array([p[0] for p in picked]), np.stack([p[1] for p in picked])
-    for h in range(x.KH):
-        bad = wrong(got[:, h], sums[:, h], rows)
-        assert not bad.any(), (h, [(i, int(rows[i])) for i in np.nonzero(bad.any((1, 2)))[0][:8]])
+    sees = [np.array(runs(m + 1), np.int64).reshape(-1, 2) for m in lens]
+    for keys in (False, True):
+        q, out = torch.zeros(n, x.KH, G, x.D, device=DEV), torch.full((n, x.KH, G, x.D), math.nan, device=DEV)
+        places = [(7 * g + 3) % x.D for g in range(G)]
+        if keys:
+            for g, place in enumerate(places):
+                q[:, :, g, place] = 40.0
+        zq.attention_paged_dev(x.cache, x.tables, q, out, n, H, dev(lens), 1.0, seq_of=None if seq_of is None else dev(seq_of),
+                               workspace=ws, workspace_bytes=need, **more)
+        got = out.cpu().numpy()
+        for h in range(x.KH):
+            every = x.before(h, None)
+            for g in sorted({0, 1, 2, G - 1} & set(range(G))) if keys else range(G):
+                rows, sums = x.before(h, places[g]) if keys else every
+                r = np.array([(rows[y[:, 1]] - rows[y[:, 0]]).sum() for y in sees])
+                t = np.stack([(sums[y[:, 1]] - sums[y[:, 0]]).sum(0) for y in sees])
+                for i in np.nonzero(r == 0)[0]:  # none counts: all do
+                    r[i] = max(sum(b - a for a, b in sees[i]), 1)
+                    t[i] = sum((every[1][b] - every[1][a] for a, b in sees[i]), np.zeros(x.D, np.int64))
+                bad = wrong(got[:, h, g], t, r)
+                assert not bad.any(), (keys, h, g, [(i, lens[i] + 1) for i in np.nonzero(bad.any(1))[0][:8]])
 
 
 EDGES = [4095, 4096, 4097, 4096 + 127, 4096 + 128, 4096 + 129, 4224 + 16, 4300]  # 4096 keys are what a workgroup has ahead
@@ -113,15 +126,11 @@ def test_long_pairs_of_selected_pages(zq, kind):
     select = x.rng.permutation(P.cdiv(9000, 16))[:268]
     select[[5, 100, 266]] = [-1, 5000, 2 ** 30]
 
-    def rows_of(n):
-        count, total = 0, np.zeros((8, 64), np.int64)
-        for p in select[:min(268, P.cdiv(n, 16))]:
-            a, b = int(p) * 16, min(int(p) * 16 + 16, n)
-            if 0 <= p < 5000 and a < b:
-                count, total = count + b - a, total + x.before[b] - x.before[a]
-        return max(count, 1), total
+    def runs(n):
+        pages = [int(p) * 16 for p in select[:min(268, P.cdiv(n, 16))] if 0 <= p < 5000]
+        return [(p, min(p + 16, n)) for p in pages if p < n]
     lens = [8999] * 20 + [4095 + i for i in range(40)] + [99, 2000, 0, 4290]
-    check(zq, x, 2, lens, None, 570, 64, select=select, select_rows=rows_of)
+    check(zq, x, 2, lens, None, 570, 64, select=select, runs=runs)
 
 
 @gpu
@@ -143,12 +152,10 @@ def test_long_shares_of_selected_pages(zq, kind, D, G):
     select = np.sort(x.rng.permutation(P.cdiv(40000, 64))[:300])
     select[-1] = P.cdiv(40000, 64) - 1
 
-    def rows_of(n):
-        which = select[:min(300, P.cdiv(n, 64))]
-        runs = [(int(p) * 64, min(int(p) * 64 + 64, n)) for p in which if p * 64 < n]
-        return sum(b - a for a, b in runs), sum(x.before[b] - x.before[a] for a, b in runs)
+    def runs(n):
+        return [(int(p) * 64, min(int(p) * 64 + 64, n)) for p in select[:min(300, P.cdiv(n, 64))] if p * 64 < n]
     lens = [39999 - 7 * (i % 5) if i % 9 else 3000 + i for i in range(200)]
-    check(zq, x, G, lens, None, 700, 200, select=select, select_rows=rows_of)
+    check(zq, x, G, lens, None, 700, 200, select=select, runs=runs)
 
 
 @gpu

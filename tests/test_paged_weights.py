@@ -100,3 +100,36 @@ def test_many_rows_far_below_the_first(zq, kind, queries, n, spare, depth):
                 want = share(x, rows + 1)
                 assert np.abs(got[i, h, :32] - want).max() <= low, (i, x, np.abs(got[i, h, :32] - want).max() / want)
                 assert np.abs(got[i, h, 32:] - 1).max() <= all_, (i, x, np.abs(got[i, h, 32:] - 1).max())
+
+
+@gpu
+@pytest.mark.parametrize("queries", [1, 9])
+def test_values_and_keys_below_the_least_normal_number(zq, queries):
+    """An fp16 cache's rows are exact there too: values of 2^-24 .. 2^-21, and keys that make two scores of 0 and of 12 with
+    queries of 3 * 2^24."""
+    D, ps, G, n = 64, 16, 4, 700
+    rng = np.random.default_rng(3)
+    pages = P.cdiv(n, ps)
+    v = rng.integers(-8, 9, (n, D))
+    one = rng.integers(0, 2, n)
+    k = np.zeros((pages * ps, D))
+    k[:n, 5] = 4 * 2.0 ** -24 * one
+    held = np.full((pages * ps, D), math.nan)
+    held[:n] = v * 2.0 ** -24
+    pool = [torch.from_numpy(x.reshape(pages, 1, ps, D)).half().to(DEV) for x in (k, held)]
+    cache = zq.KVPaged(*pool, pages, 1, D, ps)
+    tables = zq.PageTables(dev(np.arange(pages)[None]), None, 1, pages, pages, ps)
+    q = torch.zeros(queries, G, D, device=DEV)
+    q[:, :, 5] = 3 * 2.0 ** 24
+    out = torch.full_like(q, math.nan)
+    lens = list(range(n - queries, n))
+    need = zq.attention_paged_workspace_bytes(cache, tables, queries, G)
+    ws = torch.empty(need, dtype=torch.uint8, device=DEV)
+    zq.attention_paged_dev(cache, tables, q, out, queries, G, dev(lens), 1.0, seq_of=None if queries == 1 else dev([0] * queries),
+                           workspace=ws, workspace_bytes=need)
+    got = out.cpu().double().numpy()
+    for i, r in enumerate(lens):
+        w = np.where(one[:r + 1] == 1, 1.0, math.exp(-12.0))
+        want, size = (w[:, None] * v[:r + 1]).sum(0) / w.sum(), (w[:, None] * np.abs(v[:r + 1])).sum(0) / w.sum()
+        # (the scores' rounding, 4 * 12 + 12 units, and sums of at most 3 * 700 / 4 additions, in values and weights)
+        assert (np.abs(got[i] * 2.0 ** 24 - want) <= 2 * (60 + 525) * U * size + 2.0 ** -22 * size).all(), i
